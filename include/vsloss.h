@@ -388,7 +388,123 @@ size_t vsl_depth_metrics_workspace_bytes(const vsl_depth_metrics_desc* desc);
 int vsl_depth_metrics(const vsl_depth_metrics_desc* desc, float* metrics, void* workspace, size_t workspace_bytes,
                       void* stream);
 
-/* Library version, e.g. 200 for 0.2.0 (the first with the 200-byte vsl_head), 210 for 0.2.1 (the *_checked calls). */
+/*
+ * Losses over a set of classes: the tokens of a vocabulary, or the depth bins of a pixel (a row is a token or a pixel).
+ * No counterpart in the reference, whose distillation trainers compare features and disparities
+ * (Python/Trainer_distilation.py:1208-1330); these serve heads that answer with a distribution.
+ *
+ * Conventions of the entry points below
+ *   - element types: VSL_TYPE_*; all statistics, sums and losses are float32 or wider;
+ *   - a matrix is row-major with `*_stride` ELEMENTS between its rows (>= its width); the last dimension has stride 1;
+ *   - a logit of -infinity is a class that is masked out.  A row in which nothing is left (every logit, or every teacher
+ *     value, -infinity) adds nothing and gets a zero gradient.  NaN or +infinity in a row makes its results NaN;
+ *   - an index or target outside the vocabulary (other than ignore_index) is never used as an address: its row's loss
+ *     and gradients are NaN;
+ *   - results are deterministic: no floating-point atomics, every sum in a fixed order;
+ *   - limits: 0 <= rows < 2^31, 1 <= vocab < 2^30, 1 <= k <= min(vocab, VSL_MAX_TOP).  rows == 0 is a valid call.
+ */
+#define VSL_TYPE_F32 0
+#define VSL_TYPE_BF16 1
+#define VSL_TYPE_F16 2
+
+#define VSL_REDUCE_NONE 0 /* one loss per row                                                       */
+#define VSL_REDUCE_SUM 1
+#define VSL_REDUCE_MEAN 2 /* divided by the sum of the weights / the number of rows that count; 0 if that is 0 */
+
+#define VSL_MAX_TOP 256
+
+/*
+ * The k largest logits of every row, larger first, ties to the lower index, NaN above +infinity; and, when `lse` is
+ * given, the row's log sum of exp(logit / temperature).  One pass over the logits.
+ * values: [rows,k] of the logits' type; indices: [rows,k]; lse: [rows] or NULL.
+ * workspace: vsl_top_logits_workspace_bytes(desc) bytes (may be 0), 256-byte aligned.
+ */
+typedef struct vsl_top_desc {
+  int64_t rows, vocab, stride;
+  int32_t k, type;
+  float temperature;
+  uint32_t reserved;
+  const void* logits;
+} vsl_top_desc;
+
+size_t vsl_top_logits_workspace_bytes(const vsl_top_desc* desc);
+int vsl_top_logits(const vsl_top_desc* desc, void* values, int32_t* indices, float* lse, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/*
+ * Distillation from a teacher's top logits, temperature T:
+ *   teacher_lse == NULL: q = softmax of the k values / T;
+ *   teacher_lse given (log sum exp(teacher logit / T) over the whole vocabulary): q_j = exp(value_j / T - lse), and what
+ *   is left, q_t = max(0, 1 - sum q), is one further class that the student meets with the sum of its other
+ *   probabilities, p_t (left out where the student has no other class);
+ *   p = softmax(logits / T);  row loss = weight * T^2 * (sum_j q_j log(q_j / p_j) + q_t log(q_t / p_t)).
+ * A row of weight 0 is not looked at.  An index that occurs twice counts with the sum of its q.
+ *
+ * vsl_distill_fwd: row_loss [rows] (weighted); loss and divisor: one float each, the reduced loss and the sum of the
+ * weights (both NULL for VSL_REDUCE_NONE); stats: float [VSL_DISTILL_STATS * rows], what the backward call needs.
+ * vsl_distill_bwd: g_loss: one float, or [rows] for VSL_REDUCE_NONE -> grad: [rows,vocab] of the logits' type, every
+ * element written.  The descriptor is the forward call's; `stats` and `divisor` are its outputs.
+ */
+#define VSL_DISTILL_STATS 8
+typedef struct vsl_distill_desc {
+  int64_t rows, vocab, stride;
+  int32_t k, type;
+  int32_t value_type;    /* VSL_TYPE_* of teacher_values */
+  int32_t index_bytes;   /* 4 or 8: int32 or int64 teacher_indices */
+  int32_t reduction;     /* VSL_REDUCE_* */
+  float temperature;
+  const void* logits;
+  const void* teacher_values;  /* [rows,k] */
+  const void* teacher_indices; /* [rows,k] */
+  const float* teacher_lse;    /* [rows] or NULL */
+  const float* weights;        /* [rows] or NULL: all 1 */
+} vsl_distill_desc;
+
+size_t vsl_distill_workspace_bytes(const vsl_distill_desc* desc);
+int vsl_distill_fwd(const vsl_distill_desc* desc, float* row_loss, float* loss, float* divisor, float* stats,
+                    void* workspace, size_t workspace_bytes, void* stream);
+int vsl_distill_bwd(const vsl_distill_desc* desc, const float* stats, const float* divisor, const float* g_loss,
+                    void* grad, int64_t grad_stride, void* stream);
+
+/*
+ * Softmax cross entropy of z = hidden weight^T + bias, in pieces of the vocabulary: the logits are never kept.
+ *   row loss = lse - z[target] + z_loss * lse^2,  lse = log sum exp z;  rows with target == ignore_index count nothing.
+ * hidden [rows,dim], weight [vocab,dim], bias [vocab] or NULL, all of one type; target [rows].  Products run on the
+ * matrix cores with float32 accumulation; in the backward call the derivative of a logit is rounded to the operands'
+ * type before it meets weight and hidden (scaled by its largest value, so that float16 keeps it).
+ * A class whose bias is -infinity is masked out, whatever its weights hold.
+ *
+ * vsl_linear_ce_fwd: row_loss [rows]; stats [2][rows], the maximum of a row's logits and the log2 of its sum of
+ * exponentials above that (kept apart: a maximum of float32's lowest value would swallow the logarithm); loss and
+ * divisor: one float each, the reduced loss and the number of rows that count (both NULL for VSL_REDUCE_NONE).
+ * vsl_linear_ce_bwd: g_loss: one float, or [rows] for VSL_REDUCE_NONE; stats and divisor are the forward call's outputs.
+ * grad_hidden [rows,dim], grad_weight [vocab,dim], grad_bias [vocab], contiguous, of the operands' type; each may be
+ * NULL.  Workspaces: the matching *_workspace_bytes (grad_mask: bit 0 hidden, 1 weight, 2 bias), 256-byte aligned.
+ * Further limits: rows < 2^28, 1 <= dim < 2^24, rows * vocab < 2^37, rows * dim < 2^36, vocab * dim < 2^36 (each size
+ * rounded up to a multiple of 256).
+ */
+typedef struct vsl_linear_ce_desc {
+  int64_t rows, vocab, dim, hidden_stride, weight_stride;
+  int64_t ignore_index;
+  int32_t type, reduction;
+  float z_loss;
+  uint32_t reserved;
+  const void* hidden;
+  const void* weight;
+  const void* bias;
+  const int64_t* target;
+} vsl_linear_ce_desc;
+
+size_t vsl_linear_ce_fwd_workspace_bytes(const vsl_linear_ce_desc* desc);
+int vsl_linear_ce_fwd(const vsl_linear_ce_desc* desc, float* row_loss, float* stats, float* loss, float* divisor,
+                      void* workspace, size_t workspace_bytes, void* stream);
+size_t vsl_linear_ce_bwd_workspace_bytes(const vsl_linear_ce_desc* desc, uint32_t grad_mask);
+int vsl_linear_ce_bwd(const vsl_linear_ce_desc* desc, const float* stats, const float* divisor, const float* g_loss,
+                      void* grad_hidden, void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/* Library version, e.g. 200 for 0.2.0 (the first with the 200-byte vsl_head), 210 for 0.2.1 (the *_checked calls),
+ * 220 for 0.2.2 (the losses over a set of classes). */
 int vsl_version(void);
 
 #ifdef __cplusplus

@@ -21,7 +21,7 @@ LOSS_TOTAL, LOSS_PHOTO, LOSS_SMOOTH, LOSS_SCALE0 = 0, 1, 2, 3
 LOSS_SLOTS = 3 + MAX_SCALES
 STATIC_SCRATCH_BYTES = 4 << 20
 
-MIN_VERSION = 210
+MIN_VERSION = 220
 EXPORTS = ("vsl_loss_workspace_bytes", "vsl_loss_forward", "vsl_loss_backward", "vsl_identity_min",
            "vsl_loss_forward_heads", "vsl_loss_backward_heads", "vsl_loss_forward_heads_checked",
            "vsl_loss_backward_heads_checked", "vsl_loss_forward_static",
@@ -34,6 +34,9 @@ EXPORTS = ("vsl_loss_workspace_bytes", "vsl_loss_forward", "vsl_loss_backward", 
            "vsl_warp_multi_workspace_bytes", "vsl_warp_multi_fwd", "vsl_warp_multi_bwd",
            "vsl_affinity_loss_workspace_bytes", "vsl_affinity_loss_fwd", "vsl_affinity_loss_bwd",
            "vsl_mean_inv_depth_workspace_bytes", "vsl_mean_inv_depth_fwd", "vsl_mean_inv_depth_bwd",
+           "vsl_top_logits_workspace_bytes", "vsl_top_logits",
+           "vsl_distill_workspace_bytes", "vsl_distill_fwd", "vsl_distill_bwd",
+           "vsl_linear_ce_fwd_workspace_bytes", "vsl_linear_ce_fwd", "vsl_linear_ce_bwd_workspace_bytes", "vsl_linear_ce_bwd",
            "vsl_debug_fused_occupancy", "vsl_debug_quot", "vsl_debug_time_fused", "vsl_last_error_string", "vsl_version")
 
 
@@ -107,6 +110,42 @@ class DepthMetricsDesc(ctypes.Structure):
         ("crop_y0", ctypes.c_int32), ("crop_y1", ctypes.c_int32), ("crop_x0", ctypes.c_int32), ("crop_x1", ctypes.c_int32),
         ("clamp_min", ctypes.c_float), ("clamp_max", ctypes.c_float), ("reserved", ctypes.c_uint32),
         ("depth", ctypes.c_void_p), ("depth_gt", ctypes.c_void_p),
+    ]
+
+
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
+REDUCE_NONE, REDUCE_SUM, REDUCE_MEAN = 0, 1, 2
+MAX_TOP = 256
+DISTILL_STATS = 8
+
+
+class TopDesc(ctypes.Structure):
+    """Mirror of ``vsl_top_desc`` (include/vsloss.h)."""
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("vocab", ctypes.c_int64), ("stride", ctypes.c_int64),
+        ("k", ctypes.c_int32), ("type", ctypes.c_int32), ("temperature", ctypes.c_float), ("reserved", ctypes.c_uint32),
+        ("logits", ctypes.c_void_p),
+    ]
+
+
+class DistillDesc(ctypes.Structure):
+    """Mirror of ``vsl_distill_desc`` (include/vsloss.h)."""
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("vocab", ctypes.c_int64), ("stride", ctypes.c_int64),
+        ("k", ctypes.c_int32), ("type", ctypes.c_int32), ("value_type", ctypes.c_int32), ("index_bytes", ctypes.c_int32),
+        ("reduction", ctypes.c_int32), ("temperature", ctypes.c_float),
+        ("logits", ctypes.c_void_p), ("teacher_values", ctypes.c_void_p), ("teacher_indices", ctypes.c_void_p),
+        ("teacher_lse", ctypes.c_void_p), ("weights", ctypes.c_void_p),
+    ]
+
+
+class LinearCeDesc(ctypes.Structure):
+    """Mirror of ``vsl_linear_ce_desc`` (include/vsloss.h)."""
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("vocab", ctypes.c_int64), ("dim", ctypes.c_int64),
+        ("hidden_stride", ctypes.c_int64), ("weight_stride", ctypes.c_int64), ("ignore_index", ctypes.c_int64),
+        ("type", ctypes.c_int32), ("reduction", ctypes.c_int32), ("z_loss", ctypes.c_float), ("reserved", ctypes.c_uint32),
+        ("hidden", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("target", ctypes.c_void_p),
     ]
 
 
@@ -205,6 +244,15 @@ def _load():
     lib.vsl_mean_inv_depth_fwd.argtypes = [P, P, P, SZ, I, I, I, F, F, P]
     lib.vsl_mean_inv_depth_bwd.restype = ctypes.c_int
     lib.vsl_mean_inv_depth_bwd.argtypes = [P, P, P, I, I, I, I, F, F, P]
+    TD, DD, CD, U = ctypes.POINTER(TopDesc), ctypes.POINTER(DistillDesc), ctypes.POINTER(LinearCeDesc), ctypes.c_uint32
+    for name, restype, args in (
+            ("vsl_top_logits_workspace_bytes", SZ, [TD]), ("vsl_top_logits", I, [TD, P, P, P, P, SZ, P]),
+            ("vsl_distill_workspace_bytes", SZ, [DD]), ("vsl_distill_fwd", I, [DD, P, P, P, P, P, SZ, P]),
+            ("vsl_distill_bwd", I, [DD, P, P, P, P, ctypes.c_int64, P]),
+            ("vsl_linear_ce_fwd_workspace_bytes", SZ, [CD]), ("vsl_linear_ce_fwd", I, [CD, P, P, P, P, P, SZ, P]),
+            ("vsl_linear_ce_bwd_workspace_bytes", SZ, [CD, U]), ("vsl_linear_ce_bwd", I, [CD, P, P, P, P, P, P, P, SZ, P])):
+        fn = getattr(lib, name)
+        fn.restype, fn.argtypes = restype, args
     lib.vsl_last_error_string.restype = ctypes.c_char_p
     lib.vsl_last_error_string.argtypes = []
     lib.vsl_version.restype = ctypes.c_int

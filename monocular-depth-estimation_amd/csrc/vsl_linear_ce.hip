@@ -1,0 +1,768 @@
+// libvsloss.so -- softmax cross entropy of z = hidden weight^T + bias, forward and backward, in pieces of the vocabulary:
+//
+//   forward    z tile by tile on the matrix cores; each tile leaves the maximum and the sum of exponentials of its classes
+//              for every row, and the target's logit; a small kernel joins them into lse and the row losses.
+//   backward   for a piece of the vocabulary: z again, d = g (p (1 + 2 z_loss lse) - [class == target]) rounded to the
+//              operands' type and written as [rows, piece] and as [piece, rows]; then
+//              grad_hidden += d weight_piece (float32 across the pieces) and grad_weight_piece = d^T hidden.
+//
+// All three products are C[M,N] = A[M,K] B[N,K]^T with K contiguous in both operands, so that one main loop serves them:
+// the transposed weight and hidden that the two gradient products need are laid out once per call.  Recomputing z costs
+// a fourth product (a third more operations than keeping the logits) and spares rows * vocab float32 of memory traffic.
+#include "vsl_vocab.hpp"
+
+namespace vsl_vocab {
+namespace {
+
+static_assert(sizeof(vsl_linear_ce_desc) == 96, "C-ABI struct layout changed");
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kTile = 128;       // rows and columns of an output tile
+constexpr int kThreads = 256;    // four waves, 64 x 64 of the tile each
+constexpr int kBlockBytes = 128; // bytes of K that one step of the main loop takes from every row of A and B
+constexpr int kLds = 2 * 2 * kTile * kBlockBytes;
+
+template <typename T>
+struct Kind {
+  static constexpr int E = 16 / (int)sizeof(T);             // elements of a 16-byte piece
+  static constexpr int BK = kBlockBytes / (int)sizeof(T);   // elements of K per step
+};
+
+// One 16-byte piece of A (row = lane % 32) and of B (column = lane % 32) per lane; the two halves of the wave hold
+// neighbouring pieces of K.  Float32 takes the four elements of a piece one after the other: which K meet in one
+// instruction does not matter as long as A and B agree.
+__device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c, const __bf16*) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c, const _Float16*) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c, const float*) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[i]), __uint_as_float(b[i]), c, 0, 0, 0);
+  return c;
+}
+
+// Operands of a product: A [M, >= kblocks * BK], B [N, ...], rows `lda`, `ldb` elements apart.
+struct Operands {
+  const void* A;
+  const void* B;
+  int64_t lda, ldb;
+  int M, N, kblocks;
+};
+
+// C tile of a wave: acc[i][j] covers rows 32 i.. and columns 32 j.. of its 64 x 64; register r of a lane is row
+// (r & 3) + 8 (r >> 2) + 4 (lane >> 5), column lane & 31.
+struct Tile {
+  f32x16 acc[2][2];
+};
+
+// Rows of A and B go through LDS 128 bytes at a time, two buffers deep, straight from global memory.  A row is one line
+// of eight 16-byte pieces; piece p of row r lies at p ^ (r & 7), so that eight rows read at one piece touch all banks.
+template <typename T>
+__device__ __forceinline__ void tile_product(const Operands& op, int m0, int n0, int k0, int k1, char* lds, Tile& t) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int wm = wave >> 1, wn = wave & 1;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) t.acc[i][j][r] = 0.0f;
+  const char* src[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int at = ((i & 3) * 4 + wave) * 64 + lane, row = at >> 3, piece = (at & 7) ^ (row & 7);
+    src[i] = i < 4 ? (const char*)op.A + (int64_t)min(m0 + row, op.M - 1) * op.lda * (int)sizeof(T)
+                   : (const char*)op.B + (int64_t)min(n0 + row, op.N - 1) * op.ldb * (int)sizeof(T);
+    src[i] += (int64_t)k0 * kBlockBytes + piece * 16;
+  }
+  auto fetch = [&](int buffer) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      char* dst = lds + buffer * (2 * kTile * kBlockBytes) + (i < 4 ? 0 : kTile * kBlockBytes) + ((i & 3) * 4 + wave) * 1024;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src[i],
+                                       (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+      src[i] += kBlockBytes;
+    }
+  };
+  if (k0 < k1) fetch(0);
+  for (int k = k0; k < k1; ++k) {
+    const int buffer = (k - k0) & 1;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's share of the step's rows is in LDS
+    __syncthreads();                                  // everyone's is, and the other buffer has been read
+    if (k + 1 < k1) fetch(buffer ^ 1);
+    const char* a = lds + buffer * (2 * kTile * kBlockBytes) + (wm * 64 + (lane & 31)) * kBlockBytes;
+    const char* b = lds + buffer * (2 * kTile * kBlockBytes) + kTile * kBlockBytes + (wn * 64 + (lane & 31)) * kBlockBytes;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int piece = ((2 * s + (lane >> 5)) ^ (lane & 7)) * 16;
+      u32x4 fa[2], fb[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        fa[i] = *(const u32x4*)(a + i * 32 * kBlockBytes + piece);
+        fb[i] = *(const u32x4*)(b + i * 32 * kBlockBytes + piece);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) t.acc[i][j] = mma(fa[i], fb[j], t.acc[i][j], (const T*)nullptr);
+    }
+  }
+  __syncthreads();
+}
+
+// Workgroups are dealt to the 8 XCDs in turn; every XCD gets a contiguous run of tiles, walked in columns of eight rows of
+// tiles, so that the operands' panels meet in one L2.
+__device__ __forceinline__ void tile_of(int64_t block, int64_t tiles_m, int64_t tiles_n, int& tm, int& tn) {
+  const int64_t n = tiles_m * tiles_n, per = n / 8, extra = n % 8, xcd = block % 8;
+  const int64_t i = xcd * per + min(xcd, extra) + block / 8;
+  const int64_t group = 8 * tiles_n, first = i / group * 8, height = min((int64_t)8, tiles_m - first);
+  tm = (int)(first + i % group % height);
+  tn = (int)(i % group / height);
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// forward: A = weight (rows of C are classes), B = hidden (columns are rows of the loss)
+// ------------------------------------------------------------------------------------------------------------------
+struct LogitArgs {
+  Operands op;
+  const void* bias;
+  const int64_t* target;
+  int64_t class0;      // first class of the piece
+  int64_t rows_padded;
+  // forward
+  float2* partial;     // [tiles_m][rows_padded] maximum and sum
+  float* target_logit; // [rows]
+  // backward
+  const float* stats;  // [2][rows] maximum and log2 of the sum above it
+  const float* row_scale;
+  float z_loss;
+  void* delta;         // [rows_padded][ldd]
+  int64_t ldd;
+  void* delta_t;       // [padded classes of the piece][rows_padded]
+};
+
+template <typename T>
+__device__ __forceinline__ float add_bias(float z, const void* bias, int64_t v) {
+  if (!bias) return z;
+  const float b = (float)((const T*)bias)[v];
+  return b == ninf() ? b : z + b;  // a masked class stays masked whatever its weights hold
+}
+
+// derivative of lse + z_loss lse^2 with respect to lse
+__device__ __forceinline__ float slope_of(float z_loss, float top, float ls) {
+  return z_loss == 0.0f ? 1.0f : fmaf(2.0f * z_loss, fmaf(ls, kLn2, top), 1.0f);
+}
+
+template <typename T, bool DELTA>
+__global__ __launch_bounds__(kThreads) void k_ce_logits(LogitArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[kLds];
+  const int tm_count = (a.op.M + kTile - 1) / kTile, tn_count = (a.op.N + kTile - 1) / kTile;
+  int tm, tn;
+  tile_of(blockIdx.x, tm_count, tn_count, tm, tn);
+  const int m0 = tm * kTile, n0 = tn * kTile;
+  Tile t;
+  tile_product<T>(a.op, m0, n0, 0, a.op.kblocks, lds, t);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
+  const int half = lane >> 5;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int col = wn * 64 + j * 32 + (lane & 31), row = n0 + col;
+    const bool live = row < a.op.N;
+    const int64_t target = live ? a.target[row] - a.class0 : -1;
+    float m = ninf();
+    if (!DELTA) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int v = m0 + wm * 64 + i * 32 + (r & 3) + 8 * (r >> 2) + 4 * half;
+          float z = ninf();
+          if (v < a.op.M) {
+            z = add_bias<T>(t.acc[i][j][r], a.bias, a.class0 + v);
+            if (v == target) a.target_logit[row] = z;
+          }
+          t.acc[i][j][r] = z;
+          m = __builtin_elementwise_maximum(m, z);
+        }
+      const float ref = exp_ref(m);
+      float s = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s += exp_of(t.acc[i][j][r], ref, kLog2e);
+      MaxSum q{m, s};
+      q = join(q, {__shfl_xor(q.m, 32, 64), __shfl_xor(q.s, 32, 64)}, kLog2e);
+      if (half == 0) ((float2*)lds)[wm * kTile + col] = make_float2(q.m, q.s);
+    } else {
+      const float scale = live ? a.row_scale[row] : 0.0f;
+      const float top = live ? a.stats[row] : 0.0f, ls = live ? a.stats[a.op.N + row] : 0.0f;
+      const float slope = slope_of(a.z_loss, top, ls);
+      T* d = (T*)a.delta + (int64_t)row * a.ldd;
+      T* dt = (T*)a.delta_t + row;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const int v0 = m0 + wm * 64 + i * 32 + 8 * r4 + 4 * half;
+          T out[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int v = v0 + e;
+            float g = 0.0f;
+            if (v < a.op.M && scale != 0.0f) {
+              const float z = add_bias<T>(t.acc[i][j][r4 * 4 + e], a.bias, a.class0 + v);
+              g = scale * (slope * __builtin_amdgcn_exp2f(fmaf(z - top, kLog2e, -ls)) - (v == target ? 1.0f : 0.0f));
+            }
+            out[e] = (T)g;
+          }
+          if (a.delta)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[v0 + e] = out[e];
+          if (a.delta_t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dt[(int64_t)(v0 + e) * a.rows_padded] = out[e];
+        }
+    }
+  }
+  if (!DELTA) {
+    __syncthreads();
+    const int col = threadIdx.x;
+    if (col < kTile) {
+      const float2 x = ((float2*)lds)[col], y = ((float2*)lds)[kTile + col];
+      const MaxSum q = join({x.x, x.y}, {y.x, y.y}, kLog2e);
+      a.partial[(int64_t)tm * a.rows_padded + n0 + col] = make_float2(q.m, q.s);
+    }
+  }
+}
+
+// 16 rows a block, 16 lanes each: joins the tiles' maxima and sums.
+__global__ __launch_bounds__(kThreads) void k_ce_rows(const float2* __restrict__ partial, int64_t rows_padded, int tiles,
+                                                      const float* __restrict__ target_logit,
+                                                      const int64_t* __restrict__ target, int64_t ignore_index, int64_t vocab,
+                                                      float z_loss, int64_t rows, float* __restrict__ row_loss,
+                                                      float* __restrict__ stats) {
+  __shared__ float2 part[16][16];
+  const int r = threadIdx.x & 15, g = threadIdx.x >> 4;
+  const int64_t row = (int64_t)blockIdx.x * 16 + r;
+  MaxSum q{ninf(), 0.0f};
+  if (row < rows)
+    for (int i = g; i < tiles; i += 16) {
+      const float2 p = partial[(int64_t)i * rows_padded + row];
+      q = join(q, {p.x, p.y}, kLog2e);
+    }
+  part[g][r] = make_float2(q.m, q.s);
+  __syncthreads();
+  if (g == 0 && row < rows) {
+    for (int i = 1; i < 16; ++i) q = join(q, {part[i][r].x, part[i][r].y}, kLog2e);
+    const float ls = log2_sum(q), lse = log_sum(q, 1.0f);
+    float m = q.m, loss = 0.0f;
+    const int64_t t = target[row];
+    if (t != ignore_index) {
+      if (t < 0 || t >= vocab) loss = m = qnan();
+      else if (m != ninf()) loss = fmaf(ls, kLn2, m - target_logit[row]) + (z_loss == 0.0f ? 0.0f : z_loss * lse * lse);
+    }
+    row_loss[row] = loss;
+    stats[row] = m;
+    stats[rows + row] = ls;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// backward: scales of the rows
+// ------------------------------------------------------------------------------------------------------------------
+struct ScaleArgs {
+  const float* g_loss;
+  const float* divisor;
+  const float* stats;
+  const int64_t* target;
+  int64_t ignore_index, rows, rows_padded;
+  int reduction;
+  float z_loss, unit;  // unit: what the largest derivative is scaled to
+  float* partial;      // maxima of the blocks of k_ce_largest; NULL: every row has the same g and no z_loss
+  int partials;
+  float* row_scale;    // [rows_padded]
+  float* out_scale;    // one float: what the products are multiplied by at the end
+};
+__device__ __forceinline__ float row_gradient(const ScaleArgs& a, int64_t row) {
+  if (a.target[row] == a.ignore_index || a.stats[row] == ninf()) return 0.0f;
+  float g = a.g_loss[a.reduction == VSL_REDUCE_NONE ? row : 0];
+  if (a.reduction == VSL_REDUCE_MEAN) g = *a.divisor == 0.0f ? 0.0f : g / *a.divisor;
+  return g;
+}
+__device__ __forceinline__ float block_max(float v, float* red) {
+  v = group_all<64>(v, MaxF());
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(red[0], red[1]),
+                                       __builtin_elementwise_maximum(red[2], red[3]));
+}
+__global__ __launch_bounds__(kThreads) void k_ce_largest(ScaleArgs a) {
+  __shared__ float red[4];
+  float m = 0.0f;
+  for (int64_t r = (int64_t)blockIdx.x * kThreads + threadIdx.x; r < a.rows; r += (int64_t)gridDim.x * kThreads) {
+    const float g = row_gradient(a, r);
+    if (g != 0.0f)
+      m = __builtin_elementwise_maximum(m, fabsf(g) * fmaxf(1.0f, fabsf(slope_of(a.z_loss, a.stats[r], a.stats[a.rows + r]))));
+  }
+  m = block_max(m, red);
+  if (threadIdx.x == 0) a.partial[blockIdx.x] = m;
+}
+__global__ __launch_bounds__(kThreads) void k_ce_scale(ScaleArgs a) {
+  __shared__ float red[4];
+  float largest;
+  if (a.partial) {
+    largest = block_max((int)threadIdx.x < a.partials ? a.partial[threadIdx.x] : 0.0f, red);
+  } else {
+    largest = fabsf(a.g_loss[0]);
+    if (a.reduction == VSL_REDUCE_MEAN) largest = *a.divisor == 0.0f ? 0.0f : largest / *a.divisor;
+  }
+  const int64_t r = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (r < a.rows_padded) {
+    const float g = r < a.rows ? row_gradient(a, r) : 0.0f;
+    a.row_scale[r] = g == 0.0f ? 0.0f : g / largest * a.unit;
+  }
+  if (r == 0) *a.out_scale = largest / a.unit;
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// layouts
+// ------------------------------------------------------------------------------------------------------------------
+// out [rows, cols_padded] = in [rows, cols], zeros behind
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_pad(const T* __restrict__ in, int64_t stride, int64_t rows, int cols,
+                                                  int cols_padded, T* __restrict__ out) {
+  const int64_t n = rows * cols_padded;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) {
+    const int64_t r = i / cols_padded;
+    const int c = (int)(i - r * cols_padded);
+    out[i] = c < cols ? in[r * stride + c] : (T)0.0f;
+  }
+}
+
+// out [cols, rows_padded] = in^T, zeros behind; a row that cannot contribute (its scale is 0, or its bias is -infinity)
+// reads as zeros, so that a NaN in it does not meet the zero of its derivative
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_transpose(const T* __restrict__ in, int64_t stride, int64_t rows, int cols,
+                                                        int64_t rows_padded, const float* __restrict__ scale,
+                                                        const T* __restrict__ bias, T* __restrict__ out) {
+  __shared__ T tile[64][65];
+  const int64_t tiles_c = (cols + 63) / 64;
+  const int64_t r0 = blockIdx.x / tiles_c * 64;
+  const int c0 = (int)(blockIdx.x % tiles_c) * 64;
+  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+  for (int i = y; i < 64; i += 4) {
+    const int64_t r = r0 + i;
+    const int c = c0 + x;
+    T v = (T)0.0f;
+    if (r < rows && c < cols && !(scale && scale[r] == 0.0f) && !(bias && (float)bias[r] == ninf())) v = in[r * stride + c];
+    tile[i][x] = v;
+  }
+  __syncthreads();
+  for (int i = y; i < 64; i += 4)
+    if (c0 + i < cols) out[(int64_t)(c0 + i) * rows_padded + r0 + x] = tile[x][i];
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// the two gradient products
+// ------------------------------------------------------------------------------------------------------------------
+struct GradArgs {
+  Operands op;
+  int splits;              // of K
+  bool add;                // to what `sum` holds
+  float* sum;              // [splits][M][N], or NULL: straight to `out`
+  void* out;               // [M][N] of the operands' type
+  const float* out_scale;
+};
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_ce_grad(GradArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[kLds];
+  const int tm_count = (a.op.M + kTile - 1) / kTile, tn_count = (a.op.N + kTile - 1) / kTile;
+  const int tiles = tm_count * tn_count, split = blockIdx.x / tiles;
+  int tm, tn;
+  tile_of(blockIdx.x % tiles, tm_count, tn_count, tm, tn);
+  const int per = (a.op.kblocks + a.splits - 1) / a.splits;
+  const int k0 = min(split * per, a.op.kblocks), k1 = min(k0 + per, a.op.kblocks);
+  const int m0 = tm * kTile, n0 = tn * kTile;
+  Tile t;
+  tile_product<T>(a.op, m0, n0, k0, k1, lds, t);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
+  const float scale = a.sum ? 1.0f : *a.out_scale;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int row = m0 + wm * 64 + i * 32 + (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5);
+        const int col = n0 + wn * 64 + j * 32 + (lane & 31);
+        if (row >= a.op.M || col >= a.op.N) continue;
+        const int64_t at = (int64_t)row * a.op.N + col;
+        if (a.sum) {
+          float* p = a.sum + (int64_t)split * a.op.M * a.op.N + at;
+          *p = a.add ? *p + t.acc[i][j][r] : t.acc[i][j][r];
+        } else {
+          ((T*)a.out)[at] = (T)(scale * t.acc[i][j][r]);
+        }
+      }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_ce_finish(const float* __restrict__ sum, int splits, int64_t n,
+                                                        const float* __restrict__ out_scale, T* __restrict__ out) {
+  const float scale = *out_scale;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) {
+    float v = sum[i];
+    for (int s = 1; s < splits; ++s) v += sum[s * n + i];
+    out[i] = (T)(scale * v);
+  }
+}
+
+// grad_bias: a block per class sums its row of d^T, the values that grad_weight is made of
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_ce_bias(const T* __restrict__ delta_t, int64_t rows_padded,
+                                                      const float* __restrict__ out_scale, T* __restrict__ out) {
+  __shared__ float red[4];
+  const T* d = delta_t + (int64_t)blockIdx.x * rows_padded;
+  float s = 0.0f;
+  for (int64_t i = threadIdx.x; i < rows_padded / Kind<T>::E; i += kThreads) {
+    float x[Kind<T>::E];
+    unpack(load16(d + i * Kind<T>::E), x, (const T*)nullptr);
+#pragma unroll
+    for (int e = 0; e < Kind<T>::E; ++e) s += x[e];
+  }
+  s = block_add<4>(s, red);
+  if (threadIdx.x == 0) out[blockIdx.x] = (T)(s * *out_scale);
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// host
+// ------------------------------------------------------------------------------------------------------------------
+int size_of(int type) { return type == VSL_TYPE_F32 ? 4 : 2; }
+int64_t round_up(int64_t v, int64_t to) { return ceil_div(v, to) * to; }
+
+int check_ce(const vsl_linear_ce_desc* d) {
+  if (!d) return fail(VSL_ERR_INVALID_ARGUMENT, "linear_ce: descriptor is null");
+  if (d->type != VSL_TYPE_F32 && d->type != VSL_TYPE_BF16 && d->type != VSL_TYPE_F16)
+    return fail(VSL_ERR_INVALID_ARGUMENT, "linear_ce: unknown element type");
+  if (d->rows < 0 || d->rows >= (1LL << 28) || d->vocab < 1 || d->vocab >= (1LL << 30) || d->dim < 1 || d->dim >= (1LL << 24))
+    return fail(VSL_ERR_INVALID_ARGUMENT, "linear_ce: need 0 <= rows < 2^28, 1 <= vocab < 2^30, 1 <= dim < 2^24");
+  if (round_up(d->rows, 256) * round_up(d->vocab, 256) >= (1LL << 37) ||
+      round_up(d->rows, 256) * round_up(d->dim, 256) >= (1LL << 36) || round_up(d->vocab, 256) * round_up(d->dim, 256) >= (1LL << 36))
+    return fail(VSL_ERR_INVALID_ARGUMENT, "linear_ce: need rows * vocab < 2^37, rows * dim < 2^36 and vocab * dim < 2^36");
+  if (d->hidden_stride < d->dim || d->weight_stride < d->dim || d->hidden_stride >= (1LL << 40) || d->weight_stride >= (1LL << 40))
+    return fail(VSL_ERR_INVALID_ARGUMENT, "linear_ce: row strides must be at least dim");
+  if (d->reduction < VSL_REDUCE_NONE || d->reduction > VSL_REDUCE_MEAN)
+    return fail(VSL_ERR_INVALID_ARGUMENT, "linear_ce: unknown reduction");
+  if (!(d->z_loss >= 0.0f) || d->z_loss > 1e30f) return fail(VSL_ERR_INVALID_ARGUMENT, "linear_ce: z_loss must be finite and not negative");
+  if (!d->weight || (d->rows > 0 && (!d->hidden || !d->target))) return fail(VSL_ERR_INVALID_ARGUMENT, "linear_ce: NULL tensor");
+  const int s = size_of(d->type);
+  if ((uintptr_t)d->hidden % s || (uintptr_t)d->weight % s || (uintptr_t)d->bias % s)
+    return fail(VSL_ERR_INVALID_ARGUMENT, "linear_ce: misaligned tensor");
+  return VSL_OK;
+}
+
+// An operand goes to the main loop as it is when its rows are whole 128-byte blocks that 16-byte loads may read.
+bool ready(const void* p, int64_t stride, int64_t dim, int type) {
+  const int s = size_of(type);
+  return (uintptr_t)p % 16 == 0 && stride * s % 16 == 0 && dim * s % kBlockBytes == 0;
+}
+
+struct Arena {
+  char* base;
+  size_t used = 0;
+  void* take(size_t bytes) {
+    void* p = base ? base + used : nullptr;
+    used += up256(bytes);
+    return p;
+  }
+};
+
+struct Layout {
+  int64_t rows_padded, dim_padded;
+  bool copy_hidden, copy_weight;
+};
+Layout layout_of(const vsl_linear_ce_desc* d) {
+  Layout l;
+  l.rows_padded = round_up(d->rows, kTile);
+  l.dim_padded = round_up(d->dim, kBlockBytes / size_of(d->type));
+  l.copy_hidden = !ready(d->hidden, d->hidden_stride, d->dim, d->type);
+  l.copy_weight = !ready(d->weight, d->weight_stride, d->dim, d->type);
+  return l;
+}
+
+struct Forward {
+  void *hidden, *weight;
+  float2* partial;
+  float* target_logit;
+  void* sums;
+  size_t total;
+};
+Forward forward_workspace(const vsl_linear_ce_desc* d, void* base) {
+  const Layout l = layout_of(d);
+  const int s = size_of(d->type);
+  Arena a{(char*)base};
+  Forward f{};
+  f.hidden = l.copy_hidden ? a.take((size_t)d->rows * l.dim_padded * s) : nullptr;
+  f.weight = l.copy_weight ? a.take((size_t)d->vocab * l.dim_padded * s) : nullptr;
+  f.partial = (float2*)a.take((size_t)ceil_div(d->vocab, kTile) * l.rows_padded * sizeof(float2));
+  f.target_logit = (float*)a.take((size_t)d->rows * 4);
+  f.sums = a.take(sum_workspace_bytes(d->rows));
+  f.total = a.used;
+  return f;
+}
+
+// Pieces of the vocabulary whose derivatives hold at most this many elements: 128 MiB in 16 bits, twice, stays in the
+// last-level cache between the kernel that writes them and the two products that read them.
+constexpr int64_t kPieceElements = 1LL << 26;
+
+struct Backward {
+  Layout l;
+  int64_t piece, pieces, vocab_padded;
+  int splits_h, splits_w;
+  void *hidden, *weight, *hidden_t, *weight_t, *delta, *delta_t;
+  float *sum_h, *sum_w, *row_scale, *out_scale, *largest;
+  size_t total;
+};
+int splits_of(int64_t M, int64_t N, int64_t K, int type) {
+  const int64_t tiles = ceil_div(M, kTile) * ceil_div(N, kTile), blocks = ceil_div(K * size_of(type), kBlockBytes);
+  int64_t s = 512 / tiles;
+  if (s > blocks / 8) s = blocks / 8;
+  return (int)(s < 1 ? 1 : s);
+}
+Backward backward_workspace(const vsl_linear_ce_desc* d, uint32_t mask, void* base) {
+  Backward b{};
+  b.l = layout_of(d);
+  const int s = size_of(d->type);
+  b.piece = kPieceElements / (b.l.rows_padded > 0 ? b.l.rows_padded : 1) / kTile * kTile;
+  if (b.piece < kTile) b.piece = kTile;
+  if (b.piece > round_up(d->vocab, kTile)) b.piece = round_up(d->vocab, kTile);
+  b.pieces = ceil_div(d->vocab, b.piece);
+  b.vocab_padded = round_up(d->vocab, kTile);
+  const bool gh = mask & 1, gw = mask & 2, gb = mask & 4;
+  Arena a{(char*)base};
+  b.hidden = b.l.copy_hidden ? a.take((size_t)d->rows * b.l.dim_padded * s) : nullptr;
+  b.weight = b.l.copy_weight ? a.take((size_t)d->vocab * b.l.dim_padded * s) : nullptr;
+  b.hidden_t = gw ? a.take((size_t)d->dim * b.l.rows_padded * s) : nullptr;
+  b.weight_t = gh ? a.take((size_t)d->dim * b.vocab_padded * s) : nullptr;
+  b.delta = gh ? a.take((size_t)b.l.rows_padded * b.piece * s) : nullptr;
+  b.delta_t = gw || gb ? a.take((size_t)b.l.rows_padded * b.piece * s) : nullptr;
+  b.splits_h = splits_of(d->rows, d->dim, b.piece, d->type);
+  b.splits_w = splits_of(d->vocab < b.piece ? d->vocab : b.piece, d->dim, b.l.rows_padded, d->type);
+  b.sum_h = gh && (b.pieces > 1 || b.splits_h > 1) ? (float*)a.take((size_t)b.splits_h * d->rows * d->dim * 4) : nullptr;
+  b.sum_w = gw && b.splits_w > 1 ? (float*)a.take((size_t)b.splits_w * b.piece * d->dim * 4) : nullptr;
+  b.row_scale = (float*)a.take((size_t)b.l.rows_padded * 4);
+  b.out_scale = (float*)a.take(4);
+  b.largest = (float*)a.take(256 * 4);
+  b.total = a.used;
+  return b;
+}
+
+dim3 linear_grid(int64_t n) {
+  const int64_t b = ceil_div(n, kThreads);
+  return dim3((unsigned)(b < 1 ? 1 : (b > 65536 ? 65536 : b)));
+}
+
+template <typename T>
+void launch_pad(const void* in, int64_t stride, int64_t rows, int64_t cols, int64_t cols_padded, void* out, hipStream_t s) {
+  hipLaunchKernelGGL(k_pad<T>, linear_grid(rows * cols_padded), dim3(kThreads), 0, s, (const T*)in, stride, rows, (int)cols,
+                     (int)cols_padded, (T*)out);
+}
+template <typename T>
+void launch_transpose(const void* in, int64_t stride, int64_t rows, int64_t cols, int64_t rows_padded, const float* scale,
+                      const void* bias, void* out, hipStream_t s) {
+  hipLaunchKernelGGL(k_transpose<T>, dim3((unsigned)(ceil_div(rows_padded, 64) * ceil_div(cols, 64))), dim3(kThreads), 0, s,
+                     (const T*)in, stride, rows, (int)cols, rows_padded, scale, (const T*)bias, (T*)out);
+}
+
+template <typename T>
+void run_forward(const vsl_linear_ce_desc* d, const Forward& f, float* row_loss, float* stats, float* loss, float* divisor,
+                 hipStream_t s) {
+  const Layout l = layout_of(d);
+  LogitArgs a{};
+  if (l.copy_hidden) launch_pad<T>(d->hidden, d->hidden_stride, d->rows, d->dim, l.dim_padded, f.hidden, s);
+  if (l.copy_weight) launch_pad<T>(d->weight, d->weight_stride, d->vocab, d->dim, l.dim_padded, f.weight, s);
+  a.op = {l.copy_weight ? f.weight : d->weight, l.copy_hidden ? f.hidden : d->hidden,
+          l.copy_weight ? l.dim_padded : d->weight_stride, l.copy_hidden ? l.dim_padded : d->hidden_stride,
+          (int)d->vocab, (int)d->rows, (int)(l.dim_padded / Kind<T>::BK)};
+  a.bias = d->bias;
+  a.target = d->target;
+  a.rows_padded = l.rows_padded;
+  a.partial = f.partial;
+  a.target_logit = f.target_logit;
+  const int tiles = (int)ceil_div(d->vocab, kTile);
+  hipLaunchKernelGGL((k_ce_logits<T, false>), dim3((unsigned)(tiles * (l.rows_padded / kTile))), dim3(kThreads), 0, s, a);
+  hipLaunchKernelGGL(k_ce_rows, dim3((unsigned)ceil_div(d->rows, 16)), dim3(kThreads), 0, s, (const float2*)f.partial,
+                     l.rows_padded, tiles, (const float*)f.target_logit, d->target, d->ignore_index, d->vocab, d->z_loss,
+                     d->rows, row_loss, stats);
+  if (d->reduction != VSL_REDUCE_NONE)
+    launch_sum(row_loss, nullptr, d->target, d->ignore_index, d->rows, d->reduction, f.sums, loss, divisor, s);
+}
+
+template <typename T>
+void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* stats, const float* divisor, const float* g_loss,
+                  T* grad_hidden, T* grad_weight, T* grad_bias, hipStream_t s) {
+  const Layout& l = b.l;
+  ScaleArgs sc{};
+  sc.g_loss = g_loss;
+  sc.divisor = divisor;
+  sc.stats = stats;
+  sc.target = d->target;
+  sc.ignore_index = d->ignore_index;
+  sc.rows = d->rows;
+  sc.rows_padded = l.rows_padded;
+  sc.reduction = d->reduction;
+  sc.z_loss = d->z_loss;
+  // float16 keeps 2^-14 as its smallest normal number: with the largest derivative at 2^12 (twice that is the largest
+  // value of a row's sum of two terms) a probability down to 2^-26 of it keeps all its bits
+  sc.unit = sizeof(T) == 2 && !__is_same(T, __bf16) ? 4096.0f : 1.0f;
+  sc.row_scale = b.row_scale;
+  sc.out_scale = b.out_scale;
+  if (d->reduction == VSL_REDUCE_NONE || d->z_loss != 0.0f) {
+    const int64_t n = ceil_div(d->rows, kThreads);
+    sc.partial = b.largest;
+    sc.partials = (int)(n > 256 ? 256 : n);
+    hipLaunchKernelGGL(k_ce_largest, dim3(sc.partials), dim3(kThreads), 0, s, sc);
+  }
+  hipLaunchKernelGGL(k_ce_scale, dim3((unsigned)ceil_div(l.rows_padded, kThreads)), dim3(kThreads), 0, s, sc);
+  if (l.copy_hidden) launch_pad<T>(d->hidden, d->hidden_stride, d->rows, d->dim, l.dim_padded, b.hidden, s);
+  if (l.copy_weight) launch_pad<T>(d->weight, d->weight_stride, d->vocab, d->dim, l.dim_padded, b.weight, s);
+  const T* hidden = (const T*)(l.copy_hidden ? b.hidden : d->hidden);
+  const T* weight = (const T*)(l.copy_weight ? b.weight : d->weight);
+  const int64_t ldh = l.copy_hidden ? l.dim_padded : d->hidden_stride, ldw = l.copy_weight ? l.dim_padded : d->weight_stride;
+  if (grad_weight) launch_transpose<T>(hidden, ldh, d->rows, d->dim, l.rows_padded, b.row_scale, nullptr, b.hidden_t, s);
+  if (grad_hidden) launch_transpose<T>(weight, ldw, d->vocab, d->dim, b.vocab_padded, nullptr, d->bias, b.weight_t, s);
+  for (int64_t p = 0; p < b.pieces; ++p) {
+    const int64_t v0 = p * b.piece, classes = d->vocab - v0 < b.piece ? d->vocab - v0 : b.piece;
+    const int64_t padded = round_up(classes, kTile);
+    LogitArgs a{};
+    a.op = {weight + v0 * ldw, hidden, ldw, ldh, (int)classes, (int)d->rows, (int)(l.dim_padded / Kind<T>::BK)};
+    a.bias = d->bias;
+    a.target = d->target;
+    a.class0 = v0;
+    a.rows_padded = l.rows_padded;
+    a.stats = stats;
+    a.row_scale = b.row_scale;
+    a.z_loss = d->z_loss;
+    a.delta = grad_hidden ? b.delta : nullptr;
+    a.ldd = b.piece;
+    a.delta_t = grad_weight || grad_bias ? b.delta_t : nullptr;
+    hipLaunchKernelGGL((k_ce_logits<T, true>), dim3((unsigned)(padded / kTile * (l.rows_padded / kTile))), dim3(kThreads), 0,
+                       s, a);
+    if (grad_hidden) {
+      GradArgs g{};
+      g.op = {b.delta, (const T*)b.weight_t + v0, b.piece, b.vocab_padded, (int)d->rows, (int)d->dim, (int)(padded / Kind<T>::BK)};
+      g.splits = b.splits_h;
+      g.add = p > 0;
+      g.sum = b.sum_h;
+      g.out = grad_hidden;
+      g.out_scale = b.out_scale;
+      const int64_t tiles = ceil_div(d->rows, kTile) * ceil_div(d->dim, kTile);
+      hipLaunchKernelGGL(k_ce_grad<T>, dim3((unsigned)(tiles * g.splits)), dim3(kThreads), 0, s, g);
+    }
+    if (grad_weight) {
+      GradArgs g{};
+      g.op = {b.delta_t, b.hidden_t, l.rows_padded, l.rows_padded, (int)classes, (int)d->dim, (int)(l.rows_padded / Kind<T>::BK)};
+      g.splits = b.splits_w;
+      g.sum = b.sum_w;
+      g.out = grad_weight + v0 * d->dim;
+      g.out_scale = b.out_scale;
+      const int64_t tiles = ceil_div(classes, kTile) * ceil_div(d->dim, kTile);
+      hipLaunchKernelGGL(k_ce_grad<T>, dim3((unsigned)(tiles * g.splits)), dim3(kThreads), 0, s, g);
+      if (g.sum)
+        hipLaunchKernelGGL(k_ce_finish<T>, linear_grid(classes * d->dim), dim3(kThreads), 0, s, (const float*)g.sum, g.splits,
+                           classes * d->dim, (const float*)b.out_scale, (T*)g.out);
+    }
+    if (grad_bias)
+      hipLaunchKernelGGL(k_ce_bias<T>, dim3((unsigned)classes), dim3(kThreads), 0, s, (const T*)b.delta_t, l.rows_padded,
+                         (const float*)b.out_scale, grad_bias + v0);
+  }
+  if (grad_hidden && b.sum_h)
+    hipLaunchKernelGGL(k_ce_finish<T>, linear_grid(d->rows * d->dim), dim3(kThreads), 0, s, (const float*)b.sum_h, b.splits_h,
+                       d->rows * d->dim, (const float*)b.out_scale, grad_hidden);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_zero(T* p, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) p[i] = (T)0.0f;
+}
+// no rows: the gradients of the shared operands are zero
+template <typename T>
+void zero_shared(const vsl_linear_ce_desc* d, void* grad_weight, void* grad_bias, hipStream_t s) {
+  if (grad_weight)
+    hipLaunchKernelGGL(k_zero<T>, linear_grid(d->vocab * d->dim), dim3(kThreads), 0, s, (T*)grad_weight, d->vocab * d->dim);
+  if (grad_bias) hipLaunchKernelGGL(k_zero<T>, linear_grid(d->vocab), dim3(kThreads), 0, s, (T*)grad_bias, d->vocab);
+}
+
+int check_space(const void* workspace, size_t have, size_t need) {
+  if (have < need) return fail(VSL_ERR_WORKSPACE_TOO_SMALL, "linear_ce: workspace too small");
+  if (need && (!workspace || (uintptr_t)workspace % 256))
+    return fail(VSL_ERR_INVALID_ARGUMENT, "linear_ce: workspace must be 256-byte aligned and not NULL");
+  return VSL_OK;
+}
+
+}  // namespace
+}  // namespace vsl_vocab
+
+using namespace vsl_vocab;
+
+extern "C" {
+
+size_t vsl_linear_ce_fwd_workspace_bytes(const vsl_linear_ce_desc* d) {
+  return check_ce(d) ? 0 : forward_workspace(d, nullptr).total;
+}
+
+int vsl_linear_ce_fwd(const vsl_linear_ce_desc* d, float* row_loss, float* stats, float* loss, float* divisor, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  if (int rc = check_ce(d)) return rc;
+  if (d->rows > 0 && (!row_loss || !stats)) return fail(VSL_ERR_INVALID_ARGUMENT, "linear_ce: NULL output");
+  if (d->reduction != VSL_REDUCE_NONE && (!loss || !divisor)) return fail(VSL_ERR_INVALID_ARGUMENT, "linear_ce: NULL loss");
+  const Forward f = forward_workspace(d, workspace);
+  if (int rc = check_space(workspace, workspace_bytes, f.total)) return rc;
+  hipStream_t s = (hipStream_t)stream;
+  if (d->rows == 0) {
+    if (d->reduction != VSL_REDUCE_NONE) launch_sum(row_loss, nullptr, d->target, d->ignore_index, 0, d->reduction, f.sums, loss, divisor, s);
+  } else if (d->type == VSL_TYPE_F32) {
+    run_forward<float>(d, f, row_loss, stats, loss, divisor, s);
+  } else if (d->type == VSL_TYPE_BF16) {
+    run_forward<__bf16>(d, f, row_loss, stats, loss, divisor, s);
+  } else {
+    run_forward<_Float16>(d, f, row_loss, stats, loss, divisor, s);
+  }
+  return launch_status("linear_ce");
+}
+
+size_t vsl_linear_ce_bwd_workspace_bytes(const vsl_linear_ce_desc* d, uint32_t grad_mask) {
+  return check_ce(d) || d->rows == 0 ? 0 : backward_workspace(d, grad_mask, nullptr).total;
+}
+
+int vsl_linear_ce_bwd(const vsl_linear_ce_desc* d, const float* stats, const float* divisor, const float* g_loss, void* grad_hidden,
+                      void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_ce(d)) return rc;
+  hipStream_t s = (hipStream_t)stream;
+  if (d->rows == 0) {
+    if (d->type == VSL_TYPE_F32) zero_shared<float>(d, grad_weight, grad_bias, s);
+    else zero_shared<_Float16>(d, grad_weight, grad_bias, s);  // zero has the same bits in both 16-bit types
+    return launch_status("linear_ce backward");
+  }
+  if (!stats || !g_loss || (d->reduction == VSL_REDUCE_MEAN && !divisor))
+    return fail(VSL_ERR_INVALID_ARGUMENT, "linear_ce backward: NULL tensor");
+  if (!grad_hidden && !grad_weight && !grad_bias) return VSL_OK;
+  const uint32_t mask = (grad_hidden ? 1u : 0u) | (grad_weight ? 2u : 0u) | (grad_bias ? 4u : 0u);
+  const Backward b = backward_workspace(d, mask, workspace);
+  if (int rc = check_space(workspace, workspace_bytes, b.total)) return rc;
+  if (d->type == VSL_TYPE_F32)
+    run_backward<float>(d, b, stats, divisor, g_loss, (float*)grad_hidden, (float*)grad_weight, (float*)grad_bias, s);
+  else if (d->type == VSL_TYPE_BF16)
+    run_backward<__bf16>(d, b, stats, divisor, g_loss, (__bf16*)grad_hidden, (__bf16*)grad_weight, (__bf16*)grad_bias, s);
+  else
+    run_backward<_Float16>(d, b, stats, divisor, g_loss, (_Float16*)grad_hidden, (_Float16*)grad_weight, (_Float16*)grad_bias, s);
+  return launch_status("linear_ce backward");
+}
+
+}  // extern "C"

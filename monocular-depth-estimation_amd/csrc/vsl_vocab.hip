@@ -1,0 +1,1045 @@
+// libvsloss.so -- losses over a set of classes, the part that works on logits in hand: the k largest logits of every row
+// (what a teacher hands on) and the distillation of a student from them, forward and backward; and the reduction of row
+// losses that the linear cross entropy (vsl_linear_ce.hip) shares.
+//
+// A row is a token over a large vocabulary or a pixel over its depth bins, so there are two programs for each operator:
+// "rows" keeps a whole short row in the registers of 16 or 64 lanes, "stream" walks a long row, or a segment of it when
+// there are few rows, with a running maximum and sum per thread.  Both read every logit once per direction.
+#include "vsl_vocab.hpp"
+
+namespace vsl_vocab {
+
+static_assert(sizeof(vsl_top_desc) == 48 && sizeof(vsl_distill_desc) == 88, "C-ABI struct layout changed");
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr int64_t kMaxBlocks = 1 << 20;  // blocks of one launch; kernels walk further items in steps of the grid
+
+// ------------------------------------------------------------------------------------------------------------------
+// reduced loss
+// ------------------------------------------------------------------------------------------------------------------
+constexpr int kSumBlocks = 256;
+constexpr int64_t kSumRows = 4096;  // rows a block of the first pass takes at least
+
+__device__ __forceinline__ void finish_sum(double total, double count, int reduction, float* loss, float* divisor) {
+  *loss = (float)(reduction == VSL_REDUCE_MEAN ? (count == 0.0 ? 0.0 : total / count) : total);
+  *divisor = (float)count;
+}
+
+__device__ __forceinline__ void block_sum2(double& a, double& b, double* red) {
+  for (int m = 32; m >= 1; m >>= 1) {
+    a += __shfl_xor(a, m, 64);
+    b += __shfl_xor(b, m, 64);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    red[2 * (threadIdx.x >> 6)] = a;
+    red[2 * (threadIdx.x >> 6) + 1] = b;
+  }
+  __syncthreads();
+  a = b = 0.0;
+  for (int w = 0; w < kWaves; ++w) {
+    a += red[2 * w];
+    b += red[2 * w + 1];
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void k_sum_rows(const float* __restrict__ row_loss, const float* __restrict__ weights,
+                                                       const int64_t* __restrict__ target, int64_t ignore_index, int64_t rows,
+                                                       int64_t per_block, int reduction, double* __restrict__ partial,
+                                                       float* __restrict__ loss, float* __restrict__ divisor) {
+  __shared__ double red[2 * kWaves];
+  const int64_t r0 = blockIdx.x * per_block, r1 = min(rows, r0 + per_block);
+  double total = 0.0, count = 0.0;
+  for (int64_t r = r0 + threadIdx.x; r < r1; r += kThreads) {
+    total += (double)row_loss[r];
+    count += weights ? (double)weights[r] : target ? (target[r] == ignore_index ? 0.0 : 1.0) : 1.0;
+  }
+  block_sum2(total, count, red);
+  if (threadIdx.x) return;
+  if (gridDim.x == 1) {
+    finish_sum(total, count, reduction, loss, divisor);
+  } else {
+    partial[2 * blockIdx.x] = total;
+    partial[2 * blockIdx.x + 1] = count;
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void k_sum_final(const double* __restrict__ partial, int n, int reduction,
+                                                        float* __restrict__ loss, float* __restrict__ divisor) {
+  __shared__ double red[2 * kWaves];
+  double total = (int)threadIdx.x < n ? partial[2 * threadIdx.x] : 0.0;
+  double count = (int)threadIdx.x < n ? partial[2 * threadIdx.x + 1] : 0.0;
+  block_sum2(total, count, red);
+  if (threadIdx.x == 0) finish_sum(total, count, reduction, loss, divisor);
+}
+static_assert(kSumBlocks <= kThreads, "one thread of k_sum_final per block of k_sum_rows");
+
+int sum_blocks(int64_t rows) {
+  const int64_t b = ceil_div(rows, kSumRows);
+  return (int)(b < 1 ? 1 : (b > kSumBlocks ? kSumBlocks : b));
+}
+
+}  // namespace
+
+size_t sum_workspace_bytes(int64_t rows) { return up256((size_t)sum_blocks(rows) * 2 * sizeof(double)); }
+
+void launch_sum(const float* row_loss, const float* weights, const int64_t* target, int64_t ignore_index, int64_t rows,
+                int reduction, void* partial, float* loss, float* divisor, hipStream_t s) {
+  const int n = sum_blocks(rows);
+  hipLaunchKernelGGL(k_sum_rows, dim3(n), dim3(kThreads), 0, s, row_loss, weights, target, ignore_index, rows,
+                     ceil_div(rows, n), reduction, (double*)partial, loss, divisor);
+  if (n > 1)
+    hipLaunchKernelGGL(k_sum_final, dim3(1), dim3(kThreads), 0, s, (const double*)partial, n, reduction, loss, divisor);
+}
+
+namespace {
+
+// ------------------------------------------------------------------------------------------------------------------
+// keys: unsigned integers that order as (value, lower index first); 0 is below every key of an element
+// ------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ unsigned ordered32(unsigned b) {
+  if ((b & 0x7FFFFFFFu) > 0x7F800000u) return 0xFFFFFFFFu;  // NaN: above +infinity
+  if (b == 0x80000000u) b = 0u;                             // -0 ties with +0
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ unsigned unordered32(unsigned o) { return o & 0x80000000u ? o & 0x7FFFFFFFu : ~o; }
+__device__ __forceinline__ unsigned ordered16(unsigned b, unsigned inf) {
+  if ((b & 0x7FFFu) > inf) return 0xFFFFu;
+  if (b == 0x8000u) b = 0u;
+  return b & 0x8000u ? ~b & 0xFFFFu : b | 0x8000u;
+}
+__device__ __forceinline__ unsigned unordered16(unsigned o) { return o & 0x8000u ? o & 0x7FFFu : ~o & 0xFFFFu; }
+
+// short rows: value and index share 32 bits for the 16-bit types (an index fits the lower half), 64 for float32
+template <typename T>
+struct RowKey {
+  typedef unsigned K;
+  static constexpr unsigned kInf = sizeof(T) == 2 && __is_same(T, __bf16) ? 0x7F80u : 0x7C00u;
+  static __device__ __forceinline__ K make(u32x4 r, int e, int index) {
+    const unsigned b = (r[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
+    return ordered16(b, kInf) << 16 | (0xFFFFu - (unsigned)index);
+  }
+  static __device__ __forceinline__ int index(K k) { return (int)(0xFFFFu - (k & 0xFFFFu)); }
+  static __device__ __forceinline__ T value(K k) { return __builtin_bit_cast(T, (unsigned short)unordered16(k >> 16)); }
+};
+template <>
+struct RowKey<float> {
+  typedef unsigned long long K;
+  static __device__ __forceinline__ K make(u32x4 r, int e, int index) {
+    return (unsigned long long)ordered32(r[e]) << 32 | (0xFFFFFFFFu - (unsigned)index);
+  }
+  static __device__ __forceinline__ int index(K k) { return (int)(0xFFFFFFFFu - (unsigned)k); }
+  static __device__ __forceinline__ float value(K k) { return __uint_as_float(unordered32((unsigned)(k >> 32))); }
+};
+
+// ------------------------------------------------------------------------------------------------------------------
+// top logits
+// ------------------------------------------------------------------------------------------------------------------
+struct TopArgs {
+  const void* logits;
+  void* values;
+  int* indices;
+  float* lse;
+  unsigned long long* keys;  // [rows][segs][k], stream only
+  float* stat;               // [rows][segs][2] running maximum and sum, stream only
+  int64_t rows, stride;
+  int V, k, segs, seg_len;
+  float c, inv_t;            // log2(e) / temperature, 1 / temperature
+};
+
+// Short rows: L lanes hold NV vectors each.  Every round takes the group's largest key and removes it.
+template <typename T, int L, int NV>
+__global__ __launch_bounds__(kThreads) void k_top_rows(TopArgs a) {
+  constexpr int E = Vec<T>::E, G = kThreads / L;
+  typedef typename RowKey<T>::K K;
+  const int lane = threadIdx.x % L;
+  for (int64_t r0 = (int64_t)blockIdx.x * G; r0 < a.rows; r0 += (int64_t)gridDim.x * G) {
+    const int64_t row = r0 + threadIdx.x / L;
+    const bool live = row < a.rows;  // whole groups: the lanes of a group agree
+    const T* x = (const T*)a.logits + (live ? row : 0) * a.stride;
+    K key[NV * E];
+    MaxSum t{ninf(), 0.0f};
+    float xs[NV][E];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int i = (v * L + lane) * E;
+      u32x4 r = load_row(x, i, i < a.V ? a.V : i);
+      unpack(r, xs[v], (const T*)nullptr);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        key[v * E + e] = i + e < a.V ? RowKey<T>::make(r, e, i + e) : (K)0;
+        t.m = __builtin_elementwise_maximum(t.m, xs[v][e]);
+      }
+    }
+    if (a.lse) {
+      t.m = group_all<L>(t.m, MaxF());
+      const float ref = exp_ref(t.m);
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int e = 0; e < E; ++e) t.s += exp_of(xs[v][e], ref, a.c);
+      t.s = group_all<L>(t.s, AddF());
+      if (live && lane == 0) a.lse[row] = log_sum(t, a.inv_t);
+    }
+    K mine = 0;
+    for (int j = 0; j < a.k; ++j) {
+      K best = 0;
+#pragma unroll
+      for (int e = 0; e < NV * E; ++e) best = best > key[e] ? best : key[e];
+      best = group_all<L>(best, MaxU());
+#pragma unroll
+      for (int e = 0; e < NV * E; ++e) key[e] = key[e] == best ? (K)0 : key[e];
+      if (j % L == lane) mine = best;
+      if ((j % L == L - 1 || j == a.k - 1) && live && lane <= j % L) {
+        const int64_t at = row * a.k + j - j % L + lane;
+        ((T*)a.values)[at] = RowKey<T>::value(mine);
+        a.indices[at] = RowKey<T>::index(mine);
+      }
+    }
+  }
+}
+
+// Long rows.  A key is (ordered value, ~index).  The k-th largest of the 256 threads' maxima over the first tile is a
+// bound that at least k elements reach; the elements that do are collected, and whenever more than kTrigger are there the
+// k largest of them are kept and the bound rises to the k-th.
+constexpr int kTrigger = 512;
+constexpr int kBuffer = 4096;  // kTrigger + one tile of at most kThreads * 8 elements, as a power of two for the sort
+static_assert(kTrigger + kThreads * 8 <= kBuffer && VSL_MAX_TOP <= kTrigger, "candidate buffer");
+
+// Bitonic sort, larger first, of n = 2^p keys in LDS.
+__device__ __forceinline__ void sort_keys(unsigned long long* buf, int n) {
+  for (int size = 2; size <= n; size <<= 1)
+    for (int step = size >> 1; step >= 1; step >>= 1) {
+      __syncthreads();
+      for (int p = threadIdx.x; p < n / 2; p += kThreads) {
+        const int i = 2 * p - (p & (step - 1)), j = i + step;
+        const unsigned long long u = buf[i], v = buf[j];
+        if ((u < v) == ((i & size) == 0)) {
+          buf[i] = v;
+          buf[j] = u;
+        }
+      }
+    }
+  __syncthreads();
+}
+// sorts the first `count` keys; the rest up to the next power of two becomes 0
+__device__ __forceinline__ void sort_count(unsigned long long* buf, int count) {
+  int n = 2;
+  while (n < count) n <<= 1;
+  for (int i = count + threadIdx.x; i < n; i += kThreads) buf[i] = 0ull;
+  sort_keys(buf, n);
+}
+
+__device__ __forceinline__ float key_floor(unsigned long long key) {
+  // a float that no element of a key >= `key` lies below; NaN keys: +infinity (a NaN is not below it)
+  const unsigned o = (unsigned)(key >> 32);
+  return o == 0u ? ninf() : o > 0xFF800000u ? __uint_as_float(0x7F800000u) : __uint_as_float(unordered32(o));
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_top_stream(TopArgs a) {
+  constexpr int E = Vec<T>::E, kTile = kThreads * E;
+  __shared__ unsigned long long buf[kBuffer];
+  __shared__ int count;
+  __shared__ float red[2 * kWaves];
+  const int tid = threadIdx.x;
+  const int64_t items = a.rows * a.segs;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t row = item / a.segs;
+    const int seg = (int)(item % a.segs);
+    const T* x = (const T*)a.logits + row * a.stride;
+    const int e0 = seg * a.seg_len, e1 = min(a.V, e0 + a.seg_len);  // a segment never starts behind the row
+    MaxSum t{ninf(), 0.0f};
+    unsigned long long bound = 0;
+    float floor_value = ninf();
+    for (int i0 = e0; i0 < e1; i0 += kTile) {
+      const int i = i0 + tid * E;
+      float v[E];
+      const u32x4 r = load_row(x, i, i < e1 ? e1 : i);
+      unpack(r, v, (const T*)nullptr);
+      float top = v[0];
+#pragma unroll
+      for (int e = 1; e < E; ++e) top = __builtin_elementwise_maximum(top, v[e]);
+      const float m = __builtin_elementwise_maximum(t.m, top), ref = exp_ref(m);
+      float s = t.s * exp_of(t.m, ref, a.c);
+#pragma unroll
+      for (int e = 0; e < E; ++e) s += exp_of(v[e], ref, a.c);
+      t = {m, s};
+      if (i0 == e0) {
+        unsigned long long best = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (i + e < e1) {
+            const unsigned long long key =
+                (unsigned long long)ordered32(__float_as_uint(v[e])) << 32 | (0xFFFFFFFFu - (unsigned)(i + e));
+            best = best > key ? best : key;
+          }
+        buf[tid] = best;
+        if (tid == 0) count = 0;
+        sort_keys(buf, kThreads);
+        bound = buf[a.k - 1];
+        floor_value = key_floor(bound);
+        __syncthreads();
+      }
+      if (__any(!(top < floor_value))) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const bool maybe = !(v[e] < floor_value) && i + e < e1;
+          if (__ballot(maybe) == 0) continue;
+          const unsigned long long key =
+              (unsigned long long)ordered32(__float_as_uint(v[e])) << 32 | (0xFFFFFFFFu - (unsigned)(i + e));
+          const bool pass = maybe && key >= bound;
+          const unsigned long long who = __ballot(pass);
+          if (who == 0) continue;
+          int base = 0;
+          if ((tid & 63) == __ffsll((unsigned long long)who) - 1) base = atomicAdd(&count, __popcll(who));
+          base = __builtin_amdgcn_readlane(base, __ffsll((unsigned long long)who) - 1);
+          if (pass) buf[base + __popcll(who & ((1ull << (tid & 63)) - 1))] = key;
+        }
+      }
+      __syncthreads();
+      const int n = count;
+      if (n > kTrigger) {
+        sort_count(buf, n);
+        bound = buf[a.k - 1] + 1;  // its element is kept: later ones have to be above it
+        floor_value = key_floor(bound);
+        if (tid == 0) count = a.k;
+      }
+      __syncthreads();
+    }
+    const int n = count;
+    sort_count(buf, n);
+    if (a.lse || a.segs > 1) t = block_join<kWaves>(t, red, a.c);
+    if (a.segs > 1) {
+      if (tid < a.k) a.keys[item * a.k + tid] = tid < n ? buf[tid] : 0ull;
+      if (tid == 0) {
+        a.stat[2 * item] = t.m;
+        a.stat[2 * item + 1] = t.s;
+      }
+    } else {
+      if (tid < a.k) {
+        const int at = (int)(0xFFFFFFFFu - (unsigned)buf[tid]);
+        ((T*)a.values)[row * a.k + tid] = x[at];
+        a.indices[row * a.k + tid] = at;
+      }
+      if (a.lse && tid == 0) a.lse[row] = log_sum(t, a.inv_t);
+    }
+    __syncthreads();
+  }
+}
+
+// joins the segments of a row: segs * k <= kBuffer keys
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_top_join(TopArgs a) {
+  __shared__ unsigned long long buf[kBuffer];
+  __shared__ float red[2 * kWaves];
+  const int tid = threadIdx.x;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const int n = a.segs * a.k;
+    for (int i = tid; i < n; i += kThreads) buf[i] = a.keys[row * n + i];
+    sort_count(buf, n);
+    if (tid < a.k) {
+      const int at = (int)(0xFFFFFFFFu - (unsigned)buf[tid]);
+      ((T*)a.values)[row * a.k + tid] = ((const T*)a.logits)[row * a.stride + at];
+      a.indices[row * a.k + tid] = at;
+    }
+    if (a.lse) {
+      MaxSum t{ninf(), 0.0f};
+      for (int s = tid; s < a.segs; s += kThreads)
+        t = join(t, {a.stat[2 * (row * a.segs + s)], a.stat[2 * (row * a.segs + s) + 1]}, a.c);
+      t = block_join<kWaves>(t, red, a.c);
+      if (tid == 0) a.lse[row] = log_sum(t, a.inv_t);
+    }
+    __syncthreads();
+  }
+}
+
+int vec_of(int type) { return type == VSL_TYPE_F32 ? 4 : 8; }
+// a row of at most this many elements stays in registers
+int64_t short_row(int type) { return 256 * vec_of(type); }
+
+struct Split {
+  int segs, seg_len;
+};
+// Segments of a long row: enough blocks for the 256 CUs when there are few rows, whole tiles each, at most `most`.
+Split split_row(int64_t rows, int64_t V, int tile, int most) {
+  const int64_t tiles = ceil_div(V, tile);
+  int64_t segs = ceil_div(1024, rows < 1 ? 1 : rows);
+  if (segs > tiles) segs = tiles;
+  if (segs > most) segs = most;
+  if (segs < 1) segs = 1;
+  const int64_t per = ceil_div(tiles, segs);
+  return {(int)ceil_div(tiles, per), (int)(per * tile)};
+}
+
+int grid_of(int64_t items) { return (int)(items < 1 ? 1 : (items > kMaxBlocks ? kMaxBlocks : items)); }
+
+Split top_split(const vsl_top_desc* d) {
+  if (d->vocab <= short_row(d->type)) return {1, (int)d->vocab};
+  return split_row(d->rows, d->vocab, kThreads * vec_of(d->type), kBuffer / d->k);
+}
+
+bool bad_type(int t) { return t != VSL_TYPE_F32 && t != VSL_TYPE_BF16 && t != VSL_TYPE_F16; }
+
+int check_matrix(const char* what, int64_t rows, int64_t vocab, int64_t stride, int type) {
+  if (bad_type(type)) return fail(VSL_ERR_INVALID_ARGUMENT, std::string(what) + ": unknown element type");
+  if (rows < 0 || rows >= (1LL << 31) || vocab < 1 || vocab >= (1LL << 30))
+    return fail(VSL_ERR_INVALID_ARGUMENT, std::string(what) + ": need 0 <= rows < 2^31 and 1 <= vocab < 2^30");
+  if (stride < vocab || stride >= (1LL << 40))
+    return fail(VSL_ERR_INVALID_ARGUMENT, std::string(what) + ": the row stride must be at least vocab");
+  return VSL_OK;
+}
+int check_top(const vsl_top_desc* d) {
+  if (!d) return fail(VSL_ERR_INVALID_ARGUMENT, "top_logits: descriptor is null");
+  if (int rc = check_matrix("top_logits", d->rows, d->vocab, d->stride, d->type)) return rc;
+  if (d->k < 1 || d->k > VSL_MAX_TOP || d->k > d->vocab)
+    return fail(VSL_ERR_INVALID_ARGUMENT, "top_logits: need 1 <= k <= min(vocab, 256)");
+  if (!(d->temperature > 0.0f) || d->temperature > 1e30f || d->temperature < 1e-30f)
+    return fail(VSL_ERR_INVALID_ARGUMENT, "top_logits: temperature must be positive and finite");
+  return VSL_OK;
+}
+
+template <typename T>
+void launch_top(const TopArgs& a, bool rows_program, hipStream_t s) {
+  if (rows_program) {
+    const int nv = (int)ceil_div(a.V, Vec<T>::E);
+    const dim3 b(kThreads);
+    const dim3 g16(grid_of(ceil_div(a.rows, kThreads / 16))), g64(grid_of(ceil_div(a.rows, kThreads / 64)));
+    if (nv <= 16) hipLaunchKernelGGL((k_top_rows<T, 16, 1>), g16, b, 0, s, a);
+    else if (nv <= 32) hipLaunchKernelGGL((k_top_rows<T, 16, 2>), g16, b, 0, s, a);
+    else if (nv <= 64) hipLaunchKernelGGL((k_top_rows<T, 16, 4>), g16, b, 0, s, a);
+    else if (nv <= 128) hipLaunchKernelGGL((k_top_rows<T, 64, 2>), g64, b, 0, s, a);
+    else hipLaunchKernelGGL((k_top_rows<T, 64, 4>), g64, b, 0, s, a);
+    return;
+  }
+  hipLaunchKernelGGL(k_top_stream<T>, dim3(grid_of(a.rows * a.segs)), dim3(kThreads), 0, s, a);
+  if (a.segs > 1) hipLaunchKernelGGL(k_top_join<T>, dim3(grid_of(a.rows)), dim3(kThreads), 0, s, a);
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// distillation from top logits
+// ------------------------------------------------------------------------------------------------------------------
+struct DistillArgs {
+  const void* logits;
+  const void* values;
+  const void* indices;
+  const float* lse;
+  const float* weights;
+  float* row_loss;
+  float* stats;        // planes of `rows`, RowStats
+  float* partial;      // [rows][segs][2], stream only
+  const float* divisor;  // backward: of the mean
+  const float* g_loss;
+  void* grad;
+  int64_t rows, stride, grad_stride;
+  int V, k, segs, seg_len, value_type, index_bytes, reduction;
+  float c;             // log2(e) / temperature
+  float ih, il;        // 1 / temperature as a sum of two floats
+  float temperature;
+};
+
+__device__ __forceinline__ float teacher_value(const DistillArgs& a, int64_t at) {
+  if (a.value_type == VSL_TYPE_F32) return ((const float*)a.values)[at];
+  if (a.value_type == VSL_TYPE_BF16) return (float)((const __bf16*)a.values)[at];
+  return (float)((const _Float16*)a.values)[at];
+}
+// -1 for an index outside the vocabulary
+__device__ __forceinline__ int teacher_index(const DistillArgs& a, int64_t at) {
+  const int64_t i = a.index_bytes == 8 ? ((const int64_t*)a.indices)[at] : (int64_t)((const int*)a.indices)[at];
+  return i < 0 || i >= a.V ? -1 : (int)i;
+}
+
+// log q = v / T - base - log_sum.  The exponent is kept in two floats: rounded to one it would be off by half an ulp of its
+// size, and that error of every q would land in q_t = 1 - sum q, which is small.
+struct LogQ {
+  float hi, lo;
+  __device__ __forceinline__ float log() const { return hi + lo; }
+  __device__ __forceinline__ float q() const { return hi == ninf() ? 0.0f : expf(hi) * (1.0f + lo); }
+};
+struct TeacherSum {
+  float base, log_sum;  // lse and 0 where it is given; the largest value / T and the log of the sum above it otherwise
+};
+__device__ __forceinline__ LogQ log_q(const DistillArgs& a, float v, TeacherSum t) {
+  if (v == ninf()) return {ninf(), 0.0f};
+  const float p = __fmul_rn(v, a.ih);
+  const float pe = fmaf(v, a.il, fmaf(v, a.ih, -p));
+  const float s = __fsub_rn(p, t.base), b = __fsub_rn(s, p);
+  const float err = __fadd_rn(__fsub_rn(p, __fsub_rn(s, b)), __fsub_rn(-t.base, b));
+  const float h = __fsub_rn(s, t.log_sum), g = __fsub_rn(h, s);
+  return {h, pe + err + __fadd_rn(__fsub_rn(s, __fsub_rn(h, g)), __fsub_rn(-t.log_sum, g))};
+}
+
+// weight of a row, its share of the upstream gradient and the factor T of the derivative
+__device__ __forceinline__ float row_scale(const DistillArgs& a, int64_t row, float w) {
+  float g = a.g_loss[a.reduction == VSL_REDUCE_NONE ? row : 0];
+  if (a.reduction == VSL_REDUCE_MEAN) {
+    const float n = *a.divisor;
+    g = n == 0.0f ? 0.0f : g / n;
+  }
+  return g * w * a.temperature;
+}
+
+struct RowStats {
+  float m, ls;        // p = 2^((x - m) c - ls); m = +inf: the row adds nothing
+  float tm, tls;      // the same over the classes that are not the teacher's
+  float qt, total;    // the teacher's rest; sum of all q
+  TeacherSum teacher;
+  __device__ __forceinline__ void store(const DistillArgs& a, int64_t row) const {
+    const float v[VSL_DISTILL_STATS] = {m, ls, tm, tls, qt, total, teacher.base, teacher.log_sum};
+#pragma unroll
+    for (int p = 0; p < VSL_DISTILL_STATS; ++p) a.stats[p * a.rows + row] = v[p];
+  }
+  __device__ __forceinline__ void load(const DistillArgs& a, int64_t row) {
+    float v[VSL_DISTILL_STATS];
+#pragma unroll
+    for (int p = 0; p < VSL_DISTILL_STATS; ++p) v[p] = a.stats[p * a.rows + row];
+    m = v[0], ls = v[1], tm = v[2], tls = v[3], qt = v[4], total = v[5], teacher = {v[6], v[7]};
+  }
+  __device__ __forceinline__ bool dead() const { return m == __uint_as_float(0x7F800000u); }
+  __device__ __forceinline__ float p(float x, float c) const { return __builtin_amdgcn_exp2f(fmaf(x - m, c, -ls)); }
+  // log2 of the other classes' share
+  __device__ __forceinline__ float log2_rest(float c) const { return fmaf(tm - m, c, tls - ls); }
+  // derivative of the other classes: coefficient() 2^((x - base()) c - base_log())
+  __device__ __forceinline__ bool rest() const { return qt > 0.0f; }
+  __device__ __forceinline__ float base() const { return rest() ? tm : m; }
+  __device__ __forceinline__ float base_log() const { return rest() ? tls : ls; }
+  __device__ __forceinline__ float coefficient(float c) const {
+    return rest() ? fmaf(total, __builtin_amdgcn_exp2f(log2_rest(c)), -qt) : total;
+  }
+  __device__ __forceinline__ void poison() { m = ls = total = qnan(); }
+};
+__device__ __forceinline__ RowStats dead_row() { return {__uint_as_float(0x7F800000u), 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, {0.0f, 0.0f}}; }
+
+// loss of a row from its sums: cross = sum q (log q - log p), mass = sum q; rest: the classes that are not the teacher's
+__device__ __forceinline__ float finish_row(RowStats& st, float cross, float mass, bool with_rest, MaxSum rest, float c) {
+  st.qt = st.tm = st.tls = 0.0f;
+  st.total = mass;
+  if (with_rest && rest.m != ninf()) {
+    st.tm = rest.m;
+    st.tls = log2_sum(rest);
+    st.qt = fmaxf(0.0f, 1.0f - mass);
+    if (st.qt > 0.0f) cross += st.qt * (logf(st.qt) - st.log2_rest(c) * kLn2);
+    st.total = mass + st.qt;
+  }
+  return cross;
+}
+
+// Short rows: L lanes hold NV vectors each; q is scattered into an LDS table of the row, -1 where a class is not the
+// teacher's.
+template <typename T, int L, int NV, bool GRAD>
+__global__ __launch_bounds__(kThreads) void k_distill_rows(DistillArgs a) {
+  constexpr int E = Vec<T>::E, G = kThreads / L, W = L * NV * E;
+  __shared__ float table[G][W];
+  const int lane = threadIdx.x % L, group = threadIdx.x / L;
+  float* tab = table[group];
+  const unsigned long long members = (~0ull >> (64 - L)) << (((threadIdx.x & 63) / L) * L);
+  for (int64_t r0 = (int64_t)blockIdx.x * G; r0 < a.rows; r0 += (int64_t)gridDim.x * G) {
+    const int64_t row = r0 + group;
+    const bool live = row < a.rows;
+    const float w = !live ? 0.0f : a.weights ? a.weights[row] : 1.0f;
+    const T* x = (const T*)a.logits + row * a.stride;
+    RowStats st = dead_row();
+    if (GRAD && live) st.load(a, row);
+    const bool skip = w == 0.0f || (GRAD && st.dead());  // the lanes of a group agree
+    float xs[NV][E];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int i = (v * L + lane) * E;
+      const u32x4 r = load_row(x, i, skip ? i : i < a.V ? a.V : i);
+      unpack(r, xs[v], (const T*)nullptr);
+#pragma unroll
+      for (int e = 0; e < E; e += 4) *(f32x4*)&tab[i + e] = f32x4{-1.0f, -1.0f, -1.0f, -1.0f};
+    }
+    __builtin_amdgcn_wave_barrier();
+    // the teacher
+    TeacherSum teacher{0.0f, 0.0f};
+    const int k = skip ? 0 : a.k;
+    if (GRAD) {
+      teacher = st.teacher;
+    } else if (a.lse) {
+      if (!skip) teacher.base = a.lse[row];
+    } else {
+      MaxSum t{ninf(), 0.0f};
+      for (int j = lane; j < k; j += L) t.m = __builtin_elementwise_maximum(t.m, teacher_value(a, row * a.k + j));
+      t.m = group_all<L>(t.m, MaxF());
+      const float ref = exp_ref(t.m);
+      for (int j = lane; j < k; j += L) t.s += exp_of(teacher_value(a, row * a.k + j), ref, a.c);
+      t.s = group_all<L>(t.s, AddF());
+      teacher = {t.m * a.ih, log2_sum(t) * kLn2};
+    }
+    bool bad = false, twice = false;
+    float mass = 0.0f, cross = 0.0f;
+    for (int j = lane; j < k; j += L) {
+      const int at = teacher_index(a, row * a.k + j);
+      const LogQ lq = log_q(a, teacher_value(a, row * a.k + j), teacher);
+      const float q = lq.q();
+      mass += q;
+      if (q != 0.0f) cross += q * lq.log();
+      bad |= at < 0;
+      if (at >= 0) twice |= atomicExch(&tab[at], q) != -1.0f;
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (__ballot(twice) & members) {  // an index occurs twice: one lane sums its q in the teacher's order
+      for (int j = lane; j < k; j += L) {
+        const int at = teacher_index(a, row * a.k + j);
+        if (at >= 0) tab[at] = -1.0f;
+      }
+      __builtin_amdgcn_wave_barrier();
+      if (lane == 0)
+        for (int j = 0; j < k; ++j) {
+          const int at = teacher_index(a, row * a.k + j);
+          const float q = log_q(a, teacher_value(a, row * a.k + j), teacher).q();
+          if (at >= 0) tab[at] = (tab[at] == -1.0f ? 0.0f : tab[at]) + q;
+        }
+      __builtin_amdgcn_wave_barrier();
+    }
+    bad = (__ballot(bad) & members) != 0;
+    float q[NV][E];
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int e = 0; e < E; e += 4) {
+        const f32x4 t = *(const f32x4*)&tab[(v * L + lane) * E + e];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) q[v][e + u] = t[u];
+      }
+    __builtin_amdgcn_wave_barrier();
+    if (!GRAD) {
+      MaxSum all{ninf(), 0.0f}, rest{ninf(), 0.0f};
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          all.m = __builtin_elementwise_maximum(all.m, xs[v][e]);
+          if (q[v][e] == -1.0f) rest.m = __builtin_elementwise_maximum(rest.m, xs[v][e]);
+        }
+      all.m = group_all<L>(all.m, MaxF());
+      rest.m = group_all<L>(rest.m, MaxF());
+      // the other classes from their own maximum: they may lie far below the teacher's
+      const float ref = exp_ref(all.m), rest_ref = exp_ref(rest.m);
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float qe = q[v][e];
+          const bool member = qe != -1.0f;
+          const float ex = exp_of(xs[v][e], member ? ref : rest_ref, a.c);
+          all.s += member ? ex : 0.0f;
+          rest.s += member ? 0.0f : ex;
+          if (member && qe != 0.0f) cross -= qe * ((xs[v][e] - ref) * a.ih);
+        }
+      all.s = group_all<L>(all.s, AddF()) + (rest.s = group_all<L>(rest.s, AddF())) * exp_of(rest.m, ref, a.c);
+      cross = group_all<L>(cross, AddF());
+      mass = group_all<L>(mass, AddF());
+      st.m = all.m;
+      st.ls = log2_sum(all);
+      st.teacher = teacher;
+      float loss = finish_row(st, cross + mass * (st.ls * kLn2), mass, a.lse != nullptr, rest, a.c) * a.temperature *
+                   a.temperature * w;
+      if (st.ls != st.ls) st.poison();  // NaN or +infinity among the logits
+      if (skip || teacher.base == ninf() || st.m == ninf()) {
+        st = dead_row();
+        loss = 0.0f;
+      }
+      if (bad) {
+        st.poison();
+        loss = qnan();
+      }
+      if (live && lane == 0) {
+        st.store(a, row);
+        a.row_loss[row] = loss;
+      }
+    } else if (live) {
+      const float g = skip ? 0.0f : row_scale(a, row, w);
+      const float co = g * st.coefficient(a.c), base = st.base(), base_log = st.base_log();
+      T* out = (T*)a.grad + row * a.grad_stride;
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        const int i = (v * L + lane) * E;
+        float d[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const bool member = q[v][e] != -1.0f;
+          const float ex = __builtin_amdgcn_exp2f(fmaf(xs[v][e] - (member ? st.m : base), a.c, -(member ? st.ls : base_log)));
+          d[e] = skip ? 0.0f : member ? g * fmaf(st.total, ex, -q[v][e]) : co * ex;
+        }
+        if (i + E <= a.V) {
+          store16(out + i, pack(d, (const T*)nullptr));
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (i + e < a.V) out[i + e] = (T)d[e];
+        }
+      }
+    }
+  }
+}
+
+// Closes a long row: the first k threads hold the teacher's entries.  `rest`: sums over the classes that are not the
+// teacher's when there is a rest class, over all classes otherwise.
+template <typename T>
+__device__ __forceinline__ void close_row(const DistillArgs& a, int64_t row, float w, MaxSum rest, int* index, float* red) {
+  const int tid = threadIdx.x;
+  const T* x = (const T*)a.logits + row * a.stride;
+  const bool mine = tid < a.k;
+  const float value = mine ? teacher_value(a, row * a.k + tid) : ninf();
+  const int at = mine ? teacher_index(a, row * a.k + tid) : 0;
+  if (mine) index[tid] = at;
+  TeacherSum teacher;
+  if (a.lse) {
+    teacher = {a.lse[row], 0.0f};
+  } else {
+    const MaxSum t = block_join<kWaves>({value, value == ninf() ? 0.0f : 1.0f}, red, a.c);
+    teacher = {t.m * a.ih, log2_sum(t) * kLn2};
+  }
+  const bool bad = __syncthreads_or(mine && at < 0);
+  bool first = mine && at >= 0;
+  for (int j = 0; j < tid && first; ++j) first = index[j] != at;
+  const float z = mine && at >= 0 ? (float)x[at] : ninf();
+  MaxSum all = rest;
+  if (a.lse) {
+    const MaxSum seen = block_join<kWaves>({first ? z : ninf(), first && z != ninf() ? 1.0f : 0.0f}, red, a.c);
+    all = join(rest, seen, a.c);
+  }
+  RowStats st;
+  st.m = all.m;
+  st.ls = log2_sum(all);
+  st.teacher = teacher;
+  const LogQ lq = log_q(a, value, teacher);
+  const float q = mine ? lq.q() : 0.0f;
+  const float log_p = (z - all.m) * a.ih - st.ls * kLn2;
+  const float cross = block_add<kWaves>(q != 0.0f ? q * (lq.log() - log_p) : 0.0f, red);
+  const float mass = block_add<kWaves>(q, red);
+  float loss = finish_row(st, cross, mass, a.lse != nullptr, rest, a.c) * a.temperature * a.temperature * w;
+  if (st.ls != st.ls) st.poison();  // NaN or +infinity among the logits
+  if (teacher.base == ninf() || st.m == ninf()) {
+    st = dead_row();
+    loss = 0.0f;
+  }
+  if (bad) {
+    st.poison();
+    loss = qnan();
+  }
+  if (tid == 0) {
+    st.store(a, row);
+    a.row_loss[row] = loss;
+  }
+}
+
+constexpr int kMaxSegment = 1 << 17;  // elements of a segment: one bit of LDS each says whether the class is the teacher's
+
+template <typename T, bool REST>
+__global__ __launch_bounds__(kThreads) void k_distill_stream(DistillArgs a) {
+  constexpr int E = Vec<T>::E, kTile = kThreads * E;
+  __shared__ unsigned bits[REST ? kMaxSegment / 32 : 1];
+  __shared__ int index[VSL_MAX_TOP];
+  __shared__ float red[2 * kWaves];
+  const int tid = threadIdx.x;
+  const int64_t items = a.rows * a.segs;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t row = item / a.segs;
+    const int seg = (int)(item % a.segs);
+    const float w = a.weights ? a.weights[row] : 1.0f;
+    if (w == 0.0f) {  // the whole block agrees
+      if (tid == 0 && seg == 0) {
+        dead_row().store(a, row);
+        a.row_loss[row] = 0.0f;
+      }
+      continue;
+    }
+    const T* x = (const T*)a.logits + row * a.stride;
+    const int e0 = seg * a.seg_len, e1 = min(a.V, e0 + a.seg_len);
+    if (REST) {
+      for (int i = tid; i < (e1 - e0 + 31) / 32; i += kThreads) bits[i] = 0u;
+      __syncthreads();
+      if (tid < a.k) {
+        const int at = teacher_index(a, row * a.k + tid);
+        if (at >= e0 && at < e1) atomicOr(&bits[(at - e0) >> 5], 1u << ((at - e0) & 31));
+      }
+      __syncthreads();
+    }
+    MaxSum t{ninf(), 0.0f};
+    for (int i0 = e0; i0 < e1; i0 += kTile) {
+      const int i = i0 + tid * E;
+      float v[E];
+      unpack(load_row(x, i, i < e1 ? e1 : i), v, (const T*)nullptr);
+      if (REST && i < e1) {
+        const unsigned own = (bits[(i - e0) >> 5] >> ((i - e0) & 31)) & ((1u << E) - 1);
+        if (own)
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (own >> e & 1) v[e] = ninf();
+      }
+      float top = v[0];
+#pragma unroll
+      for (int e = 1; e < E; ++e) top = __builtin_elementwise_maximum(top, v[e]);
+      const float m = __builtin_elementwise_maximum(t.m, top), ref = exp_ref(m);
+      float s = t.s * exp_of(t.m, ref, a.c);
+#pragma unroll
+      for (int e = 0; e < E; ++e) s += exp_of(v[e], ref, a.c);
+      t = {m, s};
+    }
+    t = block_join<kWaves>(t, red, a.c);
+    if (a.segs == 1) {
+      close_row<T>(a, row, w, t, index, red);
+    } else if (tid == 0) {
+      a.partial[2 * item] = t.m;
+      a.partial[2 * item + 1] = t.s;
+    }
+    __syncthreads();
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_distill_join(DistillArgs a) {
+  __shared__ int index[VSL_MAX_TOP];
+  __shared__ float red[2 * kWaves];
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const float w = a.weights ? a.weights[row] : 1.0f;
+    if (w != 0.0f) {
+      MaxSum t{ninf(), 0.0f};
+      for (int s = threadIdx.x; s < a.segs; s += kThreads)
+        t = join(t, {a.partial[2 * (row * a.segs + s)], a.partial[2 * (row * a.segs + s) + 1]}, a.c);
+      t = block_join<kWaves>(t, red, a.c);
+      close_row<T>(a, row, w, t, index, red);
+    }
+    __syncthreads();
+  }
+}
+
+// The gradient of a long row: every class as if it were not the teacher's, then, behind a barrier, the teacher's own.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_distill_grad(DistillArgs a) {
+  constexpr int E = Vec<T>::E, kTile = kThreads * E;
+  __shared__ int index[VSL_MAX_TOP];
+  __shared__ float share[VSL_MAX_TOP];
+  const int tid = threadIdx.x;
+  const int64_t items = a.rows * a.segs;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t row = item / a.segs;
+    const int seg = (int)(item % a.segs);
+    const float w = a.weights ? a.weights[row] : 1.0f;
+    RowStats st;
+    st.load(a, row);
+    const bool skip = w == 0.0f || st.dead();
+    const T* x = (const T*)a.logits + row * a.stride;
+    T* out = (T*)a.grad + row * a.grad_stride;
+    const int e0 = seg * a.seg_len, e1 = min(a.V, e0 + a.seg_len);
+    const float g = skip ? 0.0f : row_scale(a, row, w);
+    const float co = g * st.coefficient(a.c), base = st.base(), base_log = st.base_log();
+    int at = -1;
+    if (!skip && tid < a.k) {
+      at = teacher_index(a, row * a.k + tid);
+      index[tid] = at;
+      share[tid] = log_q(a, teacher_value(a, row * a.k + tid), st.teacher).q();
+    }
+    for (int i0 = e0; i0 < e1; i0 += kTile) {
+      const int i = i0 + tid * E;
+      if (i >= e1) break;
+      float d[E];
+      if (skip) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) d[e] = 0.0f;
+      } else {
+        unpack(load_row(x, i, e1), d, (const T*)nullptr);
+#pragma unroll
+        for (int e = 0; e < E; ++e) d[e] = co * __builtin_amdgcn_exp2f(fmaf(d[e] - base, a.c, -base_log));
+      }
+      if (i + E <= e1) {
+        store16(out + i, pack(d, (const T*)nullptr));
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (i + e < e1) out[i + e] = (T)d[e];
+      }
+    }
+    __syncthreads();
+    if (at >= e0 && at < e1) {
+      float q = 0.0f;
+      for (int j = 0; j < a.k; ++j)
+        if (index[j] == at) q += share[j];
+      out[at] = (T)(g * fmaf(st.total, st.p((float)x[at], a.c), -q));  // entries of one index write the same value
+    }
+    __syncthreads();
+  }
+}
+
+int check_distill(const vsl_distill_desc* d) {
+  if (!d) return fail(VSL_ERR_INVALID_ARGUMENT, "distill: descriptor is null");
+  if (int rc = check_matrix("distill", d->rows, d->vocab, d->stride, d->type)) return rc;
+  if (d->k < 1 || d->k > VSL_MAX_TOP || d->k > d->vocab)
+    return fail(VSL_ERR_INVALID_ARGUMENT, "distill: need 1 <= k <= min(vocab, 256)");
+  if (bad_type(d->value_type)) return fail(VSL_ERR_INVALID_ARGUMENT, "distill: unknown type of the teacher's values");
+  if (d->index_bytes != 4 && d->index_bytes != 8)
+    return fail(VSL_ERR_INVALID_ARGUMENT, "distill: teacher indices must be int32 or int64");
+  if (d->reduction < VSL_REDUCE_NONE || d->reduction > VSL_REDUCE_MEAN)
+    return fail(VSL_ERR_INVALID_ARGUMENT, "distill: unknown reduction");
+  if (!(d->temperature > 0.0f) || d->temperature > 1e18f || d->temperature < 1e-18f)
+    return fail(VSL_ERR_INVALID_ARGUMENT, "distill: temperature must be positive and finite");
+  if (d->rows > 0 && (!d->logits || !d->teacher_values || !d->teacher_indices))
+    return fail(VSL_ERR_INVALID_ARGUMENT, "distill: NULL tensor");
+  return VSL_OK;
+}
+
+Split distill_split(const vsl_distill_desc* d) {
+  if (d->vocab <= short_row(d->type)) return {1, (int)d->vocab};
+  const int tile = kThreads * vec_of(d->type);
+  Split s = split_row(d->rows, d->vocab, tile, 1 << 20);
+  if (s.seg_len > kMaxSegment) {
+    s.seg_len = kMaxSegment;
+    s.segs = (int)ceil_div(d->vocab, kMaxSegment);
+  }
+  return s;
+}
+
+DistillArgs distill_args(const vsl_distill_desc* d) {
+  DistillArgs a{};
+  const Split sp = distill_split(d);
+  a.logits = d->logits;
+  a.values = d->teacher_values;
+  a.indices = d->teacher_indices;
+  a.lse = d->teacher_lse;
+  a.weights = d->weights;
+  a.rows = d->rows;
+  a.stride = d->stride;
+  a.V = (int)d->vocab;
+  a.k = d->k;
+  a.segs = sp.segs;
+  a.seg_len = sp.seg_len;
+  a.value_type = d->value_type;
+  a.index_bytes = d->index_bytes;
+  a.reduction = d->reduction;
+  const double inv = 1.0 / (double)d->temperature;
+  a.c = (float)(inv * 1.4426950408889634);
+  a.ih = (float)inv;
+  a.il = (float)(inv - (double)a.ih);
+  a.temperature = d->temperature;
+  return a;
+}
+
+template <typename T, bool GRAD>
+void launch_distill(const DistillArgs& a, hipStream_t s) {
+  const dim3 b(kThreads);
+  if (a.V <= 256 * Vec<T>::E) {
+    const int nv = (int)ceil_div(a.V, Vec<T>::E);
+    const dim3 g16(grid_of(ceil_div(a.rows, kThreads / 16))), g64(grid_of(ceil_div(a.rows, kThreads / 64)));
+    if (nv <= 16) hipLaunchKernelGGL((k_distill_rows<T, 16, 1, GRAD>), g16, b, 0, s, a);
+    else if (nv <= 32) hipLaunchKernelGGL((k_distill_rows<T, 16, 2, GRAD>), g16, b, 0, s, a);
+    else if (nv <= 64) hipLaunchKernelGGL((k_distill_rows<T, 16, 4, GRAD>), g16, b, 0, s, a);
+    else if (nv <= 128) hipLaunchKernelGGL((k_distill_rows<T, 64, 2, GRAD>), g64, b, 0, s, a);
+    else hipLaunchKernelGGL((k_distill_rows<T, 64, 4, GRAD>), g64, b, 0, s, a);
+    return;
+  }
+  const dim3 g(grid_of(a.rows * a.segs));
+  if (GRAD) {
+    hipLaunchKernelGGL(k_distill_grad<T>, g, b, 0, s, a);
+    return;
+  }
+  if (a.lse) hipLaunchKernelGGL((k_distill_stream<T, true>), g, b, 0, s, a);
+  else hipLaunchKernelGGL((k_distill_stream<T, false>), g, b, 0, s, a);
+  if (a.segs > 1) hipLaunchKernelGGL(k_distill_join<T>, dim3(grid_of(a.rows)), b, 0, s, a);
+}
+
+int check_workspace(const char* what, const void* workspace, size_t have, size_t need) {
+  if (have < need) return fail(VSL_ERR_WORKSPACE_TOO_SMALL, std::string(what) + ": workspace too small");
+  if (need && (!workspace || (uintptr_t)workspace % 256))
+    return fail(VSL_ERR_INVALID_ARGUMENT, std::string(what) + ": workspace must be 256-byte aligned and not NULL");
+  return VSL_OK;
+}
+
+}  // namespace
+}  // namespace vsl_vocab
+
+using namespace vsl_vocab;
+
+extern "C" {
+
+size_t vsl_top_logits_workspace_bytes(const vsl_top_desc* d) {
+  if (check_top(d)) return 0;
+  const Split sp = top_split(d);
+  if (sp.segs == 1) return 0;
+  return up256((size_t)d->rows * sp.segs * d->k * 8) + up256((size_t)d->rows * sp.segs * 8);
+}
+
+int vsl_top_logits(const vsl_top_desc* d, void* values, int32_t* indices, float* lse, void* workspace, size_t workspace_bytes,
+                   void* stream) {
+  if (int rc = check_top(d)) return rc;
+  if (d->rows == 0) return VSL_OK;
+  if (!d->logits || !values || !indices) return fail(VSL_ERR_INVALID_ARGUMENT, "top_logits: NULL tensor");
+  if (int rc = check_workspace("top_logits", workspace, workspace_bytes, vsl_top_logits_workspace_bytes(d))) return rc;
+  const Split sp = top_split(d);
+  TopArgs a{};
+  a.logits = d->logits;
+  a.values = values;
+  a.indices = indices;
+  a.lse = lse;
+  a.keys = (unsigned long long*)workspace;
+  a.stat = (float*)((char*)workspace + up256((size_t)d->rows * sp.segs * d->k * 8));
+  a.rows = d->rows;
+  a.stride = d->stride;
+  a.V = (int)d->vocab;
+  a.k = d->k;
+  a.segs = sp.segs;
+  a.seg_len = sp.seg_len;
+  a.c = (float)(1.4426950408889634 / (double)d->temperature);
+  a.inv_t = (float)(1.0 / (double)d->temperature);
+  const bool rows_program = d->vocab <= short_row(d->type);
+  hipStream_t s = (hipStream_t)stream;
+  if (d->type == VSL_TYPE_F32) launch_top<float>(a, rows_program, s);
+  else if (d->type == VSL_TYPE_BF16) launch_top<__bf16>(a, rows_program, s);
+  else launch_top<_Float16>(a, rows_program, s);
+  return launch_status("top_logits");
+}
+
+size_t vsl_distill_workspace_bytes(const vsl_distill_desc* d) {
+  if (!d || d->rows < 0 || d->vocab < 1 || bad_type(d->type)) return 0;
+  const Split sp = distill_split(d);
+  return (sp.segs > 1 ? up256((size_t)d->rows * sp.segs * 8) : 0) + sum_workspace_bytes(d->rows);
+}
+
+int vsl_distill_fwd(const vsl_distill_desc* d, float* row_loss, float* loss, float* divisor, float* stats, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+  if (int rc = check_distill(d)) return rc;
+  if (d->reduction != VSL_REDUCE_NONE && (!loss || !divisor)) return fail(VSL_ERR_INVALID_ARGUMENT, "distill: NULL loss");
+  if (d->rows > 0 && (!row_loss || !stats)) return fail(VSL_ERR_INVALID_ARGUMENT, "distill: NULL output");
+  if (int rc = check_workspace("distill", workspace, workspace_bytes, vsl_distill_workspace_bytes(d))) return rc;
+  hipStream_t s = (hipStream_t)stream;
+  DistillArgs a = distill_args(d);
+  a.row_loss = row_loss;
+  a.stats = stats;
+  const size_t part = a.segs > 1 ? up256((size_t)d->rows * a.segs * 8) : 0;
+  a.partial = (float*)workspace;
+  if (d->rows > 0) {
+    if (d->type == VSL_TYPE_F32) launch_distill<float, false>(a, s);
+    else if (d->type == VSL_TYPE_BF16) launch_distill<__bf16, false>(a, s);
+    else launch_distill<_Float16, false>(a, s);
+  }
+  if (d->reduction != VSL_REDUCE_NONE)
+    launch_sum(row_loss, d->weights, nullptr, 0, d->rows, d->reduction, (char*)workspace + part, loss, divisor, s);
+  return launch_status("distill");
+}
+
+int vsl_distill_bwd(const vsl_distill_desc* d, const float* stats, const float* divisor, const float* g_loss, void* grad,
+                    int64_t grad_stride, void* stream) {
+  if (int rc = check_distill(d)) return rc;
+  if (d->rows == 0) return VSL_OK;
+  if (!stats || !g_loss || !grad || (d->reduction == VSL_REDUCE_MEAN && !divisor))
+    return fail(VSL_ERR_INVALID_ARGUMENT, "distill backward: NULL tensor");
+  if (grad_stride < d->vocab || grad_stride >= (1LL << 40))
+    return fail(VSL_ERR_INVALID_ARGUMENT, "distill backward: the gradient's row stride must be at least vocab");
+  DistillArgs a = distill_args(d);
+  a.stats = (float*)stats;
+  a.divisor = divisor;
+  a.g_loss = g_loss;
+  a.grad = grad;
+  a.grad_stride = grad_stride;
+  hipStream_t s = (hipStream_t)stream;
+  if (d->type == VSL_TYPE_F32) launch_distill<float, true>(a, s);
+  else if (d->type == VSL_TYPE_BF16) launch_distill<__bf16, true>(a, s);
+  else launch_distill<_Float16, true>(a, s);
+  return launch_status("distill backward");
+}
+
+}  // extern "C"

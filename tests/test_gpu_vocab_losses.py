@@ -1,0 +1,549 @@
+"""GPU parity of the losses over a set of classes (mde_amd.vocab_losses) against float64 on the CPU, at the sizes and masks
+where they can go wrong.  Every tolerance is a bound on float32 arithmetic (tests/vocab_oracle.py) plus half a step of the
+type an output is rounded to."""
+import math
+
+import pytest
+import torch
+
+import vocab_oracle as O
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+INF = float("inf")
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def logits(rows, vocab, seed, dtype, scale=2.5):
+    return (torch.randn(rows, vocab, generator=gen(seed)) * scale).to(dtype)
+
+
+def close(got, want, tol, what):
+    got, want = got.double().cpu(), want.double().cpu()
+    assert got.shape == want.shape
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), what
+    inf = torch.isinf(want)
+    assert torch.equal(got[inf], want[inf]), what
+    on = torch.isfinite(want)
+    tol = (torch.zeros_like(want) + tol)[on]
+    off = (got[on] - want[on]).abs()
+    assert bool((off <= tol).all()), "%s: off by %.3g, allowed %.3g" % (
+        what, off[(off - tol).argmax()], tol[(off - tol).argmax()])
+
+
+# ------------------------------------------------------------------ top logits
+def check_top(x, k, temperature=1.0):
+    import mde_amd.vocab_losses as L
+    top = L.top_logits(x, k, temperature)
+    x2 = x.reshape(-1, x.shape[-1]).cpu()
+    v, i, lse = O.top_logits(x2, k, temperature)
+    assert top.values.shape == x.shape[:-1] + (k,) and top.values.dtype == x.dtype and top.indices.dtype == torch.int32
+    assert torch.equal(top.indices.reshape(-1, k).cpu().long(), i)
+    close(top.values.reshape(-1, k), v, 0.0, "values")
+    # a row that holds +infinity or NaN has no log sum
+    lse = torch.where(torch.isnan(x2.double()).any(1) | (x2 == INF).any(1), torch.full_like(lse, float("nan")), lse)
+    close(top.lse.reshape(-1), lse, O.exponent_error(x2, temperature) + O.sum_error(x2.shape[1]) + 4 * O.U * lse.abs(), "lse")
+    return top
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab,k", [
+    (1, 1, 1), (3, 2, 2), (5, 7, 7), (33, 64, 5), (17, 96, 8), (40, 127, 3), (9, 128, 16), (6, 129, 129), (4, 255, 17),
+    (7, 512, 33), (3, 700, 64), (2, 1024, 256), (3, 1025, 20), (2, 2048, 9), (2, 2049, 100), (1, 4097, 1), (3, 5000, 64),
+    (1, 33333, 256), (2, 70001, 128), (1200, 2500, 4)])
+def test_top_logits(rows, vocab, k, dtype):
+    x = logits(rows, vocab, rows * 7 + vocab, dtype).to(DEV)
+    check_top(x, k)
+    if vocab > 64:
+        check_top(x, k, temperature=3.5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [50, 300, 1500, 9001])
+def test_top_logits_of_ties_masks_and_specials(vocab, dtype):
+    k = 40
+    x = torch.zeros(12, vocab)
+    x[1] = 1.0                                              # every element ties
+    x[2] = -INF                                             # nothing left
+    x[3, 7:] = -INF                                         # fewer live classes than k
+    x[4] = torch.finfo(dtype).min                           # masks of the type's lowest value
+    x[5, vocab - 1] = INF
+    x[6, 3], x[6, 11], x[6, 5] = float("nan"), float("nan"), INF
+    x[7] = torch.arange(vocab)                              # ascending: the worst order for a running bound
+    x[8] = -torch.arange(vocab)
+    x[9, ::2] = -0.0                                        # -0 and +0 are one value
+    x[10] = torch.randint(0, 3, (vocab,), generator=gen(vocab)).float()
+    x[11, : vocab // 2] = -INF
+    check_top(x.to(dtype).to(DEV), k)
+
+
+def test_top_logits_of_strided_rows_leading_dimensions_and_no_rows():
+    import mde_amd.vocab_losses as L
+    base = logits(24, 400, 3, torch.bfloat16).to(DEV)
+    check_top(base[::2, 3:203], 11)                         # rows that start 6 bytes off any 16
+    check_top(base.reshape(2, 3, 4, 400), 5)
+    check_top(base[:, 1:], 9)
+    check_top(logits(6, 9000, 4, torch.float16).to(DEV)[:, 5:8998], 32)
+    maps = logits(2 * 12 * 20, 33, 5, torch.float32).reshape(2, 12, 20, 33).permute(0, 3, 1, 2).to(DEV)   # [B,C,H,W]
+    check_top(maps.movedim(1, -1), 4)
+    check_top(maps.contiguous().movedim(1, -1), 4)
+    check_top(base[0], 6)                                   # one row without a leading dimension
+    x64 = logits(3, 50, 6, torch.float32).double().to(DEV)
+    assert L.top_logits(x64, 2).values.dtype == torch.float32
+    top = L.top_logits(base[:0], 5)
+    assert top.values.shape == (0, 5) and top.lse.shape == (0,)
+    one = torch.zeros(1, 64, device=DEV).expand(5, 64)      # rows of stride 0
+    check_top(one, 3)
+
+
+# ------------------------------------------------------------------ distillation
+def teacher(rows, vocab, k, seed, dtype, live=None):
+    g = gen(seed)
+    idx = torch.stack([torch.randperm(live or vocab, generator=g)[:k] for _ in range(rows)])
+    val = (torch.randn(rows, k, generator=g) * 1.5 + 4).sort(1, descending=True).values.to(dtype)
+    return val, idx
+
+
+def check_distill(x, val, idx, lse=None, temperature=1.0, weights=None, upstream=None, reduction="sum"):
+    """All three reductions share the kernels; row losses and the gradient against the definition."""
+    import mde_amd.vocab_losses as L
+    dtype, rows, vocab = x.dtype, x.shape[0], x.shape[1]
+    loss, grad, size = O.distill(x, val, idx, lse, temperature, weights)
+    dev = lambda t: None if t is None else t.to(DEV)
+    a = x if x.is_cuda else x.to(DEV)
+    a = a.detach().requires_grad_(True)
+    args = (dev(val), dev(idx), dev(lse))
+    rows_out = L.topk_distillation_loss(a, *args, temperature=temperature, weights=dev(weights), reduction="none")
+    t = temperature
+    rel = O.exponent_error(x, t) + O.exponent_error(val, t) + 2 * O.sum_error(vocab) + 16 * O.U
+    if lse is not None:
+        rel += 8 * O.U * finite(lse)
+    w = torch.ones(rows) if weights is None else weights.cpu().abs()
+    span = finite(x) / t + finite(val) / t + (finite(lse) if lse is not None else 0) + math.log(vocab) + 1
+    close(rows_out, loss, 4 * rel * w.double() * t * t * (1 + span * 2 ** -4), "row losses")
+    if upstream is None:
+        upstream = torch.randn(rows, generator=gen(1))
+    (got,) = torch.autograd.grad(rows_out, a, upstream.to(DEV))
+    want = grad * upstream.double()[:, None]
+    assert got.dtype == dtype and got.shape == a.shape
+    tol = 4 * rel * size * upstream.double().abs()[:, None] + (O.HALF_STEP[dtype] + 4 * O.U) * want.abs() + O.TINY[dtype]
+    close(got, want, torch.nan_to_num(tol), "gradient")
+    # the reductions
+    total = L.topk_distillation_loss(a, *args, temperature=t, weights=dev(weights), reduction="sum")
+    mean = L.topk_distillation_loss(a, *args, temperature=t, weights=dev(weights), reduction="mean")
+    ws = float(rows if weights is None else weights.double().sum())
+    s = rows_out.detach().double().sum().cpu()
+    close(total.detach(), s, 2 * O.U * s.abs() if torch.isfinite(s) else 0.0, "sum")
+    close(mean.detach(), s / ws if ws else torch.zeros((), dtype=torch.float64), 4 * O.U * s.abs() / max(ws, 1e-30) if torch.isfinite(s) else 0.0, "mean")
+    (gm,) = torch.autograd.grad(mean, a, torch.tensor(0.5, device=DEV))
+    gw = grad * (0.5 / ws if ws else 0.0)
+    tol = 4 * rel * size * (0.5 / ws if ws else 0.0) + (O.HALF_STEP[dtype] + 8 * O.U) * gw.abs() + O.TINY[dtype]
+    close(gm, gw, torch.nan_to_num(tol), "gradient of the mean")
+    return rows_out, got
+
+
+def finite(x):
+    return O.finite_max(x.double())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("rows,vocab,k", [
+    (1, 1, 1), (3, 2, 1), (5, 9, 4), (37, 64, 8), (20, 96, 8), (13, 127, 16), (18, 128, 8), (6, 200, 150), (5, 300, 20),
+    (4, 512, 256), (3, 900, 33), (2, 1024, 8), (3, 1030, 17), (2, 2048, 64), (2, 2051, 64), (1, 8191, 256), (3, 6000, 5),
+    (1, 140001, 64)])
+def test_distillation(rows, vocab, k, tail, dtype):
+    x = logits(rows, vocab, rows + vocab, dtype)
+    val, idx = teacher(rows, vocab, k, vocab * 3 + k, dtype)
+    t = 1.0 if vocab % 2 else 2.5
+    lse = None
+    if tail:
+        lse = (torch.logsumexp(val.double() / t, 1) + 0.2 * torch.rand(rows, generator=gen(5), dtype=torch.float64)).float()
+    weights = None if rows < 3 else torch.rand(rows, generator=gen(6)) * (torch.arange(rows) % 3 != 1)
+    check_distill(x, val, idx, lse, t, weights)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [70, 260, 1500, 5001])
+@pytest.mark.parametrize("tail", [False, True])
+def test_distillation_of_masked_rows_repeated_indices_and_specials(vocab, tail, dtype):
+    rows, k = 14, 12
+    x = logits(rows, vocab, 11, dtype)
+    val, idx = teacher(rows, vocab, k, 12, torch.float32)
+    lse = (torch.logsumexp(val.double(), 1) + 0.1).float() if tail else None
+    x[1] = -INF                                             # the student has nothing left
+    val[2] = -INF                                           # nor has the teacher
+    if tail:
+        lse[2] = -INF
+    x[3, idx[3, 2]] = -INF                                  # the student masks a class the teacher believes in: +inf
+    val[4, 5:] = -INF                                       # the teacher knows fewer than k
+    idx[4, 5:] = idx[4, 5:6]                                # (padded with one index)
+    idx[5, 1], idx[5, 7] = idx[5, 0], idx[5, 0]             # the same index three times
+    keep = torch.zeros(vocab, dtype=torch.bool)
+    keep[idx[6]] = True
+    x[6, ~keep] = -INF                                      # the student has no other class
+    idx[7, 3] = vocab                                       # outside: NaN, never an address
+    idx[8, 0] = -1
+    x[9, :] = torch.finfo(dtype).min                        # masks of the lowest value: a uniform row
+    x[10, idx[10]] += 40                                    # the student is sure: the rest class almost vanishes
+    if dtype != torch.float16:
+        x[11, idx[11]] += 300                               # ... and does so beyond float32
+    weights = torch.ones(rows)
+    weights[12] = 0.0
+    x[12] = float("nan")                                    # not looked at
+    x[13, 3] = float("nan")
+    import mde_amd.vocab_losses as L
+    a = x.to(DEV).requires_grad_(True)
+    out = L.topk_distillation_loss(a, val.to(DEV), idx.to(DEV), None if lse is None else lse.to(DEV), weights=weights.to(DEV),
+                                   reduction="none")
+    (g,) = torch.autograd.grad(out, a, torch.ones(rows, device=DEV))
+    out, g = out.detach().cpu(), g.cpu()
+    assert out[1] == 0 and out[2] == 0 and out[12] == 0
+    assert not g[1].any() and not g[2].any() and not g[12].any()
+    assert out[3] == INF and bool(torch.isfinite(g[3]).all())
+    for bad in (7, 8, 13):
+        assert bool(torch.isnan(out[bad])) and bool(torch.isnan(g[bad]).all())
+    good = [0, 3, 4, 5, 6, 9, 10, 11]
+    # the exponents of rows 9..11 are large, and the bound grows with the largest of the rows that are checked together
+    for rows_ in ([0, 3, 4, 5, 6], [9], [10], [11]):
+        sel = torch.tensor(rows_)
+        check_distill(x[sel], val[sel], idx[sel], None if lse is None else lse[sel])
+    assert len(good) == 8
+
+
+def test_distillation_strides_types_and_no_rows():
+    import mde_amd.vocab_losses as L
+    val, idx = teacher(6, 300, 9, 21, torch.bfloat16)
+    wide = logits(12, 420, 22, torch.float16).to(DEV)
+    x = wide[::2, 7:307]
+    check_distill(x, val, idx)                              # strided rows, teacher of another type, int64 indices
+    check_distill(x, val, idx.int())
+    wide = logits(4, 9200, 23, torch.bfloat16).to(DEV)
+    val, idx = teacher(4, 9111, 9, 24, torch.float16)
+    check_distill(wide[:, 3:9114], val, idx, (torch.logsumexp(val.double(), 1) + 0.3).float())
+    check_distill(wide[:, 3:9114], val, idx, weights=torch.zeros(4))
+    val, idx = teacher(40, 33, 5, 25, torch.float32)        # [B,C,H,W] maps through movedim: the gradient comes back in place
+    maps = logits(40, 33, 26, torch.float32).reshape(2, 4, 5, 33).permute(0, 3, 1, 2).to(DEV).requires_grad_(True)
+    out = L.topk_distillation_loss(maps.movedim(1, -1), val.reshape(2, 4, 5, 5).to(DEV), idx.reshape(2, 4, 5, 5).to(DEV),
+                                   reduction="none")
+    assert out.shape == (2, 4, 5)
+    out.sum().backward()
+    flat = maps.detach().movedim(1, -1).reshape(40, 33)
+    _, grad, size = O.distill(flat, val, idx)
+    close(maps.grad.movedim(1, -1).reshape(40, 33), grad, size * 1e-5, "gradient of maps")
+    empty = torch.empty(0, 33, device=DEV, requires_grad=True)
+    for reduction, shape in (("none", (0,)), ("mean", ()), ("sum", ())):
+        out = L.topk_distillation_loss(empty, val[:0].to(DEV), idx[:0].to(DEV), reduction=reduction)
+        assert out.shape == shape and float(out.detach().sum()) == 0.0
+        out.sum().backward()
+    assert empty.grad.shape == (0, 33)
+
+
+def test_distillation_gradient_against_differences():
+    import mde_amd.vocab_losses as L
+    x = logits(3, 50, 31, torch.float32)
+    val, idx = teacher(3, 50, 6, 32, torch.float32)
+    lse = (torch.logsumexp(val.double() / 2, 1) + 0.2).float()
+    a = x.to(DEV).requires_grad_(True)
+    loss = L.topk_distillation_loss(a, val.to(DEV), idx.to(DEV), lse.to(DEV), temperature=2.0, reduction="sum")
+    (g,) = torch.autograd.grad(loss, a)
+    step = torch.sign(torch.randn(3, 50, generator=gen(33)))
+    h = 1e-2
+    f = lambda s: O.distill(x.double() + s * h * step, val, idx, lse, 2.0)[0].sum()
+    slope = (f(1) - f(-1)) / (2 * h)                        # h^2 / 6 of a third derivative below 8 per row
+    assert abs(float((g.cpu().double() * step).sum()) - float(slope)) <= 3 * 8 * h * h / 6 + 1e-4
+
+
+# ------------------------------------------------------------------ linear cross entropy
+def ce_inputs(rows, vocab, dim, dtype, seed, bias):
+    g = gen(seed)
+    h = torch.randn(rows, dim, generator=g).to(dtype)
+    w = (torch.randn(vocab, dim, generator=g) * (2.5 / math.sqrt(dim))).to(dtype)
+    b = (torch.randn(vocab, generator=g) * 0.5).to(dtype) if bias else None
+    t = torch.randint(vocab, (rows,), generator=g)
+    return h, w, b, t
+
+
+def check_ce(h, w, b, t, ignore_index=-100, z_loss=0.0, on_device=None, upstream=None):
+    import mde_amd.vocab_losses as L
+    dtype, rows, (vocab, dim) = h.dtype, h.shape[0], w.shape
+    loss, lse, z, ds = O.linear_ce(h, w, t, b, ignore_index, z_loss)
+    ha, wa = on_device if on_device else (h.to(DEV), w.to(DEV))
+    ha, wa = ha.detach().requires_grad_(True), wa.detach().requires_grad_(True)
+    ba = b.to(DEV).requires_grad_(True) if b is not None else None
+    out = L.linear_cross_entropy(ha, wa, t.to(DEV), ba, ignore_index=ignore_index, z_loss=z_loss, reduction="none")
+    habs, wabs = torch.nan_to_num(h.double().abs()), torch.nan_to_num(w.double().abs())
+    live = torch.isfinite(z)
+    zerr = ((dim + 2) * O.U * (habs @ wabs.T) + 2 * O.U * z.abs()).masked_fill(~live, 0).max(1).values   # of any class of a row
+    zmax = z.abs().masked_fill(~live, 0).max(1).values
+    lerr = zerr + 8 * O.U * (zmax + 1) + O.sum_error(vocab) + 64 * O.U
+    tol = 2 * lerr + 4 * O.U * zmax + z_loss * 2 * (lse.abs() + 1) * (lerr + 4 * O.U * lse.abs())
+    tol = torch.where((t == ignore_index) | (lse == -INF), torch.zeros_like(tol), tol)   # such rows are exactly 0
+    close(out.detach(), loss, tol, "row losses")
+    if upstream is None:
+        upstream = torch.randn(rows, generator=gen(2))
+    leaves = [ha, wa] + ([ba] if ba is not None else [])
+    grads = torch.autograd.grad(out, leaves, upstream.to(DEV), retain_graph=True)
+
+    def check_grads(grads, u, extra):
+        u = u.double()[:, None]
+        live_rows = (ds != 0).any(1) | torch.isnan(ds).any(1)
+        ud = torch.where(live_rows[:, None], ds * u, torch.zeros_like(ds))
+        half = O.HALF_STEP[dtype]
+        # the derivative: p's relative error, 1 - p's cancellation, its rounding to the operands' type (below the smallest
+        # normal of float16, 2^-14 under 2^12 of scale, the step is fixed)
+        umax = float(u.abs().max())
+        floor = umax * (1 + float((2 * z_loss * lse[torch.isfinite(lse)].abs()).max() if z_loss else 0)) * 2.0 ** -37 \
+            if dtype == torch.float16 else 0.0
+        p = (z - lse[:, None]).exp().masked_fill(~live, 0) * (1 + 2 * z_loss * lse.abs()[:, None])
+        perr = (4 * lerr[:, None] + 8 * O.U) * p + 4 * O.U
+        derr = torch.nan_to_num((perr * u.abs() + ud.abs() * half * (1 + extra) + floor) * live_rows[:, None])
+        h0 = torch.where(live_rows[:, None], h.double().cpu(), torch.zeros_like(h.double().cpu()))
+        w0 = w.double().cpu()
+        if b is not None:
+            w0 = torch.where((b == -INF)[:, None], torch.zeros_like(w0), w0)
+        n = max(rows, vocab) + 4
+        want = ud @ w0
+        close(grads[0], want, torch.nan_to_num(derr @ w0.abs() + n * O.U * (ud.abs() @ w0.abs()) + (half + 8 * O.U) * want.abs()) + O.TINY[dtype], "grad hidden")
+        want = ud.T @ h0
+        close(grads[1], want, torch.nan_to_num(derr.T @ h0.abs() + n * O.U * (ud.abs().T @ h0.abs()) + (half + 8 * O.U) * want.abs()) + O.TINY[dtype], "grad weight")
+        if b is not None:
+            want = ud.sum(0)
+            close(grads[2], want, torch.nan_to_num(derr.sum(0) + n * O.U * ud.abs().sum(0) + (half + 8 * O.U) * want.abs()) + O.TINY[dtype], "grad bias")
+
+    check_grads(grads, upstream, 0.01)
+    count = int((t != ignore_index).sum())
+    mean = L.linear_cross_entropy(ha, wa, t.to(DEV), ba, ignore_index=ignore_index, z_loss=z_loss)
+    s = out.detach().double().sum().cpu()
+    close(mean.detach(), s / count if count else torch.zeros((), dtype=torch.float64), 4 * O.U * s.abs() if torch.isfinite(s) else 0.0, "mean")
+    g = torch.autograd.grad(mean, leaves, torch.tensor(3.0, device=DEV), retain_graph=True)
+    check_grads(g, torch.full((rows,), 3.0 / max(count, 1)), 0.01)
+    total = L.linear_cross_entropy(ha, wa, t.to(DEV), ba, ignore_index=ignore_index, z_loss=z_loss, reduction="sum")
+    close(total.detach(), s, 2 * O.U * s.abs() if torch.isfinite(s) else 0.0, "sum")
+    # one gradient at a time gives the same bits as all of them
+    for i, leaf in enumerate(leaves):
+        (alone,) = torch.autograd.grad(mean, [leaf], torch.tensor(3.0, device=DEV), retain_graph=True)
+        assert torch.equal(torch.nan_to_num(alone.float()), torch.nan_to_num(g[i].float()))
+    return out, grads
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab,dim", [
+    (1, 1, 1), (1, 5, 3), (2, 100, 64), (5, 1003, 192), (16, 260, 100), (128, 128, 64), (129, 127, 65), (130, 300, 128),
+    (257, 1000, 72), (300, 64, 256), (1000, 130, 40), (64, 5000, 320), (700, 257, 513)])
+def test_linear_cross_entropy(rows, vocab, dim, dtype):
+    h, w, b, t = ce_inputs(rows, vocab, dim, dtype, rows * 3 + vocab, bias=vocab % 2 == 1)
+    if rows > 4:
+        t[torch.rand(rows, generator=gen(9)) < 0.2] = -100
+    check_ce(h, w, b, t, z_loss=1e-2 if dim % 3 == 0 else 0.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_cross_entropy_masks_and_specials(dtype):
+    rows, vocab, dim = 40, 150, 48
+    h, w, b, t = ce_inputs(rows, vocab, dim, dtype, 77, bias=True)
+    b[140:] = -INF                                          # a padded vocabulary
+    t[t >= 140] = 0
+    w[145:] = float("nan")                                  # whatever it holds
+    t[3], t[4] = 7, 7                                       # ignore_index may be an ordinary class
+    h[3] = float("nan")                                     # in a row that does not count
+    h[4, 5] = INF
+    check_ce(h, w, b, t, ignore_index=7)
+    t[8] = 141                                              # the target is masked out: +inf, finite gradients
+    check_ce(h, w, b, t, ignore_index=7)
+    b[:] = -INF                                             # nothing left in any row
+    out, grads = check_ce(h, w, b, t, ignore_index=7)
+    assert not out.any() and not any(g.any() for g in grads)
+    h, w, b, t = ce_inputs(rows, vocab, dim, dtype, 78, bias=False)
+    check_ce(h, w, None, torch.full((rows,), -100))         # no row counts
+    for bad in (vocab, -1, 2 ** 40):
+        t2 = t.clone()
+        t2[5] = bad
+        check_ce(h, w, None, t2)                            # NaN, loudly
+
+
+def test_linear_cross_entropy_strides_alignment_and_no_rows():
+    import mde_amd.vocab_losses as L
+    for dtype in TYPES:
+        h, w, b, t = ce_inputs(70, 200, 192, dtype, 81, bias=True)
+        wide_h, wide_w = torch.zeros(140, 260, dtype=dtype, device=DEV), torch.zeros(400, 250, dtype=dtype, device=DEV)
+        wide_h[::2, 3:195], wide_w[::2, 5:197] = h.to(DEV), w.to(DEV)      # rows that start off any 16 bytes
+        check_ce(h, w, b, t, on_device=(wide_h[::2, 3:195], wide_w[::2, 5:197]))
+        wide_h = torch.zeros(70, 256, dtype=dtype, device=DEV)
+        wide_h[:, :192] = h.to(DEV)
+        check_ce(h, w, b, t, on_device=(wide_h[:, :192], w.to(DEV)))       # strided and aligned: read in place
+    h, w, b, t = ce_inputs(24, 31, 16, torch.float32, 82, bias=True)
+    maps = h.reshape(2, 3, 4, 16).to(DEV)
+    out = L.linear_cross_entropy(maps, w.to(DEV), t.reshape(2, 3, 4).int().to(DEV), b.to(DEV), reduction="none")
+    loss = O.linear_ce(h, w, t, b)[0]
+    close(out, loss.reshape(2, 3, 4), 1e-4, "leading dimensions, int32 targets")
+    hh, ww, bb = (x.to(DEV).requires_grad_(True) for x in (h[:0], w, b))
+    for reduction in ("none", "sum", "mean"):
+        out = L.linear_cross_entropy(hh, ww, t[:0].to(DEV), bb, reduction=reduction)
+        assert float(out.detach().sum()) == 0.0
+        out.sum().backward()
+    assert hh.grad.shape == (0, 16) and not ww.grad.any() and not bb.grad.any()
+
+
+def test_linear_cross_entropy_several_pieces_of_the_vocabulary():
+    """rows * classes above one piece (2^26 derivatives): the pieces' sums join, the last one is ragged."""
+    import mde_amd.vocab_losses as L
+    rows, vocab, dim = 2048, 70001, 64
+    g = torch.Generator(device=DEV).manual_seed(5)
+    h = torch.randn(rows, dim, generator=g, device=DEV).bfloat16().requires_grad_(True)
+    w = (torch.randn(vocab, dim, generator=g, device=DEV) * 0.3).bfloat16().requires_grad_(True)
+    t = torch.randint(vocab, (rows,), generator=g, device=DEV)
+    loss = L.linear_cross_entropy(h, w, t)
+    gh, gw = torch.autograd.grad(loss, (h, w))
+    with torch.no_grad():
+        z = h.double() @ w.double().T
+        lse = torch.logsumexp(z, 1, keepdim=True)
+        want = (lse[:, 0] - z.gather(1, t[:, None])[:, 0]).mean()
+        d = (z - lse).exp_()
+        d[torch.arange(rows, device=DEV), t] -= 1
+        d /= rows
+        wh, ww = d @ w.double(), d.T.contiguous() @ h.double()
+        # half a step of bfloat16 for every derivative and for the result
+        th = d.abs() @ w.double().abs() * (2 ** -8 + 2 ** -16) + wh.abs() * 2 ** -8 + 1e-12
+        tw = d.abs().T.contiguous() @ h.double().abs() * (2 ** -8 + 2 ** -16) + ww.abs() * 2 ** -8 + 1e-12
+    assert abs(float(loss) - float(want)) <= 1e-5 * float(want)
+    assert bool(((gh.double() - wh).abs() <= th).all()) and bool(((gw.double() - ww).abs() <= tw).all())
+
+
+# ------------------------------------------------------------------ the three together, streams, graphs, hooks
+def test_teacher_and_student_together():
+    """A distillation step over shared pixels: the teacher's top logits, the student against them and against the labels,
+    both losses into one head."""
+    import mde_amd.vocab_losses as L
+    rows, bins, dim, k, t = 500, 80, 64, 6, 2.0
+    h, w, b, target = ce_inputs(rows, bins, dim, torch.float32, 91, bias=True)
+    tx = logits(rows, bins, 92, torch.float32)
+    top = L.top_logits(tx.to(DEV), k, t)
+    hh, ww, bb = (x.to(DEV).requires_grad_(True) for x in (h, w, b))
+    kd = L.topk_distillation_loss(hh @ ww.T + bb, top.values, top.indices, top.lse, temperature=t)
+    ce = L.linear_cross_entropy(hh, ww, target.to(DEV), bb)
+    (0.7 * kd + 0.3 * ce).backward()
+    h6, w6, b6 = (x.double().requires_grad_(True) for x in (h, w, b))
+    z = h6 @ w6.T + b6
+    v, i, lse = O.top_logits(tx, k, t)
+    logq = v / t - lse[:, None]
+    logp = torch.log_softmax(z / t, 1)
+    member = torch.zeros(rows, bins, dtype=torch.bool).scatter_(1, i, True)
+    qt = 1 - logq.exp().sum(1)
+    rest = torch.logsumexp(logp.masked_fill(member, -INF), 1)
+    kl = (logq.exp() * (logq - logp.gather(1, i))).sum(1) + qt * (qt.log() - rest)
+    want = 0.7 * t * t * kl.mean() + 0.3 * torch.nn.functional.cross_entropy(z, target)
+    want.backward()
+    assert abs(float(0.7 * kd + 0.3 * ce) - float(want)) <= 1e-5 * float(want)
+    for got, ref in ((hh.grad, h6.grad), (ww.grad, w6.grad), (bb.grad, b6.grad)):
+        assert float((got.cpu().double() - ref).norm()) <= 1e-5 * float(ref.norm())
+
+
+def both(L, s):
+    top = L.top_logits(s["teacher"], 5)
+    kd = L.topk_distillation_loss(s["x"], top.values, top.indices, top.lse)
+    ce = L.linear_cross_entropy(s["h"], s["w"], s["t"], z_loss=1e-4)
+    return (kd.detach(), ce.detach()) + torch.autograd.grad(kd + ce, (s["x"], s["h"], s["w"]))
+
+
+def state(rows, vocab, dim, dtype, seed):
+    h, w, _, t = ce_inputs(rows, vocab, dim, dtype, seed, bias=False)
+    x, tx = logits(rows, vocab, seed + 1, dtype), logits(rows, vocab, seed + 2, dtype)
+    return {"h": h.to(DEV).requires_grad_(True), "w": w.to(DEV).requires_grad_(True), "t": t.to(DEV),
+            "x": x.to(DEV).requires_grad_(True), "teacher": tx.to(DEV)}
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_repeated_calls_and_side_streams_give_the_same_bits(dtype):
+    import mde_amd.vocab_losses as L
+    for rows, vocab, dim in ((40, 130, 64), (9, 5000, 100)):
+        s = state(rows, vocab, dim, dtype, 101)
+        first = both(L, s)
+        torch.cuda.synchronize()
+        side, other = torch.cuda.Stream(), torch.cuda.Stream()
+        outs = []
+        for st in (side, other):                            # two calls under way at once
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                outs.append(both(L, s))
+        torch.cuda.synchronize()
+        for out in outs:
+            assert all(torch.equal(a, b) for a, b in zip(first, out))
+
+
+def test_captured_and_replayed():
+    """Two graphs, captured one after the other, replayed in turn on changing inputs with eager work between."""
+    import mde_amd.vocab_losses as L
+    states = [state(40, 130, 64, torch.bfloat16, 111), state(12, 6000, 96, torch.float32, 121)]
+    graphs = []
+    side = torch.cuda.Stream()
+    for s in states:
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            both(L, s)                                      # warm-up; its autograd graph is gone before the capture
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = both(L, s)
+        graphs.append((g, out))
+    for turn in range(4):
+        for s in states:
+            with torch.no_grad():
+                for name in ("x", "h", "w", "teacher"):
+                    s[name].mul_(0.9).add_(0.01 * turn)
+        for g, _ in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for s, (_, out) in zip(states, graphs):
+            assert all(torch.equal(a, b) for a, b in zip(out, both(L, s)))
+
+
+def test_saved_tensors_may_move_between_forward_and_backward():
+    import mde_amd.vocab_losses as L
+    s = state(20, 3000, 64, torch.float32, 131)
+    want = both(L, s)
+    with torch.autograd.graph.save_on_cpu():
+        top = L.top_logits(s["teacher"], 5)
+        loss = L.topk_distillation_loss(s["x"], top.values, top.indices, top.lse) \
+            + L.linear_cross_entropy(s["h"], s["w"], s["t"], z_loss=1e-4)
+    filler = [torch.full((20, 3000), float("nan"), device=DEV) for _ in range(4)]   # over anything that was given back
+    got = torch.autograd.grad(loss, (s["x"], s["h"], s["w"]))
+    assert all(torch.equal(a, b) for a, b in zip(want[2:], got)) and len(filler) == 4
+
+
+def test_refusals_on_the_device():
+    import mde_amd.vocab_losses as L
+    x = torch.zeros(4, 20, device=DEV)
+    v, i = torch.zeros(4, 3, device=DEV), torch.zeros(4, 3, dtype=torch.int32, device=DEV)
+    bad = [
+        lambda: L.top_logits(x.cpu(), 3), lambda: L.top_logits(x, 0), lambda: L.top_logits(x, 21),
+        lambda: L.top_logits(torch.zeros(2, 500, device=DEV), 257), lambda: L.top_logits(x.int(), 3),
+        lambda: L.top_logits(x, 3, temperature=0.0), lambda: L.top_logits(x, 3, temperature=float("nan")),
+        lambda: L.top_logits(x[:, :0], 1), lambda: L.top_logits(x.sum(), 1),
+        lambda: L.topk_distillation_loss(x, v, i.float()), lambda: L.topk_distillation_loss(x, v[:3], i[:3]),
+        lambda: L.topk_distillation_loss(x, v, i[:, :2]), lambda: L.topk_distillation_loss(x, v, i.cpu()),
+        lambda: L.topk_distillation_loss(x, v, i, torch.zeros(3, device=DEV)),
+        lambda: L.topk_distillation_loss(x, v, i, weights=torch.zeros(4, 1, device=DEV)),
+        lambda: L.topk_distillation_loss(x, v, i, reduction="batchmean"),
+        lambda: L.topk_distillation_loss(x, v, i, temperature=-1.0),
+        lambda: L.topk_distillation_loss(x[:, :2], v, i),
+        lambda: L.linear_cross_entropy(x, x[:, :5], i[:, 0]), lambda: L.linear_cross_entropy(x, x.half(), i[:, 0]),
+        lambda: L.linear_cross_entropy(x, x, i), lambda: L.linear_cross_entropy(x, x, v[:, 0]),
+        lambda: L.linear_cross_entropy(x, x, i[:, 0].bool()), lambda: L.linear_cross_entropy(x, x, i[:, 0].cpu()),
+        lambda: L.linear_cross_entropy(x, x, i[:, 0], x[0]), lambda: L.linear_cross_entropy(x, x, i[:, 0], x[:, 0].half()),
+        lambda: L.linear_cross_entropy(x, x, i[:, 0], z_loss=-1.0),
+        lambda: L.linear_cross_entropy(x, x, i[:, 0], reduction="max"),
+    ]
+    for n, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            print("accepted: %d" % n)
+    with pytest.raises(RuntimeError):                       # no second derivatives
+        y = x.clone().requires_grad_(True)
+        (g,) = torch.autograd.grad(L.topk_distillation_loss(y, v, i), y, create_graph=True)
+        g.sum().backward()
