@@ -18,10 +18,23 @@ static_assert(sizeof(vsl_linear_ce_desc) == 96, "C-ABI struct layout changed");
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int kTile = 128;       // rows and columns of an output tile
-constexpr int kThreads = 256;    // four waves, 64 x 64 of the tile each
+constexpr int kThreads = 256;    // of the kernels around the products
 constexpr int kBlockBytes = 128; // bytes of K that one step of the main loop takes from every row of A and B
-constexpr int kLds = 2 * 2 * kTile * kBlockBytes;
+constexpr int kPad = 256;        // rows and classes are laid out in multiples of the larger tile
+
+// Shape of an output tile: BM x BN, WM x WN waves, each with IM x JN blocks of 32 x 32.
+template <int BM_, int BN_, int WM_, int WN_>
+struct Shape {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
+  static constexpr int kThreads = 64 * WM * WN;
+  static constexpr int IM = BM / WM / 32, JN = BN / WN / 32;
+  static constexpr int kBuffer = (BM + BN) * kBlockBytes;  // LDS of one step
+  static constexpr int kLds = 2 * kBuffer;
+  static constexpr int kFetch = kBuffer / (kThreads * 16);  // 16-byte pieces per thread and step, A's first
+  static constexpr int kFetchA = BM * kBlockBytes / (kThreads * 16);
+};
+typedef Shape<256, 256, 2, 4> Large;
+typedef Shape<128, 128, 2, 2> Small;
 
 template <typename T>
 struct Kind {
@@ -53,64 +66,102 @@ struct Operands {
   int M, N, kblocks;
 };
 
-// C tile of a wave: acc[i][j] covers rows 32 i.. and columns 32 j.. of its 64 x 64; register r of a lane is row
+// C tile of a wave: acc[i][j] covers rows 32 i.. and columns 32 j.. of its part; register r of a lane is row
 // (r & 3) + 8 (r >> 2) + 4 (lane >> 5), column lane & 31.
+template <typename S>
 struct Tile {
-  f32x16 acc[2][2];
+  f32x16 acc[S::IM][S::JN];
 };
 
 // Rows of A and B go through LDS 128 bytes at a time, two buffers deep, straight from global memory.  A row is one line
-// of eight 16-byte pieces; piece p of row r lies at p ^ (r & 7), so that eight rows read at one piece touch all banks.
-template <typename T>
-__device__ __forceinline__ void tile_product(const Operands& op, int m0, int n0, int k0, int k1, char* lds, Tile& t) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int wm = wave >> 1, wn = wave & 1;
+// of eight 16-byte pieces; piece p of row r lies at p ^ ((r >> 1) & 7), so that sixteen rows read at one
+// piece touch all 64 banks (with r & 7 half of the reads' cycles were conflicts).
+// A step is four rounds; each round's fragments are read while the round before multiplies.  The barrier stands before the
+// last round, whose fragments are in registers by then: behind it the buffer is free for the step after next, and the
+// next step's first fragments are read under the last round's multiplications.
+template <typename T, typename S>
+__device__ __forceinline__ void tile_product(const Operands& op, int m0, int n0, int k0, int k1, char* lds, Tile<S>& t) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / S::WN, wn = wave % S::WN;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < S::IM; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < S::JN; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) t.acc[i][j][r] = 0.0f;
-  const char* src[8];
+  if (k0 >= k1) return;
+  const char* src[S::kFetch];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int at = ((i & 3) * 4 + wave) * 64 + lane, row = at >> 3, piece = (at & 7) ^ (row & 7);
-    src[i] = i < 4 ? (const char*)op.A + (int64_t)min(m0 + row, op.M - 1) * op.lda * (int)sizeof(T)
-                   : (const char*)op.B + (int64_t)min(n0 + row, op.N - 1) * op.ldb * (int)sizeof(T);
+  for (int i = 0; i < S::kFetch; ++i) {
+    const int at = (i < S::kFetchA ? i : i - S::kFetchA) * S::kThreads + tid, row = at >> 3, piece = (at & 7) ^ ((row >> 1) & 7);
+    src[i] = i < S::kFetchA ? (const char*)op.A + (int64_t)min(m0 + row, op.M - 1) * op.lda * (int)sizeof(T)
+                            : (const char*)op.B + (int64_t)min(n0 + row, op.N - 1) * op.ldb * (int)sizeof(T);
     src[i] += (int64_t)k0 * kBlockBytes + piece * 16;
   }
   auto fetch = [&](int buffer) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      char* dst = lds + buffer * (2 * kTile * kBlockBytes) + (i < 4 ? 0 : kTile * kBlockBytes) + ((i & 3) * 4 + wave) * 1024;
+    for (int i = 0; i < S::kFetch; ++i) {
+      char* dst = lds + buffer * S::kBuffer + (i * S::kThreads + wave * 64) * 16;
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src[i],
                                        (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
       src[i] += kBlockBytes;
     }
   };
-  if (k0 < k1) fetch(0);
-  for (int k = k0; k < k1; ++k) {
-    const int buffer = (k - k0) & 1;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's share of the step's rows is in LDS
-    __syncthreads();                                  // everyone's is, and the other buffer has been read
-    if (k + 1 < k1) fetch(buffer ^ 1);
-    const char* a = lds + buffer * (2 * kTile * kBlockBytes) + (wm * 64 + (lane & 31)) * kBlockBytes;
-    const char* b = lds + buffer * (2 * kTile * kBlockBytes) + kTile * kBlockBytes + (wn * 64 + (lane & 31)) * kBlockBytes;
+  auto wait = [&]() {  // this wave's pieces are in LDS and its reads are done; then everyone's are
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  const char* a = lds + (wm * S::IM * 32 + (lane & 31)) * kBlockBytes;
+  const char* b = lds + (S::BM + wn * S::JN * 32 + (lane & 31)) * kBlockBytes;
+  u32x4 fa[2][S::IM], fb[2][S::JN];
+  auto read = [&](int set, int buffer, int round) {
+    const int piece = ((2 * round + (lane >> 5)) ^ ((lane >> 1) & 7)) * 16 + buffer * S::kBuffer;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const int piece = ((2 * s + (lane >> 5)) ^ (lane & 7)) * 16;
-      u32x4 fa[2], fb[2];
+    for (int i = 0; i < S::IM; ++i) fa[set][i] = *(const u32x4*)(a + i * 32 * kBlockBytes + piece);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        fa[i] = *(const u32x4*)(a + i * 32 * kBlockBytes + piece);
-        fb[i] = *(const u32x4*)(b + i * 32 * kBlockBytes + piece);
-      }
+    for (int j = 0; j < S::JN; ++j) fb[set][j] = *(const u32x4*)(b + j * 32 * kBlockBytes + piece);
+  };
+  auto multiply = [&](int set) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < S::IM; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) t.acc[i][j] = mma(fa[i], fb[j], t.acc[i][j], (const T*)nullptr);
+      for (int j = 0; j < S::JN; ++j) t.acc[i][j] = mma(fa[set][i], fb[set][j], t.acc[i][j], (const T*)nullptr);
+  };
+  auto interleave = [&]() {  // a round's reads go out one by one behind its multiplications, and stay in their round
+    constexpr int kMma = S::IM * S::JN * (sizeof(T) == 4 ? 4 : 1), kRead = S::IM + S::JN;
+    constexpr int kEach = kMma / (kRead + 2) < 1 ? 1 : kMma / (kRead + 2);
+#pragma unroll
+    for (int i = 0; i < kRead; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
+    __builtin_amdgcn_sched_group_barrier(0x008, kMma - kRead * kEach, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  fetch(0);
+  wait();
+  if (k0 + 1 < k1) fetch(1);
+  read(0, 0, 0);
+  auto rounds = [&](int buffer) {  // the first three
+#pragma unroll
+    for (int round = 0; round < 3; ++round) {
+      read((round + 1) & 1, buffer, round + 1);
+      multiply(round & 1);
+      interleave();
+    }
+  };
+  for (int k = k0; k < k1 - 1; ++k) {
+    const int buffer = (k - k0) & 1;
+    rounds(buffer);
+    wait();
+    if (k + 2 < k1) fetch(buffer);
+    read(0, buffer ^ 1, 0);
+    multiply(1);
+    interleave();
   }
+  rounds((k1 - 1 - k0) & 1);
+  multiply(1);
   __syncthreads();
 }
 
@@ -157,29 +208,50 @@ __device__ __forceinline__ float slope_of(float z_loss, float top, float ls) {
   return z_loss == 0.0f ? 1.0f : fmaf(2.0f * z_loss, fmaf(ls, kLn2, top), 1.0f);
 }
 
-template <typename T, bool DELTA>
-__global__ __launch_bounds__(kThreads) void k_ce_logits(LogitArgs a) {
-  __shared__ __attribute__((aligned(16))) char lds[kLds];
-  const int tm_count = (a.op.M + kTile - 1) / kTile, tn_count = (a.op.N + kTile - 1) / kTile;
+// Four 16-bit values a lane, of four lanes in a row, transposed: lane q of the four ends with value q of each.
+__device__ __forceinline__ uint2 transpose4(uint2 x) {
+  const unsigned q = threadIdx.x & 3;
+  const unsigned got = dpp<kXor2>(q < 2 ? x.y : x.x);
+  const unsigned a = q < 2 ? x.x : got, b = q < 2 ? got : x.y;  // values 2 (q / 2).. of lanes q & 1 and (q & 1) + 2
+  const unsigned lows = (a & 0xFFFFu) | b << 16, highs = a >> 16 | (b & 0xFFFF0000u);
+  const unsigned other = dpp<kXor1>(q & 1 ? lows : highs);
+  const unsigned even = q & 1 ? other : lows, odd = q & 1 ? highs : other;  // lanes 0, 2 and lanes 1, 3
+  return {(even & 0xFFFFu) | odd << 16, even >> 16 | (odd & 0xFFFF0000u)};
+}
+template <typename T>
+__device__ __forceinline__ uint2 pack4(const float (&g)[4]) {
+  union {
+    T t[4];
+    uint2 u;
+  } p;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) p.t[e] = (T)g[e];
+  return p.u;
+}
+
+template <typename T, typename S, bool DELTA>
+__global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[S::kLds];
+  const int tm_count = (a.op.M + S::BM - 1) / S::BM, tn_count = (a.op.N + S::BN - 1) / S::BN;
   int tm, tn;
   tile_of(blockIdx.x, tm_count, tn_count, tm, tn);
-  const int m0 = tm * kTile, n0 = tn * kTile;
-  Tile t;
-  tile_product<T>(a.op, m0, n0, 0, a.op.kblocks, lds, t);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
+  const int m0 = tm * S::BM, n0 = tn * S::BN;
+  Tile<S> t;
+  tile_product<T, S>(a.op, m0, n0, 0, a.op.kblocks, lds, t);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
   const int half = lane >> 5;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int col = wn * 64 + j * 32 + (lane & 31), row = n0 + col;
+  for (int j = 0; j < S::JN; ++j) {
+    const int col = (wn * S::JN + j) * 32 + (lane & 31), row = n0 + col;
     const bool live = row < a.op.N;
     const int64_t target = live ? a.target[row] - a.class0 : -1;
     float m = ninf();
     if (!DELTA) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < S::IM; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int v = m0 + wm * 64 + i * 32 + (r & 3) + 8 * (r >> 2) + 4 * half;
+          const int v = m0 + (wm * S::IM + i) * 32 + (r & 3) + 8 * (r >> 2) + 4 * half;
           float z = ninf();
           if (v < a.op.M) {
             z = add_bias<T>(t.acc[i][j][r], a.bias, a.class0 + v);
@@ -191,49 +263,75 @@ __global__ __launch_bounds__(kThreads) void k_ce_logits(LogitArgs a) {
       const float ref = exp_ref(m);
       float s = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < S::IM; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) s += exp_of(t.acc[i][j][r], ref, kLog2e);
       MaxSum q{m, s};
       q = join(q, {__shfl_xor(q.m, 32, 64), __shfl_xor(q.s, 32, 64)}, kLog2e);
-      if (half == 0) ((float2*)lds)[wm * kTile + col] = make_float2(q.m, q.s);
+      if (half == 0) ((float2*)lds)[wm * S::BN + col] = make_float2(q.m, q.s);
     } else {
       const float scale = live ? a.row_scale[row] : 0.0f;
       const float top = live ? a.stats[row] : 0.0f, ls = live ? a.stats[a.op.N + row] : 0.0f;
       const float slope = slope_of(a.z_loss, top, ls);
       T* d = (T*)a.delta + (int64_t)row * a.ldd;
-      T* dt = (T*)a.delta_t + row;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < S::IM; ++i) {
+        const int v32 = m0 + (wm * S::IM + i) * 32;
 #pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-          const int v0 = m0 + wm * 64 + i * 32 + 8 * r4 + 4 * half;
-          T out[4];
+        for (int r8 = 0; r8 < 2; ++r8) {  // two groups of 8 classes, four of each in either half of the wave
+          float g[2][4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int v = v0 + e;
-            float g = 0.0f;
-            if (v < a.op.M && scale != 0.0f) {
-              const float z = add_bias<T>(t.acc[i][j][r4 * 4 + e], a.bias, a.class0 + v);
-              g = scale * (slope * __builtin_amdgcn_exp2f(fmaf(z - top, kLog2e, -ls)) - (v == target ? 1.0f : 0.0f));
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int v = v32 + 16 * r8 + 8 * u + 4 * half + e;
+              float x = 0.0f;
+              if (v < a.op.M && scale != 0.0f) {
+                const float z = add_bias<T>(t.acc[i][j][r8 * 8 + u * 4 + e], a.bias, a.class0 + v);
+                x = scale * (slope * __builtin_amdgcn_exp2f(fmaf(z - top, kLog2e, -ls)) - (v == target ? 1.0f : 0.0f));
+              }
+              g[u][e] = x;
             }
-            out[e] = (T)g;
+          if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const int v0 = v32 + 16 * r8 + 8 * u + 4 * half;
+              if (a.delta) *(f32x4*)(d + v0) = f32x4{g[u][0], g[u][1], g[u][2], g[u][3]};
+              if (a.delta_t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) ((T*)a.delta_t)[(int64_t)(v0 + e) * a.rows_padded + row] = g[u][e];
+            }
+          } else {
+            const uint2 p0 = pack4<T>(g[0]), p1 = pack4<T>(g[1]);
+            if (a.delta) {
+              // the halves trade: the lower lanes get all 8 classes of the first group, the upper ones those of the second
+              const auto x = __builtin_amdgcn_permlane32_swap(p0.x, p1.x, false, false);
+              const auto y = __builtin_amdgcn_permlane32_swap(p0.y, p1.y, false, false);
+              *(u32x4*)(d + v32 + 16 * r8 + 8 * half) = u32x4{x[0], y[0], x[1], y[1]};
+            }
+            if (a.delta_t) {
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                const int v = v32 + 16 * r8 + 8 * u + 4 * half + (lane & 3);
+                *(uint2*)((T*)a.delta_t + (int64_t)v * a.rows_padded + (row & ~3)) = transpose4(u ? p1 : p0);
+              }
+            }
           }
-          if (a.delta)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) d[v0 + e] = out[e];
-          if (a.delta_t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) dt[(int64_t)(v0 + e) * a.rows_padded] = out[e];
         }
+      }
     }
   }
   if (!DELTA) {
     __syncthreads();
     const int col = threadIdx.x;
-    if (col < kTile) {
-      const float2 x = ((float2*)lds)[col], y = ((float2*)lds)[kTile + col];
-      const MaxSum q = join({x.x, x.y}, {y.x, y.y}, kLog2e);
+    if (col < S::BN) {
+      float2 x = ((float2*)lds)[col];
+      MaxSum q{x.x, x.y};
+#pragma unroll
+      for (int w = 1; w < S::WM; ++w) {
+        x = ((float2*)lds)[w * S::BN + col];
+        q = join(q, {x.x, x.y}, kLog2e);
+      }
       a.partial[(int64_t)tm * a.rows_padded + n0 + col] = make_float2(q.m, q.s);
     }
   }
@@ -371,45 +469,65 @@ __global__ __launch_bounds__(kThreads) void k_transpose(const T* __restrict__ in
 // the two gradient products
 // ------------------------------------------------------------------------------------------------------------------
 struct GradArgs {
-  Operands op;
+  Operands op;             // A: [M features, K], B: [N rows or classes, K]
   int splits;              // of K
   bool add;                // to what `sum` holds
-  float* sum;              // [splits][M][N], or NULL: straight to `out`
-  void* out;               // [M][N] of the operands' type
+  bool whole;              // four features in a row are one aligned store
+  float* sum;              // [splits][N][M], or NULL: straight to `out`
+  void* out;               // [N][M] of the operands' type
   const float* out_scale;
 };
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void k_ce_grad(GradArgs a) {
-  __shared__ __attribute__((aligned(16))) char lds[kLds];
-  const int tm_count = (a.op.M + kTile - 1) / kTile, tn_count = (a.op.N + kTile - 1) / kTile;
+template <typename T, typename S>
+__global__ __launch_bounds__(S::kThreads) void k_ce_grad(GradArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[S::kLds];
+  const int tm_count = (a.op.M + S::BM - 1) / S::BM, tn_count = (a.op.N + S::BN - 1) / S::BN;
   const int tiles = tm_count * tn_count, split = blockIdx.x / tiles;
   int tm, tn;
   tile_of(blockIdx.x % tiles, tm_count, tn_count, tm, tn);
   const int per = (a.op.kblocks + a.splits - 1) / a.splits;
   const int k0 = min(split * per, a.op.kblocks), k1 = min(k0 + per, a.op.kblocks);
-  const int m0 = tm * kTile, n0 = tn * kTile;
-  Tile t;
-  tile_product<T>(a.op, m0, n0, k0, k1, lds, t);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
+  const int m0 = tm * S::BM, n0 = tn * S::BN;
+  Tile<S> t;
+  tile_product<T, S>(a.op, m0, n0, k0, k1, lds, t);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
   const float scale = a.sum ? 1.0f : *a.out_scale;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int j = 0; j < S::JN; ++j) {
+    const int row = n0 + (wn * S::JN + j) * 32 + (lane & 31);
+    if (row >= a.op.N) continue;
+    const int64_t at = (int64_t)row * a.op.M;
+    float* sum = a.sum ? a.sum + (int64_t)split * a.op.M * a.op.N + at : nullptr;
+    T* out = (T*)a.out + at;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int i = 0; i < S::IM; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int row = m0 + wm * 64 + i * 32 + (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5);
-        const int col = n0 + wn * 64 + j * 32 + (lane & 31);
-        if (row >= a.op.M || col >= a.op.N) continue;
-        const int64_t at = (int64_t)row * a.op.N + col;
-        if (a.sum) {
-          float* p = a.sum + (int64_t)split * a.op.M * a.op.N + at;
-          *p = a.add ? *p + t.acc[i][j][r] : t.acc[i][j][r];
+      for (int r4 = 0; r4 < 4; ++r4) {
+        const int m = m0 + (wm * S::IM + i) * 32 + 8 * r4 + 4 * (lane >> 5);
+        float g[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) g[e] = scale * t.acc[i][j][4 * r4 + e];
+        if (a.whole && m < a.op.M) {
+          if (sum) {
+            f32x4* p = (f32x4*)(sum + m);
+            f32x4 v{g[0], g[1], g[2], g[3]};
+            if (a.add) v += *p;
+            *p = v;
+          } else if constexpr (sizeof(T) == 4) {
+            *(f32x4*)(out + m) = f32x4{g[0], g[1], g[2], g[3]};
+          } else {
+            *(uint2*)(out + m) = pack4<T>(g);
+          }
         } else {
-          ((T*)a.out)[at] = (T)(scale * t.acc[i][j][r]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (m + e < a.op.M) {
+              if (sum) sum[m + e] = a.add ? sum[m + e] + g[e] : g[e];
+              else out[m + e] = (T)g[e];
+            }
         }
       }
+  }
 }
 
 template <typename T>
@@ -425,12 +543,12 @@ __global__ __launch_bounds__(kThreads) void k_ce_finish(const float* __restrict_
 
 // grad_bias: a block per class sums its row of d^T, the values that grad_weight is made of
 template <typename T>
-__global__ __launch_bounds__(kThreads) void k_ce_bias(const T* __restrict__ delta_t, int64_t rows_padded,
+__global__ __launch_bounds__(kThreads) void k_ce_bias(const T* __restrict__ delta_t, int64_t rows_padded, int64_t rows,
                                                       const float* __restrict__ out_scale, T* __restrict__ out) {
   __shared__ float red[4];
   const T* d = delta_t + (int64_t)blockIdx.x * rows_padded;
   float s = 0.0f;
-  for (int64_t i = threadIdx.x; i < rows_padded / Kind<T>::E; i += kThreads) {
+  for (int64_t i = threadIdx.x; i < rows / Kind<T>::E; i += kThreads) {
     float x[Kind<T>::E];
     unpack(load16(d + i * Kind<T>::E), x, (const T*)nullptr);
 #pragma unroll
@@ -489,7 +607,7 @@ struct Layout {
 };
 Layout layout_of(const vsl_linear_ce_desc* d) {
   Layout l;
-  l.rows_padded = round_up(d->rows, kTile);
+  l.rows_padded = round_up(d->rows, kPad);
   l.dim_padded = round_up(d->dim, kBlockBytes / size_of(d->type));
   l.copy_hidden = !ready(d->hidden, d->hidden_stride, d->dim, d->type);
   l.copy_weight = !ready(d->weight, d->weight_stride, d->dim, d->type);
@@ -510,7 +628,7 @@ Forward forward_workspace(const vsl_linear_ce_desc* d, void* base) {
   Forward f{};
   f.hidden = l.copy_hidden ? a.take((size_t)d->rows * l.dim_padded * s) : nullptr;
   f.weight = l.copy_weight ? a.take((size_t)d->vocab * l.dim_padded * s) : nullptr;
-  f.partial = (float2*)a.take((size_t)ceil_div(d->vocab, kTile) * l.rows_padded * sizeof(float2));
+  f.partial = (float2*)a.take((size_t)ceil_div(d->vocab, Small::BM) * l.rows_padded * sizeof(float2));
   f.target_logit = (float*)a.take((size_t)d->rows * 4);
   f.sums = a.take(sum_workspace_bytes(d->rows));
   f.total = a.used;
@@ -529,8 +647,13 @@ struct Backward {
   float *sum_h, *sum_w, *row_scale, *out_scale, *largest;
   size_t total;
 };
+bool large_tiles(int64_t M, int64_t N, int type) {
+  return type != VSL_TYPE_F32 && ceil_div(M, Large::BM) * ceil_div(N, Large::BN) >= 256;
+}
+// Tiles of a product, and into how many parts its K is cut so that there are enough of them for the 256 CUs.
 int splits_of(int64_t M, int64_t N, int64_t K, int type) {
-  const int64_t tiles = ceil_div(M, kTile) * ceil_div(N, kTile), blocks = ceil_div(K * size_of(type), kBlockBytes);
+  if (large_tiles(M, N, type)) return 1;
+  const int64_t tiles = ceil_div(M, Small::BM) * ceil_div(N, Small::BN), blocks = ceil_div(K * size_of(type), kBlockBytes);
   int64_t s = 512 / tiles;
   if (s > blocks / 8) s = blocks / 8;
   return (int)(s < 1 ? 1 : s);
@@ -539,11 +662,11 @@ Backward backward_workspace(const vsl_linear_ce_desc* d, uint32_t mask, void* ba
   Backward b{};
   b.l = layout_of(d);
   const int s = size_of(d->type);
-  b.piece = kPieceElements / (b.l.rows_padded > 0 ? b.l.rows_padded : 1) / kTile * kTile;
-  if (b.piece < kTile) b.piece = kTile;
-  if (b.piece > round_up(d->vocab, kTile)) b.piece = round_up(d->vocab, kTile);
+  b.piece = kPieceElements / (b.l.rows_padded > 0 ? b.l.rows_padded : 1) / kPad * kPad;
+  if (b.piece < kPad) b.piece = kPad;
+  if (b.piece > round_up(d->vocab, kPad)) b.piece = round_up(d->vocab, kPad);
   b.pieces = ceil_div(d->vocab, b.piece);
-  b.vocab_padded = round_up(d->vocab, kTile);
+  b.vocab_padded = round_up(d->vocab, kPad);
   const bool gh = mask & 1, gw = mask & 2, gb = mask & 4;
   Arena a{(char*)base};
   b.hidden = b.l.copy_hidden ? a.take((size_t)d->rows * b.l.dim_padded * s) : nullptr;
@@ -552,8 +675,8 @@ Backward backward_workspace(const vsl_linear_ce_desc* d, uint32_t mask, void* ba
   b.weight_t = gh ? a.take((size_t)d->dim * b.vocab_padded * s) : nullptr;
   b.delta = gh ? a.take((size_t)b.l.rows_padded * b.piece * s) : nullptr;
   b.delta_t = gw || gb ? a.take((size_t)b.l.rows_padded * b.piece * s) : nullptr;
-  b.splits_h = splits_of(d->rows, d->dim, b.piece, d->type);
-  b.splits_w = splits_of(d->vocab < b.piece ? d->vocab : b.piece, d->dim, b.l.rows_padded, d->type);
+  b.splits_h = splits_of(d->dim, d->rows, b.piece, d->type);
+  b.splits_w = splits_of(d->dim, d->vocab < b.piece ? d->vocab : b.piece, b.l.rows_padded, d->type);
   b.sum_h = gh && (b.pieces > 1 || b.splits_h > 1) ? (float*)a.take((size_t)b.splits_h * d->rows * d->dim * 4) : nullptr;
   b.sum_w = gw && b.splits_w > 1 ? (float*)a.take((size_t)b.splits_w * b.piece * d->dim * 4) : nullptr;
   b.row_scale = (float*)a.take((size_t)b.l.rows_padded * 4);
@@ -580,6 +703,31 @@ void launch_transpose(const void* in, int64_t stride, int64_t rows, int64_t cols
                      (const T*)in, stride, rows, (int)cols, rows_padded, scale, (const T*)bias, (T*)out);
 }
 
+template <typename T, typename S, bool DELTA>
+int launch_logits_as(const LogitArgs& a, hipStream_t s) {
+  const int64_t tm = ceil_div(a.op.M, S::BM), tn = ceil_div(a.op.N, S::BN);
+  hipLaunchKernelGGL((k_ce_logits<T, S, DELTA>), dim3((unsigned)(tm * tn)), dim3(S::kThreads), 0, s, a);
+  return (int)tm;
+}
+template <typename T, bool DELTA>
+int launch_logits(const LogitArgs& a, bool large, hipStream_t s) {  // returns the rows of tiles
+  if constexpr (sizeof(T) == 2)
+    if (large) return launch_logits_as<T, Large, DELTA>(a, s);
+  return launch_logits_as<T, Small, DELTA>(a, s);
+}
+template <typename T, typename S>
+void launch_grad_as(const GradArgs& g, hipStream_t s) {
+  const int64_t tiles = ceil_div(g.op.M, S::BM) * ceil_div(g.op.N, S::BN);
+  hipLaunchKernelGGL((k_ce_grad<T, S>), dim3((unsigned)(tiles * g.splits)), dim3(S::kThreads), 0, s, g);
+}
+template <typename T>
+void launch_grad(GradArgs g, int type, hipStream_t s) {
+  g.whole = g.op.M % 4 == 0 && (uintptr_t)g.out % 16 == 0;
+  if constexpr (sizeof(T) == 2)
+    if (large_tiles(g.op.M, g.op.N, type)) return launch_grad_as<T, Large>(g, s);
+  launch_grad_as<T, Small>(g, s);
+}
+
 template <typename T>
 void run_forward(const vsl_linear_ce_desc* d, const Forward& f, float* row_loss, float* stats, float* loss, float* divisor,
                  hipStream_t s) {
@@ -595,8 +743,7 @@ void run_forward(const vsl_linear_ce_desc* d, const Forward& f, float* row_loss,
   a.rows_padded = l.rows_padded;
   a.partial = f.partial;
   a.target_logit = f.target_logit;
-  const int tiles = (int)ceil_div(d->vocab, kTile);
-  hipLaunchKernelGGL((k_ce_logits<T, false>), dim3((unsigned)(tiles * (l.rows_padded / kTile))), dim3(kThreads), 0, s, a);
+  const int tiles = launch_logits<T, false>(a, large_tiles(a.op.M, a.op.N, d->type), s);
   hipLaunchKernelGGL(k_ce_rows, dim3((unsigned)ceil_div(d->rows, 16)), dim3(kThreads), 0, s, (const float2*)f.partial,
                      l.rows_padded, tiles, (const float*)f.target_logit, d->target, d->ignore_index, d->vocab, d->z_loss,
                      d->rows, row_loss, stats);
@@ -639,7 +786,9 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
   if (grad_hidden) launch_transpose<T>(weight, ldw, d->vocab, d->dim, b.vocab_padded, nullptr, d->bias, b.weight_t, s);
   for (int64_t p = 0; p < b.pieces; ++p) {
     const int64_t v0 = p * b.piece, classes = d->vocab - v0 < b.piece ? d->vocab - v0 : b.piece;
-    const int64_t padded = round_up(classes, kTile);
+    const bool large = large_tiles(classes, d->rows, d->type);
+    const int64_t tile = large ? Large::BM : Small::BM;  // square: what the derivative kernel covers in both directions
+    const int64_t padded = round_up(classes, tile), rows_covered = round_up(d->rows, tile);
     LogitArgs a{};
     a.op = {weight + v0 * ldw, hidden, ldw, ldh, (int)classes, (int)d->rows, (int)(l.dim_padded / Kind<T>::BK)};
     a.bias = d->bias;
@@ -652,35 +801,32 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
     a.delta = grad_hidden ? b.delta : nullptr;
     a.ldd = b.piece;
     a.delta_t = grad_weight || grad_bias ? b.delta_t : nullptr;
-    hipLaunchKernelGGL((k_ce_logits<T, true>), dim3((unsigned)(padded / kTile * (l.rows_padded / kTile))), dim3(kThreads), 0,
-                       s, a);
+    launch_logits<T, true>(a, large, s);
     if (grad_hidden) {
       GradArgs g{};
-      g.op = {b.delta, (const T*)b.weight_t + v0, b.piece, b.vocab_padded, (int)d->rows, (int)d->dim, (int)(padded / Kind<T>::BK)};
+      g.op = {(const T*)b.weight_t + v0, b.delta, b.vocab_padded, b.piece, (int)d->dim, (int)d->rows, (int)(padded / Kind<T>::BK)};
       g.splits = b.splits_h;
       g.add = p > 0;
       g.sum = b.sum_h;
       g.out = grad_hidden;
       g.out_scale = b.out_scale;
-      const int64_t tiles = ceil_div(d->rows, kTile) * ceil_div(d->dim, kTile);
-      hipLaunchKernelGGL(k_ce_grad<T>, dim3((unsigned)(tiles * g.splits)), dim3(kThreads), 0, s, g);
+      launch_grad<T>(g, d->type, s);
     }
     if (grad_weight) {
       GradArgs g{};
-      g.op = {b.delta_t, b.hidden_t, l.rows_padded, l.rows_padded, (int)classes, (int)d->dim, (int)(l.rows_padded / Kind<T>::BK)};
+      g.op = {b.hidden_t, b.delta_t, l.rows_padded, l.rows_padded, (int)d->dim, (int)classes, (int)(rows_covered / Kind<T>::BK)};
       g.splits = b.splits_w;
       g.sum = b.sum_w;
       g.out = grad_weight + v0 * d->dim;
       g.out_scale = b.out_scale;
-      const int64_t tiles = ceil_div(classes, kTile) * ceil_div(d->dim, kTile);
-      hipLaunchKernelGGL(k_ce_grad<T>, dim3((unsigned)(tiles * g.splits)), dim3(kThreads), 0, s, g);
+      launch_grad<T>(g, d->type, s);
       if (g.sum)
         hipLaunchKernelGGL(k_ce_finish<T>, linear_grid(classes * d->dim), dim3(kThreads), 0, s, (const float*)g.sum, g.splits,
                            classes * d->dim, (const float*)b.out_scale, (T*)g.out);
     }
     if (grad_bias)
       hipLaunchKernelGGL(k_ce_bias<T>, dim3((unsigned)classes), dim3(kThreads), 0, s, (const T*)b.delta_t, l.rows_padded,
-                         (const float*)b.out_scale, grad_bias + v0);
+                         rows_covered, (const float*)b.out_scale, grad_bias + v0);
   }
   if (grad_hidden && b.sum_h)
     hipLaunchKernelGGL(k_ce_finish<T>, linear_grid(d->rows * d->dim), dim3(kThreads), 0, s, (const float*)b.sum_h, b.splits_h,
