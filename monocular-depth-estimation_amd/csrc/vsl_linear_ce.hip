@@ -430,39 +430,72 @@ __global__ __launch_bounds__(kThreads) void k_ce_scale(ScaleArgs a) {
 // ------------------------------------------------------------------------------------------------------------------
 // layouts
 // ------------------------------------------------------------------------------------------------------------------
-// out [rows, cols_padded] = in [rows, cols], zeros behind
+// out [rows, cols_padded] = in [rows, cols], zeros behind: 16 bytes a thread, from rows that may start anywhere
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_pad(const T* __restrict__ in, int64_t stride, int64_t rows, int cols,
                                                   int cols_padded, T* __restrict__ out) {
-  const int64_t n = rows * cols_padded;
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) {
-    const int64_t r = i / cols_padded;
-    const int c = (int)(i - r * cols_padded);
-    out[i] = c < cols ? in[r * stride + c] : (T)0.0f;
-  }
+  constexpr int E = Kind<T>::E;
+  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+  for (int64_t r = (int64_t)blockIdx.x * 4 + y; r < rows; r += (int64_t)gridDim.x * 4)
+    for (int c = x * E; c < cols_padded; c += 64 * E) {
+      float v[E];
+      if (c + E <= cols) {
+        *(u32x4*)(out + r * cols_padded + c) = load16(in + r * stride + c);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = c + e < cols ? (float)in[r * stride + c + e] : 0.0f;
+        *(u32x4*)(out + r * cols_padded + c) = pack(v, (const T*)nullptr);
+      }
+    }
 }
 
 // out [cols, rows_padded] = in^T, zeros behind; a row that cannot contribute (its scale is 0, or its bias is -infinity)
-// reads as zeros, so that a NaN in it does not meet the zero of its derivative
+// reads as zeros, so that a NaN in it does not meet the zero of its derivative.  in: rows the main loop could take.
+template <typename T>
+__device__ __forceinline__ bool contributes(int64_t r, int64_t rows, const float* scale, const T* bias) {
+  return r < rows && !(scale && scale[r] == 0.0f) && !(bias && (float)bias[r] == ninf());
+}
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_transpose(const T* __restrict__ in, int64_t stride, int64_t rows, int cols,
                                                         int64_t rows_padded, const float* __restrict__ scale,
                                                         const T* __restrict__ bias, T* __restrict__ out) {
-  __shared__ T tile[64][65];
   const int64_t tiles_c = (cols + 63) / 64;
   const int64_t r0 = blockIdx.x / tiles_c * 64;
   const int c0 = (int)(blockIdx.x % tiles_c) * 64;
-  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
-  for (int i = y; i < 64; i += 4) {
-    const int64_t r = r0 + i;
-    const int c = c0 + x;
-    T v = (T)0.0f;
-    if (r < rows && c < cols && !(scale && scale[r] == 0.0f) && !(bias && (float)bias[r] == ninf())) v = in[r * stride + c];
-    tile[i][x] = v;
+  if constexpr (sizeof(T) == 2) {
+    // A thread takes eight columns of two rows and leaves eight words of two rows each in the columns' lines; a line is
+    // 32 words, turned by four words per group of eight columns so that the groups' words meet in different banks.
+    __shared__ __attribute__((aligned(16))) unsigned tile[64 * 32];
+    {
+      const int g = threadIdx.x & 7, rp = threadIdx.x >> 3, c = c0 + 8 * g;
+      const int64_t r = r0 + 2 * rp;
+      const u32x4 none{0u, 0u, 0u, 0u};
+      const u32x4 x = c < cols && contributes(r, rows, scale, bias) ? *(const u32x4*)(in + r * stride + c) : none;
+      const u32x4 y = c < cols && contributes(r + 1, rows, scale, bias) ? *(const u32x4*)(in + (r + 1) * stride + c) : none;
+      unsigned* t = tile + 8 * g * 32 + ((rp + 4 * g) & 31);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        t[(2 * i) * 32] = (x[i] & 0xFFFFu) | y[i] << 16;
+        t[(2 * i + 1) * 32] = x[i] >> 16 | (y[i] & 0xFFFF0000u);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int at = i * kThreads + threadIdx.x, c = at >> 3, piece = at & 7;
+      if (c0 + c < cols)
+        *(u32x4*)(out + (int64_t)(c0 + c) * rows_padded + r0 + 8 * piece) =
+            *(const u32x4*)(tile + c * 32 + ((4 * piece + 4 * (c >> 3)) & 31));
+    }
+  } else {
+    __shared__ T tile[64][65];
+    const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+    for (int i = y; i < 64; i += 4)
+      tile[i][x] = c0 + x < cols && contributes(r0 + i, rows, scale, bias) ? in[(r0 + i) * stride + c0 + x] : (T)0.0f;
+    __syncthreads();
+    for (int i = y; i < 64; i += 4)
+      if (c0 + i < cols) out[(int64_t)(c0 + i) * rows_padded + r0 + x] = tile[x][i];
   }
-  __syncthreads();
-  for (int i = y; i < 64; i += 4)
-    if (c0 + i < cols) out[(int64_t)(c0 + i) * rows_padded + r0 + x] = tile[x][i];
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -530,14 +563,35 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_grad(GradArgs a) {
   }
 }
 
+// out = out_scale * the sum of the splits, in their order: four elements a thread, the splits dealt to the four waves
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_ce_finish(const float* __restrict__ sum, int splits, int64_t n,
                                                         const float* __restrict__ out_scale, T* __restrict__ out) {
+  __shared__ f32x4 part[3][64];
   const float scale = *out_scale;
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) {
-    float v = sum[i];
-    for (int s = 1; s < splits; ++s) v += sum[s * n + i];
-    out[i] = (T)(scale * v);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int per = (splits + 3) / 4, s0 = wave * per, s1 = min(splits, s0 + per);
+  for (int64_t i0 = (int64_t)blockIdx.x * 256; i0 < n; i0 += (int64_t)gridDim.x * 256) {
+    const int64_t i = i0 + 4 * lane;
+    f32x4 v{0.0f, 0.0f, 0.0f, 0.0f};
+    if (n % 4 == 0) {
+      if (i < n)
+        for (int s = s0; s < s1; ++s) v += *(const f32x4*)(sum + s * n + i);
+    } else {
+      for (int s = s0; s < s1; ++s)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (i + e < n) v[e] += sum[s * n + i + e];
+    }
+    __syncthreads();
+    if (wave) part[wave - 1][lane] = v;
+    __syncthreads();
+    if (wave) continue;
+#pragma unroll
+    for (int w = 0; w < 3; ++w) v += part[w][lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (i + e < n) out[i + e] = (T)(scale * v[e]);
   }
 }
 
@@ -647,8 +701,10 @@ struct Backward {
   float *sum_h, *sum_w, *row_scale, *out_scale, *largest;
   size_t total;
 };
+// The large tile reads half as much per product and needs enough tiles for the 256 CUs, and not more padding than it saves.
 bool large_tiles(int64_t M, int64_t N, int type) {
-  return type != VSL_TYPE_F32 && ceil_div(M, Large::BM) * ceil_div(N, Large::BN) >= 256;
+  const int64_t large = ceil_div(M, Large::BM) * ceil_div(N, Large::BN), small = ceil_div(M, Small::BM) * ceil_div(N, Small::BN);
+  return type != VSL_TYPE_F32 && large >= 256 && large * 4 * 8 <= small * 9;
 }
 // Tiles of a product, and into how many parts its K is cut so that there are enough of them for the 256 CUs.
 int splits_of(int64_t M, int64_t N, int64_t K, int type) {
@@ -693,7 +749,7 @@ dim3 linear_grid(int64_t n) {
 
 template <typename T>
 void launch_pad(const void* in, int64_t stride, int64_t rows, int64_t cols, int64_t cols_padded, void* out, hipStream_t s) {
-  hipLaunchKernelGGL(k_pad<T>, linear_grid(rows * cols_padded), dim3(kThreads), 0, s, (const T*)in, stride, rows, (int)cols,
+  hipLaunchKernelGGL(k_pad<T>, dim3((unsigned)(ceil_div(rows, 4) < 16384 ? ceil_div(rows, 4) : 16384)), dim3(kThreads), 0, s, (const T*)in, stride, rows, (int)cols,
                      (int)cols_padded, (T*)out);
 }
 template <typename T>
