@@ -189,7 +189,9 @@ struct LogitArgs {
   float* target_logit; // [rows]
   // backward
   const float* stats;  // [2][rows] maximum and log2 of the sum above it
-  const float* row_scale;
+  const float* row_scale;  // NULL: `unit` for every row that counts
+  float unit;
+  int64_t ignore_index;
   float z_loss;
   void* delta;         // [rows_padded][ldd]
   int64_t ldd;
@@ -270,8 +272,9 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
       q = join(q, {__shfl_xor(q.m, 32, 64), __shfl_xor(q.s, 32, 64)}, kLog2e);
       if (half == 0) ((float2*)lds)[wm * S::BN + col] = make_float2(q.m, q.s);
     } else {
-      const float scale = live ? a.row_scale[row] : 0.0f;
-      const float top = live ? a.stats[row] : 0.0f, ls = live ? a.stats[a.op.N + row] : 0.0f;
+      const float top = live ? a.stats[row] : ninf(), ls = live ? a.stats[a.op.N + row] : 0.0f;
+      const float scale = !live || top == ninf() || target + a.class0 == a.ignore_index ? 0.0f
+                          : a.row_scale ? a.row_scale[row] : a.unit;
       const float slope = slope_of(a.z_loss, top, ls);
       T* d = (T*)a.delta + (int64_t)row * a.ldd;
 #pragma unroll
@@ -372,24 +375,38 @@ __global__ __launch_bounds__(kThreads) void k_ce_rows(const float2* __restrict__
 // ------------------------------------------------------------------------------------------------------------------
 // backward: scales of the rows
 // ------------------------------------------------------------------------------------------------------------------
+// What the products are multiplied by at the end.  Where every row has the same gradient g, the derivatives are made for
+// a gradient of `unit` and this is g / unit; where they differ (one per row, or by z_loss) the derivatives are made for
+// gradients scaled so that the largest becomes `unit`, and this is that largest / unit.
+struct OutScale {
+  const float* g_loss;    // NULL: `given` holds the scale
+  const float* divisor;   // NULL: 1
+  const float* given;
+  float unit;
+  __device__ __forceinline__ float gradient() const {
+    if (!divisor) return *g_loss;
+    return *divisor == 0.0f ? 0.0f : *g_loss / *divisor;
+  }
+  __device__ __forceinline__ float get() const { return g_loss ? gradient() / unit : *given; }
+};
+
 struct ScaleArgs {
   const float* g_loss;
-  const float* divisor;
+  const float* divisor;  // NULL: 1
   const float* stats;
   const int64_t* target;
   int64_t ignore_index, rows, rows_padded;
-  int reduction;
-  float z_loss, unit;  // unit: what the largest derivative is scaled to
-  float* partial;      // maxima of the blocks of k_ce_largest; NULL: every row has the same g and no z_loss
+  bool per_row;          // g_loss holds one gradient per row
+  float z_loss, unit;    // unit: what the largest derivative is scaled to
+  float* partial;        // maxima of the blocks of k_ce_largest
   int partials;
-  float* row_scale;    // [rows_padded]
-  float* out_scale;    // one float: what the products are multiplied by at the end
+  float* row_scale;      // [rows_padded]
+  float* out_scale;      // one float
 };
 __device__ __forceinline__ float row_gradient(const ScaleArgs& a, int64_t row) {
   if (a.target[row] == a.ignore_index || a.stats[row] == ninf()) return 0.0f;
-  float g = a.g_loss[a.reduction == VSL_REDUCE_NONE ? row : 0];
-  if (a.reduction == VSL_REDUCE_MEAN) g = *a.divisor == 0.0f ? 0.0f : g / *a.divisor;
-  return g;
+  const OutScale g{a.g_loss + (a.per_row ? row : 0), a.divisor, nullptr, 1.0f};
+  return g.gradient();
 }
 __device__ __forceinline__ float block_max(float v, float* red) {
   v = group_all<64>(v, MaxF());
@@ -412,13 +429,7 @@ __global__ __launch_bounds__(kThreads) void k_ce_largest(ScaleArgs a) {
 }
 __global__ __launch_bounds__(kThreads) void k_ce_scale(ScaleArgs a) {
   __shared__ float red[4];
-  float largest;
-  if (a.partial) {
-    largest = block_max((int)threadIdx.x < a.partials ? a.partial[threadIdx.x] : 0.0f, red);
-  } else {
-    largest = fabsf(a.g_loss[0]);
-    if (a.reduction == VSL_REDUCE_MEAN) largest = *a.divisor == 0.0f ? 0.0f : largest / *a.divisor;
-  }
+  const float largest = block_max((int)threadIdx.x < a.partials ? a.partial[threadIdx.x] : 0.0f, red);
   const int64_t r = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   if (r < a.rows_padded) {
     const float g = r < a.rows ? row_gradient(a, r) : 0.0f;
@@ -449,16 +460,24 @@ __global__ __launch_bounds__(kThreads) void k_pad(const T* __restrict__ in, int6
     }
 }
 
-// out [cols, rows_padded] = in^T, zeros behind; a row that cannot contribute (its scale is 0, or its bias is -infinity)
-// reads as zeros, so that a NaN in it does not meet the zero of its derivative.  in: rows the main loop could take.
-template <typename T>
-__device__ __forceinline__ bool contributes(int64_t r, int64_t rows, const float* scale, const T* bias) {
-  return r < rows && !(scale && scale[r] == 0.0f) && !(bias && (float)bias[r] == ninf());
-}
+// out [cols, rows_padded] = in^T, zeros behind; a row that cannot contribute (its target is ignored, no class of it is
+// left, its scale is 0, or, of the weight, its bias is -infinity) reads as zeros, so that a NaN in it does not meet the
+// zero of its derivative.  in: rows the main loop could take.
+struct Contributes {
+  const int64_t* target;
+  const float* stats;
+  const float* scale;
+  const void* bias;
+  int64_t ignore_index;
+  template <typename T>
+  __device__ __forceinline__ bool row(int64_t r) const {
+    if (target && (target[r] == ignore_index || stats[r] == ninf())) return false;
+    return !(scale && scale[r] == 0.0f) && !(bias && (float)((const T*)bias)[r] == ninf());
+  }
+};
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_transpose(const T* __restrict__ in, int64_t stride, int64_t rows, int cols,
-                                                        int64_t rows_padded, const float* __restrict__ scale,
-                                                        const T* __restrict__ bias, T* __restrict__ out) {
+                                                        int64_t rows_padded, Contributes with, T* __restrict__ out) {
   const int64_t tiles_c = (cols + 63) / 64;
   const int64_t r0 = blockIdx.x / tiles_c * 64;
   const int c0 = (int)(blockIdx.x % tiles_c) * 64;
@@ -470,8 +489,8 @@ __global__ __launch_bounds__(kThreads) void k_transpose(const T* __restrict__ in
       const int g = threadIdx.x & 7, rp = threadIdx.x >> 3, c = c0 + 8 * g;
       const int64_t r = r0 + 2 * rp;
       const u32x4 none{0u, 0u, 0u, 0u};
-      const u32x4 x = c < cols && contributes(r, rows, scale, bias) ? *(const u32x4*)(in + r * stride + c) : none;
-      const u32x4 y = c < cols && contributes(r + 1, rows, scale, bias) ? *(const u32x4*)(in + (r + 1) * stride + c) : none;
+      const u32x4 x = c < cols && r < rows && with.row<T>(r) ? *(const u32x4*)(in + r * stride + c) : none;
+      const u32x4 y = c < cols && r + 1 < rows && with.row<T>(r + 1) ? *(const u32x4*)(in + (r + 1) * stride + c) : none;
       unsigned* t = tile + 8 * g * 32 + ((rp + 4 * g) & 31);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -491,7 +510,7 @@ __global__ __launch_bounds__(kThreads) void k_transpose(const T* __restrict__ in
     __shared__ T tile[64][65];
     const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
     for (int i = y; i < 64; i += 4)
-      tile[i][x] = c0 + x < cols && contributes(r0 + i, rows, scale, bias) ? in[(r0 + i) * stride + c0 + x] : (T)0.0f;
+      tile[i][x] = c0 + x < cols && r0 + i < rows && with.row<T>(r0 + i) ? in[(r0 + i) * stride + c0 + x] : (T)0.0f;
     __syncthreads();
     for (int i = y; i < 64; i += 4)
       if (c0 + i < cols) out[(int64_t)(c0 + i) * rows_padded + r0 + x] = tile[x][i];
@@ -508,7 +527,7 @@ struct GradArgs {
   bool whole;              // four features in a row are one aligned store
   float* sum;              // [splits][N][M], or NULL: straight to `out`
   void* out;               // [N][M] of the operands' type
-  const float* out_scale;
+  OutScale scale;
 };
 
 template <typename T, typename S>
@@ -524,7 +543,7 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_grad(GradArgs a) {
   Tile<S> t;
   tile_product<T, S>(a.op, m0, n0, k0, k1, lds, t);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
-  const float scale = a.sum ? 1.0f : *a.out_scale;
+  const float scale = a.sum ? 1.0f : a.scale.get();
 #pragma unroll
   for (int j = 0; j < S::JN; ++j) {
     const int row = n0 + (wn * S::JN + j) * 32 + (lane & 31);
@@ -566,9 +585,9 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_grad(GradArgs a) {
 // out = out_scale * the sum of the splits, in their order: four elements a thread, the splits dealt to the four waves
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_ce_finish(const float* __restrict__ sum, int splits, int64_t n,
-                                                        const float* __restrict__ out_scale, T* __restrict__ out) {
+                                                        OutScale out_scale, T* __restrict__ out) {
   __shared__ f32x4 part[3][64];
-  const float scale = *out_scale;
+  const float scale = out_scale.get();
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int per = (splits + 3) / 4, s0 = wave * per, s1 = min(splits, s0 + per);
   for (int64_t i0 = (int64_t)blockIdx.x * 256; i0 < n; i0 += (int64_t)gridDim.x * 256) {
@@ -598,7 +617,7 @@ __global__ __launch_bounds__(kThreads) void k_ce_finish(const float* __restrict_
 // grad_bias: a block per class sums its row of d^T, the values that grad_weight is made of
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_ce_bias(const T* __restrict__ delta_t, int64_t rows_padded, int64_t rows,
-                                                      const float* __restrict__ out_scale, T* __restrict__ out) {
+                                                      OutScale out_scale, T* __restrict__ out) {
   __shared__ float red[4];
   const T* d = delta_t + (int64_t)blockIdx.x * rows_padded;
   float s = 0.0f;
@@ -609,7 +628,7 @@ __global__ __launch_bounds__(kThreads) void k_ce_bias(const T* __restrict__ delt
     for (int e = 0; e < Kind<T>::E; ++e) s += x[e];
   }
   s = block_add<4>(s, red);
-  if (threadIdx.x == 0) out[blockIdx.x] = (T)(s * *out_scale);
+  if (threadIdx.x == 0) out[blockIdx.x] = (T)(s * out_scale.get());
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -753,10 +772,10 @@ void launch_pad(const void* in, int64_t stride, int64_t rows, int64_t cols, int6
                      (int)cols_padded, (T*)out);
 }
 template <typename T>
-void launch_transpose(const void* in, int64_t stride, int64_t rows, int64_t cols, int64_t rows_padded, const float* scale,
-                      const void* bias, void* out, hipStream_t s) {
+void launch_transpose(const void* in, int64_t stride, int64_t rows, int64_t cols, int64_t rows_padded, const Contributes& with,
+                      void* out, hipStream_t s) {
   hipLaunchKernelGGL(k_transpose<T>, dim3((unsigned)(ceil_div(rows_padded, 64) * ceil_div(cols, 64))), dim3(kThreads), 0, s,
-                     (const T*)in, stride, rows, (int)cols, rows_padded, scale, (const T*)bias, (T*)out);
+                     (const T*)in, stride, rows, (int)cols, rows_padded, with, (T*)out);
 }
 
 template <typename T, typename S, bool DELTA>
@@ -811,35 +830,42 @@ template <typename T>
 void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* stats, const float* divisor, const float* g_loss,
                   T* grad_hidden, T* grad_weight, T* grad_bias, hipStream_t s) {
   const Layout& l = b.l;
-  ScaleArgs sc{};
-  sc.g_loss = g_loss;
-  sc.divisor = divisor;
-  sc.stats = stats;
-  sc.target = d->target;
-  sc.ignore_index = d->ignore_index;
-  sc.rows = d->rows;
-  sc.rows_padded = l.rows_padded;
-  sc.reduction = d->reduction;
-  sc.z_loss = d->z_loss;
-  // float16 keeps 2^-14 as its smallest normal number: with the largest derivative at 2^12 (twice that is the largest
-  // value of a row's sum of two terms) a probability down to 2^-26 of it keeps all its bits
-  sc.unit = sizeof(T) == 2 && !__is_same(T, __bf16) ? 4096.0f : 1.0f;
-  sc.row_scale = b.row_scale;
-  sc.out_scale = b.out_scale;
-  if (d->reduction == VSL_REDUCE_NONE || d->z_loss != 0.0f) {
+  // float16 keeps 2^-14 as its smallest normal number: with the largest gradient at 2^12 (a derivative is at most that) a
+  // probability down to 2^-26 keeps all its bits
+  const float unit = __is_same(T, _Float16) ? 4096.0f : 1.0f;
+  const float* mean_of = d->reduction == VSL_REDUCE_MEAN ? divisor : nullptr;
+  const bool uniform = d->reduction != VSL_REDUCE_NONE && d->z_loss == 0.0f;
+  const float* row_scale = uniform ? nullptr : b.row_scale;
+  const OutScale scale = uniform ? OutScale{g_loss, mean_of, nullptr, unit} : OutScale{nullptr, nullptr, b.out_scale, unit};
+  if (!uniform) {
+    ScaleArgs sc{};
+    sc.g_loss = g_loss;
+    sc.divisor = mean_of;
+    sc.stats = stats;
+    sc.target = d->target;
+    sc.ignore_index = d->ignore_index;
+    sc.rows = d->rows;
+    sc.rows_padded = l.rows_padded;
+    sc.per_row = d->reduction == VSL_REDUCE_NONE;
+    sc.z_loss = d->z_loss;
+    sc.unit = unit;
+    sc.row_scale = b.row_scale;
+    sc.out_scale = b.out_scale;
     const int64_t n = ceil_div(d->rows, kThreads);
     sc.partial = b.largest;
     sc.partials = (int)(n > 256 ? 256 : n);
     hipLaunchKernelGGL(k_ce_largest, dim3(sc.partials), dim3(kThreads), 0, s, sc);
+    hipLaunchKernelGGL(k_ce_scale, dim3((unsigned)ceil_div(l.rows_padded, kThreads)), dim3(kThreads), 0, s, sc);
   }
-  hipLaunchKernelGGL(k_ce_scale, dim3((unsigned)ceil_div(l.rows_padded, kThreads)), dim3(kThreads), 0, s, sc);
   if (l.copy_hidden) launch_pad<T>(d->hidden, d->hidden_stride, d->rows, d->dim, l.dim_padded, b.hidden, s);
   if (l.copy_weight) launch_pad<T>(d->weight, d->weight_stride, d->vocab, d->dim, l.dim_padded, b.weight, s);
   const T* hidden = (const T*)(l.copy_hidden ? b.hidden : d->hidden);
   const T* weight = (const T*)(l.copy_weight ? b.weight : d->weight);
   const int64_t ldh = l.copy_hidden ? l.dim_padded : d->hidden_stride, ldw = l.copy_weight ? l.dim_padded : d->weight_stride;
-  if (grad_weight) launch_transpose<T>(hidden, ldh, d->rows, d->dim, l.rows_padded, b.row_scale, nullptr, b.hidden_t, s);
-  if (grad_hidden) launch_transpose<T>(weight, ldw, d->vocab, d->dim, b.vocab_padded, nullptr, d->bias, b.weight_t, s);
+  if (grad_weight) launch_transpose<T>(hidden, ldh, d->rows, d->dim, l.rows_padded,
+                                        Contributes{d->target, stats, row_scale, nullptr, d->ignore_index}, b.hidden_t, s);
+  if (grad_hidden) launch_transpose<T>(weight, ldw, d->vocab, d->dim, b.vocab_padded,
+                                        Contributes{nullptr, nullptr, nullptr, d->bias, 0}, b.weight_t, s);
   for (int64_t p = 0; p < b.pieces; ++p) {
     const int64_t v0 = p * b.piece, classes = d->vocab - v0 < b.piece ? d->vocab - v0 : b.piece;
     const bool large = large_tiles(classes, d->rows, d->type);
@@ -852,7 +878,9 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
     a.class0 = v0;
     a.rows_padded = l.rows_padded;
     a.stats = stats;
-    a.row_scale = b.row_scale;
+    a.row_scale = row_scale;
+    a.unit = unit;
+    a.ignore_index = d->ignore_index;
     a.z_loss = d->z_loss;
     a.delta = grad_hidden ? b.delta : nullptr;
     a.ldd = b.piece;
@@ -865,7 +893,7 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
       g.add = p > 0;
       g.sum = b.sum_h;
       g.out = grad_hidden;
-      g.out_scale = b.out_scale;
+      g.scale = scale;
       launch_grad<T>(g, d->type, s);
     }
     if (grad_weight) {
@@ -874,19 +902,19 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
       g.splits = b.splits_w;
       g.sum = b.sum_w;
       g.out = grad_weight + v0 * d->dim;
-      g.out_scale = b.out_scale;
+      g.scale = scale;
       launch_grad<T>(g, d->type, s);
       if (g.sum)
         hipLaunchKernelGGL(k_ce_finish<T>, linear_grid(classes * d->dim), dim3(kThreads), 0, s, (const float*)g.sum, g.splits,
-                           classes * d->dim, (const float*)b.out_scale, (T*)g.out);
+                           classes * d->dim, scale, (T*)g.out);
     }
     if (grad_bias)
       hipLaunchKernelGGL(k_ce_bias<T>, dim3((unsigned)classes), dim3(kThreads), 0, s, (const T*)b.delta_t, l.rows_padded,
-                         rows_covered, (const float*)b.out_scale, grad_bias + v0);
+                         rows_covered, scale, grad_bias + v0);
   }
   if (grad_hidden && b.sum_h)
     hipLaunchKernelGGL(k_ce_finish<T>, linear_grid(d->rows * d->dim), dim3(kThreads), 0, s, (const float*)b.sum_h, b.splits_h,
-                       d->rows * d->dim, (const float*)b.out_scale, grad_hidden);
+                       d->rows * d->dim, scale, grad_hidden);
 }
 
 template <typename T>

@@ -35,21 +35,29 @@ class TopLogits(NamedTuple):
     lse: torch.Tensor       # [...], float32: log sum exp(logits / temperature) over the whole vocabulary
 
 
+# The checks below and the calls run once per loss and step; where rows are few they are most of the time (a few
+# microseconds each way), so they ask for whole numbers instead of building torch objects and leave alone what fits.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
 def _floating(t: torch.Tensor, name: str) -> torch.Tensor:
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError("%s must be a GPU tensor (there is no CPU implementation)" % name)
-    if t.dtype == torch.float64:
-        t = t.float()
     if t.dtype not in _TYPES:
-        raise ValueError("%s must be float32, bfloat16 or float16, not %s" % (name, t.dtype))
+        if t.dtype != torch.float64:
+            raise ValueError("%s must be float32, bfloat16 or float16, not %s" % (name, t.dtype))
+        t = t.float()
     return t
 
 
 def _matrix(t: torch.Tensor, name: str) -> torch.Tensor:
     """[..., n] as [rows, n] whose rows may be strided and whose elements are not."""
-    if t.dim() < 1 or t.shape[-1] < 1:
+    if t.dim() != 2:
+        if t.dim() < 1:
+            raise ValueError("%s needs a last dimension of at least 1" % name)
+        t = t.reshape(t.shape[:-1].numel(), t.shape[-1])
+    if t.shape[1] < 1:
         raise ValueError("%s needs a last dimension of at least 1" % name)
-    t = t.reshape(-1, t.shape[-1]) if t.numel() else t.reshape(t.shape[:-1].numel(), t.shape[-1])
     if t.stride(1) != 1 or t.stride(0) < t.shape[1]:
         t = t.contiguous()
     return t
@@ -60,7 +68,7 @@ def _row_stride(t: torch.Tensor) -> int:
 
 
 def _on(t: torch.Tensor, name: str, like: torch.Tensor) -> None:
-    if t.device != like.device:
+    if t.get_device() != like.get_device():
         raise ValueError("%s is on %s, not on %s" % (name, t.device, like.device))
 
 
@@ -71,7 +79,23 @@ def _per_row(t: Optional[torch.Tensor], name: str, shape, like: torch.Tensor) ->
     _on(t, name, like)
     if t.shape != shape:
         raise ValueError("%s must have the shape of the rows, %s, not %s" % (name, tuple(shape), tuple(t.shape)))
-    return t.detach().reshape(-1).float().contiguous()
+    if t.dim() != 1:
+        t = t.reshape(-1)
+    return (t if t.dtype == torch.float32 else t.float()).contiguous()
+
+
+def _once(backward):
+    """once_differentiable without its cost where no second derivative can be asked for."""
+    with_graph = once_differentiable(backward)
+
+    def call(ctx, g):
+        return with_graph(ctx, g) if torch.is_grad_enabled() else backward(ctx, g)
+
+    return call
+
+
+def _differentiable(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def _reduction(name: str) -> int:
@@ -87,16 +111,28 @@ def _temperature(value) -> float:
     return value
 
 
-def _workspace(nbytes: int, like: torch.Tensor) -> Optional[torch.Tensor]:
-    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
+def _bytes(n: int, like: torch.Tensor) -> torch.Tensor:
+    return torch.empty(n, dtype=torch.uint8, device=like.device)
+
+
+def _floats(n: int, like: torch.Tensor) -> torch.Tensor:
+    return torch.empty(n, dtype=torch.float32, device=like.device)
 
 
 def _ptr(t: Optional[torch.Tensor]):
     return t.data_ptr() if t is not None else None
 
 
-def _stream(t: torch.Tensor):
-    return torch.cuda.current_stream(t.device).cuda_stream
+def _run(like: torch.Tensor, call, *args) -> None:
+    """A library call on the current stream of the tensor's device, which need not be the current device."""
+    index = like.get_device()
+    if index == torch.cuda.current_device():
+        rc = call(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = call(*args, _raw_stream(index))
+    if rc:
+        _abi.check(rc)
 
 
 # ------------------------------------------------------------------ top logits
@@ -115,10 +151,9 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLog
     values = torch.empty(shape + (k,), dtype=x.dtype, device=x.device)
     indices = torch.empty(shape + (k,), dtype=torch.int32, device=x.device)
     lse = torch.empty(shape, dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
-        ws = _workspace(_lib.vsl_top_logits_workspace_bytes(ctypes.byref(d)), x)
-        _abi.check(_lib.vsl_top_logits(ctypes.byref(d), values.data_ptr(), indices.data_ptr(), lse.data_ptr(), _ptr(ws),
-                                       ws.numel() if ws is not None else 0, _stream(x)))
+    nbytes = _lib.vsl_top_logits_workspace_bytes(ctypes.byref(d))
+    ws = _bytes(nbytes, x)
+    _run(x, _lib.vsl_top_logits, ctypes.byref(d), values.data_ptr(), indices.data_ptr(), lse.data_ptr(), ws.data_ptr(), nbytes)
     return TopLogits(values, indices, lse)
 
 
@@ -130,35 +165,44 @@ def _distill_desc(x, values, indices, lse, weights, temperature, reduction):
                             teacher_indices=indices.data_ptr(), teacher_lse=_ptr(lse), weights=_ptr(weights))
 
 
+def _distill_forward(x, values, indices, lse, weights, temperature, reduction):
+    """The loss, and what the backward call needs of the rows: statistics and, behind them, the divisor of the mean.  The
+    workspace and, where they are summed, the row losses share that allocation: all are small beside the logits."""
+    rows = x.shape[0]
+    d = _distill_desc(x, values, indices, lse, weights, temperature, reduction)
+    nbytes = _lib.vsl_distill_workspace_bytes(ctypes.byref(d))
+    head = (4 * (_abi.DISTILL_STATS * rows + 1) + 255) // 256 * 256
+    kept = _bytes(head + nbytes + 4 * rows, x)
+    base = kept.data_ptr()
+    if reduction == _abi.REDUCE_NONE:
+        out = _floats(rows, x)
+        _run(x, _lib.vsl_distill_fwd, ctypes.byref(d), out.data_ptr(), None, None, base, base + head, nbytes)
+    else:
+        out = _floats((), x)
+        _run(x, _lib.vsl_distill_fwd, ctypes.byref(d), base + head + nbytes, out.data_ptr(),
+             base + 4 * _abi.DISTILL_STATS * rows, base, base + head, nbytes)
+    return out, kept
+
+
 class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, values, indices, lse, weights, temperature, reduction):
-        rows = x.shape[0]
-        d = _distill_desc(x, values, indices, lse, weights, temperature, reduction)
-        row_loss = torch.empty(rows, dtype=torch.float32, device=x.device)
-        stats = torch.empty(_abi.DISTILL_STATS * rows, dtype=torch.float32, device=x.device)
-        loss = divisor = None
-        if reduction != _abi.REDUCE_NONE:
-            loss, divisor = (torch.empty((), dtype=torch.float32, device=x.device) for _ in range(2))
-        with torch.cuda.device(x.device):
-            ws = _workspace(_lib.vsl_distill_workspace_bytes(ctypes.byref(d)), x)
-            _abi.check(_lib.vsl_distill_fwd(ctypes.byref(d), row_loss.data_ptr(), _ptr(loss), _ptr(divisor), stats.data_ptr(),
-                                            ws.data_ptr(), ws.numel(), _stream(x)))
-        ctx.save_for_backward(x, values, indices, lse, weights, stats, divisor)
+        out, kept = _distill_forward(x, values, indices, lse, weights, temperature, reduction)
+        ctx.save_for_backward(x, values, indices, weights, kept)
         ctx.cfg = (temperature, reduction)
-        return row_loss if loss is None else loss
+        return out
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g):
         # the descriptor is made anew: a saved-tensor hook may have moved what it points to
-        x, values, indices, lse, weights, stats, divisor = ctx.saved_tensors
-        d = _distill_desc(x, values, indices, lse, weights, *ctx.cfg)
-        g = g.float().contiguous()
+        x, values, indices, weights, kept = ctx.saved_tensors
+        d = _distill_desc(x, values, indices, None, weights, *ctx.cfg)
+        g = g.contiguous()
         grad = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        with torch.cuda.device(x.device):
-            _abi.check(_lib.vsl_distill_bwd(ctypes.byref(d), stats.data_ptr(), _ptr(divisor), g.data_ptr(), grad.data_ptr(),
-                                            x.shape[1], _stream(x)))
+        base = kept.data_ptr()
+        _run(x, _lib.vsl_distill_bwd, ctypes.byref(d), base, base + 4 * _abi.DISTILL_STATS * x.shape[0], g.data_ptr(),
+             grad.data_ptr(), x.shape[1])
         return grad, None, None, None, None, None, None
 
 
@@ -174,23 +218,23 @@ def topk_distillation_loss(logits: torch.Tensor, teacher_values: torch.Tensor, t
     probabilities; it is left out of a row where the student has no other class.  ``weights`` [...]: a row of weight 0 is
     not looked at; ``"mean"`` divides by their sum.  The teacher's tensors and the weights carry no gradient."""
     logits = _floating(logits, "logits")
-    values = _floating(teacher_values, "teacher_values").detach()
-    indices = teacher_indices
-    shape = logits.shape[:-1]
+    values, indices, shape = _floating(teacher_values, "teacher_values"), teacher_indices, logits.shape[:-1]
     _on(values, "teacher_values", logits)
     _on(indices, "teacher_indices", logits)
     if indices.dtype not in (torch.int32, torch.int64):
         raise ValueError("teacher_indices must be int32 or int64, not %s" % indices.dtype)
-    if values.shape != indices.shape or values.shape[:-1] != shape or values.dim() < 1:
+    if values.shape != indices.shape or values.dim() < 1 or values.shape[:-1] != shape:
         raise ValueError("teacher_values and teacher_indices must both be [..., k] over the rows of logits")
     x = _matrix(logits, "logits")
     k = values.shape[-1]
     if not 1 <= k <= min(x.shape[1], _abi.MAX_TOP):
         raise ValueError("the teacher's k must lie in 1..min(classes, %d), not %d" % (_abi.MAX_TOP, k))
-    loss = _Distill.apply(x, values.reshape(x.shape[0], k).contiguous(), indices.reshape(x.shape[0], k).contiguous(),
-                          _per_row(teacher_lse, "teacher_lse", shape, logits), _per_row(weights, "weights", shape, logits),
-                          _temperature(temperature), _reduction(reduction))
-    return loss.reshape(shape) if reduction == "none" else loss
+    if values.dim() != 2:
+        values, indices = values.reshape(x.shape[0], k), indices.reshape(x.shape[0], k)
+    args = (x, values.contiguous(), indices.contiguous(), _per_row(teacher_lse, "teacher_lse", shape, logits),
+            _per_row(weights, "weights", shape, logits), _temperature(temperature), _reduction(reduction))
+    loss = _Distill.apply(*args) if _differentiable(x) else _distill_forward(*args)[0]
+    return loss.reshape(shape) if reduction == "none" and len(shape) != 1 else loss
 
 
 # ------------------------------------------------------------------ linear cross entropy
@@ -201,38 +245,46 @@ def _linear_ce_desc(hidden, weight, bias, target, ignore_index, z_loss, reductio
                              bias=_ptr(bias), target=target.data_ptr())
 
 
+def _linear_ce_forward(hidden, weight, bias, target, ignore_index, z_loss, reduction):
+    """The loss, and what the backward call needs of the rows: statistics and, behind them, the divisor of the mean."""
+    d = _linear_ce_desc(hidden, weight, bias, target, ignore_index, z_loss, reduction)
+    rows = hidden.shape[0]
+    kept = _floats(2 * rows + 1, hidden)
+    nbytes = _lib.vsl_linear_ce_fwd_workspace_bytes(ctypes.byref(d))
+    if reduction == _abi.REDUCE_NONE:
+        out, ws = _floats(rows, hidden), _bytes(nbytes, hidden)
+        _run(hidden, _lib.vsl_linear_ce_fwd, ctypes.byref(d), out.data_ptr(), kept.data_ptr(), None, None, ws.data_ptr(), nbytes)
+    else:
+        out, ws = _floats((), hidden), _bytes(nbytes + 4 * rows, hidden)   # the row losses are scratch behind the workspace
+        _run(hidden, _lib.vsl_linear_ce_fwd, ctypes.byref(d), ws.data_ptr() + nbytes, kept.data_ptr(), out.data_ptr(),
+             kept.data_ptr() + 8 * rows, ws.data_ptr(), nbytes)
+    return out, kept
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, bias, target, ignore_index, z_loss, reduction):
-        d = _linear_ce_desc(hidden, weight, bias, target, ignore_index, z_loss, reduction)
-        row_loss = torch.empty(hidden.shape[0], dtype=torch.float32, device=hidden.device)
-        stats = torch.empty(2 * hidden.shape[0], dtype=torch.float32, device=hidden.device)
-        loss = divisor = None
-        if reduction != _abi.REDUCE_NONE:
-            loss, divisor = (torch.empty((), dtype=torch.float32, device=hidden.device) for _ in range(2))
-        with torch.cuda.device(hidden.device):
-            ws = _workspace(_lib.vsl_linear_ce_fwd_workspace_bytes(ctypes.byref(d)), hidden)
-            _abi.check(_lib.vsl_linear_ce_fwd(ctypes.byref(d), row_loss.data_ptr(), stats.data_ptr(), _ptr(loss), _ptr(divisor),
-                                              _ptr(ws), ws.numel() if ws is not None else 0, _stream(hidden)))
-        ctx.save_for_backward(hidden, weight, bias, target, stats, divisor)
+        out, kept = _linear_ce_forward(hidden, weight, bias, target, ignore_index, z_loss, reduction)
+        ctx.save_for_backward(hidden, weight, bias, target, kept)
         ctx.cfg = (ignore_index, z_loss, reduction)
-        return row_loss if loss is None else loss
+        return out
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g):
-        hidden, weight, bias, target, stats, divisor = ctx.saved_tensors
+        hidden, weight, bias, target, kept = ctx.saved_tensors
         d = _linear_ce_desc(hidden, weight, bias, target, *ctx.cfg)   # anew: a saved-tensor hook may have moved them
-        g = g.float().contiguous()
-        grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and ctx.needs_input_grad[i] else None
-                 for i, t in enumerate((hidden, weight, bias))]
-        mask = sum(1 << i for i, t in enumerate(grads) if t is not None)
-        with torch.cuda.device(hidden.device):
-            ws = _workspace(_lib.vsl_linear_ce_bwd_workspace_bytes(ctypes.byref(d), mask), hidden)
-            _abi.check(_lib.vsl_linear_ce_bwd(ctypes.byref(d), stats.data_ptr(), _ptr(divisor), g.data_ptr(),
-                                              _ptr(grads[0]), _ptr(grads[1]), _ptr(grads[2]), _ptr(ws),
-                                              ws.numel() if ws is not None else 0, _stream(hidden)))
-        return grads[0], grads[1], grads[2], None, None, None, None
+        g = g.contiguous()
+        need = ctx.needs_input_grad
+        g_hidden = torch.empty(hidden.shape, dtype=hidden.dtype, device=hidden.device) if need[0] else None
+        g_weight = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) if need[1] else None
+        g_bias = torch.empty(bias.shape, dtype=bias.dtype, device=bias.device) if bias is not None and need[2] else None
+        mask = (g_hidden is not None) | (g_weight is not None) << 1 | (g_bias is not None) << 2
+        nbytes = _lib.vsl_linear_ce_bwd_workspace_bytes(ctypes.byref(d), mask)
+        ws = _bytes(nbytes, hidden)
+        _run(hidden, _lib.vsl_linear_ce_bwd, ctypes.byref(d), kept.data_ptr(), kept.data_ptr() + 8 * hidden.shape[0],
+             g.data_ptr(), _ptr(g_hidden), _ptr(g_weight), _ptr(g_bias), ws.data_ptr(), nbytes)
+        return g_hidden, g_weight, g_bias, None, None, None, None
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor,
@@ -265,7 +317,9 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     z_loss = float(z_loss)
     if not 0.0 <= z_loss <= 1e30:
         raise ValueError("z_loss must be finite and not negative")
-    x = _matrix(hidden, "hidden")
-    loss = _LinearCrossEntropy.apply(x, _matrix(weight, "weight"), bias, target.reshape(-1).long().contiguous(),
-                                     int(ignore_index), z_loss, _reduction(reduction))
-    return loss.reshape(target.shape) if reduction == "none" else loss
+    if target.dim() != 1:
+        target = target.reshape(-1)
+    args = (_matrix(hidden, "hidden"), _matrix(weight, "weight"), bias, target.long().contiguous(), int(ignore_index), z_loss,
+            _reduction(reduction))
+    loss = _LinearCrossEntropy.apply(*args) if _differentiable(*args[:3]) else _linear_ce_forward(*args)[0]
+    return loss.reshape(hidden.shape[:-1]) if reduction == "none" and hidden.dim() != 2 else loss
