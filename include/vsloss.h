@@ -401,7 +401,8 @@ int vsl_depth_metrics(const vsl_depth_metrics_desc* desc, float* metrics, void* 
  *   - an index or target outside the vocabulary (other than ignore_index) is never used as an address: its row's loss
  *     and gradients are NaN;
  *   - results are deterministic: no floating-point atomics, every sum in a fixed order;
- *   - limits: 0 <= rows < 2^31, 1 <= vocab < 2^30, 1 <= k <= min(vocab, VSL_MAX_TOP).  rows == 0 is a valid call.
+ *   - limits: 0 <= rows < 2^31, 1 <= vocab < 2^30, 1 <= k <= min(vocab, VSL_MAX_TOP), 1e-4 <= temperature <= 1e4.
+ *     rows == 0 is a valid call.
  */
 #define VSL_TYPE_F32 0
 #define VSL_TYPE_BF16 1
@@ -441,7 +442,8 @@ int vsl_top_logits(const vsl_top_desc* desc, void* values, int32_t* indices, flo
  * A row of weight 0 is not looked at.  An index that occurs twice counts with the sum of its q.
  *
  * vsl_distill_fwd: row_loss [rows] (weighted); loss and divisor: one float each, the reduced loss and the sum of the
- * weights (both NULL for VSL_REDUCE_NONE); stats: float [VSL_DISTILL_STATS * rows], what the backward call needs.
+ * weights (both NULL for VSL_REDUCE_NONE); stats: float [rows][VSL_DISTILL_STATS], 16-byte aligned, what the
+ * backward call needs.
  * vsl_distill_bwd: g_loss: one float, or [rows] for VSL_REDUCE_NONE -> grad: [rows,vocab] of the logits' type, every
  * element written.  The descriptor is the forward call's; `stats` and `divisor` are its outputs.
  */

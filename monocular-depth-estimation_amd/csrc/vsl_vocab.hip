@@ -105,30 +105,29 @@ __device__ __forceinline__ unsigned ordered32(unsigned b) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ unsigned unordered32(unsigned o) { return o & 0x80000000u ? o & 0x7FFFFFFFu : ~o; }
-__device__ __forceinline__ unsigned ordered16(unsigned b, unsigned inf) {
-  if ((b & 0x7FFFu) > inf) return 0xFFFFu;
-  if (b == 0x8000u) b = 0u;
-  return b & 0x8000u ? ~b & 0xFFFFu : b | 0x8000u;
-}
-__device__ __forceinline__ unsigned unordered16(unsigned o) { return o & 0x8000u ? o & 0x7FFFu : ~o & 0xFFFFu; }
 
-// short rows: value and index share 32 bits for the 16-bit types (an index fits the lower half), 64 for float32
+// Short rows: a 16-bit value as a float has at least 13 zero bits at the end, so value and index share 32 bits; float32
+// takes 64.  make: a NaN has to be a positive one (which orders above +infinity), the callers see to it.
 template <typename T>
 struct RowKey {
   typedef unsigned K;
-  static constexpr unsigned kInf = sizeof(T) == 2 && __is_same(T, __bf16) ? 0x7F80u : 0x7C00u;
-  static __device__ __forceinline__ K make(u32x4 r, int e, int index) {
-    const unsigned b = (r[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
-    return ordered16(b, kInf) << 16 | (0xFFFFu - (unsigned)index);
+  static constexpr unsigned kIndex = 2047u;  // a short row has at most 2048 classes
+  static __device__ __forceinline__ K make(float x, int index) {
+    const unsigned b = __float_as_uint(x + 0.0f);  // -0 ties with +0
+    const unsigned o = b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
+    return (o & ~kIndex) | (kIndex - (unsigned)index);
   }
-  static __device__ __forceinline__ int index(K k) { return (int)(0xFFFFu - (k & 0xFFFFu)); }
-  static __device__ __forceinline__ T value(K k) { return __builtin_bit_cast(T, (unsigned short)unordered16(k >> 16)); }
+  static __device__ __forceinline__ int index(K k) { return (int)(kIndex - (k & kIndex)); }
+  static __device__ __forceinline__ T value(K k) {
+    const unsigned o = k & ~kIndex;
+    return (T)__uint_as_float((o & 0x80000000u ? o & 0x7FFFFFFFu : ~o) & ~kIndex);
+  }
 };
 template <>
 struct RowKey<float> {
   typedef unsigned long long K;
-  static __device__ __forceinline__ K make(u32x4 r, int e, int index) {
-    return (unsigned long long)ordered32(r[e]) << 32 | (0xFFFFFFFFu - (unsigned)index);
+  static __device__ __forceinline__ K make(float x, int index) {
+    return (unsigned long long)ordered32(__float_as_uint(x)) << 32 | (0xFFFFFFFFu - (unsigned)index);
   }
   static __device__ __forceinline__ int index(K k) { return (int)(0xFFFFFFFFu - (unsigned)k); }
   static __device__ __forceinline__ float value(K k) { return __uint_as_float(unordered32((unsigned)(k >> 32))); }
@@ -149,7 +148,26 @@ struct TopArgs {
   float c, inv_t;            // log2(e) / temperature, 1 / temperature
 };
 
-// Short rows: L lanes hold NV vectors each.  Every round takes the group's largest key and removes it.
+// A lane's own keys, larger first: the odd-even merge network, N a power of two.
+template <int N, typename K>
+__device__ __forceinline__ void sort_own(K (&key)[N]) {
+#pragma unroll
+  for (int p = 1; p < N; p <<= 1)
+#pragma unroll
+    for (int q = p; q >= 1; q >>= 1)
+#pragma unroll
+      for (int j = q % p; j + q < N; j += 2 * q)
+#pragma unroll
+        for (int i = 0; i < q; ++i)
+          if (i + j + q < N && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+            const K a = key[i + j], b = key[i + j + q];
+            key[i + j] = a > b ? a : b;
+            key[i + j + q] = a > b ? b : a;
+          }
+}
+
+// Short rows: L lanes hold NV vectors each.  Every lane sorts its keys; every round takes the largest of the group's first
+// ones, and its lane moves on to its next.
 template <typename T, int L, int NV>
 __global__ __launch_bounds__(kThreads) void k_top_rows(TopArgs a) {
   constexpr int E = Vec<T>::E, G = kThreads / L;
@@ -159,38 +177,47 @@ __global__ __launch_bounds__(kThreads) void k_top_rows(TopArgs a) {
     const int64_t row = r0 + threadIdx.x / L;
     const bool live = row < a.rows;  // whole groups: the lanes of a group agree
     const T* x = (const T*)a.logits + (live ? row : 0) * a.stride;
-    K key[NV * E];
-    MaxSum t{ninf(), 0.0f};
     float xs[NV][E];
+    MaxSum t{ninf(), 0.0f};
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int i = (v * L + lane) * E;
-      u32x4 r = load_row(x, i, i < a.V ? a.V : i);
-      unpack(r, xs[v], (const T*)nullptr);
+      unpack(load_row(x, i, i < a.V ? a.V : i), xs[v], (const T*)nullptr);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        key[v * E + e] = i + e < a.V ? RowKey<T>::make(r, e, i + e) : (K)0;
-        t.m = __builtin_elementwise_maximum(t.m, xs[v][e]);
-      }
+      for (int e = 0; e < E; ++e) t.m = __builtin_elementwise_maximum(t.m, xs[v][e]);
     }
-    if (a.lse) {
-      t.m = group_all<L>(t.m, MaxF());
-      const float ref = exp_ref(t.m);
+    if (__any(t.m != t.m)) {
 #pragma unroll
       for (int v = 0; v < NV; ++v)
 #pragma unroll
-        for (int e = 0; e < E; ++e) t.s += exp_of(xs[v][e], ref, a.c);
+        for (int e = 0; e < E; ++e) xs[v][e] = xs[v][e] != xs[v][e] ? qnan() : xs[v][e];
+    }
+    K key[NV * E];
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int i = (v * L + lane) * E + e;
+        key[v * E + e] = i < a.V ? RowKey<T>::make(xs[v][e], i) : (K)0;
+      }
+    if (a.lse) {
+      t.m = group_all<L>(t.m, MaxF());
+      const Exponent ex(exp_ref(t.m), a.c);
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int e = 0; e < E; ++e) t.s += ex(xs[v][e]);
       t.s = group_all<L>(t.s, AddF());
       if (live && lane == 0) a.lse[row] = log_sum(t, a.inv_t);
     }
+    sort_own<NV * E>(key);
     K mine = 0;
     for (int j = 0; j < a.k; ++j) {
-      K best = 0;
+      const K best = group_all<L>(key[0], MaxU());
+      const bool taken = key[0] == best;  // by one lane: no key occurs twice, and 0 follows the last
 #pragma unroll
-      for (int e = 0; e < NV * E; ++e) best = best > key[e] ? best : key[e];
-      best = group_all<L>(best, MaxU());
-#pragma unroll
-      for (int e = 0; e < NV * E; ++e) key[e] = key[e] == best ? (K)0 : key[e];
+      for (int e = 0; e < NV * E - 1; ++e) key[e] = taken ? key[e + 1] : key[e];
+      key[NV * E - 1] = taken ? (K)0 : key[NV * E - 1];
       if (j % L == lane) mine = best;
       if ((j % L == L - 1 || j == a.k - 1) && live && lane <= j % L) {
         const int64_t at = row * a.k + j - j % L + lane;
@@ -201,11 +228,13 @@ __global__ __launch_bounds__(kThreads) void k_top_rows(TopArgs a) {
   }
 }
 
-// Long rows.  A key is (ordered value, ~index).  The k-th largest of the 256 threads' maxima over the first tile is a
-// bound that at least k elements reach; the elements that do are collected, and whenever more than kTrigger are there the
-// k largest of them are kept and the bound rises to the k-th.
-constexpr int kTrigger = 512;
-constexpr int kBuffer = 4096;  // kTrigger + one tile of at most kThreads * 8 elements, as a power of two for the sort
+// Long rows, kGroup vectors a thread at a time, the next ones under way meanwhile.  A key is (ordered value, ~index).
+// The k-th largest of the 256 threads' maxima over the first group is a bound that at least k elements reach; the elements
+// that do are collected, and whenever more than kTrigger are there the k largest of them are kept and the bound rises to
+// the k-th.  A group of which more passes than the buffer holds (rising rows) is collected again, vector by vector.
+constexpr int kGroup = 2;
+constexpr int kTrigger = 512;  // at most; see trigger below
+constexpr int kBuffer = 4096;  // kTrigger + one vector of each thread, as a power of two for the sort
 static_assert(kTrigger + kThreads * 8 <= kBuffer && VSL_MAX_TOP <= kTrigger, "candidate buffer");
 
 // Bitonic sort, larger first, of n = 2^p keys in LDS.
@@ -238,9 +267,40 @@ __device__ __forceinline__ float key_floor(unsigned long long key) {
   return o == 0u ? ninf() : o > 0xFF800000u ? __uint_as_float(0x7F800000u) : __uint_as_float(unordered32(o));
 }
 
+// N vectors of a thread, kThreads vectors apart
+template <typename T, int N>
+__device__ __forceinline__ void load_group(const T* x, int i0, int end, u32x4 (&r)[N]) {
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    const int i = i0 + (u * kThreads + (int)threadIdx.x) * Vec<T>::E;
+    r[u] = load_row(x, i, i < end ? end : i);
+  }
+}
+// running maximum and sum over a group; returns the group's maximum
+template <typename T, int N>
+__device__ __forceinline__ float add_group(const float (&v)[N][Vec<T>::E], MaxSum& t, float c) {
+  float top = v[0][0];
+#pragma unroll
+  for (int u = 0; u < N; ++u)
+#pragma unroll
+    for (int e = 0; e < Vec<T>::E; ++e) top = __builtin_elementwise_maximum(top, v[u][e]);
+  const float m = __builtin_elementwise_maximum(t.m, top), ref = exp_ref(m);
+  const Exponent ex(ref, c);
+  float s = t.s * exp_of(t.m, ref, c), s2 = 0.0f;
+#pragma unroll
+  for (int u = 0; u < N; ++u)
+#pragma unroll
+    for (int e = 0; e < Vec<T>::E; e += 2) {
+      s += ex(v[u][e]);
+      s2 += ex(v[u][e + 1]);
+    }
+  t = {m, s + s2};
+  return top;
+}
+
 template <typename T>
-__global__ __launch_bounds__(kThreads) void k_top_stream(TopArgs a) {
-  constexpr int E = Vec<T>::E, kTile = kThreads * E;
+__global__ __launch_bounds__(kThreads, 4) void k_top_stream(TopArgs a) {
+  constexpr int E = Vec<T>::E, kSpan = kThreads * E * kGroup;
   __shared__ unsigned long long buf[kBuffer];
   __shared__ int count;
   __shared__ float red[2 * kWaves];
@@ -254,27 +314,51 @@ __global__ __launch_bounds__(kThreads) void k_top_stream(TopArgs a) {
     MaxSum t{ninf(), 0.0f};
     unsigned long long bound = 0;
     float floor_value = ninf();
-    for (int i0 = e0; i0 < e1; i0 += kTile) {
-      const int i = i0 + tid * E;
-      float v[E];
-      const u32x4 r = load_row(x, i, i < e1 ? e1 : i);
-      unpack(r, v, (const T*)nullptr);
-      float top = v[0];
+    int kept = 0;  // keys in the buffer, as every thread knows it
+    const int trigger = min(kTrigger, a.k + 128);  // sorting 256 keys is cheaper than collecting by a loose bound
+    auto key_of = [&](float v, int i) {
+      return (unsigned long long)ordered32(__float_as_uint(v)) << 32 | (0xFFFFFFFFu - (unsigned)i);
+    };
+    auto collect = [&](const float (&v)[E], int i) {
 #pragma unroll
-      for (int e = 1; e < E; ++e) top = __builtin_elementwise_maximum(top, v[e]);
-      const float m = __builtin_elementwise_maximum(t.m, top), ref = exp_ref(m);
-      float s = t.s * exp_of(t.m, ref, a.c);
+      for (int e = 0; e < E; ++e)
+        if (!(v[e] < floor_value)) {  // few lanes, and soon hardly any
+          const unsigned long long key = key_of(v[e], i + e);
+          if (key >= bound && i + e < e1) {
+            const int at = atomicAdd(&count, 1);
+            if (at < kBuffer) buf[at] = key;
+          }
+        }
+    };
+    auto settle = [&]() {  // everyone has collected: take the count, keep the k largest if there are many
+      __syncthreads();
+      kept = count;
+      __syncthreads();
+      if (kept <= trigger || kept > kBuffer) return;
+      sort_count(buf, kept);
+      bound = buf[a.k - 1] + 1;  // its element is kept: later ones have to be above it
+      floor_value = key_floor(bound);
+      if (tid == 0) count = a.k;
+      kept = a.k;
+      __syncthreads();
+    };
+    u32x4 next[kGroup];
+    load_group(x, e0, e1, next);
+    for (int i0 = e0; i0 < e1; i0 += kSpan) {
+      float v[kGroup][E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) s += exp_of(v[e], ref, a.c);
-      t = {m, s};
+      for (int u = 0; u < kGroup; ++u) unpack(next[u], v[u], (const T*)nullptr);
+      if (i0 + kSpan < e1) load_group(x, i0 + kSpan, e1, next);
+      const float top = add_group<T>(v, t, a.c);
       if (i0 == e0) {
         unsigned long long best = 0;
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (i + e < e1) {
-            const unsigned long long key =
-                (unsigned long long)ordered32(__float_as_uint(v[e])) << 32 | (0xFFFFFFFFu - (unsigned)(i + e));
-            best = best > key ? best : key;
+        for (int u = 0; u < kGroup; ++u)
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const int i = i0 + (u * kThreads + tid) * E + e;
+            const unsigned long long key = key_of(v[u][e], i);
+            if (i < e1 && key > best) best = key;
           }
         buf[tid] = best;
         if (tid == 0) count = 0;
@@ -283,33 +367,22 @@ __global__ __launch_bounds__(kThreads) void k_top_stream(TopArgs a) {
         floor_value = key_floor(bound);
         __syncthreads();
       }
-      if (__any(!(top < floor_value))) {
+      const int before = kept;
+      if (__any(!(top < floor_value)))
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const bool maybe = !(v[e] < floor_value) && i + e < e1;
-          if (__ballot(maybe) == 0) continue;
-          const unsigned long long key =
-              (unsigned long long)ordered32(__float_as_uint(v[e])) << 32 | (0xFFFFFFFFu - (unsigned)(i + e));
-          const bool pass = maybe && key >= bound;
-          const unsigned long long who = __ballot(pass);
-          if (who == 0) continue;
-          int base = 0;
-          if ((tid & 63) == __ffsll((unsigned long long)who) - 1) base = atomicAdd(&count, __popcll(who));
-          base = __builtin_amdgcn_readlane(base, __ffsll((unsigned long long)who) - 1);
-          if (pass) buf[base + __popcll(who & ((1ull << (tid & 63)) - 1))] = key;
+        for (int u = 0; u < kGroup; ++u) collect(v[u], i0 + (u * kThreads + tid) * E);
+      settle();
+      if (kept > kBuffer) {
+        if (tid == 0) count = before;
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < kGroup; ++u) {
+          collect(v[u], i0 + (u * kThreads + tid) * E);
+          settle();
         }
       }
-      __syncthreads();
-      const int n = count;
-      if (n > kTrigger) {
-        sort_count(buf, n);
-        bound = buf[a.k - 1] + 1;  // its element is kept: later ones have to be above it
-        floor_value = key_floor(bound);
-        if (tid == 0) count = a.k;
-      }
-      __syncthreads();
     }
-    const int n = count;
+    const int n = kept;
     sort_count(buf, n);
     if (a.lse || a.segs > 1) t = block_join<kWaves>(t, red, a.c);
     if (a.segs > 1) {
@@ -396,8 +469,8 @@ int check_top(const vsl_top_desc* d) {
   if (int rc = check_matrix("top_logits", d->rows, d->vocab, d->stride, d->type)) return rc;
   if (d->k < 1 || d->k > VSL_MAX_TOP || d->k > d->vocab)
     return fail(VSL_ERR_INVALID_ARGUMENT, "top_logits: need 1 <= k <= min(vocab, 256)");
-  if (!(d->temperature > 0.0f) || d->temperature > 1e30f || d->temperature < 1e-30f)
-    return fail(VSL_ERR_INVALID_ARGUMENT, "top_logits: temperature must be positive and finite");
+  if (!(d->temperature >= 1e-4f && d->temperature <= 1e4f))
+    return fail(VSL_ERR_INVALID_ARGUMENT, "top_logits: temperature must lie in 1e-4..1e4");
   return VSL_OK;
 }
 
@@ -428,7 +501,7 @@ struct DistillArgs {
   const float* lse;
   const float* weights;
   float* row_loss;
-  float* stats;        // planes of `rows`, RowStats
+  float* stats;        // [rows] of RowStats
   float* partial;      // [rows][segs][2], stream only
   const float* divisor;  // backward: of the mean
   const float* g_loss;
@@ -456,7 +529,12 @@ __device__ __forceinline__ int teacher_index(const DistillArgs& a, int64_t at) {
 struct LogQ {
   float hi, lo;
   __device__ __forceinline__ float log() const { return hi + lo; }
-  __device__ __forceinline__ float q() const { return hi == ninf() ? 0.0f : expf(hi) * (1.0f + lo); }
+  __device__ __forceinline__ float q() const {
+    // hi log2(e) in two floats as well: 2^p (1 + the rest)
+    const float p = __fmul_rn(hi, kLog2e), pe = fmaf(hi, kLog2e, -p);
+    const float rest = fmaf(fmaf(hi, kLog2eLow, pe), kLn2, lo), e = __builtin_amdgcn_exp2f(p);
+    return hi == ninf() ? 0.0f : fmaf(e, rest, e);
+  }
 };
 struct TeacherSum {
   float base, log_sum;  // lse and 0 where it is given; the largest value / T and the log of the sum above it otherwise
@@ -487,15 +565,14 @@ struct RowStats {
   float qt, total;    // the teacher's rest; sum of all q
   TeacherSum teacher;
   __device__ __forceinline__ void store(const DistillArgs& a, int64_t row) const {
-    const float v[VSL_DISTILL_STATS] = {m, ls, tm, tls, qt, total, teacher.base, teacher.log_sum};
-#pragma unroll
-    for (int p = 0; p < VSL_DISTILL_STATS; ++p) a.stats[p * a.rows + row] = v[p];
+    f32x4* p = (f32x4*)(a.stats + row * VSL_DISTILL_STATS);
+    p[0] = f32x4{m, ls, tm, tls};
+    p[1] = f32x4{qt, total, teacher.base, teacher.log_sum};
   }
   __device__ __forceinline__ void load(const DistillArgs& a, int64_t row) {
-    float v[VSL_DISTILL_STATS];
-#pragma unroll
-    for (int p = 0; p < VSL_DISTILL_STATS; ++p) v[p] = a.stats[p * a.rows + row];
-    m = v[0], ls = v[1], tm = v[2], tls = v[3], qt = v[4], total = v[5], teacher = {v[6], v[7]};
+    const f32x4* p = (const f32x4*)(a.stats + row * VSL_DISTILL_STATS);
+    const f32x4 u = p[0], v = p[1];
+    m = u[0], ls = u[1], tm = u[2], tls = u[3], qt = v[0], total = v[1], teacher = {v[2], v[3]};
   }
   __device__ __forceinline__ bool dead() const { return m == __uint_as_float(0x7F800000u); }
   __device__ __forceinline__ float p(float x, float c) const { return __builtin_amdgcn_exp2f(fmaf(x - m, c, -ls)); }
@@ -520,158 +597,267 @@ __device__ __forceinline__ float finish_row(RowStats& st, float cross, float mas
     st.tm = rest.m;
     st.tls = log2_sum(rest);
     st.qt = fmaxf(0.0f, 1.0f - mass);
-    if (st.qt > 0.0f) cross += st.qt * (logf(st.qt) - st.log2_rest(c) * kLn2);
+    if (st.qt > 0.0f) cross += st.qt * (__builtin_amdgcn_logf(st.qt) - st.log2_rest(c)) * kLn2;
     st.total = mass + st.qt;
   }
   return cross;
 }
 
-// Short rows: L lanes hold NV vectors each; q is scattered into an LDS table of the row, -1 where a class is not the
-// teacher's.
-template <typename T, int L, int NV, bool GRAD>
-__global__ __launch_bounds__(kThreads) void k_distill_rows(DistillArgs a) {
-  constexpr int E = Vec<T>::E, G = kThreads / L, W = L * NV * E;
-  __shared__ float table[G][W];
-  const int lane = threadIdx.x % L, group = threadIdx.x / L;
-  float* tab = table[group];
-  const unsigned long long members = (~0ull >> (64 - L)) << (((threadIdx.x & 63) / L) * L);
-  for (int64_t r0 = (int64_t)blockIdx.x * G; r0 < a.rows; r0 += (int64_t)gridDim.x * G) {
-    const int64_t row = r0 + group;
-    const bool live = row < a.rows;
-    const float w = !live ? 0.0f : a.weights ? a.weights[row] : 1.0f;
-    const T* x = (const T*)a.logits + row * a.stride;
-    RowStats st = dead_row();
-    if (GRAD && live) st.load(a, row);
-    const bool skip = w == 0.0f || (GRAD && st.dead());  // the lanes of a group agree
-    float xs[NV][E];
+// Marks the teacher's classes of a short row in a bit map of LDS (one bit a class, WORDS words a row); true for the one
+// that finds its class marked already.  A wave's LDS operations run in order, so that no barrier is needed within it.
+template <int L, int WORDS>
+__device__ __forceinline__ void clear_marks(unsigned* marks, int lane) {
+  __builtin_amdgcn_wave_barrier();
+  for (int w = lane; w < WORDS; w += L) marks[w] = 0u;
+  __builtin_amdgcn_wave_barrier();
+}
+__device__ __forceinline__ bool mark(unsigned* marks, int at) {
+  const unsigned bit = 1u << (at & 31);
+  return atomicOr(&marks[at >> 5], bit) & bit;
+}
+
+// What a group of L lanes holds of a short row: NV vectors each, and lane j the teacher's entry j (further ones are read
+// when their turn comes).  All of it is asked for at once, a turn of the loop ahead: a row is little work, and one that
+// waited for its weight before its logits, and for those before the next row, would spend its time on latency (measured
+// at 1474560 rows of 128: 250 us where the traffic takes 80).
+template <typename T, int L, int NV>
+struct ShortRow {
+  u32x4 x[NV];
+  float weight = 0.0f, lse = 0.0f, value = 0.0f, g = 0.0f;
+  int at = -1;
+  RowStats st;
+  template <bool GRAD>
+  __device__ __forceinline__ void load(const DistillArgs& a, int64_t row, int lane) {
+    if (row >= a.rows) {  // whole groups: the row stays unwritten
+#pragma unroll
+      for (int v = 0; v < NV; ++v) x[v] = u32x4{0u, 0u, 0u, 0u};
+      weight = 0.0f;
+      return;
+    }
+    const T* p = (const T*)a.logits + row * a.stride;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int i = (v * L + lane) * E;
-      const u32x4 r = load_row(x, i, skip ? i : i < a.V ? a.V : i);
-      unpack(r, xs[v], (const T*)nullptr);
+      const int i = (v * L + lane) * Vec<T>::E;
+      x[v] = load_row(p, i, i < a.V ? a.V : i);
+    }
+    weight = a.weights ? a.weights[row] : 1.0f;
+    at = lane < a.k ? teacher_index(a, row * a.k + lane) : -1;
+    value = lane < a.k ? teacher_value(a, row * a.k + lane) : ninf();
+    if (GRAD) {
+      st.load(a, row);
+      g = a.g_loss[a.reduction == VSL_REDUCE_NONE ? row : 0];
+    } else if (a.lse) {
+      lse = a.lse[row];
+    }
+  }
+  // f(entry, class or -1, value) for the lane's entries of the teacher
+  template <typename F>
+  __device__ __forceinline__ void each(const DistillArgs& a, int64_t row, int lane, int k, F f) const {
+    if (lane < k) f(lane, at, value);
+    for (int j = lane + L; j < k; j += L) f(j, teacher_index(a, row * a.k + j), teacher_value(a, row * a.k + j));
+  }
+};
+constexpr int kResident = 2048;  // blocks of 256 threads that 256 CUs hold: what walks short rows
+
+template <typename T, int L, int NV>
+__global__ __launch_bounds__(kThreads) void k_distill_rows(DistillArgs a) {
+  constexpr int E = Vec<T>::E, G = kThreads / L, W = L * NV * E;
+  __shared__ unsigned marks_of[G][W / 32];
+  __shared__ __attribute__((aligned(16))) T lines[G][W];
+  const int lane = threadIdx.x % L, group = threadIdx.x / L;
+  unsigned* marks = marks_of[group];
+  T* line = lines[group];
+  const unsigned long long members = (~0ull >> (64 - L)) << (((threadIdx.x & 63) / L) * L);
+  const int64_t step = (int64_t)gridDim.x * G;
+  ShortRow<T, L, NV> next;
+  next.template load<false>(a, (int64_t)blockIdx.x * G + group, lane);
+  for (int64_t r0 = (int64_t)blockIdx.x * G; r0 < a.rows; r0 += step) {
+    const int64_t row = r0 + group;
+    const ShortRow<T, L, NV> in = next;
+    if (r0 + step < a.rows) next.template load<false>(a, row + step, lane);
+    const bool skip = in.weight == 0.0f;  // the lanes of a group agree
+    const int k = skip ? 0 : a.k;
+    float xs[NV][E];
+    MaxSum all{ninf(), 0.0f}, rest{ninf(), 0.0f};
+    clear_marks<L, W / 32>(marks, lane);
 #pragma unroll
-      for (int e = 0; e < E; e += 4) *(f32x4*)&tab[i + e] = f32x4{-1.0f, -1.0f, -1.0f, -1.0f};
+    for (int v = 0; v < NV; ++v) {
+      *(u32x4*)(line + (v * L + lane) * E) = in.x[v];
+      unpack(in.x[v], xs[v], (const T*)nullptr);
+#pragma unroll
+      for (int e = 0; e < E; ++e) all.m = __builtin_elementwise_maximum(all.m, xs[v][e]);
     }
     __builtin_amdgcn_wave_barrier();
-    // the teacher
-    TeacherSum teacher{0.0f, 0.0f};
-    const int k = skip ? 0 : a.k;
-    if (GRAD) {
-      teacher = st.teacher;
-    } else if (a.lse) {
-      if (!skip) teacher.base = a.lse[row];
-    } else {
+    TeacherSum teacher{in.lse, 0.0f};
+    if (!a.lse) {
       MaxSum t{ninf(), 0.0f};
-      for (int j = lane; j < k; j += L) t.m = __builtin_elementwise_maximum(t.m, teacher_value(a, row * a.k + j));
+      in.each(a, row, lane, k, [&](int, int, float v) { t.m = __builtin_elementwise_maximum(t.m, v); });
       t.m = group_all<L>(t.m, MaxF());
       const float ref = exp_ref(t.m);
-      for (int j = lane; j < k; j += L) t.s += exp_of(teacher_value(a, row * a.k + j), ref, a.c);
+      in.each(a, row, lane, k, [&](int, int, float v) { t.s += exp_of(v, ref, a.c); });
       t.s = group_all<L>(t.s, AddF());
       teacher = {t.m * a.ih, log2_sum(t) * kLn2};
     }
+    all.m = group_all<L>(all.m, MaxF());
+    const float ref = exp_ref(all.m);
     bool bad = false, twice = false;
-    float mass = 0.0f, cross = 0.0f;
-    for (int j = lane; j < k; j += L) {
-      const int at = teacher_index(a, row * a.k + j);
-      const LogQ lq = log_q(a, teacher_value(a, row * a.k + j), teacher);
+    float mass = 0.0f, cross = 0.0f, seen = 0.0f;
+    in.each(a, row, lane, k, [&](int, int at, float v) {
+      const LogQ lq = log_q(a, v, teacher);
       const float q = lq.q();
       mass += q;
-      if (q != 0.0f) cross += q * lq.log();
       bad |= at < 0;
-      if (at >= 0) twice |= atomicExch(&tab[at], q) != -1.0f;
-    }
-    __builtin_amdgcn_wave_barrier();
-    if (__ballot(twice) & members) {  // an index occurs twice: one lane sums its q in the teacher's order
-      for (int j = lane; j < k; j += L) {
-        const int at = teacher_index(a, row * a.k + j);
-        if (at >= 0) tab[at] = -1.0f;
-      }
-      __builtin_amdgcn_wave_barrier();
-      if (lane == 0)
-        for (int j = 0; j < k; ++j) {
-          const int at = teacher_index(a, row * a.k + j);
-          const float q = log_q(a, teacher_value(a, row * a.k + j), teacher).q();
-          if (at >= 0) tab[at] = (tab[at] == -1.0f ? 0.0f : tab[at]) + q;
-        }
-      __builtin_amdgcn_wave_barrier();
-    }
+      if (at < 0) return;
+      const float z = (float)line[at] - ref;
+      if (q != 0.0f) cross += q * (lq.log() - z * a.ih);
+      if (mark(marks, at)) twice = true;
+      else seen += __builtin_amdgcn_exp2f(z * a.c);  // a class counts once
+    });
     bad = (__ballot(bad) & members) != 0;
-    float q[NV][E];
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
-#pragma unroll
-      for (int e = 0; e < E; e += 4) {
-        const f32x4 t = *(const f32x4*)&tab[(v * L + lane) * E + e];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) q[v][e + u] = t[u];
-      }
+    if (__ballot(twice) & members) {  // which entry came first is not the hardware's to say: the first in the teacher's order
+      seen = 0.0f;
+      in.each(a, row, lane, k, [&](int j, int at, float) {
+        bool first = at >= 0;
+        for (int u = 0; u < j && first; ++u) first = teacher_index(a, row * a.k + u) != at;
+        if (first) seen += exp_of((float)line[at], ref, a.c);
+      });
+    }
     __builtin_amdgcn_wave_barrier();
-    if (!GRAD) {
-      MaxSum all{ninf(), 0.0f}, rest{ninf(), 0.0f};
+    if (a.lse) {  // the other classes alone: the teacher's become -infinity in the line, which is read again
+      in.each(a, row, lane, k, [&](int, int at, float) {
+        if (at >= 0) line[at] = (T)ninf();
+      });
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int v = 0; v < NV; ++v) unpack(*(const u32x4*)(line + (v * L + lane) * E), xs[v], (const T*)nullptr);
+    }
+    auto sum_from = [&](float base) {
+      const Exponent ex(base, a.c);
+      float s = 0.0f, s2 = 0.0f;
 #pragma unroll
       for (int v = 0; v < NV; ++v)
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          all.m = __builtin_elementwise_maximum(all.m, xs[v][e]);
-          if (q[v][e] == -1.0f) rest.m = __builtin_elementwise_maximum(rest.m, xs[v][e]);
+        for (int e = 0; e < E; e += 2) {
+          s += ex(xs[v][e]);
+          s2 += ex(xs[v][e + 1]);
         }
-      all.m = group_all<L>(all.m, MaxF());
-      rest.m = group_all<L>(rest.m, MaxF());
-      // the other classes from their own maximum: they may lie far below the teacher's
-      const float ref = exp_ref(all.m), rest_ref = exp_ref(rest.m);
+      return group_all<L>(s + s2, AddF());
+    };
+    const float s = sum_from(ref);
+    if (a.lse) {
+      all.s = group_all<L>(seen, AddF()) + s;
+      rest = {s == 0.0f ? ninf() : all.m, s};
+      if (__any(s < 1e-20f)) {  // far below the teacher's classes: their sum from their own maximum
+        float m = ninf();
 #pragma unroll
-      for (int v = 0; v < NV; ++v)
+        for (int v = 0; v < NV; ++v)
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float qe = q[v][e];
-          const bool member = qe != -1.0f;
-          const float ex = exp_of(xs[v][e], member ? ref : rest_ref, a.c);
-          all.s += member ? ex : 0.0f;
-          rest.s += member ? 0.0f : ex;
-          if (member && qe != 0.0f) cross -= qe * ((xs[v][e] - ref) * a.ih);
-        }
-      all.s = group_all<L>(all.s, AddF()) + (rest.s = group_all<L>(rest.s, AddF())) * exp_of(rest.m, ref, a.c);
-      cross = group_all<L>(cross, AddF());
-      mass = group_all<L>(mass, AddF());
-      st.m = all.m;
-      st.ls = log2_sum(all);
-      st.teacher = teacher;
-      float loss = finish_row(st, cross + mass * (st.ls * kLn2), mass, a.lse != nullptr, rest, a.c) * a.temperature *
-                   a.temperature * w;
-      if (st.ls != st.ls) st.poison();  // NaN or +infinity among the logits
-      if (skip || teacher.base == ninf() || st.m == ninf()) {
-        st = dead_row();
-        loss = 0.0f;
+          for (int e = 0; e < E; ++e) m = __builtin_elementwise_maximum(m, xs[v][e]);
+        rest.m = group_all<L>(m, MaxF());
+        rest.s = sum_from(exp_ref(rest.m));
       }
-      if (bad) {
-        st.poison();
-        loss = qnan();
+    } else {
+      all.s = s;
+    }
+    cross = group_all<L>(cross, AddF());
+    mass = group_all<L>(mass, AddF());
+    RowStats st;
+    st.m = all.m;
+    st.ls = log2_sum(all);
+    st.teacher = teacher;
+    float loss = finish_row(st, cross + mass * (st.ls * kLn2), mass, a.lse != nullptr, rest, a.c) * a.temperature *
+                 a.temperature * in.weight;
+    if (st.ls != st.ls) st.poison();  // NaN or +infinity among the logits
+    if (skip || teacher.base == ninf() || st.m == ninf()) {
+      st = dead_row();
+      loss = 0.0f;
+    }
+    if (bad) {
+      st.poison();
+      loss = qnan();
+    }
+    if (row < a.rows && lane == 0) {
+      st.store(a, row);
+      a.row_loss[row] = loss;
+    }
+  }
+}
+
+// The gradient of a short row: every class as if it were not the teacher's goes to an LDS line, the teacher's entries
+// overwrite theirs there, and the line goes out.
+template <typename T, int L, int NV>
+__global__ __launch_bounds__(kThreads) void k_distill_rows_grad(DistillArgs a) {
+  constexpr int E = Vec<T>::E, G = kThreads / L, W = L * NV * E;
+  __shared__ unsigned marks_of[G][W / 32];
+  __shared__ __attribute__((aligned(16))) T lines[G][W];
+  const int lane = threadIdx.x % L, group = threadIdx.x / L;
+  unsigned* marks = marks_of[group];
+  T* line = lines[group];
+  const unsigned long long members = (~0ull >> (64 - L)) << (((threadIdx.x & 63) / L) * L);
+  const int64_t step = (int64_t)gridDim.x * G;
+  const float divisor = a.reduction == VSL_REDUCE_MEAN ? *a.divisor : 1.0f;
+  ShortRow<T, L, NV> next;
+  next.template load<true>(a, (int64_t)blockIdx.x * G + group, lane);
+  for (int64_t r0 = (int64_t)blockIdx.x * G; r0 < a.rows; r0 += step) {
+    const int64_t row = r0 + group;
+    const ShortRow<T, L, NV> in = next;
+    if (r0 + step < a.rows) next.template load<true>(a, row + step, lane);
+    if (row >= a.rows) continue;  // whole groups; what follows is per group
+    const RowStats& st = in.st;
+    const bool skip = in.weight == 0.0f || st.dead();
+    const float g = skip || divisor == 0.0f ? 0.0f : in.g / divisor * in.weight * a.temperature;
+    const float co = g * st.coefficient(a.c);
+    const Exponent ex(st.base(), a.c);
+    const float shift = ex.shift - st.base_log();
+    clear_marks<L, W / 32>(marks, lane);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) *(u32x4*)(line + (v * L + lane) * E) = in.x[v];
+    __builtin_amdgcn_wave_barrier();
+    // the lane's first entry, kept until the line has become the gradient's
+    const float own = lane < a.k && in.at >= 0 ? (float)line[in.at] : 0.0f;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      float d[E];
+      unpack(in.x[v], d, (const T*)nullptr);
+#pragma unroll
+      for (int e = 0; e < E; ++e) d[e] = co * __builtin_amdgcn_exp2f(fmaf(d[e], ex.c, shift));
+      if (skip) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) d[e] = 0.0f;
       }
-      if (live && lane == 0) {
-        st.store(a, row);
-        a.row_loss[row] = loss;
-      }
-    } else if (live) {
-      const float g = skip ? 0.0f : row_scale(a, row, w);
-      const float co = g * st.coefficient(a.c), base = st.base(), base_log = st.base_log();
-      T* out = (T*)a.grad + row * a.grad_stride;
+      *(u32x4*)(line + (v * L + lane) * E) = pack(d, (const T*)nullptr);
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (!skip) {
+      const T* x = (const T*)a.logits + row * a.stride;
+      bool twice = false;
+      in.each(a, row, lane, a.k, [&](int j, int at, float v) {
+        if (at < 0) return;
+        twice |= mark(marks, at);
+        const float z = j < L ? own : (float)x[at];
+        line[at] = (T)(g * fmaf(st.total, st.p(z, a.c), -log_q(a, v, st.teacher).q()));
+      });
+      if (__ballot(twice) & members)  // an index occurs twice: every entry takes the sum of its class, in the teacher's order
+        in.each(a, row, lane, a.k, [&](int, int at, float) {
+          if (at < 0) return;
+          float q = 0.0f;
+          for (int u = 0; u < a.k; ++u)
+            if (teacher_index(a, row * a.k + u) == at) q += log_q(a, teacher_value(a, row * a.k + u), st.teacher).q();
+          line[at] = (T)(g * fmaf(st.total, st.p((float)x[at], a.c), -q));
+        });
+    }
+    __builtin_amdgcn_wave_barrier();
+    T* out = (T*)a.grad + row * a.grad_stride;
 #pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        const int i = (v * L + lane) * E;
-        float d[E];
+    for (int v = 0; v < NV; ++v) {
+      const int i = (v * L + lane) * E;
+      if (i + E <= a.V) {
+        store16(out + i, *(const u32x4*)(line + i));
+      } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const bool member = q[v][e] != -1.0f;
-          const float ex = __builtin_amdgcn_exp2f(fmaf(xs[v][e] - (member ? st.m : base), a.c, -(member ? st.ls : base_log)));
-          d[e] = skip ? 0.0f : member ? g * fmaf(st.total, ex, -q[v][e]) : co * ex;
-        }
-        if (i + E <= a.V) {
-          store16(out + i, pack(d, (const T*)nullptr));
-        } else {
-#pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (i + e < a.V) out[i + e] = (T)d[e];
-        }
+        for (int e = 0; e < E; ++e)
+          if (i + e < a.V) out[i + e] = line[i + e];
       }
     }
   }
@@ -730,9 +916,10 @@ __device__ __forceinline__ void close_row(const DistillArgs& a, int64_t row, flo
 
 constexpr int kMaxSegment = 1 << 17;  // elements of a segment: one bit of LDS each says whether the class is the teacher's
 
+constexpr int kWide = 4;  // vectors a thread has under way
 template <typename T, bool REST>
 __global__ __launch_bounds__(kThreads) void k_distill_stream(DistillArgs a) {
-  constexpr int E = Vec<T>::E, kTile = kThreads * E;
+  constexpr int E = Vec<T>::E, kSpan = kThreads * E * kWide;
   __shared__ unsigned bits[REST ? kMaxSegment / 32 : 1];
   __shared__ int index[VSL_MAX_TOP];
   __shared__ float red[2 * kWaves];
@@ -761,25 +948,26 @@ __global__ __launch_bounds__(kThreads) void k_distill_stream(DistillArgs a) {
       __syncthreads();
     }
     MaxSum t{ninf(), 0.0f};
-    for (int i0 = e0; i0 < e1; i0 += kTile) {
-      const int i = i0 + tid * E;
-      float v[E];
-      unpack(load_row(x, i, i < e1 ? e1 : i), v, (const T*)nullptr);
-      if (REST && i < e1) {
-        const unsigned own = (bits[(i - e0) >> 5] >> ((i - e0) & 31)) & ((1u << E) - 1);
-        if (own)
+    u32x4 next[kWide];
+    load_group(x, e0, e1, next);
+    for (int i0 = e0; i0 < e1; i0 += kSpan) {
+      float v[kWide][E];
 #pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (own >> e & 1) v[e] = ninf();
+      for (int u = 0; u < kWide; ++u) unpack(next[u], v[u], (const T*)nullptr);
+      if (i0 + kSpan < e1) load_group(x, i0 + kSpan, e1, next);
+      if (REST) {
+#pragma unroll
+        for (int u = 0; u < kWide; ++u) {
+          const int i = i0 + (u * kThreads + tid) * E;
+          if (i >= e1) continue;
+          const unsigned own = (bits[(i - e0) >> 5] >> ((i - e0) & 31)) & ((1u << E) - 1);
+          if (own)
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+              if (own >> e & 1) v[u][e] = ninf();
+        }
       }
-      float top = v[0];
-#pragma unroll
-      for (int e = 1; e < E; ++e) top = __builtin_elementwise_maximum(top, v[e]);
-      const float m = __builtin_elementwise_maximum(t.m, top), ref = exp_ref(m);
-      float s = t.s * exp_of(t.m, ref, a.c);
-#pragma unroll
-      for (int e = 0; e < E; ++e) s += exp_of(v[e], ref, a.c);
-      t = {m, s};
+      add_group<T>(v, t, a.c);
     }
     t = block_join<kWaves>(t, red, a.c);
     if (a.segs == 1) {
@@ -828,7 +1016,9 @@ __global__ __launch_bounds__(kThreads) void k_distill_grad(DistillArgs a) {
     T* out = (T*)a.grad + row * a.grad_stride;
     const int e0 = seg * a.seg_len, e1 = min(a.V, e0 + a.seg_len);
     const float g = skip ? 0.0f : row_scale(a, row, w);
-    const float co = g * st.coefficient(a.c), base = st.base(), base_log = st.base_log();
+    const float co = g * st.coefficient(a.c);
+    const Exponent ex(st.base(), a.c);
+    const float shift = ex.shift - st.base_log();
     int at = -1;
     if (!skip && tid < a.k) {
       at = teacher_index(a, row * a.k + tid);
@@ -845,7 +1035,7 @@ __global__ __launch_bounds__(kThreads) void k_distill_grad(DistillArgs a) {
       } else {
         unpack(load_row(x, i, e1), d, (const T*)nullptr);
 #pragma unroll
-        for (int e = 0; e < E; ++e) d[e] = co * __builtin_amdgcn_exp2f(fmaf(d[e] - base, a.c, -base_log));
+        for (int e = 0; e < E; ++e) d[e] = co * __builtin_amdgcn_exp2f(fmaf(d[e], ex.c, shift));
       }
       if (i + E <= e1) {
         store16(out + i, pack(d, (const T*)nullptr));
@@ -876,8 +1066,8 @@ int check_distill(const vsl_distill_desc* d) {
     return fail(VSL_ERR_INVALID_ARGUMENT, "distill: teacher indices must be int32 or int64");
   if (d->reduction < VSL_REDUCE_NONE || d->reduction > VSL_REDUCE_MEAN)
     return fail(VSL_ERR_INVALID_ARGUMENT, "distill: unknown reduction");
-  if (!(d->temperature > 0.0f) || d->temperature > 1e18f || d->temperature < 1e-18f)
-    return fail(VSL_ERR_INVALID_ARGUMENT, "distill: temperature must be positive and finite");
+  if (!(d->temperature >= 1e-4f && d->temperature <= 1e4f))
+    return fail(VSL_ERR_INVALID_ARGUMENT, "distill: temperature must lie in 1e-4..1e4");
   if (d->rows > 0 && (!d->logits || !d->teacher_values || !d->teacher_indices))
     return fail(VSL_ERR_INVALID_ARGUMENT, "distill: NULL tensor");
   return VSL_OK;
@@ -924,12 +1114,17 @@ void launch_distill(const DistillArgs& a, hipStream_t s) {
   const dim3 b(kThreads);
   if (a.V <= 256 * Vec<T>::E) {
     const int nv = (int)ceil_div(a.V, Vec<T>::E);
-    const dim3 g16(grid_of(ceil_div(a.rows, kThreads / 16))), g64(grid_of(ceil_div(a.rows, kThreads / 64)));
-    if (nv <= 16) hipLaunchKernelGGL((k_distill_rows<T, 16, 1, GRAD>), g16, b, 0, s, a);
-    else if (nv <= 32) hipLaunchKernelGGL((k_distill_rows<T, 16, 2, GRAD>), g16, b, 0, s, a);
-    else if (nv <= 64) hipLaunchKernelGGL((k_distill_rows<T, 16, 4, GRAD>), g16, b, 0, s, a);
-    else if (nv <= 128) hipLaunchKernelGGL((k_distill_rows<T, 64, 2, GRAD>), g64, b, 0, s, a);
-    else hipLaunchKernelGGL((k_distill_rows<T, 64, 4, GRAD>), g64, b, 0, s, a);
+    auto resident = [](int64_t blocks) { return dim3((unsigned)(blocks < kResident ? blocks : kResident)); };
+    const dim3 g16 = resident(ceil_div(a.rows, kThreads / 16)), g64 = resident(ceil_div(a.rows, kThreads / 64));
+    auto launch = [&](auto fwd, auto bwd, dim3 g) {
+      if (GRAD) hipLaunchKernelGGL(bwd, g, b, 0, s, a);
+      else hipLaunchKernelGGL(fwd, g, b, 0, s, a);
+    };
+    if (nv <= 16) launch(k_distill_rows<T, 16, 1>, k_distill_rows_grad<T, 16, 1>, g16);
+    else if (nv <= 32) launch(k_distill_rows<T, 16, 2>, k_distill_rows_grad<T, 16, 2>, g16);
+    else if (nv <= 64) launch(k_distill_rows<T, 16, 4>, k_distill_rows_grad<T, 16, 4>, g16);
+    else if (nv <= 128) launch(k_distill_rows<T, 64, 2>, k_distill_rows_grad<T, 64, 2>, g64);
+    else launch(k_distill_rows<T, 64, 4>, k_distill_rows_grad<T, 64, 4>, g64);
     return;
   }
   const dim3 g(grid_of(a.rows * a.segs));

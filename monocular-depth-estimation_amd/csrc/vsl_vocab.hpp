@@ -15,7 +15,8 @@ namespace vsl_vocab {
 
 using vsl_err::fail;
 
-constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLog2e = 1.44269504088896340736f;  // and what a float leaves of it
+constexpr float kLog2eLow = (float)(1.4426950408889634 - (double)1.44269504088896340736f);
 constexpr float kLn2 = 0.693147180559945309417f;
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
@@ -79,8 +80,14 @@ __device__ __forceinline__ void store16(_Float16* p, u32x4 v) { *(u32x4_any2*)p 
 
 // Elements [i, i + E) of a row that ends at `end`, kept in their own type; what lies behind the end reads as -infinity.
 template <typename T>
+__device__ __forceinline__ unsigned ninf_word() {  // all elements of a 32-bit word -infinity
+  return sizeof(T) == 4 ? 0xFF800000u : __is_same(T, __bf16) ? 0xFF80FF80u : 0xFC00FC00u;
+}
+template <typename T>
 __device__ __forceinline__ u32x4 load_row(const T* row, int i, int end) {
   if (i + Vec<T>::E <= end) return load16(row + i);
+  const unsigned none = ninf_word<T>();
+  if (i >= end) return u32x4{none, none, none, none};
   float x[Vec<T>::E];
 #pragma unroll
   for (int e = 0; e < Vec<T>::E; ++e) x[e] = i + e < end ? (float)row[i + e] : ninf();
@@ -90,11 +97,11 @@ __device__ __forceinline__ u32x4 load_row(const T* row, int i, int end) {
 // ---- reductions over groups of 16 lanes by data-parallel primitives (no LDS), wider ones by shuffles
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
-  return __uint_as_float((unsigned)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xF, 0xF, false));
+  return __uint_as_float((unsigned)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xF, 0xF, true));
 }
 template <int CTRL>
 __device__ __forceinline__ unsigned dpp(unsigned v) {
-  return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false);
+  return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
 }
 template <int CTRL>
 __device__ __forceinline__ unsigned long long dpp(unsigned long long v) {
@@ -135,6 +142,17 @@ struct MaxSum {
 };
 __device__ __forceinline__ float exp_ref(float m) { return m == ninf() ? 0.0f : m; }  // keeps -inf - -inf out of exponents
 __device__ __forceinline__ float exp_of(float x, float ref, float c) { return __builtin_amdgcn_exp2f((x - ref) * c); }
+// The same for many x <= ref as one multiply-add and one exponential each.  Where ref * c is not finite (a row of lowest
+// values) the scale is so small that ref * c is, and still so large that the next value below ref gives 0: temperatures
+// are at least 1e-4, so |ref| is above 2^114 there and floats are at least 2^91 apart.
+struct Exponent {
+  float c, shift;
+  __device__ __forceinline__ Exponent(float ref, float scale) {
+    c = fabsf(ref * scale) < __uint_as_float(0x7F800000u) ? scale : 0x1p-80f;
+    shift = -(ref * c);
+  }
+  __device__ __forceinline__ float operator()(float x) const { return __builtin_amdgcn_exp2f(fmaf(x, c, shift)); }
+};
 __device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, float c) {
   const float m = __builtin_elementwise_maximum(a.m, b.m), r = exp_ref(m);
   return {m, a.s * exp_of(a.m, r, c) + b.s * exp_of(b.m, r, c)};

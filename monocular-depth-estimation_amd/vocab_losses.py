@@ -106,8 +106,8 @@ def _reduction(name: str) -> int:
 
 def _temperature(value) -> float:
     value = float(value)
-    if not 1e-18 <= value <= 1e18:
-        raise ValueError("temperature must be positive and finite, not %r" % value)
+    if not 1e-4 <= value <= 1e4:
+        raise ValueError("temperature must lie in 1e-4..1e4, not %r" % value)
     return value
 
 
