@@ -3,7 +3,7 @@
 // losses that the linear cross entropy (vsl_linear_ce.hip) shares.
 //
 // A row is a token over a large vocabulary or a pixel over its depth bins, so there are two programs for each operator:
-// "rows" keeps a whole short row in the registers of 16 or 64 lanes, "stream" walks a long row, or a segment of it when
+// "rows" keeps a whole short row in the registers of 8, 16 or 64 lanes, "stream" walks a long row, or a segment of it when
 // there are few rows, with a running maximum and sum per thread.  Both read every logit once per direction.
 #include "vsl_vocab.hpp"
 
@@ -229,16 +229,78 @@ __global__ __launch_bounds__(kThreads) void k_top_rows(TopArgs a) {
 }
 
 // Long rows, kGroup vectors a thread at a time, the next ones under way meanwhile.  A key is (ordered value, ~index).
-// The k-th largest of the 256 threads' maxima over the first group is a bound that at least k elements reach; the elements
-// that do are collected, and whenever more than kTrigger are there the k largest of them are kept and the bound rises to
-// the k-th.  A group of which more passes than the buffer holds (rising rows) is collected again, vector by vector.
+// First only the threads' maxima over the first kProbe groups are taken: their k-th largest is a bound that at least k
+// elements reach.  Then, from the start (what was read is in L2 still), the elements that reach the bound are collected,
+// and whenever more than `trigger` are there the k largest of them are kept and the bound rises to the k-th.  A group of
+// which more passes than the buffer holds (rising rows) is collected again, vector by vector.
+constexpr int kProbe = 4;
 constexpr int kGroup = 2;
 constexpr int kTrigger = 512;  // at most; see trigger below
 constexpr int kBuffer = 4096;  // kTrigger + one vector of each thread, as a power of two for the sort
 static_assert(kTrigger + kThreads * 8 <= kBuffer && VSL_MAX_TOP <= kTrigger, "candidate buffer");
 
-// Bitonic sort, larger first, of n = 2^p keys in LDS.
-__device__ __forceinline__ void sort_keys(unsigned long long* buf, int n) {
+// Bitonic sort, larger first, of 256 R keys: thread t holds keys t, t + 256, ...  Partners within a wave trade by
+// shuffles, within a thread by registers; only strides of 64 and 128 go through LDS and barriers.
+template <int R>
+__device__ __forceinline__ void sort_step(unsigned long long (&key)[R], unsigned long long* lds, int size, int step) {
+  const int tid = threadIdx.x;
+  if (R > 1 && step >= kThreads) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int o = r + step / kThreads;
+      if ((r * kThreads) & step || o >= R) continue;
+      const unsigned long long u = key[r], v = key[o];
+      const bool keep = (u > v) == (((r * kThreads) & size) == 0);
+      key[r] = keep ? u : v;
+      key[o] = keep ? v : u;
+    }
+    return;
+  }
+  unsigned long long other[R];
+  if (step >= 64) {
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r) lds[r * kThreads + tid] = key[r];
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r) other[r] = lds[r * kThreads + (tid ^ step)];
+  } else {
+#pragma unroll
+    for (int r = 0; r < R; ++r) other[r] = __shfl_xor(key[r], step, 64);
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int i = r * kThreads + tid;
+    const bool take_larger = ((i & size) == 0) == ((i & step) == 0);
+    key[r] = (other[r] > key[r]) == take_larger ? other[r] : key[r];
+  }
+}
+template <int R>
+__device__ __forceinline__ void sort_registers(unsigned long long (&key)[R], unsigned long long* lds) {
+#pragma unroll
+  for (int size = 2; size <= kThreads * R; size <<= 1)
+#pragma unroll
+    for (int step = size >> 1; step >= 1; step >>= 1) sort_step<R>(key, lds, size, step);
+}
+template <int R>
+__device__ __forceinline__ void sort_some(unsigned long long* buf, int count) {
+  unsigned long long key[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) key[r] = r * kThreads + (int)threadIdx.x < count ? buf[r * kThreads + threadIdx.x] : 0ull;
+  sort_registers<R>(key, buf);
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < R; ++r) buf[r * kThreads + threadIdx.x] = key[r];
+  __syncthreads();
+}
+// Sorts the first `count` keys of an LDS buffer of kBuffer, larger first, zeros behind (as far as a power of two or 256).
+// Starts behind a barrier that made the keys visible; ends with one.
+__device__ __forceinline__ void sort_count(unsigned long long* buf, int count) {
+  if (count <= kThreads) return sort_some<1>(buf, count);
+  if (count <= 2 * kThreads) return sort_some<2>(buf, count);
+  int n = 4 * kThreads;
+  while (n < count) n <<= 1;
+  for (int i = count + threadIdx.x; i < n; i += kThreads) buf[i] = 0ull;
   for (int size = 2; size <= n; size <<= 1)
     for (int step = size >> 1; step >= 1; step >>= 1) {
       __syncthreads();
@@ -252,13 +314,6 @@ __device__ __forceinline__ void sort_keys(unsigned long long* buf, int n) {
       }
     }
   __syncthreads();
-}
-// sorts the first `count` keys; the rest up to the next power of two becomes 0
-__device__ __forceinline__ void sort_count(unsigned long long* buf, int count) {
-  int n = 2;
-  while (n < count) n <<= 1;
-  for (int i = count + threadIdx.x; i < n; i += kThreads) buf[i] = 0ull;
-  sort_keys(buf, n);
 }
 
 __device__ __forceinline__ float key_floor(unsigned long long key) {
@@ -343,29 +398,42 @@ __global__ __launch_bounds__(kThreads, 4) void k_top_stream(TopArgs a) {
       __syncthreads();
     };
     u32x4 next[kGroup];
+    const int probe_end = min(e1, e0 + kProbe * kSpan);
     load_group(x, e0, e1, next);
+    float best = ninf();
+    for (int i0 = e0; i0 < probe_end; i0 += kSpan) {
+      float v[kGroup][E];
+#pragma unroll
+      for (int u = 0; u < kGroup; ++u) unpack(next[u], v[u], (const T*)nullptr);
+      if (i0 + kSpan < probe_end) load_group(x, i0 + kSpan, e1, next);
+      best = __builtin_elementwise_maximum(best, add_group<T>(v, t, a.c));
+    }
+    load_group(x, e0, e1, next);
+    {
+      // the value alone: whatever equals it reaches the bound as well.  A thread without an element says -infinity.
+      unsigned long long key[1] = {(unsigned long long)ordered32(__float_as_uint(best)) << 32};
+      sort_registers<1>(key, buf);
+      __syncthreads();
+      buf[tid] = key[0];
+      if (tid == 0) count = 0;
+      __syncthreads();
+      bound = buf[a.k - 1];
+      floor_value = key_floor(bound);
+      __syncthreads();
+    }
     for (int i0 = e0; i0 < e1; i0 += kSpan) {
       float v[kGroup][E];
 #pragma unroll
       for (int u = 0; u < kGroup; ++u) unpack(next[u], v[u], (const T*)nullptr);
       if (i0 + kSpan < e1) load_group(x, i0 + kSpan, e1, next);
-      const float top = add_group<T>(v, t, a.c);
-      if (i0 == e0) {
-        unsigned long long best = 0;
+      float top = v[0][0];
+      if (i0 < probe_end) {
 #pragma unroll
         for (int u = 0; u < kGroup; ++u)
 #pragma unroll
-          for (int e = 0; e < E; ++e) {
-            const int i = i0 + (u * kThreads + tid) * E + e;
-            const unsigned long long key = key_of(v[u][e], i);
-            if (i < e1 && key > best) best = key;
-          }
-        buf[tid] = best;
-        if (tid == 0) count = 0;
-        sort_keys(buf, kThreads);
-        bound = buf[a.k - 1];
-        floor_value = key_floor(bound);
-        __syncthreads();
+          for (int e = 0; e < E; ++e) top = __builtin_elementwise_maximum(top, v[u][e]);
+      } else {
+        top = add_group<T>(v, t, a.c);
       }
       const int before = kept;
       if (__any(!(top < floor_value)))
@@ -403,7 +471,9 @@ __global__ __launch_bounds__(kThreads, 4) void k_top_stream(TopArgs a) {
   }
 }
 
-// joins the segments of a row: segs * k <= kBuffer keys
+// Joins the segments of a row, at most kJoinKeys keys: what a block sorts in registers (800 keys through LDS took 21 us).
+constexpr int kJoinKeys = 2 * kThreads;
+static_assert(kJoinKeys <= kBuffer && kJoinKeys >= VSL_MAX_TOP, "segments of a row");
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_top_join(TopArgs a) {
   __shared__ unsigned long long buf[kBuffer];
@@ -451,7 +521,7 @@ int grid_of(int64_t items) { return (int)(items < 1 ? 1 : (items > kMaxBlocks ? 
 
 Split top_split(const vsl_top_desc* d) {
   if (d->vocab <= short_row(d->type)) return {1, (int)d->vocab};
-  return split_row(d->rows, d->vocab, kThreads * vec_of(d->type), kBuffer / d->k);
+  return split_row(d->rows, d->vocab, kThreads * vec_of(d->type), kJoinKeys / d->k);
 }
 
 bool bad_type(int t) { return t != VSL_TYPE_F32 && t != VSL_TYPE_BF16 && t != VSL_TYPE_F16; }
@@ -479,8 +549,10 @@ void launch_top(const TopArgs& a, bool rows_program, hipStream_t s) {
   if (rows_program) {
     const int nv = (int)ceil_div(a.V, Vec<T>::E);
     const dim3 b(kThreads);
+    const dim3 g8(grid_of(ceil_div(a.rows, kThreads / 8)));
     const dim3 g16(grid_of(ceil_div(a.rows, kThreads / 16))), g64(grid_of(ceil_div(a.rows, kThreads / 64)));
-    if (nv <= 16) hipLaunchKernelGGL((k_top_rows<T, 16, 1>), g16, b, 0, s, a);
+    if (nv <= 8) hipLaunchKernelGGL((k_top_rows<T, 8, 1>), g8, b, 0, s, a);
+    else if (nv <= 16) hipLaunchKernelGGL((k_top_rows<T, 8, 2>), g8, b, 0, s, a);
     else if (nv <= 32) hipLaunchKernelGGL((k_top_rows<T, 16, 2>), g16, b, 0, s, a);
     else if (nv <= 64) hipLaunchKernelGGL((k_top_rows<T, 16, 4>), g16, b, 0, s, a);
     else if (nv <= 128) hipLaunchKernelGGL((k_top_rows<T, 64, 2>), g64, b, 0, s, a);
@@ -1115,12 +1187,16 @@ void launch_distill(const DistillArgs& a, hipStream_t s) {
   if (a.V <= 256 * Vec<T>::E) {
     const int nv = (int)ceil_div(a.V, Vec<T>::E);
     auto resident = [](int64_t blocks) { return dim3((unsigned)(blocks < kResident ? blocks : kResident)); };
+    const dim3 g8 = resident(ceil_div(a.rows, kThreads / 8));
     const dim3 g16 = resident(ceil_div(a.rows, kThreads / 16)), g64 = resident(ceil_div(a.rows, kThreads / 64));
     auto launch = [&](auto fwd, auto bwd, dim3 g) {
       if (GRAD) hipLaunchKernelGGL(bwd, g, b, 0, s, a);
       else hipLaunchKernelGGL(fwd, g, b, 0, s, a);
     };
-    if (nv <= 16) launch(k_distill_rows<T, 16, 1>, k_distill_rows_grad<T, 16, 1>, g16);
+    // Fewer lanes a row share the work that every row costs among more rows: 8 lanes of two vectors against 16 of one, 128
+    // bins in bfloat16, 146 against 232 us forward.
+    if (nv <= 8) launch(k_distill_rows<T, 8, 1>, k_distill_rows_grad<T, 8, 1>, g8);
+    else if (nv <= 16) launch(k_distill_rows<T, 8, 2>, k_distill_rows_grad<T, 8, 2>, g8);
     else if (nv <= 32) launch(k_distill_rows<T, 16, 2>, k_distill_rows_grad<T, 16, 2>, g16);
     else if (nv <= 64) launch(k_distill_rows<T, 16, 4>, k_distill_rows_grad<T, 16, 4>, g16);
     else if (nv <= 128) launch(k_distill_rows<T, 64, 2>, k_distill_rows_grad<T, 64, 2>, g64);

@@ -109,13 +109,13 @@ __device__ __forceinline__ unsigned long long dpp(unsigned long long v) {
 }
 constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kMirror8 = 0x141, kMirror16 = 0x140;
 
-// all L lanes of a group (L = 16 or 64, aligned) get op over the group
+// all L lanes of a group (L = 8, 16 or 64, aligned) get op over the group
 template <int L, typename V, typename Op>
 __device__ __forceinline__ V group_all(V v, Op op) {
   v = op(v, dpp<kXor1>(v));
   v = op(v, dpp<kXor2>(v));
   v = op(v, dpp<kMirror8>(v));
-  v = op(v, dpp<kMirror16>(v));
+  if (L > 8) v = op(v, dpp<kMirror16>(v));
   if (L > 16) {
     v = op(v, (V)__shfl_xor(v, 16, 64));
     v = op(v, (V)__shfl_xor(v, 32, 64));
