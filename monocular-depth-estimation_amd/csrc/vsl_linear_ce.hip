@@ -35,6 +35,7 @@ struct Shape {
 };
 typedef Shape<256, 256, 2, 4> Large;
 typedef Shape<128, 128, 2, 2> Small;
+typedef Shape<128, 64, 4, 1> Narrow;  // few columns: rows of the loss
 
 template <typename T>
 struct Kind {
@@ -340,25 +341,37 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
   }
 }
 
-// 16 rows a block, 16 lanes each: joins the tiles' maxima and sums.
+// R rows a block, 256 / R lanes each: joins the tiles' maxima and sums, four of a lane's at a time.
+template <int R>
 __global__ __launch_bounds__(kThreads) void k_ce_rows(const float2* __restrict__ partial, int64_t rows_padded, int tiles,
                                                       const float* __restrict__ target_logit,
                                                       const int64_t* __restrict__ target, int64_t ignore_index, int64_t vocab,
                                                       float z_loss, int64_t rows, float* __restrict__ row_loss,
                                                       float* __restrict__ stats) {
-  __shared__ float2 part[16][16];
-  const int r = threadIdx.x & 15, g = threadIdx.x >> 4;
-  const int64_t row = (int64_t)blockIdx.x * 16 + r;
+  constexpr int P = kThreads / R;
+  __shared__ float2 part[P][R];
+  const int r = threadIdx.x % R, g = threadIdx.x / R;
+  const int64_t row = (int64_t)blockIdx.x * R + r;
   MaxSum q{ninf(), 0.0f};
   if (row < rows)
-    for (int i = g; i < tiles; i += 16) {
-      const float2 p = partial[(int64_t)i * rows_padded + row];
-      q = join(q, {p.x, p.y}, kLog2e);
+    for (int i = g; i < tiles; i += 4 * P) {
+      float2 p[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        p[u] = i + u * P < tiles ? partial[(int64_t)(i + u * P) * rows_padded + row] : make_float2(ninf(), 0.0f);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) q = join(q, {p[u].x, p[u].y}, kLog2e);
     }
   part[g][r] = make_float2(q.m, q.s);
-  __syncthreads();
+#pragma unroll
+  for (int n = P / 2; n >= 1; n >>= 1) {
+    __syncthreads();
+    if (g < n) {
+      q = join(q, {part[g + n][r].x, part[g + n][r].y}, kLog2e);
+      part[g][r] = make_float2(q.m, q.s);
+    }
+  }
   if (g == 0 && row < rows) {
-    for (int i = 1; i < 16; ++i) q = join(q, {part[i][r].x, part[i][r].y}, kLog2e);
     const float ls = log2_sum(q), lse = log_sum(q, 1.0f);
     float m = q.m, loss = 0.0f;
     const int64_t t = target[row];
@@ -712,27 +725,51 @@ Forward forward_workspace(const vsl_linear_ce_desc* d, void* base) {
 // last-level cache between the kernel that writes them and the two products that read them.
 constexpr int64_t kPieceElements = 1LL << 26;
 
+struct Plan {
+  int shape, splits;  // of the tiles of a product, and of its K
+};
 struct Backward {
   Layout l;
   int64_t piece, pieces, vocab_padded;
-  int splits_h, splits_w;
+  Plan plan_h, plan_w;
   void *hidden, *weight, *hidden_t, *weight_t, *delta, *delta_t;
   float *sum_h, *sum_w, *row_scale, *out_scale, *largest;
   size_t total;
 };
-// The large tile reads half as much per product and needs enough tiles for the 256 CUs, and not more padding than it saves.
-bool large_tiles(int64_t M, int64_t N, int type) {
-  const int64_t large = ceil_div(M, Large::BM) * ceil_div(N, Large::BN), small = ceil_div(M, Small::BM) * ceil_div(N, Small::BN);
-  return type != VSL_TYPE_F32 && large >= 256 && large * 4 * 8 <= small * 9;
+enum { kLarge, kSmall, kNarrow };
+struct ShapeInfo {
+  int bm, bn, slots;             // tile, and how many of it the 256 CUs hold at once
+  float step16, step32, around;  // microseconds of a step of K with all slots taken (16-bit types, float32), and of a tile's
+                                 // beginning and end
+};
+// Measured on products of 2048..8192 rows (large: 1240 TFLOP/s in bfloat16, small: 850; float32: 105).
+constexpr ShapeInfo kShapes[] = {{Large::BM, Large::BN, 256, 1.7f, 0.0f, 4.0f},
+                                 {Small::BM, Small::BN, 512, 1.3f, 5.0f, 2.5f},
+                                 {Narrow::BM, Narrow::BN, 768, 1.1f, 4.0f, 2.0f}};
+// Shape of the tiles of a product M x N over `blocks` steps of K, and into how many parts K is cut: the least of the waves
+// of tiles times their length, plus the traffic of the partial sums.  float32 leaves out the large tile: its epilogue
+// does not fit the registers, and its matrix instructions are eight times slower, so that its loads never bind.
+Plan plan_of(int64_t M, int64_t N, int64_t blocks, int type, bool may_split) {
+  Plan best{kSmall, 1};
+  double least = 1e300;
+  for (int shape = type == VSL_TYPE_F32 ? kSmall : kLarge; shape <= kNarrow; ++shape) {
+    const ShapeInfo& h = kShapes[shape];
+    const double tiles = (double)(ceil_div(M, h.bm) * ceil_div(N, h.bn));
+    const double step = type == VSL_TYPE_F32 ? h.step32 : h.step16;
+    for (int s = 1; s <= 256 && (s == 1 || (may_split && blocks / s >= 4)); s = s < 4 ? s + 1 : s + s / 2) {
+      const double waves = (double)(int64_t)((tiles * s + h.slots - 1) / h.slots);
+      double t = waves * ((double)ceil_div(blocks, s) * step + h.around);
+      if (s > 1) t += 4.0 + (double)s * (double)M * (double)N * 8.0 / 4e6;
+      if (t < least) {
+        least = t;
+        best = {shape, s};
+      }
+    }
+  }
+  return best;
 }
-// Tiles of a product, and into how many parts its K is cut so that there are enough of them for the 256 CUs.
-int splits_of(int64_t M, int64_t N, int64_t K, int type) {
-  if (large_tiles(M, N, type)) return 1;
-  const int64_t tiles = ceil_div(M, Small::BM) * ceil_div(N, Small::BN), blocks = ceil_div(K * size_of(type), kBlockBytes);
-  int64_t s = 512 / tiles;
-  if (s > blocks / 8) s = blocks / 8;
-  return (int)(s < 1 ? 1 : s);
-}
+int64_t blocks_of(int64_t K, int type) { return ceil_div(K * size_of(type), kBlockBytes); }
+
 Backward backward_workspace(const vsl_linear_ce_desc* d, uint32_t mask, void* base) {
   Backward b{};
   b.l = layout_of(d);
@@ -750,10 +787,10 @@ Backward backward_workspace(const vsl_linear_ce_desc* d, uint32_t mask, void* ba
   b.weight_t = gh ? a.take((size_t)d->dim * b.vocab_padded * s) : nullptr;
   b.delta = gh ? a.take((size_t)b.l.rows_padded * b.piece * s) : nullptr;
   b.delta_t = gw || gb ? a.take((size_t)b.l.rows_padded * b.piece * s) : nullptr;
-  b.splits_h = splits_of(d->dim, d->rows, b.piece, d->type);
-  b.splits_w = splits_of(d->dim, d->vocab < b.piece ? d->vocab : b.piece, b.l.rows_padded, d->type);
-  b.sum_h = gh && (b.pieces > 1 || b.splits_h > 1) ? (float*)a.take((size_t)b.splits_h * d->rows * d->dim * 4) : nullptr;
-  b.sum_w = gw && b.splits_w > 1 ? (float*)a.take((size_t)b.splits_w * b.piece * d->dim * 4) : nullptr;
+  b.plan_h = plan_of(d->dim, d->rows, blocks_of(b.piece, d->type), d->type, true);
+  b.plan_w = plan_of(d->dim, d->vocab < b.piece ? d->vocab : b.piece, blocks_of(d->rows, d->type), d->type, true);
+  b.sum_h = gh && (b.pieces > 1 || b.plan_h.splits > 1) ? (float*)a.take((size_t)b.plan_h.splits * d->rows * d->dim * 4) : nullptr;
+  b.sum_w = gw && b.plan_w.splits > 1 ? (float*)a.take((size_t)b.plan_w.splits * b.piece * d->dim * 4) : nullptr;
   b.row_scale = (float*)a.take((size_t)b.l.rows_padded * 4);
   b.out_scale = (float*)a.take(4);
   b.largest = (float*)a.take(256 * 4);
@@ -785,9 +822,10 @@ int launch_logits_as(const LogitArgs& a, hipStream_t s) {
   return (int)tm;
 }
 template <typename T, bool DELTA>
-int launch_logits(const LogitArgs& a, bool large, hipStream_t s) {  // returns the rows of tiles
+int launch_logits(const LogitArgs& a, int shape, hipStream_t s) {  // returns the rows of tiles
   if constexpr (sizeof(T) == 2)
-    if (large) return launch_logits_as<T, Large, DELTA>(a, s);
+    if (shape == kLarge) return launch_logits_as<T, Large, DELTA>(a, s);
+  if (shape == kNarrow) return launch_logits_as<T, Narrow, DELTA>(a, s);
   return launch_logits_as<T, Small, DELTA>(a, s);
 }
 template <typename T, typename S>
@@ -796,10 +834,12 @@ void launch_grad_as(const GradArgs& g, hipStream_t s) {
   hipLaunchKernelGGL((k_ce_grad<T, S>), dim3((unsigned)(tiles * g.splits)), dim3(S::kThreads), 0, s, g);
 }
 template <typename T>
-void launch_grad(GradArgs g, int type, hipStream_t s) {
+void launch_grad(GradArgs g, const Plan& p, hipStream_t s) {
+  g.splits = p.splits;
   g.whole = g.op.M % 4 == 0 && (uintptr_t)g.out % 16 == 0;
   if constexpr (sizeof(T) == 2)
-    if (large_tiles(g.op.M, g.op.N, type)) return launch_grad_as<T, Large>(g, s);
+    if (p.shape == kLarge) return launch_grad_as<T, Large>(g, s);
+  if (p.shape == kNarrow) return launch_grad_as<T, Narrow>(g, s);
   launch_grad_as<T, Small>(g, s);
 }
 
@@ -818,9 +858,11 @@ void run_forward(const vsl_linear_ce_desc* d, const Forward& f, float* row_loss,
   a.rows_padded = l.rows_padded;
   a.partial = f.partial;
   a.target_logit = f.target_logit;
-  const int tiles = launch_logits<T, false>(a, large_tiles(a.op.M, a.op.N, d->type), s);
-  hipLaunchKernelGGL(k_ce_rows, dim3((unsigned)ceil_div(d->rows, 16)), dim3(kThreads), 0, s, (const float2*)f.partial,
-                     l.rows_padded, tiles, (const float*)f.target_logit, d->target, d->ignore_index, d->vocab, d->z_loss,
+  const int tiles = launch_logits<T, false>(a, plan_of(a.op.M, a.op.N, a.op.kblocks, d->type, false).shape, s);
+  // few rows: more lanes each, so that no lane walks many tiles (16 rows of 512 tiles: 14 us with 16 lanes a row)
+  const int per_block = tiles > 64 && d->rows <= 2048 ? 4 : 16;
+  hipLaunchKernelGGL(per_block == 4 ? k_ce_rows<4> : k_ce_rows<16>, dim3((unsigned)ceil_div(d->rows, per_block)),
+                     dim3(kThreads), 0, s, (const float2*)f.partial, l.rows_padded, tiles, (const float*)f.target_logit, d->target, d->ignore_index, d->vocab, d->z_loss,
                      d->rows, row_loss, stats);
   if (d->reduction != VSL_REDUCE_NONE)
     launch_sum(row_loss, nullptr, d->target, d->ignore_index, d->rows, d->reduction, f.sums, loss, divisor, s);
@@ -868,9 +910,9 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
                                         Contributes{nullptr, nullptr, nullptr, d->bias, 0}, b.weight_t, s);
   for (int64_t p = 0; p < b.pieces; ++p) {
     const int64_t v0 = p * b.piece, classes = d->vocab - v0 < b.piece ? d->vocab - v0 : b.piece;
-    const bool large = large_tiles(classes, d->rows, d->type);
-    const int64_t tile = large ? Large::BM : Small::BM;  // square: what the derivative kernel covers in both directions
-    const int64_t padded = round_up(classes, tile), rows_covered = round_up(d->rows, tile);
+    const int shape = plan_of(classes, d->rows, l.dim_padded / Kind<T>::BK, d->type, false).shape;
+    // what the derivative kernel covers: whole steps of K for the two products that follow
+    const int64_t padded = round_up(classes, kShapes[shape].bm), rows_covered = round_up(d->rows, kShapes[shape].bn);
     LogitArgs a{};
     a.op = {weight + v0 * ldw, hidden, ldw, ldh, (int)classes, (int)d->rows, (int)(l.dim_padded / Kind<T>::BK)};
     a.bias = d->bias;
@@ -885,27 +927,25 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
     a.delta = grad_hidden ? b.delta : nullptr;
     a.ldd = b.piece;
     a.delta_t = grad_weight || grad_bias ? b.delta_t : nullptr;
-    launch_logits<T, true>(a, large, s);
+    launch_logits<T, true>(a, shape, s);
     if (grad_hidden) {
       GradArgs g{};
       g.op = {(const T*)b.weight_t + v0, b.delta, b.vocab_padded, b.piece, (int)d->dim, (int)d->rows, (int)(padded / Kind<T>::BK)};
-      g.splits = b.splits_h;
       g.add = p > 0;
       g.sum = b.sum_h;
       g.out = grad_hidden;
       g.scale = scale;
-      launch_grad<T>(g, d->type, s);
+      launch_grad<T>(g, b.plan_h, s);
     }
     if (grad_weight) {
       GradArgs g{};
       g.op = {b.hidden_t, b.delta_t, l.rows_padded, l.rows_padded, (int)d->dim, (int)classes, (int)(rows_covered / Kind<T>::BK)};
-      g.splits = b.splits_w;
       g.sum = b.sum_w;
       g.out = grad_weight + v0 * d->dim;
       g.scale = scale;
-      launch_grad<T>(g, d->type, s);
+      launch_grad<T>(g, b.plan_w, s);
       if (g.sum)
-        hipLaunchKernelGGL(k_ce_finish<T>, linear_grid(classes * d->dim), dim3(kThreads), 0, s, (const float*)g.sum, g.splits,
+        hipLaunchKernelGGL(k_ce_finish<T>, linear_grid(classes * d->dim), dim3(kThreads), 0, s, (const float*)g.sum, b.plan_w.splits,
                            classes * d->dim, scale, (T*)g.out);
     }
     if (grad_bias)
@@ -913,7 +953,7 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
                          rows_covered, scale, grad_bias + v0);
   }
   if (grad_hidden && b.sum_h)
-    hipLaunchKernelGGL(k_ce_finish<T>, linear_grid(d->rows * d->dim), dim3(kThreads), 0, s, (const float*)b.sum_h, b.splits_h,
+    hipLaunchKernelGGL(k_ce_finish<T>, linear_grid(d->rows * d->dim), dim3(kThreads), 0, s, (const float*)b.sum_h, b.plan_h.splits,
                        d->rows * d->dim, scale, grad_hidden);
 }
 
