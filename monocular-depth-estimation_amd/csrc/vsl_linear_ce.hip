@@ -199,11 +199,15 @@ struct LogitArgs {
   void* delta_t;       // [padded classes of the piece][rows_padded]
 };
 
-template <typename T>
-__device__ __forceinline__ float add_bias(float z, const void* bias, int64_t v) {
-  if (!bias) return z;
-  const float b = (float)((const T*)bias)[v];
-  return b == ninf() ? b : z + b;  // a masked class stays masked whatever its weights hold
+// Adds the biases of a block's classes, which lie in LDS as floats, -infinity behind the last class.
+__device__ __forceinline__ void add_bias(f32x16& z, const float* bias) {
+#pragma unroll
+  for (int r4 = 0; r4 < 4; ++r4) {
+    const f32x4 b = *(const f32x4*)(bias + 8 * r4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)  // a masked class stays masked whatever its weights hold
+      z[4 * r4 + e] = b[e] == ninf() ? b[e] : z[4 * r4 + e] + b[e];
+  }
 }
 
 // derivative of lse + z_loss lse^2 with respect to lse
@@ -243,59 +247,75 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
   tile_product<T, S>(a.op, m0, n0, 0, a.op.kblocks, lds, t);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
   const int half = lane >> 5;
+  const bool biased = a.bias || m0 + S::BM > a.op.M;
+  float* bias = (float*)(lds + S::WM * S::BN * sizeof(float2));
+  if (biased) {
+    for (int i = threadIdx.x; i < S::BM; i += S::kThreads)
+      bias[i] = m0 + i >= a.op.M ? ninf() : a.bias ? (float)((const T*)a.bias)[a.class0 + m0 + i] : 0.0f;
+    __syncthreads();
+  }
 #pragma unroll
   for (int j = 0; j < S::JN; ++j) {
     const int col = (wn * S::JN + j) * 32 + (lane & 31), row = n0 + col;
     const bool live = row < a.op.N;
     const int64_t target = live ? a.target[row] - a.class0 : -1;
-    float m = ninf();
+    // Most of an epilogue's elements are neither behind the last class nor a target: both are looked for once per 32
+    // classes (16 of them in a lane's registers).
     if (!DELTA) {
+      float m = ninf();
 #pragma unroll
-      for (int i = 0; i < S::IM; ++i)
+      for (int i = 0; i < S::IM; ++i) {
+        const int v32 = m0 + (wm * S::IM + i) * 32;
+        f32x16& z = t.acc[i][j];
+        if (biased) add_bias(z, bias + v32 - m0 + 4 * half);
+        if (target >= v32 && target < v32 + 32) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int v = m0 + (wm * S::IM + i) * 32 + (r & 3) + 8 * (r >> 2) + 4 * half;
-          float z = ninf();
-          if (v < a.op.M) {
-            z = add_bias<T>(t.acc[i][j][r], a.bias, a.class0 + v);
-            if (v == target) a.target_logit[row] = z;
-          }
-          t.acc[i][j][r] = z;
-          m = __builtin_elementwise_maximum(m, z);
+          for (int r = 0; r < 16; ++r)
+            if (v32 + (r & 3) + 8 * (r >> 2) + 4 * half == target) a.target_logit[row] = z[r];
         }
-      const float ref = exp_ref(m);
-      float s = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) m = __builtin_elementwise_maximum(m, z[r]);
+      }
+      const Exponent ex(exp_ref(m), kLog2e);
+      float s = 0.0f, s2 = 0.0f;
 #pragma unroll
       for (int i = 0; i < S::IM; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s += exp_of(t.acc[i][j][r], ref, kLog2e);
-      MaxSum q{m, s};
+        for (int r = 0; r < 16; r += 2) {
+          s += ex(t.acc[i][j][r]);
+          s2 += ex(t.acc[i][j][r + 1]);
+        }
+      MaxSum q{m, s + s2};
       q = join(q, {__shfl_xor(q.m, 32, 64), __shfl_xor(q.s, 32, 64)}, kLog2e);
       if (half == 0) ((float2*)lds)[wm * S::BN + col] = make_float2(q.m, q.s);
     } else {
       const float top = live ? a.stats[row] : ninf(), ls = live ? a.stats[a.op.N + row] : 0.0f;
       const float scale = !live || top == ninf() || target + a.class0 == a.ignore_index ? 0.0f
                           : a.row_scale ? a.row_scale[row] : a.unit;
-      const float slope = slope_of(a.z_loss, top, ls);
+      const float factor = scale * slope_of(a.z_loss, top, ls);
+      const Exponent ex(top, kLog2e);
+      const float shift = ex.shift - ls;
       T* d = (T*)a.delta + (int64_t)row * a.ldd;
 #pragma unroll
       for (int i = 0; i < S::IM; ++i) {
         const int v32 = m0 + (wm * S::IM + i) * 32;
+        f32x16& z = t.acc[i][j];
+        if (biased) add_bias(z, bias + v32 - m0 + 4 * half);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) z[r] = factor * __builtin_amdgcn_exp2f(fmaf(z[r], ex.c, shift));
+        if (target >= v32 && target < v32 + 32) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (v32 + (r & 3) + 8 * (r >> 2) + 4 * half == target) z[r] -= scale;
+        }
+        if (scale == 0.0f) {  // whatever the row holds
+#pragma unroll
+          for (int r = 0; r < 16; ++r) z[r] = 0.0f;
+        }
 #pragma unroll
         for (int r8 = 0; r8 < 2; ++r8) {  // two groups of 8 classes, four of each in either half of the wave
-          float g[2][4];
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int v = v32 + 16 * r8 + 8 * u + 4 * half + e;
-              float x = 0.0f;
-              if (v < a.op.M && scale != 0.0f) {
-                const float z = add_bias<T>(t.acc[i][j][r8 * 8 + u * 4 + e], a.bias, a.class0 + v);
-                x = scale * (slope * __builtin_amdgcn_exp2f(fmaf(z - top, kLog2e, -ls)) - (v == target ? 1.0f : 0.0f));
-              }
-              g[u][e] = x;
-            }
+          const float g[2][4] = {{z[8 * r8], z[8 * r8 + 1], z[8 * r8 + 2], z[8 * r8 + 3]},
+                                 {z[8 * r8 + 4], z[8 * r8 + 5], z[8 * r8 + 6], z[8 * r8 + 7]}};
           if constexpr (sizeof(T) == 4) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -322,6 +342,7 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
             }
           }
         }
+        __builtin_amdgcn_sched_barrier(0);  // blocks one after the other: mixed they need more registers than there are
       }
     }
   }
@@ -627,21 +648,27 @@ __global__ __launch_bounds__(kThreads) void k_ce_finish(const float* __restrict_
   }
 }
 
-// grad_bias: a block per class sums its row of d^T, the values that grad_weight is made of
+// grad_bias: sums of the rows of d^T, the values that grad_weight is made of; a block per class and part of its row
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_ce_bias(const T* __restrict__ delta_t, int64_t rows_padded, int64_t rows,
-                                                      OutScale out_scale, T* __restrict__ out) {
+                                                      int classes, int parts, float* __restrict__ sum, OutScale out_scale,
+                                                      T* __restrict__ out) {
   __shared__ float red[4];
-  const T* d = delta_t + (int64_t)blockIdx.x * rows_padded;
+  const int c = blockIdx.x % classes, part = blockIdx.x / classes;
+  const T* d = delta_t + (int64_t)c * rows_padded;
+  const int64_t vectors = rows / Kind<T>::E, per = (vectors + parts - 1) / parts;
+  const int64_t end = min(vectors, (part + 1) * per);
   float s = 0.0f;
-  for (int64_t i = threadIdx.x; i < rows / Kind<T>::E; i += kThreads) {
+  for (int64_t i = part * per + threadIdx.x; i < end; i += kThreads) {
     float x[Kind<T>::E];
     unpack(load16(d + i * Kind<T>::E), x, (const T*)nullptr);
 #pragma unroll
     for (int e = 0; e < Kind<T>::E; ++e) s += x[e];
   }
   s = block_add<4>(s, red);
-  if (threadIdx.x == 0) out[blockIdx.x] = (T)(s * out_scale.get());
+  if (threadIdx.x) return;
+  if (sum) sum[(int64_t)part * classes + c] = s;
+  else out[c] = (T)(s * out_scale.get());
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -725,6 +752,8 @@ Forward forward_workspace(const vsl_linear_ce_desc* d, void* base) {
 // last-level cache between the kernel that writes them and the two products that read them.
 constexpr int64_t kPieceElements = 1LL << 26;
 
+constexpr int64_t kBiasBlocks = 1024;
+
 struct Plan {
   int shape, splits;  // of the tiles of a product, and of its K
 };
@@ -733,7 +762,7 @@ struct Backward {
   int64_t piece, pieces, vocab_padded;
   Plan plan_h, plan_w;
   void *hidden, *weight, *hidden_t, *weight_t, *delta, *delta_t;
-  float *sum_h, *sum_w, *row_scale, *out_scale, *largest;
+  float *sum_h, *sum_w, *sum_b, *row_scale, *out_scale, *largest;
   size_t total;
 };
 enum { kLarge, kSmall, kNarrow };
@@ -756,7 +785,7 @@ Plan plan_of(int64_t M, int64_t N, int64_t blocks, int type, bool may_split) {
     const ShapeInfo& h = kShapes[shape];
     const double tiles = (double)(ceil_div(M, h.bm) * ceil_div(N, h.bn));
     const double step = type == VSL_TYPE_F32 ? h.step32 : h.step16;
-    for (int s = 1; s <= 256 && (s == 1 || (may_split && blocks / s >= 4)); s = s < 4 ? s + 1 : s + s / 2) {
+    for (int s = 1; s <= 256 && (s == 1 || (may_split && blocks / s >= 4)); s = s < 16 ? s + 1 : s + s / 4) {
       const double waves = (double)(int64_t)((tiles * s + h.slots - 1) / h.slots);
       double t = waves * ((double)ceil_div(blocks, s) * step + h.around);
       if (s > 1) t += 4.0 + (double)s * (double)M * (double)N * 8.0 / 4e6;
@@ -791,6 +820,7 @@ Backward backward_workspace(const vsl_linear_ce_desc* d, uint32_t mask, void* ba
   b.plan_w = plan_of(d->dim, d->vocab < b.piece ? d->vocab : b.piece, blocks_of(d->rows, d->type), d->type, true);
   b.sum_h = gh && (b.pieces > 1 || b.plan_h.splits > 1) ? (float*)a.take((size_t)b.plan_h.splits * d->rows * d->dim * 4) : nullptr;
   b.sum_w = gw && b.plan_w.splits > 1 ? (float*)a.take((size_t)b.plan_w.splits * b.piece * d->dim * 4) : nullptr;
+  b.sum_b = gb && d->rows >= 8192 && d->vocab <= kBiasBlocks / 2 ? (float*)a.take(kBiasBlocks * 4) : nullptr;
   b.row_scale = (float*)a.take((size_t)b.l.rows_padded * 4);
   b.out_scale = (float*)a.take(4);
   b.largest = (float*)a.take(256 * 4);
@@ -948,9 +978,15 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
         hipLaunchKernelGGL(k_ce_finish<T>, linear_grid(classes * d->dim), dim3(kThreads), 0, s, (const float*)g.sum, b.plan_w.splits,
                            classes * d->dim, scale, (T*)g.out);
     }
-    if (grad_bias)
-      hipLaunchKernelGGL(k_ce_bias<T>, dim3((unsigned)classes), dim3(kThreads), 0, s, (const T*)b.delta_t, l.rows_padded,
-                         rows_covered, scale, grad_bias + v0);
+    if (grad_bias) {
+      // few classes: their rows in parts, so that more than a block per class works on them
+      const int parts = b.sum_b ? (int)(kBiasBlocks / classes < 1 ? 1 : kBiasBlocks / classes) : 1;
+      hipLaunchKernelGGL(k_ce_bias<T>, dim3((unsigned)(classes * parts)), dim3(kThreads), 0, s, (const T*)b.delta_t,
+                         l.rows_padded, rows_covered, (int)classes, parts, parts > 1 ? b.sum_b : nullptr, scale, grad_bias + v0);
+      if (parts > 1)
+        hipLaunchKernelGGL(k_ce_finish<T>, linear_grid(classes), dim3(kThreads), 0, s, (const float*)b.sum_b, parts, classes,
+                           scale, grad_bias + v0);
+    }
   }
   if (grad_hidden && b.sum_h)
     hipLaunchKernelGGL(k_ce_finish<T>, linear_grid(d->rows * d->dim), dim3(kThreads), 0, s, (const float*)b.sum_h, b.plan_h.splits,
