@@ -748,9 +748,10 @@ Forward forward_workspace(const vsl_linear_ce_desc* d, void* base) {
   return f;
 }
 
-// Pieces of the vocabulary whose derivatives hold at most this many elements: 128 MiB in 16 bits, twice, stays in the
-// last-level cache between the kernel that writes them and the two products that read them.
-constexpr int64_t kPieceElements = 1LL << 26;
+// Pieces of the vocabulary whose derivatives hold at most this many elements: 256 MiB in 16 bits, twice.  Smaller pieces
+// would stay in the last-level cache, but every piece reads and writes grad_hidden's sums: at 8192 x 131072 x 4096 in
+// bfloat16 2^26, 2^27 and 2^28 elements take 29.6, 29.3 and 29.3 ms.
+constexpr int64_t kPieceElements = 1LL << 27;
 
 constexpr int64_t kBiasBlocks = 1024;
 
