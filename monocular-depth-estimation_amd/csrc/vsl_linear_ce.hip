@@ -9,6 +9,15 @@
 // All three products are C[M,N] = A[M,K] B[N,K]^T with K contiguous in both operands, so that one main loop serves them:
 // the transposed weight and hidden that the two gradient products need are laid out once per call.  Recomputing z costs
 // a fourth product (a third more operations than keeping the logits) and spares rows * vocab float32 of memory traffic.
+//
+// Float32 has two forms.  The direct one uses the float32 matrix instructions (105 TFLOP/s here).  The split one writes
+// every float as the sum of three bfloat16, x = h + m + l, which holds all of its 24 bits, and multiplies
+// x y = l h + m m + h l + m h + h m + h h; what it leaves out (m l, l m, l l) is below 2^-24 of the product, as a float32
+// product's own rounding is, and the sums stay float32.  Six bfloat16 products run 2.7 times faster than one float32
+// product; their operands are laid out as three planes per row, and the main loop walks the six pairs of planes one after
+// the other, smallest first.
+#include <type_traits>
+
 #include "vsl_vocab.hpp"
 
 namespace vsl_vocab {
@@ -59,13 +68,19 @@ __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c, const float*) 
   return c;
 }
 
-// Operands of a product: A [M, >= kblocks * BK], B [N, ...], rows `lda`, `ldb` elements apart.
+// Operands of a product: A [M, >= kblocks * BK], B [N, ...], rows `lda`, `ldb` elements apart; in the split form the
+// planes of a row are plane_a, plane_b elements apart.
 struct Operands {
   const void* A;
   const void* B;
   int64_t lda, ldb;
   int M, N, kblocks;
+  int64_t plane_a, plane_b;
 };
+constexpr int kPairs = 6;
+// planes of pair p, two bits each: l h, m m, h l, m h, h m, h h (h = 0, m = 1, l = 2)
+__device__ __forceinline__ int pair_a(int p) { return (0x046 >> (2 * p)) & 3; }
+__device__ __forceinline__ int pair_b(int p) { return (0x124 >> (2 * p)) & 3; }
 
 // C tile of a wave: acc[i][j] covers rows 32 i.. and columns 32 j.. of its part; register r of a lane is row
 // (r & 3) + 8 (r >> 2) + 4 (lane >> 5), column lane & 31.
@@ -80,7 +95,8 @@ struct Tile {
 // A step is four rounds; each round's fragments are read while the round before multiplies.  The barrier stands before the
 // last round, whose fragments are in registers by then: behind it the buffer is free for the step after next, and the
 // next step's first fragments are read under the last round's multiplications.
-template <typename T, typename S>
+// T: the operands' type; steps [k0, k1) of kblocks, or of kPairs * kblocks in the split form.
+template <typename T, typename S, bool SPLIT>
 __device__ __forceinline__ void tile_product(const Operands& op, int m0, int n0, int k0, int k1, char* lds, Tile<S>& t) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / S::WN, wn = wave % S::WN;
@@ -92,20 +108,36 @@ __device__ __forceinline__ void tile_product(const Operands& op, int m0, int n0,
       for (int r = 0; r < 16; ++r) t.acc[i][j][r] = 0.0f;
   if (k0 >= k1) return;
   const char* src[S::kFetch];
+  int pair = 0, at_k = k0;
+  int64_t offset_a = (int64_t)k0 * kBlockBytes, offset_b = offset_a;
+  if (SPLIT) {
+    pair = k0 / op.kblocks;
+    at_k = k0 - pair * op.kblocks;
+    offset_a = pair_a(pair) * op.plane_a * (int)sizeof(T) + (int64_t)at_k * kBlockBytes;
+    offset_b = pair_b(pair) * op.plane_b * (int)sizeof(T) + (int64_t)at_k * kBlockBytes;
+  }
 #pragma unroll
   for (int i = 0; i < S::kFetch; ++i) {
     const int at = (i < S::kFetchA ? i : i - S::kFetchA) * S::kThreads + tid, row = at >> 3, piece = (at & 7) ^ ((row >> 1) & 7);
     src[i] = i < S::kFetchA ? (const char*)op.A + (int64_t)min(m0 + row, op.M - 1) * op.lda * (int)sizeof(T)
                             : (const char*)op.B + (int64_t)min(n0 + row, op.N - 1) * op.ldb * (int)sizeof(T);
-    src[i] += (int64_t)k0 * kBlockBytes + piece * 16;
+    src[i] += (i < S::kFetchA ? offset_a : offset_b) + piece * 16;
   }
   auto fetch = [&](int buffer) {
+    int64_t next_a = kBlockBytes, next_b = kBlockBytes;
+    if (SPLIT && ++at_k == op.kblocks) {  // on to the next pair of planes, from its beginning
+      const int64_t back = (int64_t)(op.kblocks - 1) * kBlockBytes;
+      next_a = (pair_a(pair + 1) - pair_a(pair)) * op.plane_a * (int)sizeof(T) - back;
+      next_b = (pair_b(pair + 1) - pair_b(pair)) * op.plane_b * (int)sizeof(T) - back;
+      at_k = 0;
+      ++pair;
+    }
 #pragma unroll
     for (int i = 0; i < S::kFetch; ++i) {
       char* dst = lds + buffer * S::kBuffer + (i * S::kThreads + wave * 64) * 16;
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src[i],
                                        (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
-      src[i] += kBlockBytes;
+      src[i] += i < S::kFetchA ? next_a : next_b;
     }
   };
   auto wait = [&]() {  // this wave's pieces are in LDS and its reads are done; then everyone's are
@@ -194,9 +226,10 @@ struct LogitArgs {
   float unit;
   int64_t ignore_index;
   float z_loss;
-  void* delta;         // [rows_padded][ldd]
-  int64_t ldd;
-  void* delta_t;       // [padded classes of the piece][rows_padded]
+  void* delta;         // [rows_padded][ldd], planes plane_d apart
+  int64_t ldd, plane_d;
+  void* delta_t;       // [padded classes of the piece][ldt], planes rows_padded apart
+  int64_t ldt;
 };
 
 // Adds the biases of a block's classes, which lie in LDS as floats, -infinity behind the last class.
@@ -236,15 +269,24 @@ __device__ __forceinline__ uint2 pack4(const float (&g)[4]) {
   return p.u;
 }
 
-template <typename T, typename S, bool DELTA>
+// z -> its part that bfloat16 holds, and what is left of it
+__device__ __forceinline__ float take_plane(float& z) {
+  const float h = (float)(__bf16)z;
+  z -= h;
+  return h;
+}
+
+// T: the tensors' type; SPLIT: float32 by planes of bfloat16
+template <typename T, typename S, bool DELTA, bool SPLIT>
 __global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
+  typedef std::conditional_t<SPLIT, __bf16, T> O;
   __shared__ __attribute__((aligned(16))) char lds[S::kLds];
   const int tm_count = (a.op.M + S::BM - 1) / S::BM, tn_count = (a.op.N + S::BN - 1) / S::BN;
   int tm, tn;
   tile_of(blockIdx.x, tm_count, tn_count, tm, tn);
   const int m0 = tm * S::BM, n0 = tn * S::BN;
   Tile<S> t;
-  tile_product<T, S>(a.op, m0, n0, 0, a.op.kblocks, lds, t);
+  tile_product<O, S, SPLIT>(a.op, m0, n0, 0, (SPLIT ? kPairs : 1) * a.op.kblocks, lds, t);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
   const int half = lane >> 5;
   const bool biased = a.bias || m0 + S::BM > a.op.M;
@@ -295,7 +337,7 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
       const float factor = scale * slope_of(a.z_loss, top, ls);
       const Exponent ex(top, kLog2e);
       const float shift = ex.shift - ls;
-      T* d = (T*)a.delta + (int64_t)row * a.ldd;
+      O* d = (O*)a.delta + (int64_t)row * a.ldd;
 #pragma unroll
       for (int i = 0; i < S::IM; ++i) {
         const int v32 = m0 + (wm * S::IM + i) * 32;
@@ -314,30 +356,40 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
         }
 #pragma unroll
         for (int r8 = 0; r8 < 2; ++r8) {  // two groups of 8 classes, four of each in either half of the wave
-          const float g[2][4] = {{z[8 * r8], z[8 * r8 + 1], z[8 * r8 + 2], z[8 * r8 + 3]},
-                                 {z[8 * r8 + 4], z[8 * r8 + 5], z[8 * r8 + 6], z[8 * r8 + 7]}};
-          if constexpr (sizeof(T) == 4) {
+          if constexpr (sizeof(O) == 4) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-              const int v0 = v32 + 16 * r8 + 8 * u + 4 * half;
-              if (a.delta) *(f32x4*)(d + v0) = f32x4{g[u][0], g[u][1], g[u][2], g[u][3]};
+              const int v0 = v32 + 16 * r8 + 8 * u + 4 * half, r = 8 * r8 + 4 * u;
+              if (a.delta) *(f32x4*)(d + v0) = f32x4{z[r], z[r + 1], z[r + 2], z[r + 3]};
               if (a.delta_t)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) ((T*)a.delta_t)[(int64_t)(v0 + e) * a.rows_padded + row] = g[u][e];
+                for (int e = 0; e < 4; ++e) ((O*)a.delta_t)[(int64_t)(v0 + e) * a.ldt + row] = z[r + e];
             }
           } else {
-            const uint2 p0 = pack4<T>(g[0]), p1 = pack4<T>(g[1]);
-            if (a.delta) {
-              // the halves trade: the lower lanes get all 8 classes of the first group, the upper ones those of the second
-              const auto x = __builtin_amdgcn_permlane32_swap(p0.x, p1.x, false, false);
-              const auto y = __builtin_amdgcn_permlane32_swap(p0.y, p1.y, false, false);
-              *(u32x4*)(d + v32 + 16 * r8 + 8 * half) = u32x4{x[0], y[0], x[1], y[1]};
-            }
-            if (a.delta_t) {
 #pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                const int v = v32 + 16 * r8 + 8 * u + 4 * half + (lane & 3);
-                *(uint2*)((T*)a.delta_t + (int64_t)v * a.rows_padded + (row & ~3)) = transpose4(u ? p1 : p0);
+            for (int plane = 0; plane < (SPLIT ? 3 : 1); ++plane) {
+              float g[2][4];
+#pragma unroll
+              for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  float rest = z[8 * r8 + 4 * u + e];
+                  g[u][e] = SPLIT ? take_plane(rest) : rest;
+                  z[8 * r8 + 4 * u + e] = rest;
+                }
+              const uint2 p0 = pack4<O>(g[0]), p1 = pack4<O>(g[1]);
+              if (a.delta) {
+                // the halves trade: the lower lanes get all 8 classes of the first group, the upper ones those of the second
+                const auto x = __builtin_amdgcn_permlane32_swap(p0.x, p1.x, false, false);
+                const auto y = __builtin_amdgcn_permlane32_swap(p0.y, p1.y, false, false);
+                *(u32x4*)(d + plane * a.plane_d + v32 + 16 * r8 + 8 * half) = u32x4{x[0], y[0], x[1], y[1]};
+              }
+              if (a.delta_t) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                  const int v = v32 + 16 * r8 + 8 * u + 4 * half + (lane & 3);
+                  *(uint2*)((O*)a.delta_t + (int64_t)v * a.ldt + plane * a.rows_padded + (row & ~3)) = transpose4(u ? p1 : p0);
+                }
               }
             }
           }
@@ -494,6 +546,51 @@ __global__ __launch_bounds__(kThreads) void k_pad(const T* __restrict__ in, int6
     }
 }
 
+// out [rows][3][cols_padded]: the planes of in [rows, cols], zeros behind.  The first plane is cut off instead of rounded
+// where rounding would leave bfloat16's range.
+struct Planes {
+  u32x4 h, m, l;
+};
+__device__ __forceinline__ Planes planes_of(const float (&v)[8]) {
+  bf16x8 h, m, l;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float x = v[e];
+    h[e] = (__bf16)x;
+    if (fabsf((float)h[e]) == __uint_as_float(0x7F800000u)) h[e] = (__bf16)__uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
+    x -= (float)h[e];
+    m[e] = (__bf16)x;
+    x -= (float)m[e];
+    l[e] = (__bf16)x;
+  }
+  return {__builtin_bit_cast(u32x4, h), __builtin_bit_cast(u32x4, m), __builtin_bit_cast(u32x4, l)};
+}
+__global__ __launch_bounds__(kThreads) void k_split(const float* __restrict__ in, int64_t stride, int64_t rows, int cols,
+                                                    int cols_padded, __bf16* __restrict__ out) {
+  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+  for (int64_t r = (int64_t)blockIdx.x * 4 + y; r < rows; r += (int64_t)gridDim.x * 4)
+    for (int c = x * 8; c < cols_padded; c += 64 * 8) {
+      const float* p = in + r * stride + c;
+      float v[8];
+      if (c + 8 <= cols) {
+        const u32x4 a = load16(p), b = load16(p + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] = __uint_as_float(a[e]);
+          v[4 + e] = __uint_as_float(b[e]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? p[e] : 0.0f;
+      }
+      const Planes q = planes_of(v);
+      __bf16* o = out + r * 3 * cols_padded + c;
+      *(u32x4*)o = q.h;
+      *(u32x4*)(o + cols_padded) = q.m;
+      *(u32x4*)(o + 2 * (int64_t)cols_padded) = q.l;
+    }
+}
+
 // out [cols, rows_padded] = in^T, zeros behind; a row that cannot contribute (its target is ignored, no class of it is
 // left, its scale is 0, or, of the weight, its bias is -infinity) reads as zeros, so that a NaN in it does not meet the
 // zero of its derivative.  in: rows the main loop could take.
@@ -551,6 +648,33 @@ __global__ __launch_bounds__(kThreads) void k_transpose(const T* __restrict__ in
   }
 }
 
+// The same by planes: out [cols][3][rows_padded].
+__global__ __launch_bounds__(kThreads) void k_transpose_split(const float* __restrict__ in, int64_t stride, int64_t rows,
+                                                              int cols, int64_t rows_padded, Contributes with,
+                                                              __bf16* __restrict__ out) {
+  __shared__ float tile[64][65];
+  const int64_t tiles_c = (cols + 63) / 64;
+  const int64_t r0 = blockIdx.x / tiles_c * 64;
+  const int c0 = (int)(blockIdx.x % tiles_c) * 64;
+  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+  for (int i = y; i < 64; i += 4)
+    tile[i][x] = c0 + x < cols && r0 + i < rows && with.row<float>(r0 + i) ? in[(r0 + i) * stride + c0 + x] : 0.0f;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int at = i * kThreads + threadIdx.x, c = at >> 3, piece = at & 7;
+    if (c0 + c >= cols) continue;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = tile[8 * piece + e][c];
+    const Planes q = planes_of(v);
+    __bf16* o = out + (int64_t)(c0 + c) * 3 * rows_padded + r0 + 8 * piece;
+    *(u32x4*)o = q.h;
+    *(u32x4*)(o + rows_padded) = q.m;
+    *(u32x4*)(o + 2 * rows_padded) = q.l;
+  }
+}
+
 // ------------------------------------------------------------------------------------------------------------------
 // the two gradient products
 // ------------------------------------------------------------------------------------------------------------------
@@ -564,18 +688,18 @@ struct GradArgs {
   OutScale scale;
 };
 
-template <typename T, typename S>
+template <typename T, typename S, bool SPLIT>
 __global__ __launch_bounds__(S::kThreads) void k_ce_grad(GradArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[S::kLds];
   const int tm_count = (a.op.M + S::BM - 1) / S::BM, tn_count = (a.op.N + S::BN - 1) / S::BN;
   const int tiles = tm_count * tn_count, split = blockIdx.x / tiles;
   int tm, tn;
   tile_of(blockIdx.x % tiles, tm_count, tn_count, tm, tn);
-  const int per = (a.op.kblocks + a.splits - 1) / a.splits;
-  const int k0 = min(split * per, a.op.kblocks), k1 = min(k0 + per, a.op.kblocks);
+  const int steps = (SPLIT ? kPairs : 1) * a.op.kblocks, per = (steps + a.splits - 1) / a.splits;
+  const int k0 = min(split * per, steps), k1 = min(k0 + per, steps);
   const int m0 = tm * S::BM, n0 = tn * S::BN;
   Tile<S> t;
-  tile_product<T, S>(a.op, m0, n0, k0, k1, lds, t);
+  tile_product<std::conditional_t<SPLIT, __bf16, T>, S, SPLIT>(a.op, m0, n0, k0, k1, lds, t);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
   const float scale = a.sum ? 1.0f : a.scale.get();
 #pragma unroll
@@ -649,21 +773,24 @@ __global__ __launch_bounds__(kThreads) void k_ce_finish(const float* __restrict_
 }
 
 // grad_bias: sums of the rows of d^T, the values that grad_weight is made of; a block per class and part of its row
-template <typename T>
-__global__ __launch_bounds__(kThreads) void k_ce_bias(const T* __restrict__ delta_t, int64_t rows_padded, int64_t rows,
-                                                      int classes, int parts, float* __restrict__ sum, OutScale out_scale,
-                                                      T* __restrict__ out) {
+template <typename T, bool SPLIT>
+__global__ __launch_bounds__(kThreads) void k_ce_bias(const void* __restrict__ delta_t, int64_t ldt, int64_t rows_padded,
+                                                      int64_t rows, int classes, int parts, float* __restrict__ sum,
+                                                      OutScale out_scale, T* __restrict__ out) {
+  typedef std::conditional_t<SPLIT, __bf16, T> O;
   __shared__ float red[4];
   const int c = blockIdx.x % classes, part = blockIdx.x / classes;
-  const T* d = delta_t + (int64_t)c * rows_padded;
-  const int64_t vectors = rows / Kind<T>::E, per = (vectors + parts - 1) / parts;
+  const int64_t vectors = rows / Kind<O>::E, per = (vectors + parts - 1) / parts;
   const int64_t end = min(vectors, (part + 1) * per);
   float s = 0.0f;
-  for (int64_t i = part * per + threadIdx.x; i < end; i += kThreads) {
-    float x[Kind<T>::E];
-    unpack(load16(d + i * Kind<T>::E), x, (const T*)nullptr);
+  for (int plane = SPLIT ? 2 : 0; plane >= 0; --plane) {
+    const O* d = (const O*)delta_t + (int64_t)c * ldt + plane * rows_padded;
+    for (int64_t i = part * per + threadIdx.x; i < end; i += kThreads) {
+      float x[Kind<O>::E];
+      unpack(load16(d + i * Kind<O>::E), x, (const O*)nullptr);
 #pragma unroll
-    for (int e = 0; e < Kind<T>::E; ++e) s += x[e];
+      for (int e = 0; e < Kind<O>::E; ++e) s += x[e];
+    }
   }
   s = block_add<4>(s, red);
   if (threadIdx.x) return;
@@ -714,16 +841,66 @@ struct Arena {
   }
 };
 
+struct Plan {
+  int shape, splits;  // of the tiles of a product, and of its K
+  double time;        // estimated, microseconds
+};
+enum { kLarge, kSmall, kNarrow };
+struct ShapeInfo {
+  int bm, bn, slots;             // tile, and how many of it the 256 CUs hold at once
+  float step16, step32, around;  // microseconds of a step of K with all slots taken (16-bit types, float32), and of a tile's
+                                 // beginning and end
+};
+// Measured on products of 2048..8192 rows (large: 1240 TFLOP/s in bfloat16, small: 850; float32: 105).
+constexpr ShapeInfo kShapes[] = {{Large::BM, Large::BN, 256, 1.7f, 0.0f, 4.0f},
+                                 {Small::BM, Small::BN, 512, 1.3f, 5.0f, 2.5f},
+                                 {Narrow::BM, Narrow::BN, 768, 1.1f, 4.0f, 2.0f}};
+// Shape of the tiles of a product M x N over `blocks` steps of K, and into how many parts K is cut: the least of the waves
+// of tiles times their length, plus the traffic of the partial sums.  float32 leaves out the large tile: its epilogue
+// does not fit the registers, and its matrix instructions are eight times slower, so that its loads never bind.
+Plan plan_of(int64_t M, int64_t N, int64_t blocks, int type, bool may_split) {
+  Plan best{kSmall, 1, 1e300};
+  for (int shape = type == VSL_TYPE_F32 ? kSmall : kLarge; shape <= kNarrow; ++shape) {
+    const ShapeInfo& h = kShapes[shape];
+    const double tiles = (double)(ceil_div(M, h.bm) * ceil_div(N, h.bn));
+    const double step = type == VSL_TYPE_F32 ? h.step32 : h.step16;
+    for (int s = 1; s <= 256 && (s == 1 || (may_split && blocks / s >= 4)); s = s < 16 ? s + 1 : s + s / 4) {
+      // a CU that holds fewer tiles than it could runs each of them faster, though not in proportion
+      const double full = (double)(int64_t)(tiles * s / h.slots), rest = tiles * s - full * h.slots;
+      const double per_cu = h.slots / 256.0, held = (double)(int64_t)((rest + 255) / 256);
+      double t = (full + (rest > 0 ? 0.1 + 0.9 * held / per_cu : 0.0)) * ((double)ceil_div(blocks, s) * step + h.around);
+      if (s > 1) t += 4.0 + (double)s * (double)M * (double)N * 8.0 / 4e6;
+      if (t < best.time) best = {shape, s, t};
+    }
+  }
+  return best;
+}
+int64_t blocks_of(int64_t K, int type) { return ceil_div(K * size_of(type), kBlockBytes); }
+
+
+// How the operands of the products lie: elements of `size` bytes, `planes` of them a value, BK elements a step.
 struct Layout {
+  bool split;          // float32 by planes of bfloat16
+  int type, size, planes;
   int64_t rows_padded, dim_padded;
   bool copy_hidden, copy_weight;
+  int64_t steps(int64_t K) const { return (split ? kPairs : 1) * blocks_of(K, type); }
 };
 Layout layout_of(const vsl_linear_ce_desc* d) {
-  Layout l;
+  Layout l{};
   l.rows_padded = round_up(d->rows, kPad);
-  l.dim_padded = round_up(d->dim, kBlockBytes / size_of(d->type));
-  l.copy_hidden = !ready(d->hidden, d->hidden_stride, d->dim, d->type);
-  l.copy_weight = !ready(d->weight, d->weight_stride, d->dim, d->type);
+  if (d->type == VSL_TYPE_F32) {
+    // the planes are worth writing (10 bytes a value) where they save more on the logits than that
+    const double direct = plan_of(d->vocab, d->rows, blocks_of(d->dim, VSL_TYPE_F32), VSL_TYPE_F32, false).time;
+    const double planes = plan_of(d->vocab, d->rows, kPairs * blocks_of(d->dim, VSL_TYPE_BF16), VSL_TYPE_BF16, false).time;
+    l.split = planes + 10.0 + (double)(d->rows + d->vocab) * (double)d->dim * 10.0 / 4e6 < direct;
+  }
+  l.type = l.split ? VSL_TYPE_BF16 : d->type;
+  l.size = size_of(l.type);
+  l.planes = l.split ? 3 : 1;
+  l.dim_padded = round_up(d->dim, kBlockBytes / l.size);
+  l.copy_hidden = l.split || !ready(d->hidden, d->hidden_stride, d->dim, d->type);
+  l.copy_weight = l.split || !ready(d->weight, d->weight_stride, d->dim, d->type);
   return l;
 }
 
@@ -736,7 +913,7 @@ struct Forward {
 };
 Forward forward_workspace(const vsl_linear_ce_desc* d, void* base) {
   const Layout l = layout_of(d);
-  const int s = size_of(d->type);
+  const int s = l.size * l.planes;
   Arena a{(char*)base};
   Forward f{};
   f.hidden = l.copy_hidden ? a.take((size_t)d->rows * l.dim_padded * s) : nullptr;
@@ -755,9 +932,6 @@ constexpr int64_t kPieceElements = 1LL << 27;
 
 constexpr int64_t kBiasBlocks = 1024;
 
-struct Plan {
-  int shape, splits;  // of the tiles of a product, and of its K
-};
 struct Backward {
   Layout l;
   int64_t piece, pieces, vocab_padded;
@@ -766,44 +940,10 @@ struct Backward {
   float *sum_h, *sum_w, *sum_b, *row_scale, *out_scale, *largest;
   size_t total;
 };
-enum { kLarge, kSmall, kNarrow };
-struct ShapeInfo {
-  int bm, bn, slots;             // tile, and how many of it the 256 CUs hold at once
-  float step16, step32, around;  // microseconds of a step of K with all slots taken (16-bit types, float32), and of a tile's
-                                 // beginning and end
-};
-// Measured on products of 2048..8192 rows (large: 1240 TFLOP/s in bfloat16, small: 850; float32: 105).
-constexpr ShapeInfo kShapes[] = {{Large::BM, Large::BN, 256, 1.7f, 0.0f, 4.0f},
-                                 {Small::BM, Small::BN, 512, 1.3f, 5.0f, 2.5f},
-                                 {Narrow::BM, Narrow::BN, 768, 1.1f, 4.0f, 2.0f}};
-// Shape of the tiles of a product M x N over `blocks` steps of K, and into how many parts K is cut: the least of the waves
-// of tiles times their length, plus the traffic of the partial sums.  float32 leaves out the large tile: its epilogue
-// does not fit the registers, and its matrix instructions are eight times slower, so that its loads never bind.
-Plan plan_of(int64_t M, int64_t N, int64_t blocks, int type, bool may_split) {
-  Plan best{kSmall, 1};
-  double least = 1e300;
-  for (int shape = type == VSL_TYPE_F32 ? kSmall : kLarge; shape <= kNarrow; ++shape) {
-    const ShapeInfo& h = kShapes[shape];
-    const double tiles = (double)(ceil_div(M, h.bm) * ceil_div(N, h.bn));
-    const double step = type == VSL_TYPE_F32 ? h.step32 : h.step16;
-    for (int s = 1; s <= 256 && (s == 1 || (may_split && blocks / s >= 4)); s = s < 16 ? s + 1 : s + s / 4) {
-      const double waves = (double)(int64_t)((tiles * s + h.slots - 1) / h.slots);
-      double t = waves * ((double)ceil_div(blocks, s) * step + h.around);
-      if (s > 1) t += 4.0 + (double)s * (double)M * (double)N * 8.0 / 4e6;
-      if (t < least) {
-        least = t;
-        best = {shape, s};
-      }
-    }
-  }
-  return best;
-}
-int64_t blocks_of(int64_t K, int type) { return ceil_div(K * size_of(type), kBlockBytes); }
-
 Backward backward_workspace(const vsl_linear_ce_desc* d, uint32_t mask, void* base) {
   Backward b{};
   b.l = layout_of(d);
-  const int s = size_of(d->type);
+  const int s = b.l.size * b.l.planes;
   b.piece = kPieceElements / (b.l.rows_padded > 0 ? b.l.rows_padded : 1) / kPad * kPad;
   if (b.piece < kPad) b.piece = kPad;
   if (b.piece > round_up(d->vocab, kPad)) b.piece = round_up(d->vocab, kPad);
@@ -817,8 +957,8 @@ Backward backward_workspace(const vsl_linear_ce_desc* d, uint32_t mask, void* ba
   b.weight_t = gh ? a.take((size_t)d->dim * b.vocab_padded * s) : nullptr;
   b.delta = gh ? a.take((size_t)b.l.rows_padded * b.piece * s) : nullptr;
   b.delta_t = gw || gb ? a.take((size_t)b.l.rows_padded * b.piece * s) : nullptr;
-  b.plan_h = plan_of(d->dim, d->rows, blocks_of(b.piece, d->type), d->type, true);
-  b.plan_w = plan_of(d->dim, d->vocab < b.piece ? d->vocab : b.piece, blocks_of(d->rows, d->type), d->type, true);
+  b.plan_h = plan_of(d->dim, d->rows, b.l.steps(b.piece), b.l.type, true);
+  b.plan_w = plan_of(d->dim, d->vocab < b.piece ? d->vocab : b.piece, b.l.steps(d->rows), b.l.type, true);
   b.sum_h = gh && (b.pieces > 1 || b.plan_h.splits > 1) ? (float*)a.take((size_t)b.plan_h.splits * d->rows * d->dim * 4) : nullptr;
   b.sum_w = gw && b.plan_w.splits > 1 ? (float*)a.take((size_t)b.plan_w.splits * b.piece * d->dim * 4) : nullptr;
   b.sum_b = gb && d->rows >= 8192 && d->vocab <= kBiasBlocks / 2 ? (float*)a.take(kBiasBlocks * 4) : nullptr;
@@ -834,62 +974,72 @@ dim3 linear_grid(int64_t n) {
   return dim3((unsigned)(b < 1 ? 1 : (b > 65536 ? 65536 : b)));
 }
 
-template <typename T>
+unsigned pad_blocks(int64_t rows) { return (unsigned)(ceil_div(rows, 4) < 16384 ? ceil_div(rows, 4) : 16384); }
+template <typename T, bool SPLIT>
 void launch_pad(const void* in, int64_t stride, int64_t rows, int64_t cols, int64_t cols_padded, void* out, hipStream_t s) {
-  hipLaunchKernelGGL(k_pad<T>, dim3((unsigned)(ceil_div(rows, 4) < 16384 ? ceil_div(rows, 4) : 16384)), dim3(kThreads), 0, s, (const T*)in, stride, rows, (int)cols,
-                     (int)cols_padded, (T*)out);
+  if constexpr (SPLIT)
+    hipLaunchKernelGGL(k_split, dim3(pad_blocks(rows)), dim3(kThreads), 0, s, (const float*)in, stride, rows, (int)cols,
+                       (int)cols_padded, (__bf16*)out);
+  else
+    hipLaunchKernelGGL(k_pad<T>, dim3(pad_blocks(rows)), dim3(kThreads), 0, s, (const T*)in, stride, rows, (int)cols,
+                       (int)cols_padded, (T*)out);
 }
-template <typename T>
+template <typename T, bool SPLIT>
 void launch_transpose(const void* in, int64_t stride, int64_t rows, int64_t cols, int64_t rows_padded, const Contributes& with,
                       void* out, hipStream_t s) {
-  hipLaunchKernelGGL(k_transpose<T>, dim3((unsigned)(ceil_div(rows_padded, 64) * ceil_div(cols, 64))), dim3(kThreads), 0, s,
-                     (const T*)in, stride, rows, (int)cols, rows_padded, with, (T*)out);
+  const dim3 grid((unsigned)(ceil_div(rows_padded, 64) * ceil_div(cols, 64)));
+  if constexpr (SPLIT)
+    hipLaunchKernelGGL(k_transpose_split, grid, dim3(kThreads), 0, s, (const float*)in, stride, rows, (int)cols, rows_padded,
+                       with, (__bf16*)out);
+  else
+    hipLaunchKernelGGL(k_transpose<T>, grid, dim3(kThreads), 0, s, (const T*)in, stride, rows, (int)cols, rows_padded, with,
+                       (T*)out);
 }
 
-template <typename T, typename S, bool DELTA>
+template <typename T, typename S, bool DELTA, bool SPLIT>
 int launch_logits_as(const LogitArgs& a, hipStream_t s) {
   const int64_t tm = ceil_div(a.op.M, S::BM), tn = ceil_div(a.op.N, S::BN);
-  hipLaunchKernelGGL((k_ce_logits<T, S, DELTA>), dim3((unsigned)(tm * tn)), dim3(S::kThreads), 0, s, a);
+  hipLaunchKernelGGL((k_ce_logits<T, S, DELTA, SPLIT>), dim3((unsigned)(tm * tn)), dim3(S::kThreads), 0, s, a);
   return (int)tm;
 }
-template <typename T, bool DELTA>
+template <typename T, bool DELTA, bool SPLIT>
 int launch_logits(const LogitArgs& a, int shape, hipStream_t s) {  // returns the rows of tiles
-  if constexpr (sizeof(T) == 2)
-    if (shape == kLarge) return launch_logits_as<T, Large, DELTA>(a, s);
-  if (shape == kNarrow) return launch_logits_as<T, Narrow, DELTA>(a, s);
-  return launch_logits_as<T, Small, DELTA>(a, s);
+  if constexpr (sizeof(T) == 2 || SPLIT)
+    if (shape == kLarge) return launch_logits_as<T, Large, DELTA, SPLIT>(a, s);
+  if (shape == kNarrow) return launch_logits_as<T, Narrow, DELTA, SPLIT>(a, s);
+  return launch_logits_as<T, Small, DELTA, SPLIT>(a, s);
 }
-template <typename T, typename S>
+template <typename T, typename S, bool SPLIT>
 void launch_grad_as(const GradArgs& g, hipStream_t s) {
   const int64_t tiles = ceil_div(g.op.M, S::BM) * ceil_div(g.op.N, S::BN);
-  hipLaunchKernelGGL((k_ce_grad<T, S>), dim3((unsigned)(tiles * g.splits)), dim3(S::kThreads), 0, s, g);
+  hipLaunchKernelGGL((k_ce_grad<T, S, SPLIT>), dim3((unsigned)(tiles * g.splits)), dim3(S::kThreads), 0, s, g);
 }
-template <typename T>
+template <typename T, bool SPLIT>
 void launch_grad(GradArgs g, const Plan& p, hipStream_t s) {
   g.splits = p.splits;
   g.whole = g.op.M % 4 == 0 && (uintptr_t)g.out % 16 == 0;
-  if constexpr (sizeof(T) == 2)
-    if (p.shape == kLarge) return launch_grad_as<T, Large>(g, s);
-  if (p.shape == kNarrow) return launch_grad_as<T, Narrow>(g, s);
-  launch_grad_as<T, Small>(g, s);
+  if constexpr (sizeof(T) == 2 || SPLIT)
+    if (p.shape == kLarge) return launch_grad_as<T, Large, SPLIT>(g, s);
+  if (p.shape == kNarrow) return launch_grad_as<T, Narrow, SPLIT>(g, s);
+  launch_grad_as<T, Small, SPLIT>(g, s);
 }
 
-template <typename T>
-void run_forward(const vsl_linear_ce_desc* d, const Forward& f, float* row_loss, float* stats, float* loss, float* divisor,
-                 hipStream_t s) {
-  const Layout l = layout_of(d);
+template <typename T, bool SPLIT>
+void run_forward(const vsl_linear_ce_desc* d, const Layout& l, const Forward& f, float* row_loss, float* stats, float* loss,
+                 float* divisor, hipStream_t s) {
+  typedef std::conditional_t<SPLIT, __bf16, T> O;
   LogitArgs a{};
-  if (l.copy_hidden) launch_pad<T>(d->hidden, d->hidden_stride, d->rows, d->dim, l.dim_padded, f.hidden, s);
-  if (l.copy_weight) launch_pad<T>(d->weight, d->weight_stride, d->vocab, d->dim, l.dim_padded, f.weight, s);
+  if (l.copy_hidden) launch_pad<T, SPLIT>(d->hidden, d->hidden_stride, d->rows, d->dim, l.dim_padded, f.hidden, s);
+  if (l.copy_weight) launch_pad<T, SPLIT>(d->weight, d->weight_stride, d->vocab, d->dim, l.dim_padded, f.weight, s);
   a.op = {l.copy_weight ? f.weight : d->weight, l.copy_hidden ? f.hidden : d->hidden,
-          l.copy_weight ? l.dim_padded : d->weight_stride, l.copy_hidden ? l.dim_padded : d->hidden_stride,
-          (int)d->vocab, (int)d->rows, (int)(l.dim_padded / Kind<T>::BK)};
+          l.copy_weight ? l.planes * l.dim_padded : d->weight_stride, l.copy_hidden ? l.planes * l.dim_padded : d->hidden_stride,
+          (int)d->vocab, (int)d->rows, (int)(l.dim_padded / Kind<O>::BK), l.dim_padded, l.dim_padded};
   a.bias = d->bias;
   a.target = d->target;
   a.rows_padded = l.rows_padded;
   a.partial = f.partial;
   a.target_logit = f.target_logit;
-  const int tiles = launch_logits<T, false>(a, plan_of(a.op.M, a.op.N, a.op.kblocks, d->type, false).shape, s);
+  const int tiles = launch_logits<T, false, SPLIT>(a, plan_of(a.op.M, a.op.N, l.steps(d->dim), l.type, false).shape, s);
   // few rows: more lanes each, so that no lane walks many tiles (16 rows of 512 tiles: 14 us with 16 lanes a row)
   const int per_block = tiles > 64 && d->rows <= 2048 ? 4 : 16;
   hipLaunchKernelGGL(per_block == 4 ? k_ce_rows<4> : k_ce_rows<16>, dim3((unsigned)ceil_div(d->rows, per_block)),
@@ -899,9 +1049,10 @@ void run_forward(const vsl_linear_ce_desc* d, const Forward& f, float* row_loss,
     launch_sum(row_loss, nullptr, d->target, d->ignore_index, d->rows, d->reduction, f.sums, loss, divisor, s);
 }
 
-template <typename T>
+template <typename T, bool SPLIT>
 void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* stats, const float* divisor, const float* g_loss,
                   T* grad_hidden, T* grad_weight, T* grad_bias, hipStream_t s) {
+  typedef std::conditional_t<SPLIT, __bf16, T> O;
   const Layout& l = b.l;
   // float16 keeps 2^-14 as its smallest normal number: with the largest gradient at 2^12 (a derivative is at most that) a
   // probability down to 2^-26 keeps all its bits
@@ -930,22 +1081,27 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
     hipLaunchKernelGGL(k_ce_largest, dim3(sc.partials), dim3(kThreads), 0, s, sc);
     hipLaunchKernelGGL(k_ce_scale, dim3((unsigned)ceil_div(l.rows_padded, kThreads)), dim3(kThreads), 0, s, sc);
   }
-  if (l.copy_hidden) launch_pad<T>(d->hidden, d->hidden_stride, d->rows, d->dim, l.dim_padded, b.hidden, s);
-  if (l.copy_weight) launch_pad<T>(d->weight, d->weight_stride, d->vocab, d->dim, l.dim_padded, b.weight, s);
-  const T* hidden = (const T*)(l.copy_hidden ? b.hidden : d->hidden);
-  const T* weight = (const T*)(l.copy_weight ? b.weight : d->weight);
-  const int64_t ldh = l.copy_hidden ? l.dim_padded : d->hidden_stride, ldw = l.copy_weight ? l.dim_padded : d->weight_stride;
-  if (grad_weight) launch_transpose<T>(hidden, ldh, d->rows, d->dim, l.rows_padded,
-                                        Contributes{d->target, stats, row_scale, nullptr, d->ignore_index}, b.hidden_t, s);
-  if (grad_hidden) launch_transpose<T>(weight, ldw, d->vocab, d->dim, b.vocab_padded,
-                                        Contributes{nullptr, nullptr, nullptr, d->bias, 0}, b.weight_t, s);
+  if (l.copy_hidden) launch_pad<T, SPLIT>(d->hidden, d->hidden_stride, d->rows, d->dim, l.dim_padded, b.hidden, s);
+  if (l.copy_weight) launch_pad<T, SPLIT>(d->weight, d->weight_stride, d->vocab, d->dim, l.dim_padded, b.weight, s);
+  const O* hidden = (const O*)(l.copy_hidden ? b.hidden : d->hidden);
+  const O* weight = (const O*)(l.copy_weight ? b.weight : d->weight);
+  const int64_t ldh = l.copy_hidden ? l.planes * l.dim_padded : d->hidden_stride;
+  const int64_t ldw = l.copy_weight ? l.planes * l.dim_padded : d->weight_stride;
+  // the transposed operands come from rows the main loop could take, by planes from the tensors themselves
+  if (grad_weight)
+    launch_transpose<T, SPLIT>(SPLIT ? d->hidden : hidden, SPLIT ? d->hidden_stride : ldh, d->rows, d->dim, l.rows_padded,
+                               Contributes{d->target, stats, row_scale, nullptr, d->ignore_index}, b.hidden_t, s);
+  if (grad_hidden)
+    launch_transpose<T, SPLIT>(SPLIT ? d->weight : weight, SPLIT ? d->weight_stride : ldw, d->vocab, d->dim, b.vocab_padded,
+                               Contributes{nullptr, nullptr, nullptr, d->bias, 0}, b.weight_t, s);
   for (int64_t p = 0; p < b.pieces; ++p) {
     const int64_t v0 = p * b.piece, classes = d->vocab - v0 < b.piece ? d->vocab - v0 : b.piece;
-    const int shape = plan_of(classes, d->rows, l.dim_padded / Kind<T>::BK, d->type, false).shape;
+    const int shape = plan_of(classes, d->rows, l.steps(d->dim), l.type, false).shape;
     // what the derivative kernel covers: whole steps of K for the two products that follow
     const int64_t padded = round_up(classes, kShapes[shape].bm), rows_covered = round_up(d->rows, kShapes[shape].bn);
     LogitArgs a{};
-    a.op = {weight + v0 * ldw, hidden, ldw, ldh, (int)classes, (int)d->rows, (int)(l.dim_padded / Kind<T>::BK)};
+    a.op = {weight + v0 * ldw, hidden, ldw, ldh, (int)classes, (int)d->rows, (int)(l.dim_padded / Kind<O>::BK), l.dim_padded,
+            l.dim_padded};
     a.bias = d->bias;
     a.target = d->target;
     a.class0 = v0;
@@ -956,25 +1112,29 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
     a.ignore_index = d->ignore_index;
     a.z_loss = d->z_loss;
     a.delta = grad_hidden ? b.delta : nullptr;
-    a.ldd = b.piece;
+    a.ldd = l.planes * b.piece;
+    a.plane_d = b.piece;
+    a.ldt = l.planes * l.rows_padded;
     a.delta_t = grad_weight || grad_bias ? b.delta_t : nullptr;
-    launch_logits<T, true>(a, shape, s);
+    launch_logits<T, true, SPLIT>(a, shape, s);
     if (grad_hidden) {
       GradArgs g{};
-      g.op = {(const T*)b.weight_t + v0, b.delta, b.vocab_padded, b.piece, (int)d->dim, (int)d->rows, (int)(padded / Kind<T>::BK)};
+      g.op = {(const O*)b.weight_t + v0, b.delta, l.planes * b.vocab_padded, l.planes * b.piece, (int)d->dim, (int)d->rows,
+              (int)(padded / Kind<O>::BK), b.vocab_padded, b.piece};
       g.add = p > 0;
       g.sum = b.sum_h;
       g.out = grad_hidden;
       g.scale = scale;
-      launch_grad<T>(g, b.plan_h, s);
+      launch_grad<T, SPLIT>(g, b.plan_h, s);
     }
     if (grad_weight) {
       GradArgs g{};
-      g.op = {b.hidden_t, b.delta_t, l.rows_padded, l.rows_padded, (int)d->dim, (int)classes, (int)(rows_covered / Kind<T>::BK)};
+      g.op = {b.hidden_t, b.delta_t, l.planes * l.rows_padded, l.planes * l.rows_padded, (int)d->dim, (int)classes,
+              (int)(rows_covered / Kind<O>::BK), l.rows_padded, l.rows_padded};
       g.sum = b.sum_w;
       g.out = grad_weight + v0 * d->dim;
       g.scale = scale;
-      launch_grad<T>(g, b.plan_w, s);
+      launch_grad<T, SPLIT>(g, b.plan_w, s);
       if (g.sum)
         hipLaunchKernelGGL(k_ce_finish<T>, linear_grid(classes * d->dim), dim3(kThreads), 0, s, (const float*)g.sum, b.plan_w.splits,
                            classes * d->dim, scale, (T*)g.out);
@@ -982,8 +1142,8 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
     if (grad_bias) {
       // few classes: their rows in parts, so that more than a block per class works on them
       const int parts = b.sum_b ? (int)(kBiasBlocks / classes < 1 ? 1 : kBiasBlocks / classes) : 1;
-      hipLaunchKernelGGL(k_ce_bias<T>, dim3((unsigned)(classes * parts)), dim3(kThreads), 0, s, (const T*)b.delta_t,
-                         l.rows_padded, rows_covered, (int)classes, parts, parts > 1 ? b.sum_b : nullptr, scale, grad_bias + v0);
+      hipLaunchKernelGGL((k_ce_bias<T, SPLIT>), dim3((unsigned)(classes * parts)), dim3(kThreads), 0, s,
+                         (const void*)b.delta_t, l.planes * l.rows_padded, l.rows_padded, rows_covered, (int)classes, parts, parts > 1 ? b.sum_b : nullptr, scale, grad_bias + v0);
       if (parts > 1)
         hipLaunchKernelGGL(k_ce_finish<T>, linear_grid(classes), dim3(kThreads), 0, s, (const float*)b.sum_b, parts, classes,
                            scale, grad_bias + v0);
@@ -1034,12 +1194,11 @@ int vsl_linear_ce_fwd(const vsl_linear_ce_desc* d, float* row_loss, float* stats
   hipStream_t s = (hipStream_t)stream;
   if (d->rows == 0) {
     if (d->reduction != VSL_REDUCE_NONE) launch_sum(row_loss, nullptr, d->target, d->ignore_index, 0, d->reduction, f.sums, loss, divisor, s);
-  } else if (d->type == VSL_TYPE_F32) {
-    run_forward<float>(d, f, row_loss, stats, loss, divisor, s);
-  } else if (d->type == VSL_TYPE_BF16) {
-    run_forward<__bf16>(d, f, row_loss, stats, loss, divisor, s);
   } else {
-    run_forward<_Float16>(d, f, row_loss, stats, loss, divisor, s);
+    const Layout l = layout_of(d);
+    auto run = d->type == VSL_TYPE_BF16 ? run_forward<__bf16, false> : d->type == VSL_TYPE_F16 ? run_forward<_Float16, false>
+               : l.split ? run_forward<float, true> : run_forward<float, false>;
+    run(d, l, f, row_loss, stats, loss, divisor, s);
   }
   return launch_status("linear_ce");
 }
@@ -1064,11 +1223,12 @@ int vsl_linear_ce_bwd(const vsl_linear_ce_desc* d, const float* stats, const flo
   const Backward b = backward_workspace(d, mask, workspace);
   if (int rc = check_space(workspace, workspace_bytes, b.total)) return rc;
   if (d->type == VSL_TYPE_F32)
-    run_backward<float>(d, b, stats, divisor, g_loss, (float*)grad_hidden, (float*)grad_weight, (float*)grad_bias, s);
+    (b.l.split ? run_backward<float, true> : run_backward<float, false>)(d, b, stats, divisor, g_loss, (float*)grad_hidden,
+                                                                         (float*)grad_weight, (float*)grad_bias, s);
   else if (d->type == VSL_TYPE_BF16)
-    run_backward<__bf16>(d, b, stats, divisor, g_loss, (__bf16*)grad_hidden, (__bf16*)grad_weight, (__bf16*)grad_bias, s);
+    run_backward<__bf16, false>(d, b, stats, divisor, g_loss, (__bf16*)grad_hidden, (__bf16*)grad_weight, (__bf16*)grad_bias, s);
   else
-    run_backward<_Float16>(d, b, stats, divisor, g_loss, (_Float16*)grad_hidden, (_Float16*)grad_weight, (_Float16*)grad_bias, s);
+    run_backward<_Float16, false>(d, b, stats, divisor, g_loss, (_Float16*)grad_hidden, (_Float16*)grad_weight, (_Float16*)grad_bias, s);
   return launch_status("linear_ce backward");
 }
 
