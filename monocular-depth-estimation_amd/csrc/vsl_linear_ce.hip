@@ -414,14 +414,16 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
   }
 }
 
-// R rows a block, 256 / R lanes each: joins the tiles' maxima and sums, four of a lane's at a time.
-template <int R>
-__global__ __launch_bounds__(kThreads) void k_ce_rows(const float2* __restrict__ partial, int64_t rows_padded, int tiles,
+// R rows a block, THREADS / R lanes each: joins the tiles' maxima and sums, four of a lane's at a time.  A block that has
+// all rows also closes the reduced loss.
+template <int R, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_ce_rows(const float2* __restrict__ partial, int64_t rows_padded, int tiles,
                                                       const float* __restrict__ target_logit,
                                                       const int64_t* __restrict__ target, int64_t ignore_index, int64_t vocab,
                                                       float z_loss, int64_t rows, float* __restrict__ row_loss,
-                                                      float* __restrict__ stats) {
-  constexpr int P = kThreads / R;
+                                                      float* __restrict__ stats, int reduction, float* __restrict__ loss_out,
+                                                      float* __restrict__ divisor) {
+  constexpr int P = THREADS / R;
   __shared__ float2 part[P][R];
   const int r = threadIdx.x % R, g = threadIdx.x / R;
   const int64_t row = (int64_t)blockIdx.x * R + r;
@@ -444,17 +446,36 @@ __global__ __launch_bounds__(kThreads) void k_ce_rows(const float2* __restrict__
       part[g][r] = make_float2(q.m, q.s);
     }
   }
+  float loss = 0.0f;
+  bool counts = false;
   if (g == 0 && row < rows) {
     const float ls = log2_sum(q), lse = log_sum(q, 1.0f);
-    float m = q.m, loss = 0.0f;
+    float m = q.m;
     const int64_t t = target[row];
-    if (t != ignore_index) {
+    counts = t != ignore_index;
+    if (counts) {
       if (t < 0 || t >= vocab) loss = m = qnan();
       else if (m != ninf()) loss = fmaf(ls, kLn2, m - target_logit[row]) + (z_loss == 0.0f ? 0.0f : z_loss * lse * lse);
     }
     row_loss[row] = loss;
     stats[row] = m;
     stats[rows + row] = ls;
+  }
+  if (!loss_out) return;
+  __shared__ double sum[2][R];
+  __syncthreads();
+  if (g == 0) {
+    sum[0][r] = (double)loss;
+    sum[1][r] = counts ? 1.0 : 0.0;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double total = 0.0, count = 0.0;
+    for (int i = 0; i < R; ++i) {
+      total += sum[0][i];
+      count += sum[1][i];
+    }
+    finish_sum(total, count, reduction, loss_out, divisor);
   }
 }
 
@@ -527,27 +548,37 @@ __global__ __launch_bounds__(kThreads) void k_ce_scale(ScaleArgs a) {
 // ------------------------------------------------------------------------------------------------------------------
 // layouts
 // ------------------------------------------------------------------------------------------------------------------
-// out [rows, cols_padded] = in [rows, cols], zeros behind: 16 bytes a thread, from rows that may start anywhere
-template <typename T>
-__global__ __launch_bounds__(kThreads) void k_pad(const T* __restrict__ in, int64_t stride, int64_t rows, int cols,
-                                                  int cols_padded, T* __restrict__ out) {
-  constexpr int E = Kind<T>::E;
-  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
-  for (int64_t r = (int64_t)blockIdx.x * 4 + y; r < rows; r += (int64_t)gridDim.x * 4)
-    for (int c = x * E; c < cols_padded; c += 64 * E) {
-      float v[E];
-      if (c + E <= cols) {
-        *(u32x4*)(out + r * cols_padded + c) = load16(in + r * stride + c);
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = c + e < cols ? (float)in[r * stride + c + e] : 0.0f;
-        *(u32x4*)(out + r * cols_padded + c) = pack(v, (const T*)nullptr);
-      }
-    }
-}
+// Everything that has to be laid out for the products goes in one launch, as jobs with a run of blocks each:
+//   copy       out [rows][planes][width] = in [rows, cols], zeros behind
+//   transpose  out [cols][planes][width] = in^T, zeros behind; a row that cannot contribute (its target is ignored, no
+//              class of it is left, its scale is 0, or, of the weight, its bias is -infinity) reads as zeros, so that a NaN
+//              in it does not meet the zero of its derivative
+struct Contributes {
+  const int64_t* target;
+  const float* stats;
+  const float* scale;
+  const void* bias;
+  int64_t ignore_index;
+  template <typename T>
+  __device__ __forceinline__ bool row(int64_t r) const {
+    if (target && (target[r] == ignore_index || stats[r] == ninf())) return false;
+    return !(scale && scale[r] == 0.0f) && !(bias && (float)((const T*)bias)[r] == ninf());
+  }
+};
+struct LayoutJob {
+  const void* in;
+  void* out;
+  int64_t stride, rows, width;  // of in, of in, of out
+  int cols;
+  bool transpose;
+  Contributes with;
+  int64_t blocks;
+};
+struct LayoutJobs {
+  LayoutJob job[4];
+};
 
-// out [rows][3][cols_padded]: the planes of in [rows, cols], zeros behind.  The first plane is cut off instead of rounded
-// where rounding would leave bfloat16's range.
+// A float's three planes.  The first is cut off instead of rounded where rounding would leave bfloat16's range.
 struct Planes {
   u32x4 h, m, l;
 };
@@ -565,63 +596,70 @@ __device__ __forceinline__ Planes planes_of(const float (&v)[8]) {
   }
   return {__builtin_bit_cast(u32x4, h), __builtin_bit_cast(u32x4, m), __builtin_bit_cast(u32x4, l)};
 }
-__global__ __launch_bounds__(kThreads) void k_split(const float* __restrict__ in, int64_t stride, int64_t rows, int cols,
-                                                    int cols_padded, __bf16* __restrict__ out) {
-  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
-  for (int64_t r = (int64_t)blockIdx.x * 4 + y; r < rows; r += (int64_t)gridDim.x * 4)
-    for (int c = x * 8; c < cols_padded; c += 64 * 8) {
-      const float* p = in + r * stride + c;
-      float v[8];
-      if (c + 8 <= cols) {
-        const u32x4 a = load16(p), b = load16(p + 4);
+// eight floats of a row, zeros behind the last column
+__device__ __forceinline__ void load8(const float* p, int c, int cols, float (&v)[8]) {
+  if (c + 8 <= cols) {
+    const u32x4 a = load16(p + c), b = load16(p + c + 4);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] = __uint_as_float(a[e]);
-          v[4 + e] = __uint_as_float(b[e]);
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? p[e] : 0.0f;
-      }
-      const Planes q = planes_of(v);
-      __bf16* o = out + r * 3 * cols_padded + c;
-      *(u32x4*)o = q.h;
-      *(u32x4*)(o + cols_padded) = q.m;
-      *(u32x4*)(o + 2 * (int64_t)cols_padded) = q.l;
+    for (int e = 0; e < 4; ++e) {
+      v[e] = __uint_as_float(a[e]);
+      v[4 + e] = __uint_as_float(b[e]);
     }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? p[c + e] : 0.0f;
+  }
+}
+// 16 bytes of a row that may start anywhere, zeros behind the last column
+template <typename T>
+__device__ __forceinline__ u32x4 load_columns(const T* p, int c, int cols) {
+  if (c + Kind<T>::E <= cols) return load16(p + c);
+  float v[Kind<T>::E];
+#pragma unroll
+  for (int e = 0; e < Kind<T>::E; ++e) v[e] = c + e < cols ? (float)p[c + e] : 0.0f;
+  return pack(v, (const T*)nullptr);
+}
+template <typename O>
+__device__ __forceinline__ void store_planes(O* out, int64_t width, const Planes& q) {
+  *(u32x4*)out = q.h;
+  *(u32x4*)(out + width) = q.m;
+  *(u32x4*)(out + 2 * width) = q.l;
 }
 
-// out [cols, rows_padded] = in^T, zeros behind; a row that cannot contribute (its target is ignored, no class of it is
-// left, its scale is 0, or, of the weight, its bias is -infinity) reads as zeros, so that a NaN in it does not meet the
-// zero of its derivative.  in: rows the main loop could take.
-struct Contributes {
-  const int64_t* target;
-  const float* stats;
-  const float* scale;
-  const void* bias;
-  int64_t ignore_index;
-  template <typename T>
-  __device__ __forceinline__ bool row(int64_t r) const {
-    if (target && (target[r] == ignore_index || stats[r] == ninf())) return false;
-    return !(scale && scale[r] == 0.0f) && !(bias && (float)((const T*)bias)[r] == ninf());
+template <typename T, bool SPLIT>
+__device__ __forceinline__ void copy_job(const LayoutJob& j, int64_t block) {
+  constexpr int E = SPLIT ? 8 : Kind<T>::E;
+  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+  for (int64_t r = block * 4 + y; r < j.rows; r += j.blocks * 4) {
+    const T* p = (const T*)j.in + r * j.stride;
+    for (int64_t c = x * E; c < j.width; c += 64 * E) {
+      if constexpr (SPLIT) {
+        float v[8];
+        load8(p, (int)c, j.cols, v);
+        store_planes((__bf16*)j.out + r * 3 * j.width + c, j.width, planes_of(v));
+      } else {
+        *(u32x4*)((T*)j.out + r * j.width + c) = load_columns(p, (int)c, j.cols);
+      }
+    }
   }
-};
-template <typename T>
-__global__ __launch_bounds__(kThreads) void k_transpose(const T* __restrict__ in, int64_t stride, int64_t rows, int cols,
-                                                        int64_t rows_padded, Contributes with, T* __restrict__ out) {
-  const int64_t tiles_c = (cols + 63) / 64;
-  const int64_t r0 = blockIdx.x / tiles_c * 64;
-  const int c0 = (int)(blockIdx.x % tiles_c) * 64;
+}
+
+template <typename T, bool SPLIT>
+__device__ __forceinline__ void transpose_job(const LayoutJob& j, int64_t block, char* lds) {
+  const int64_t tiles_c = (j.cols + 63) / 64;
+  const int64_t r0 = block / tiles_c * 64;
+  const int c0 = (int)(block % tiles_c) * 64;
+  const T* in = (const T*)j.in;
   if constexpr (sizeof(T) == 2) {
     // A thread takes eight columns of two rows and leaves eight words of two rows each in the columns' lines; a line is
     // 32 words, turned by four words per group of eight columns so that the groups' words meet in different banks.
-    __shared__ __attribute__((aligned(16))) unsigned tile[64 * 32];
+    unsigned* tile = (unsigned*)lds;
     {
       const int g = threadIdx.x & 7, rp = threadIdx.x >> 3, c = c0 + 8 * g;
       const int64_t r = r0 + 2 * rp;
-      const u32x4 none{0u, 0u, 0u, 0u};
-      const u32x4 x = c < cols && r < rows && with.row<T>(r) ? *(const u32x4*)(in + r * stride + c) : none;
-      const u32x4 y = c < cols && r + 1 < rows && with.row<T>(r + 1) ? *(const u32x4*)(in + (r + 1) * stride + c) : none;
+      u32x4 x{0u, 0u, 0u, 0u}, y = x;
+      if (c < j.cols && r < j.rows && j.with.row<T>(r)) x = load_columns(in + r * j.stride, c, j.cols);
+      if (c < j.cols && r + 1 < j.rows && j.with.row<T>(r + 1)) y = load_columns(in + (r + 1) * j.stride, c, j.cols);
       unsigned* t = tile + 8 * g * 32 + ((rp + 4 * g) & 31);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -633,46 +671,42 @@ __global__ __launch_bounds__(kThreads) void k_transpose(const T* __restrict__ in
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int at = i * kThreads + threadIdx.x, c = at >> 3, piece = at & 7;
-      if (c0 + c < cols)
-        *(u32x4*)(out + (int64_t)(c0 + c) * rows_padded + r0 + 8 * piece) =
+      if (c0 + c < j.cols)
+        *(u32x4*)((T*)j.out + (int64_t)(c0 + c) * j.width + r0 + 8 * piece) =
             *(const u32x4*)(tile + c * 32 + ((4 * piece + 4 * (c >> 3)) & 31));
     }
   } else {
-    __shared__ T tile[64][65];
+    float(*tile)[65] = (float(*)[65])lds;
     const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
     for (int i = y; i < 64; i += 4)
-      tile[i][x] = c0 + x < cols && r0 + i < rows && with.row<T>(r0 + i) ? in[(r0 + i) * stride + c0 + x] : (T)0.0f;
+      tile[i][x] = c0 + x < j.cols && r0 + i < j.rows && j.with.row<T>(r0 + i) ? in[(r0 + i) * j.stride + c0 + x] : 0.0f;
     __syncthreads();
-    for (int i = y; i < 64; i += 4)
-      if (c0 + i < cols) out[(int64_t)(c0 + i) * rows_padded + r0 + x] = tile[x][i];
+    if constexpr (SPLIT) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int at = i * kThreads + threadIdx.x, c = at >> 3, piece = at & 7;
+        if (c0 + c >= j.cols) continue;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = tile[8 * piece + e][c];
+        store_planes((__bf16*)j.out + (int64_t)(c0 + c) * 3 * j.width + r0 + 8 * piece, j.width, planes_of(v));
+      }
+    } else {
+      for (int i = y; i < 64; i += 4)
+        if (c0 + i < j.cols) ((T*)j.out)[(int64_t)(c0 + i) * j.width + r0 + x] = tile[x][i];
+    }
   }
 }
 
-// The same by planes: out [cols][3][rows_padded].
-__global__ __launch_bounds__(kThreads) void k_transpose_split(const float* __restrict__ in, int64_t stride, int64_t rows,
-                                                              int cols, int64_t rows_padded, Contributes with,
-                                                              __bf16* __restrict__ out) {
-  __shared__ float tile[64][65];
-  const int64_t tiles_c = (cols + 63) / 64;
-  const int64_t r0 = blockIdx.x / tiles_c * 64;
-  const int c0 = (int)(blockIdx.x % tiles_c) * 64;
-  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
-  for (int i = y; i < 64; i += 4)
-    tile[i][x] = c0 + x < cols && r0 + i < rows && with.row<float>(r0 + i) ? in[(r0 + i) * stride + c0 + x] : 0.0f;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int at = i * kThreads + threadIdx.x, c = at >> 3, piece = at & 7;
-    if (c0 + c >= cols) continue;
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = tile[8 * piece + e][c];
-    const Planes q = planes_of(v);
-    __bf16* o = out + (int64_t)(c0 + c) * 3 * rows_padded + r0 + 8 * piece;
-    *(u32x4*)o = q.h;
-    *(u32x4*)(o + rows_padded) = q.m;
-    *(u32x4*)(o + 2 * rows_padded) = q.l;
-  }
+template <typename T, bool SPLIT>
+__global__ __launch_bounds__(kThreads) void k_layout(LayoutJobs jobs) {
+  __shared__ __attribute__((aligned(16))) char lds[64 * 65 * 4];
+  int64_t block = blockIdx.x;
+  int n = 0;
+  while (block >= jobs.job[n].blocks) block -= jobs.job[n++].blocks;  // the grid is the sum of the jobs' blocks
+  const LayoutJob& j = jobs.job[n];
+  if (j.transpose) transpose_job<T, SPLIT>(j, block, lds);
+  else copy_job<T, SPLIT>(j, block);
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -688,13 +722,22 @@ struct GradArgs {
   OutScale scale;
 };
 
+// one or both products of a piece: the first job's blocks, then the second's
+struct GradJobs {
+  GradArgs job[2];
+  unsigned first;  // blocks of the first
+};
+
 template <typename T, typename S, bool SPLIT>
-__global__ __launch_bounds__(S::kThreads) void k_ce_grad(GradArgs a) {
+__global__ __launch_bounds__(S::kThreads) void k_ce_grad(GradJobs jobs) {
+  const int which = blockIdx.x >= jobs.first ? 1 : 0;
+  const GradArgs& a = jobs.job[which];
+  const int block = blockIdx.x - (which ? jobs.first : 0u);
   __shared__ __attribute__((aligned(16))) char lds[S::kLds];
   const int tm_count = (a.op.M + S::BM - 1) / S::BM, tn_count = (a.op.N + S::BN - 1) / S::BN;
-  const int tiles = tm_count * tn_count, split = blockIdx.x / tiles;
+  const int tiles = tm_count * tn_count, split = block / tiles;
   int tm, tn;
-  tile_of(blockIdx.x % tiles, tm_count, tn_count, tm, tn);
+  tile_of(block % tiles, tm_count, tn_count, tm, tn);
   const int steps = (SPLIT ? kPairs : 1) * a.op.kblocks, per = (steps + a.splits - 1) / a.splits;
   const int k0 = min(split * per, steps), k1 = min(k0 + per, steps);
   const int m0 = tm * S::BM, n0 = tn * S::BN;
@@ -740,25 +783,40 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_grad(GradArgs a) {
   }
 }
 
-// out = out_scale * the sum of the splits, in their order: four elements a thread, the splits dealt to the four waves
+// out = scale * the sum of the splits, in their order: four elements a thread, the splits dealt to the four waves; up to
+// three sums in one launch.
+struct FinishJob {
+  const float* sum;
+  void* out;
+  int splits;
+  int64_t n;
+  int64_t blocks;
+};
+struct FinishJobs {
+  FinishJob job[3];
+  OutScale scale;
+};
 template <typename T>
-__global__ __launch_bounds__(kThreads) void k_ce_finish(const float* __restrict__ sum, int splits, int64_t n,
-                                                        OutScale out_scale, T* __restrict__ out) {
+__global__ __launch_bounds__(kThreads) void k_ce_finish(FinishJobs jobs) {
   __shared__ f32x4 part[3][64];
-  const float scale = out_scale.get();
+  int64_t block = blockIdx.x;
+  int which = 0;
+  while (block >= jobs.job[which].blocks) block -= jobs.job[which++].blocks;  // the grid is the sum of the jobs' blocks
+  const FinishJob& j = jobs.job[which];
+  const float scale = jobs.scale.get();
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int per = (splits + 3) / 4, s0 = wave * per, s1 = min(splits, s0 + per);
-  for (int64_t i0 = (int64_t)blockIdx.x * 256; i0 < n; i0 += (int64_t)gridDim.x * 256) {
+  const int per = (j.splits + 3) / 4, s0 = wave * per, s1 = min(j.splits, s0 + per);
+  for (int64_t i0 = block * 256; i0 < j.n; i0 += j.blocks * 256) {
     const int64_t i = i0 + 4 * lane;
     f32x4 v{0.0f, 0.0f, 0.0f, 0.0f};
-    if (n % 4 == 0) {
-      if (i < n)
-        for (int s = s0; s < s1; ++s) v += *(const f32x4*)(sum + s * n + i);
+    if (j.n % 4 == 0) {
+      if (i < j.n)
+        for (int s = s0; s < s1; ++s) v += *(const f32x4*)(j.sum + s * j.n + i);
     } else {
       for (int s = s0; s < s1; ++s)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (i + e < n) v[e] += sum[s * n + i + e];
+          if (i + e < j.n) v[e] += j.sum[s * j.n + i + e];
     }
     __syncthreads();
     if (wave) part[wave - 1][lane] = v;
@@ -768,7 +826,7 @@ __global__ __launch_bounds__(kThreads) void k_ce_finish(const float* __restrict_
     for (int w = 0; w < 3; ++w) v += part[w][lane];
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (i + e < n) out[i + e] = (T)(scale * v[e]);
+      if (i + e < j.n) ((T*)j.out)[i + e] = (T)(scale * v[e]);
   }
 }
 
@@ -974,27 +1032,41 @@ dim3 linear_grid(int64_t n) {
   return dim3((unsigned)(b < 1 ? 1 : (b > 65536 ? 65536 : b)));
 }
 
-unsigned pad_blocks(int64_t rows) { return (unsigned)(ceil_div(rows, 4) < 16384 ? ceil_div(rows, 4) : 16384); }
-template <typename T, bool SPLIT>
-void launch_pad(const void* in, int64_t stride, int64_t rows, int64_t cols, int64_t cols_padded, void* out, hipStream_t s) {
-  if constexpr (SPLIT)
-    hipLaunchKernelGGL(k_split, dim3(pad_blocks(rows)), dim3(kThreads), 0, s, (const float*)in, stride, rows, (int)cols,
-                       (int)cols_padded, (__bf16*)out);
-  else
-    hipLaunchKernelGGL(k_pad<T>, dim3(pad_blocks(rows)), dim3(kThreads), 0, s, (const T*)in, stride, rows, (int)cols,
-                       (int)cols_padded, (T*)out);
-}
-template <typename T, bool SPLIT>
-void launch_transpose(const void* in, int64_t stride, int64_t rows, int64_t cols, int64_t rows_padded, const Contributes& with,
-                      void* out, hipStream_t s) {
-  const dim3 grid((unsigned)(ceil_div(rows_padded, 64) * ceil_div(cols, 64)));
-  if constexpr (SPLIT)
-    hipLaunchKernelGGL(k_transpose_split, grid, dim3(kThreads), 0, s, (const float*)in, stride, rows, (int)cols, rows_padded,
-                       with, (__bf16*)out);
-  else
-    hipLaunchKernelGGL(k_transpose<T>, grid, dim3(kThreads), 0, s, (const T*)in, stride, rows, (int)cols, rows_padded, with,
-                       (T*)out);
-}
+struct LayoutLaunch {
+  LayoutJobs jobs{};
+  int n = 0;
+  int64_t blocks = 0;
+  void add(const LayoutJob& j) {
+    jobs.job[n++] = j;
+    blocks += j.blocks;
+  }
+  void copy(const void* in, int64_t stride, int64_t rows, int64_t cols, int64_t width, void* out) {
+    const int64_t b = ceil_div(rows, 4);
+    add({in, out, stride, rows, width, (int)cols, false, {}, b < 16384 ? b : 16384});
+  }
+  void transpose(const void* in, int64_t stride, int64_t rows, int64_t cols, int64_t width, const Contributes& with, void* out) {
+    add({in, out, stride, rows, width, (int)cols, true, with, width / 64 * ceil_div(cols, 64)});
+  }
+  template <typename T, bool SPLIT>
+  void run(hipStream_t s) {
+    if (n) hipLaunchKernelGGL((k_layout<T, SPLIT>), dim3((unsigned)blocks), dim3(kThreads), 0, s, jobs);
+  }
+};
+struct FinishLaunch {
+  FinishJobs jobs{};
+  int n = 0;
+  int64_t blocks = 0;
+  void add(const float* sum, int splits, int64_t elements, void* out) {
+    const int64_t b = ceil_div(elements, 256);
+    jobs.job[n++] = {sum, out, splits, elements, b < 65536 ? b : 65536};
+    blocks += jobs.job[n - 1].blocks;
+  }
+  template <typename T>
+  void run(const OutScale& scale, hipStream_t s) {
+    jobs.scale = scale;
+    if (n) hipLaunchKernelGGL(k_ce_finish<T>, dim3((unsigned)blocks), dim3(kThreads), 0, s, jobs);
+  }
+};
 
 template <typename T, typename S, bool DELTA, bool SPLIT>
 int launch_logits_as(const LogitArgs& a, hipStream_t s) {
@@ -1010,18 +1082,31 @@ int launch_logits(const LogitArgs& a, int shape, hipStream_t s) {  // returns th
   return launch_logits_as<T, Small, DELTA, SPLIT>(a, s);
 }
 template <typename T, typename S, bool SPLIT>
-void launch_grad_as(const GradArgs& g, hipStream_t s) {
-  const int64_t tiles = ceil_div(g.op.M, S::BM) * ceil_div(g.op.N, S::BN);
-  hipLaunchKernelGGL((k_ce_grad<T, S, SPLIT>), dim3((unsigned)(tiles * g.splits)), dim3(S::kThreads), 0, s, g);
+void launch_grad_as(const GradArgs* g, int n, hipStream_t s) {
+  GradJobs jobs{};
+  unsigned blocks = 0;
+  for (int i = 0; i < n; ++i) {
+    jobs.job[i] = g[i];
+    if (i) jobs.first = blocks;
+    blocks += (unsigned)(ceil_div(g[i].op.M, S::BM) * ceil_div(g[i].op.N, S::BN) * g[i].splits);
+  }
+  if (n == 1) jobs.first = blocks;
+  hipLaunchKernelGGL((k_ce_grad<T, S, SPLIT>), dim3(blocks), dim3(S::kThreads), 0, s, jobs);
 }
+// n products, one after the other in one launch where their tiles have one shape
 template <typename T, bool SPLIT>
-void launch_grad(GradArgs g, const Plan& p, hipStream_t s) {
-  g.splits = p.splits;
-  g.whole = g.op.M % 4 == 0 && (uintptr_t)g.out % 16 == 0;
+void launch_grad(GradArgs* g, const int* shape, int n, hipStream_t s) {
+  for (int i = 0; i < n; ++i) g[i].whole = g[i].op.M % 4 == 0 && (uintptr_t)g[i].out % 16 == 0;
+  if (n == 2 && shape[0] != shape[1]) {
+    launch_grad<T, SPLIT>(g, shape, 1, s);
+    launch_grad<T, SPLIT>(g + 1, shape + 1, 1, s);
+    return;
+  }
+  if (!n) return;
   if constexpr (sizeof(T) == 2 || SPLIT)
-    if (p.shape == kLarge) return launch_grad_as<T, Large, SPLIT>(g, s);
-  if (p.shape == kNarrow) return launch_grad_as<T, Narrow, SPLIT>(g, s);
-  launch_grad_as<T, Small, SPLIT>(g, s);
+    if (shape[0] == kLarge) return launch_grad_as<T, Large, SPLIT>(g, n, s);
+  if (shape[0] == kNarrow) return launch_grad_as<T, Narrow, SPLIT>(g, n, s);
+  launch_grad_as<T, Small, SPLIT>(g, n, s);
 }
 
 template <typename T, bool SPLIT>
@@ -1029,8 +1114,10 @@ void run_forward(const vsl_linear_ce_desc* d, const Layout& l, const Forward& f,
                  float* divisor, hipStream_t s) {
   typedef std::conditional_t<SPLIT, __bf16, T> O;
   LogitArgs a{};
-  if (l.copy_hidden) launch_pad<T, SPLIT>(d->hidden, d->hidden_stride, d->rows, d->dim, l.dim_padded, f.hidden, s);
-  if (l.copy_weight) launch_pad<T, SPLIT>(d->weight, d->weight_stride, d->vocab, d->dim, l.dim_padded, f.weight, s);
+  LayoutLaunch lay;
+  if (l.copy_hidden) lay.copy(d->hidden, d->hidden_stride, d->rows, d->dim, l.dim_padded, f.hidden);
+  if (l.copy_weight) lay.copy(d->weight, d->weight_stride, d->vocab, d->dim, l.dim_padded, f.weight);
+  lay.run<T, SPLIT>(s);
   a.op = {l.copy_weight ? f.weight : d->weight, l.copy_hidden ? f.hidden : d->hidden,
           l.copy_weight ? l.planes * l.dim_padded : d->weight_stride, l.copy_hidden ? l.planes * l.dim_padded : d->hidden_stride,
           (int)d->vocab, (int)d->rows, (int)(l.dim_padded / Kind<O>::BK), l.dim_padded, l.dim_padded};
@@ -1040,12 +1127,18 @@ void run_forward(const vsl_linear_ce_desc* d, const Layout& l, const Forward& f,
   a.partial = f.partial;
   a.target_logit = f.target_logit;
   const int tiles = launch_logits<T, false, SPLIT>(a, plan_of(a.op.M, a.op.N, l.steps(d->dim), l.type, false).shape, s);
-  // few rows: more lanes each, so that no lane walks many tiles (16 rows of 512 tiles: 14 us with 16 lanes a row)
-  const int per_block = tiles > 64 && d->rows <= 2048 ? 4 : 16;
-  hipLaunchKernelGGL(per_block == 4 ? k_ce_rows<4> : k_ce_rows<16>, dim3((unsigned)ceil_div(d->rows, per_block)),
-                     dim3(kThreads), 0, s, (const float2*)f.partial, l.rows_padded, tiles, (const float*)f.target_logit, d->target, d->ignore_index, d->vocab, d->z_loss,
-                     d->rows, row_loss, stats);
-  if (d->reduction != VSL_REDUCE_NONE)
+  // few rows: more lanes each, so that no lane walks many tiles (16 rows of 512 tiles: 14 us with 16 lanes a row), and
+  // where one block can hold all of them it closes the loss as well
+  const bool reduce = d->reduction != VSL_REDUCE_NONE, one = reduce && d->rows <= 64 && tiles <= 64;
+  auto rows = [&](auto kernel, int per_block, int threads) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(d->rows, per_block)), dim3(threads), 0, s, (const float2*)f.partial,
+                       l.rows_padded, tiles, (const float*)f.target_logit, d->target, d->ignore_index, d->vocab, d->z_loss,
+                       d->rows, row_loss, stats, d->reduction, one ? loss : nullptr, divisor);
+  };
+  if (one) rows(k_ce_rows<64, 1024>, 64, 1024);
+  else if (tiles > 64 && d->rows <= 2048) rows(k_ce_rows<4, kThreads>, 4, kThreads);
+  else rows(k_ce_rows<16, kThreads>, 16, kThreads);
+  if (reduce && !one)
     launch_sum(row_loss, nullptr, d->target, d->ignore_index, d->rows, d->reduction, f.sums, loss, divisor, s);
 }
 
@@ -1081,19 +1174,20 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
     hipLaunchKernelGGL(k_ce_largest, dim3(sc.partials), dim3(kThreads), 0, s, sc);
     hipLaunchKernelGGL(k_ce_scale, dim3((unsigned)ceil_div(l.rows_padded, kThreads)), dim3(kThreads), 0, s, sc);
   }
-  if (l.copy_hidden) launch_pad<T, SPLIT>(d->hidden, d->hidden_stride, d->rows, d->dim, l.dim_padded, b.hidden, s);
-  if (l.copy_weight) launch_pad<T, SPLIT>(d->weight, d->weight_stride, d->vocab, d->dim, l.dim_padded, b.weight, s);
+  LayoutLaunch lay;
+  if (l.copy_hidden) lay.copy(d->hidden, d->hidden_stride, d->rows, d->dim, l.dim_padded, b.hidden);
+  if (l.copy_weight) lay.copy(d->weight, d->weight_stride, d->vocab, d->dim, l.dim_padded, b.weight);
+  if (grad_weight)
+    lay.transpose(d->hidden, d->hidden_stride, d->rows, d->dim, l.rows_padded,
+                  Contributes{d->target, stats, row_scale, nullptr, d->ignore_index}, b.hidden_t);
+  if (grad_hidden)
+    lay.transpose(d->weight, d->weight_stride, d->vocab, d->dim, b.vocab_padded, Contributes{nullptr, nullptr, nullptr, d->bias, 0},
+                  b.weight_t);
+  lay.run<T, SPLIT>(s);
   const O* hidden = (const O*)(l.copy_hidden ? b.hidden : d->hidden);
   const O* weight = (const O*)(l.copy_weight ? b.weight : d->weight);
   const int64_t ldh = l.copy_hidden ? l.planes * l.dim_padded : d->hidden_stride;
   const int64_t ldw = l.copy_weight ? l.planes * l.dim_padded : d->weight_stride;
-  // the transposed operands come from rows the main loop could take, by planes from the tensors themselves
-  if (grad_weight)
-    launch_transpose<T, SPLIT>(SPLIT ? d->hidden : hidden, SPLIT ? d->hidden_stride : ldh, d->rows, d->dim, l.rows_padded,
-                               Contributes{d->target, stats, row_scale, nullptr, d->ignore_index}, b.hidden_t, s);
-  if (grad_hidden)
-    launch_transpose<T, SPLIT>(SPLIT ? d->weight : weight, SPLIT ? d->weight_stride : ldw, d->vocab, d->dim, b.vocab_padded,
-                               Contributes{nullptr, nullptr, nullptr, d->bias, 0}, b.weight_t, s);
   for (int64_t p = 0; p < b.pieces; ++p) {
     const int64_t v0 = p * b.piece, classes = d->vocab - v0 < b.piece ? d->vocab - v0 : b.piece;
     const int shape = plan_of(classes, d->rows, l.steps(d->dim), l.type, false).shape;
@@ -1117,41 +1211,41 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
     a.ldt = l.planes * l.rows_padded;
     a.delta_t = grad_weight || grad_bias ? b.delta_t : nullptr;
     launch_logits<T, true, SPLIT>(a, shape, s);
+    GradArgs g[2] = {};
+    int shapes[2], n = 0;
+    FinishLaunch finish;
     if (grad_hidden) {
-      GradArgs g{};
-      g.op = {(const O*)b.weight_t + v0, b.delta, l.planes * b.vocab_padded, l.planes * b.piece, (int)d->dim, (int)d->rows,
-              (int)(padded / Kind<O>::BK), b.vocab_padded, b.piece};
-      g.add = p > 0;
-      g.sum = b.sum_h;
-      g.out = grad_hidden;
-      g.scale = scale;
-      launch_grad<T, SPLIT>(g, b.plan_h, s);
+      g[n].op = {(const O*)b.weight_t + v0, b.delta, l.planes * b.vocab_padded, l.planes * b.piece, (int)d->dim, (int)d->rows,
+                 (int)(padded / Kind<O>::BK), b.vocab_padded, b.piece};
+      g[n].add = p > 0;
+      g[n].sum = b.sum_h;
+      g[n].out = grad_hidden;
+      g[n].scale = scale;
+      g[n].splits = b.plan_h.splits;
+      shapes[n++] = b.plan_h.shape;
+      if (b.sum_h && p == b.pieces - 1) finish.add(b.sum_h, b.plan_h.splits, d->rows * d->dim, grad_hidden);
     }
     if (grad_weight) {
-      GradArgs g{};
-      g.op = {b.hidden_t, b.delta_t, l.planes * l.rows_padded, l.planes * l.rows_padded, (int)d->dim, (int)classes,
-              (int)(rows_covered / Kind<O>::BK), l.rows_padded, l.rows_padded};
-      g.sum = b.sum_w;
-      g.out = grad_weight + v0 * d->dim;
-      g.scale = scale;
-      launch_grad<T, SPLIT>(g, b.plan_w, s);
-      if (g.sum)
-        hipLaunchKernelGGL(k_ce_finish<T>, linear_grid(classes * d->dim), dim3(kThreads), 0, s, (const float*)g.sum, b.plan_w.splits,
-                           classes * d->dim, scale, (T*)g.out);
+      g[n].op = {b.hidden_t, b.delta_t, l.planes * l.rows_padded, l.planes * l.rows_padded, (int)d->dim, (int)classes,
+                 (int)(rows_covered / Kind<O>::BK), l.rows_padded, l.rows_padded};
+      g[n].sum = b.sum_w;
+      g[n].out = grad_weight + v0 * d->dim;
+      g[n].scale = scale;
+      g[n].splits = b.plan_w.splits;
+      shapes[n++] = b.plan_w.shape;
+      if (b.sum_w) finish.add(b.sum_w, b.plan_w.splits, classes * d->dim, grad_weight + v0 * d->dim);
     }
+    launch_grad<T, SPLIT>(g, shapes, n, s);
     if (grad_bias) {
       // few classes: their rows in parts, so that more than a block per class works on them
       const int parts = b.sum_b ? (int)(kBiasBlocks / classes < 1 ? 1 : kBiasBlocks / classes) : 1;
       hipLaunchKernelGGL((k_ce_bias<T, SPLIT>), dim3((unsigned)(classes * parts)), dim3(kThreads), 0, s,
-                         (const void*)b.delta_t, l.planes * l.rows_padded, l.rows_padded, rows_covered, (int)classes, parts, parts > 1 ? b.sum_b : nullptr, scale, grad_bias + v0);
-      if (parts > 1)
-        hipLaunchKernelGGL(k_ce_finish<T>, linear_grid(classes), dim3(kThreads), 0, s, (const float*)b.sum_b, parts, classes,
-                           scale, grad_bias + v0);
+                         (const void*)b.delta_t, l.planes * l.rows_padded, l.rows_padded, rows_covered, (int)classes, parts,
+                         parts > 1 ? b.sum_b : nullptr, scale, grad_bias + v0);
+      if (parts > 1) finish.add(b.sum_b, parts, classes, grad_bias + v0);
     }
+    finish.run<T>(scale, s);
   }
-  if (grad_hidden && b.sum_h)
-    hipLaunchKernelGGL(k_ce_finish<T>, linear_grid(d->rows * d->dim), dim3(kThreads), 0, s, (const float*)b.sum_h, b.plan_h.splits,
-                       d->rows * d->dim, scale, grad_hidden);
 }
 
 template <typename T>

@@ -23,11 +23,6 @@ constexpr int64_t kMaxBlocks = 1 << 20;  // blocks of one launch; kernels walk f
 constexpr int kSumBlocks = 256;
 constexpr int64_t kSumRows = 4096;  // rows a block of the first pass takes at least
 
-__device__ __forceinline__ void finish_sum(double total, double count, int reduction, float* loss, float* divisor) {
-  *loss = (float)(reduction == VSL_REDUCE_MEAN ? (count == 0.0 ? 0.0 : total / count) : total);
-  *divisor = (float)count;
-}
-
 __device__ __forceinline__ void block_sum2(double& a, double& b, double* red) {
   for (int m = 32; m >= 1; m >>= 1) {
     a += __shfl_xor(a, m, 64);

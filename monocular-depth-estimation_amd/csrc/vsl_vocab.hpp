@@ -196,6 +196,12 @@ __device__ __forceinline__ float block_add(float v, float* red) {
   return t;
 }
 
+// ---- reduced loss
+__device__ __forceinline__ void finish_sum(double total, double count, int reduction, float* loss, float* divisor) {
+  *loss = (float)(reduction == VSL_REDUCE_MEAN ? (count == 0.0 ? 0.0 : total / count) : total);
+  *divisor = (float)count;
+}
+
 // ---- host side
 inline int launch_status(const char* what) {
   if (hipError_t e = hipGetLastError(); e != hipSuccess)
