@@ -23,7 +23,8 @@ def logits(rows, vocab, seed, dtype, scale=2.5):
 
 
 def close(got, want, tol, what):
-    got, want = got.double().cpu(), want.double().cpu()
+    want = want.double()
+    got = got.detach().double().to(want.device)
     assert got.shape == want.shape
     assert torch.equal(torch.isnan(got), torch.isnan(want)), what
     inf = torch.isinf(want)
@@ -271,7 +272,9 @@ def ce_inputs(rows, vocab, dim, dtype, seed, bias):
 def check_ce(h, w, b, t, ignore_index=-100, z_loss=0.0, on_device=None, upstream=None):
     import mde_amd.vocab_losses as L
     dtype, rows, (vocab, dim) = h.dtype, h.shape[0], w.shape
-    loss, lse, z, ds = O.linear_ce(h, w, t, b, ignore_index, z_loss)
+    at = DEV if rows * vocab > 1 << 20 else "cpu"           # where the definition is evaluated
+    h, w, t, b = h.to(at), w.to(at), t.to(at), None if b is None else b.to(at)
+    loss, lse, z, ds = O.linear_ce(h, w, t, b, ignore_index, z_loss, at)
     ha, wa = on_device if on_device else (h.to(DEV), w.to(DEV))
     ha, wa = ha.detach().requires_grad_(True), wa.detach().requires_grad_(True)
     ba = b.to(DEV).requires_grad_(True) if b is not None else None
@@ -290,7 +293,7 @@ def check_ce(h, w, b, t, ignore_index=-100, z_loss=0.0, on_device=None, upstream
     grads = torch.autograd.grad(out, leaves, upstream.to(DEV), retain_graph=True)
 
     def check_grads(grads, u, extra):
-        u = u.double()[:, None]
+        u = u.double().to(at)[:, None]
         live_rows = (ds != 0).any(1) | torch.isnan(ds).any(1)
         ud = torch.where(live_rows[:, None], ds * u, torch.zeros_like(ds))
         half = O.HALF_STEP[dtype]
@@ -302,15 +305,15 @@ def check_ce(h, w, b, t, ignore_index=-100, z_loss=0.0, on_device=None, upstream
         p = (z - lse[:, None]).exp().masked_fill(~live, 0) * (1 + 2 * z_loss * lse.abs()[:, None])
         perr = (4 * lerr[:, None] + 8 * O.U) * p + 4 * O.U
         derr = torch.nan_to_num((perr * u.abs() + ud.abs() * half * (1 + extra) + floor) * live_rows[:, None])
-        h0 = torch.where(live_rows[:, None], h.double().cpu(), torch.zeros_like(h.double().cpu()))
-        w0 = w.double().cpu()
+        h0 = torch.where(live_rows[:, None], h.double(), torch.zeros_like(h.double()))
+        w0 = w.double()
         if b is not None:
             w0 = torch.where((b == -INF)[:, None], torch.zeros_like(w0), w0)
         n = max(rows, vocab) + 4
         want = ud @ w0
         close(grads[0], want, torch.nan_to_num(derr @ w0.abs() + n * O.U * (ud.abs() @ w0.abs()) + (half + 8 * O.U) * want.abs()) + O.TINY[dtype], "grad hidden")
-        want = ud.T @ h0
-        close(grads[1], want, torch.nan_to_num(derr.T @ h0.abs() + n * O.U * (ud.abs().T @ h0.abs()) + (half + 8 * O.U) * want.abs()) + O.TINY[dtype], "grad weight")
+        want = ud.T.contiguous() @ h0
+        close(grads[1], want, torch.nan_to_num(derr.T.contiguous() @ h0.abs() + n * O.U * (ud.abs().T.contiguous() @ h0.abs()) + (half + 8 * O.U) * want.abs()) + O.TINY[dtype], "grad weight")
         if b is not None:
             want = ud.sum(0)
             close(grads[2], want, torch.nan_to_num(derr.sum(0) + n * O.U * ud.abs().sum(0) + (half + 8 * O.U) * want.abs()) + O.TINY[dtype], "grad bias")
@@ -318,8 +321,8 @@ def check_ce(h, w, b, t, ignore_index=-100, z_loss=0.0, on_device=None, upstream
     check_grads(grads, upstream, 0.01)
     count = int((t != ignore_index).sum())
     mean = L.linear_cross_entropy(ha, wa, t.to(DEV), ba, ignore_index=ignore_index, z_loss=z_loss)
-    s = out.detach().double().sum().cpu()
-    close(mean.detach(), s / count if count else torch.zeros((), dtype=torch.float64), 4 * O.U * s.abs() if torch.isfinite(s) else 0.0, "mean")
+    s = out.detach().double().sum().to(at)
+    close(mean.detach(), s / count if count else torch.zeros((), dtype=torch.float64, device=at), 4 * O.U * s.abs() if torch.isfinite(s) else 0.0, "mean")
     g = torch.autograd.grad(mean, leaves, torch.tensor(3.0, device=DEV), retain_graph=True)
     check_grads(g, torch.full((rows,), 3.0 / max(count, 1)), 0.01)
     total = L.linear_cross_entropy(ha, wa, t.to(DEV), ba, ignore_index=ignore_index, z_loss=z_loss, reduction="sum")
@@ -389,29 +392,44 @@ def test_linear_cross_entropy_strides_alignment_and_no_rows():
     assert hh.grad.shape == (0, 16) and not ww.grad.any() and not bb.grad.any()
 
 
-def test_linear_cross_entropy_several_pieces_of_the_vocabulary():
-    """rows * classes above one piece (2^26 derivatives): the pieces' sums join, the last one is ragged."""
-    import mde_amd.vocab_losses as L
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab,dim,bias", [
+    (1030, 4000, 330, True),        # float32 by planes; every size ragged
+    (2100, 8200, 128, False),       # the large tile
+    (2047, 8191, 96, True),
+    (65, 20000, 64, False),         # just above the narrow tile
+    (64, 20000, 200, True),         # the narrow tile, many tiles a row
+    (9000, 90, 200, True),          # many rows of few classes: the sums over the rows are cut into parts
+    (40, 3000, 1100, False)])
+def test_linear_cross_entropy_tile_shapes(rows, vocab, dim, bias, dtype):
+    h, w, b, t = ce_inputs(rows, vocab, dim, dtype, rows + vocab, bias)
+    t[torch.rand(rows, generator=gen(3)) < 0.2] = -100
+    if bias:
+        b[-5:] = -INF
+        t[t >= vocab - 5] = 1
+    check_ce(h, w, b, t, z_loss=1e-3 if bias else 0.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_cross_entropy_several_pieces_of_the_vocabulary(dtype):
+    """rows * classes above one piece (2^27 derivatives): the pieces' sums join, the last one is ragged."""
     rows, vocab, dim = 2048, 70001, 64
-    g = torch.Generator(device=DEV).manual_seed(5)
-    h = torch.randn(rows, dim, generator=g, device=DEV).bfloat16().requires_grad_(True)
-    w = (torch.randn(vocab, dim, generator=g, device=DEV) * 0.3).bfloat16().requires_grad_(True)
-    t = torch.randint(vocab, (rows,), generator=g, device=DEV)
-    loss = L.linear_cross_entropy(h, w, t)
-    gh, gw = torch.autograd.grad(loss, (h, w))
-    with torch.no_grad():
-        z = h.double() @ w.double().T
-        lse = torch.logsumexp(z, 1, keepdim=True)
-        want = (lse[:, 0] - z.gather(1, t[:, None])[:, 0]).mean()
-        d = (z - lse).exp_()
-        d[torch.arange(rows, device=DEV), t] -= 1
-        d /= rows
-        wh, ww = d @ w.double(), d.T.contiguous() @ h.double()
-        # half a step of bfloat16 for every derivative and for the result
-        th = d.abs() @ w.double().abs() * (2 ** -8 + 2 ** -16) + wh.abs() * 2 ** -8 + 1e-12
-        tw = d.abs().T.contiguous() @ h.double().abs() * (2 ** -8 + 2 ** -16) + ww.abs() * 2 ** -8 + 1e-12
-    assert abs(float(loss) - float(want)) <= 1e-5 * float(want)
-    assert bool(((gh.double() - wh).abs() <= th).all()) and bool(((gw.double() - ww).abs() <= tw).all())
+    h, w, b, t = ce_inputs(rows, vocab, dim, dtype, 5, bias=True)
+    check_ce(h, w, b, t)
+
+
+def test_linear_cross_entropy_of_lowest_values():
+    """Biases of the type's lowest value mask as -infinity does while another class is left, and tie where none is."""
+    for dtype in TYPES:
+        h, w, b, t = ce_inputs(33, 40, 64, dtype, 141, bias=True)
+        t[:] = torch.arange(33) % 30
+        b[30:] = torch.finfo(dtype).min
+        if dtype != torch.float16:                          # float16's lowest value is an ordinary logit
+            check_ce(h, w, b, t)
+            import mde_amd.vocab_losses as L
+            b[:] = torch.finfo(dtype).min
+            out = L.linear_cross_entropy(h.to(DEV), w.to(DEV), t.to(DEV), b.to(DEV), reduction="none")
+            close(out, torch.full((33,), math.log(40), dtype=torch.float64), 1e-5, "uniform rows")
 
 
 # ------------------------------------------------------------------ the three together, streams, graphs, hooks

@@ -77,13 +77,13 @@ def distill(x, values, indices, lse=None, temperature=1.0, weights=None):
     return loss, grad, size
 
 
-def linear_ce(hidden, weight, target, bias=None, ignore_index=-100, z_loss=0.0):
+def linear_ce(hidden, weight, target, bias=None, ignore_index=-100, z_loss=0.0, device="cpu"):
     """(row losses, lse, logits, dS = derivative of every row's loss), NaN rows for targets outside the vocabulary."""
-    h, w = hidden.double().cpu(), weight.double().cpu()
-    target = target.cpu().long()
+    h, w = hidden.double().to(device), weight.double().to(device)
+    target = target.to(device).long()
     z = h @ w.T
     if bias is not None:
-        b = bias.double().cpu()
+        b = bias.double().to(device)
         z = torch.where(b == -float("inf"), b, z + b)
     lse = torch.logsumexp(z, 1)
     live = target != ignore_index
@@ -94,7 +94,7 @@ def linear_ce(hidden, weight, target, bias=None, ignore_index=-100, z_loss=0.0):
     loss = torch.where(live & ~empty, loss, torch.zeros_like(loss))
     loss = torch.where(bad, torch.full_like(loss, float("nan")), loss)
     ds = (z - lse[:, None]).exp() * (1 + 2 * z_loss * lse[:, None])
-    ds[torch.arange(len(target)), at] -= 1
+    ds[torch.arange(len(target), device=device), at] -= 1
     ds = torch.where((live & ~empty)[:, None], ds, torch.zeros_like(ds))
     ds = torch.where(bad[:, None], torch.full_like(ds, float("nan")), ds)
     return loss, lse, z, ds
