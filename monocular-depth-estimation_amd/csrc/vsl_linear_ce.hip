@@ -76,7 +76,10 @@ struct Operands {
   int64_t lda, ldb;
   int M, N, kblocks;
   int64_t plane_a, plane_b;
+  int tail;  // 16-byte pieces of a row in the last block (8: it is whole); what follows them is not the row's
 };
+// what the pieces behind a row's end are read from
+__device__ const u32x4 kZeros[1] = {{0u, 0u, 0u, 0u}};
 constexpr int kPairs = 6;
 // planes of pair p, two bits each: l h, m m, h l, m h, h m, h h (h = 0, m = 1, l = 2)
 __device__ __forceinline__ int pair_a(int p) { return (0x046 >> (2 * p)) & 3; }
@@ -123,7 +126,15 @@ __device__ __forceinline__ void tile_product(const Operands& op, int m0, int n0,
                             : (const char*)op.B + (int64_t)min(n0 + row, op.N - 1) * op.ldb * (int)sizeof(T);
     src[i] += (i < S::kFetchA ? offset_a : offset_b) + piece * 16;
   }
+  int left = k1 - k0;  // steps to fetch
   auto fetch = [&](int buffer) {
+    if (!SPLIT && --left == 0 && k1 == op.kblocks && op.tail < 8) {
+#pragma unroll
+      for (int i = 0; i < S::kFetch; ++i) {
+        const int at = (i < S::kFetchA ? i : i - S::kFetchA) * S::kThreads + tid;
+        if (((at & 7) ^ ((at >> 4) & 7)) >= op.tail) src[i] = (const char*)kZeros;
+      }
+    }
     int64_t next_a = kBlockBytes, next_b = kBlockBytes;
     if (SPLIT && ++at_k == op.kblocks) {  // on to the next pair of planes, from its beginning
       const int64_t back = (int64_t)(op.kblocks - 1) * kBlockBytes;
@@ -883,10 +894,10 @@ int check_ce(const vsl_linear_ce_desc* d) {
   return VSL_OK;
 }
 
-// An operand goes to the main loop as it is when its rows are whole 128-byte blocks that 16-byte loads may read.
+// An operand goes to the main loop as it is when its rows are whole 16-byte pieces at 16-byte addresses.
 bool ready(const void* p, int64_t stride, int64_t dim, int type) {
   const int s = size_of(type);
-  return (uintptr_t)p % 16 == 0 && stride * s % 16 == 0 && dim * s % kBlockBytes == 0;
+  return (uintptr_t)p % 16 == 0 && stride * s % 16 == 0 && dim * s % 16 == 0;
 }
 
 struct Arena {
@@ -942,6 +953,7 @@ struct Layout {
   int type, size, planes;
   int64_t rows_padded, dim_padded;
   bool copy_hidden, copy_weight;
+  int tail;            // Operands::tail of the logits' products
   int64_t steps(int64_t K) const { return (split ? kPairs : 1) * blocks_of(K, type); }
 };
 Layout layout_of(const vsl_linear_ce_desc* d) {
@@ -959,6 +971,9 @@ Layout layout_of(const vsl_linear_ce_desc* d) {
   l.dim_padded = round_up(d->dim, kBlockBytes / l.size);
   l.copy_hidden = l.split || !ready(d->hidden, d->hidden_stride, d->dim, d->type);
   l.copy_weight = l.split || !ready(d->weight, d->weight_stride, d->dim, d->type);
+  // a copy is padded with zeros up to the block's end; beside an operand that is read in place only its pieces count
+  l.tail = l.copy_hidden && l.copy_weight ? 8 : (int)((d->dim * l.size % kBlockBytes + 15) / 16);
+  if (l.tail == 0) l.tail = 8;
   return l;
 }
 
@@ -1120,7 +1135,7 @@ void run_forward(const vsl_linear_ce_desc* d, const Layout& l, const Forward& f,
   lay.run<T, SPLIT>(s);
   a.op = {l.copy_weight ? f.weight : d->weight, l.copy_hidden ? f.hidden : d->hidden,
           l.copy_weight ? l.planes * l.dim_padded : d->weight_stride, l.copy_hidden ? l.planes * l.dim_padded : d->hidden_stride,
-          (int)d->vocab, (int)d->rows, (int)(l.dim_padded / Kind<O>::BK), l.dim_padded, l.dim_padded};
+          (int)d->vocab, (int)d->rows, (int)(l.dim_padded / Kind<O>::BK), l.dim_padded, l.dim_padded, l.tail};
   a.bias = d->bias;
   a.target = d->target;
   a.rows_padded = l.rows_padded;
@@ -1195,7 +1210,7 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
     const int64_t padded = round_up(classes, kShapes[shape].bm), rows_covered = round_up(d->rows, kShapes[shape].bn);
     LogitArgs a{};
     a.op = {weight + v0 * ldw, hidden, ldw, ldh, (int)classes, (int)d->rows, (int)(l.dim_padded / Kind<O>::BK), l.dim_padded,
-            l.dim_padded};
+            l.dim_padded, l.tail};
     a.bias = d->bias;
     a.target = d->target;
     a.class0 = v0;
@@ -1216,7 +1231,7 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
     FinishLaunch finish;
     if (grad_hidden) {
       g[n].op = {(const O*)b.weight_t + v0, b.delta, l.planes * b.vocab_padded, l.planes * b.piece, (int)d->dim, (int)d->rows,
-                 (int)(padded / Kind<O>::BK), b.vocab_padded, b.piece};
+                 (int)(padded / Kind<O>::BK), b.vocab_padded, b.piece, 8};
       g[n].add = p > 0;
       g[n].sum = b.sum_h;
       g[n].out = grad_hidden;
@@ -1227,7 +1242,7 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
     }
     if (grad_weight) {
       g[n].op = {b.hidden_t, b.delta_t, l.planes * l.rows_padded, l.planes * l.rows_padded, (int)d->dim, (int)classes,
-                 (int)(rows_covered / Kind<O>::BK), l.rows_padded, l.rows_padded};
+                 (int)(rows_covered / Kind<O>::BK), l.rows_padded, l.rows_padded, 8};
       g[n].sum = b.sum_w;
       g[n].out = grad_weight + v0 * d->dim;
       g[n].scale = scale;
