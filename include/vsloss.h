@@ -441,8 +441,8 @@ int vsl_top_logits(const vsl_top_desc* desc, void* values, int32_t* indices, flo
  *   p = softmax(logits / T);  row loss = weight * T^2 * (sum_j q_j log(q_j / p_j) + q_t log(q_t / p_t)).
  * A row of weight 0 is not looked at.  An index that occurs twice counts with the sum of its q.
  *
- * vsl_distill_fwd: row_loss [rows] (weighted); loss and divisor: one float each, the reduced loss and the sum of the
- * weights (both NULL for VSL_REDUCE_NONE); stats: float [rows][VSL_DISTILL_STATS], 16-byte aligned, what the
+ * vsl_distill_fwd: row_loss [rows] (weighted; scratch unless VSL_REDUCE_NONE); loss and divisor: one float each, the
+ * reduced loss and the sum of the weights (both NULL for VSL_REDUCE_NONE); stats: float [rows][VSL_DISTILL_STATS], 16-byte aligned, what the
  * backward call needs.
  * vsl_distill_bwd: g_loss: one float, or [rows] for VSL_REDUCE_NONE -> grad: [rows,vocab] of the logits' type, every
  * element written.  The descriptor is the forward call's; `stats` and `divisor` are its outputs.
@@ -476,7 +476,7 @@ int vsl_distill_bwd(const vsl_distill_desc* desc, const float* stats, const floa
  * type before it meets weight and hidden (scaled by its largest value, so that float16 keeps it).
  * A class whose bias is -infinity is masked out, whatever its weights hold.
  *
- * vsl_linear_ce_fwd: row_loss [rows]; stats [2][rows], the maximum of a row's logits and the log2 of its sum of
+ * vsl_linear_ce_fwd: row_loss [rows] (scratch unless VSL_REDUCE_NONE); stats [2][rows], the maximum of a row's logits and the log2 of its sum of
  * exponentials above that (kept apart: a maximum of float32's lowest value would swallow the logarithm); loss and
  * divisor: one float each, the reduced loss and the number of rows that count (both NULL for VSL_REDUCE_NONE).
  * vsl_linear_ce_bwd: g_loss: one float, or [rows] for VSL_REDUCE_NONE; stats and divisor are the forward call's outputs.

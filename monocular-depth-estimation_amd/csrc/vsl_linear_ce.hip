@@ -425,15 +425,15 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
   }
 }
 
-// R rows a block, THREADS / R lanes each: joins the tiles' maxima and sums, four of a lane's at a time.  A block that has
-// all rows also closes the reduced loss.
+// R rows a block, THREADS / R lanes each: joins the tiles' maxima and sums, four of a lane's at a time.  A block also sums
+// its rows' losses: closes the reduced loss if it has all rows, leaves its sums in `pairs` otherwise.
 template <int R, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_ce_rows(const float2* __restrict__ partial, int64_t rows_padded, int tiles,
                                                       const float* __restrict__ target_logit,
                                                       const int64_t* __restrict__ target, int64_t ignore_index, int64_t vocab,
                                                       float z_loss, int64_t rows, float* __restrict__ row_loss,
-                                                      float* __restrict__ stats, int reduction, float* __restrict__ loss_out,
-                                                      float* __restrict__ divisor) {
+                                                      float* __restrict__ stats, int reduction, double* __restrict__ pairs,
+                                                      float* __restrict__ loss_out, float* __restrict__ divisor) {
   constexpr int P = THREADS / R;
   __shared__ float2 part[P][R];
   const int r = threadIdx.x % R, g = threadIdx.x / R;
@@ -472,7 +472,7 @@ __global__ __launch_bounds__(THREADS) void k_ce_rows(const float2* __restrict__ 
     stats[row] = m;
     stats[rows + row] = ls;
   }
-  if (!loss_out) return;
+  if (reduction == VSL_REDUCE_NONE) return;
   __shared__ double sum[2][R];
   __syncthreads();
   if (g == 0) {
@@ -486,7 +486,12 @@ __global__ __launch_bounds__(THREADS) void k_ce_rows(const float2* __restrict__ 
       total += sum[0][i];
       count += sum[1][i];
     }
-    finish_sum(total, count, reduction, loss_out, divisor);
+    if (gridDim.x == 1) {
+      finish_sum(total, count, reduction, loss_out, divisor);
+    } else {
+      pairs[2 * blockIdx.x] = total;
+      pairs[2 * blockIdx.x + 1] = count;
+    }
   }
 }
 
@@ -981,7 +986,7 @@ struct Forward {
   void *hidden, *weight;
   float2* partial;
   float* target_logit;
-  void* sums;
+  double* pairs;
   size_t total;
 };
 Forward forward_workspace(const vsl_linear_ce_desc* d, void* base) {
@@ -993,7 +998,7 @@ Forward forward_workspace(const vsl_linear_ce_desc* d, void* base) {
   f.weight = l.copy_weight ? a.take((size_t)d->vocab * l.dim_padded * s) : nullptr;
   f.partial = (float2*)a.take((size_t)ceil_div(d->vocab, Small::BM) * l.rows_padded * sizeof(float2));
   f.target_logit = (float*)a.take((size_t)d->rows * 4);
-  f.sums = a.take(sum_workspace_bytes(d->rows));
+  f.pairs = (double*)a.take((size_t)ceil_div(d->rows, d->rows <= 2048 ? 4 : 16) * 2 * sizeof(double));
   f.total = a.used;
   return f;
 }
@@ -1142,19 +1147,19 @@ void run_forward(const vsl_linear_ce_desc* d, const Layout& l, const Forward& f,
   a.partial = f.partial;
   a.target_logit = f.target_logit;
   const int tiles = launch_logits<T, false, SPLIT>(a, plan_of(a.op.M, a.op.N, l.steps(d->dim), l.type, false).shape, s);
-  // few rows: more lanes each, so that no lane walks many tiles (16 rows of 512 tiles: 14 us with 16 lanes a row), and
-  // where one block can hold all of them it closes the loss as well
-  const bool reduce = d->reduction != VSL_REDUCE_NONE, one = reduce && d->rows <= 64 && tiles <= 64;
+  // few rows: more lanes each, so that no lane walks many tiles (16 rows of 512 tiles: 14 us with 16 lanes a row); many rows:
+  // more of them a block, so that fewer sums are left
   auto rows = [&](auto kernel, int per_block, int threads) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(d->rows, per_block)), dim3(threads), 0, s, (const float2*)f.partial,
-                       l.rows_padded, tiles, (const float*)f.target_logit, d->target, d->ignore_index, d->vocab, d->z_loss,
-                       d->rows, row_loss, stats, d->reduction, one ? loss : nullptr, divisor);
+    const unsigned blocks = (unsigned)ceil_div(d->rows, per_block);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), 0, s, (const float2*)f.partial, l.rows_padded, tiles,
+                       (const float*)f.target_logit, d->target, d->ignore_index, d->vocab, d->z_loss, d->rows, row_loss, stats,
+                       d->reduction, f.pairs, loss, divisor);
+    if (d->reduction != VSL_REDUCE_NONE && blocks > 1) launch_sum_pairs(f.pairs, blocks, d->reduction, loss, divisor, s);
   };
-  if (one) rows(k_ce_rows<64, 1024>, 64, 1024);
+  if (d->rows <= 64 && tiles <= 64) rows(k_ce_rows<64, 1024>, 64, 1024);
   else if (tiles > 64 && d->rows <= 2048) rows(k_ce_rows<4, kThreads>, 4, kThreads);
+  else if (d->rows >= 32768 || tiles <= 16) rows(k_ce_rows<64, kThreads>, 64, kThreads);
   else rows(k_ce_rows<16, kThreads>, 16, kThreads);
-  if (reduce && !one)
-    launch_sum(row_loss, nullptr, d->target, d->ignore_index, d->rows, d->reduction, f.sums, loss, divisor, s);
 }
 
 template <typename T, bool SPLIT>
@@ -1302,7 +1307,7 @@ int vsl_linear_ce_fwd(const vsl_linear_ce_desc* d, float* row_loss, float* stats
   if (int rc = check_space(workspace, workspace_bytes, f.total)) return rc;
   hipStream_t s = (hipStream_t)stream;
   if (d->rows == 0) {
-    if (d->reduction != VSL_REDUCE_NONE) launch_sum(row_loss, nullptr, d->target, d->ignore_index, 0, d->reduction, f.sums, loss, divisor, s);
+    if (d->reduction != VSL_REDUCE_NONE) launch_sum_pairs(f.pairs, 0, d->reduction, loss, divisor, s);
   } else {
     const Layout l = layout_of(d);
     auto run = d->type == VSL_TYPE_BF16 ? run_forward<__bf16, false> : d->type == VSL_TYPE_F16 ? run_forward<_Float16, false>

@@ -20,9 +20,11 @@ constexpr int64_t kMaxBlocks = 1 << 20;  // blocks of one launch; kernels walk f
 // ------------------------------------------------------------------------------------------------------------------
 // reduced loss
 // ------------------------------------------------------------------------------------------------------------------
-constexpr int kSumBlocks = 256;
-constexpr int64_t kSumRows = 4096;  // rows a block of the first pass takes at least
+constexpr int kSumBlocks = 1024;
+constexpr int64_t kSumRows = 1024;  // rows a block of the first pass takes at least
+constexpr int kFinalThreads = 1024;
 
+template <int WAVES>
 __device__ __forceinline__ void block_sum2(double& a, double& b, double* red) {
   for (int m = 32; m >= 1; m >>= 1) {
     a += __shfl_xor(a, m, 64);
@@ -34,24 +36,24 @@ __device__ __forceinline__ void block_sum2(double& a, double& b, double* red) {
   }
   __syncthreads();
   a = b = 0.0;
-  for (int w = 0; w < kWaves; ++w) {
+  for (int w = 0; w < WAVES; ++w) {
     a += red[2 * w];
     b += red[2 * w + 1];
   }
 }
 
 __global__ __launch_bounds__(kThreads) void k_sum_rows(const float* __restrict__ row_loss, const float* __restrict__ weights,
-                                                       const int64_t* __restrict__ target, int64_t ignore_index, int64_t rows,
-                                                       int64_t per_block, int reduction, double* __restrict__ partial,
-                                                       float* __restrict__ loss, float* __restrict__ divisor) {
+                                                       int64_t rows, int64_t per_block, int reduction,
+                                                       double* __restrict__ partial, float* __restrict__ loss,
+                                                       float* __restrict__ divisor) {
   __shared__ double red[2 * kWaves];
   const int64_t r0 = blockIdx.x * per_block, r1 = min(rows, r0 + per_block);
   double total = 0.0, count = 0.0;
   for (int64_t r = r0 + threadIdx.x; r < r1; r += kThreads) {
     total += (double)row_loss[r];
-    count += weights ? (double)weights[r] : target ? (target[r] == ignore_index ? 0.0 : 1.0) : 1.0;
+    count += weights ? (double)weights[r] : 1.0;
   }
-  block_sum2(total, count, red);
+  block_sum2<kWaves>(total, count, red);
   if (threadIdx.x) return;
   if (gridDim.x == 1) {
     finish_sum(total, count, reduction, loss, divisor);
@@ -61,15 +63,17 @@ __global__ __launch_bounds__(kThreads) void k_sum_rows(const float* __restrict__
   }
 }
 
-__global__ __launch_bounds__(kThreads) void k_sum_final(const double* __restrict__ partial, int n, int reduction,
-                                                        float* __restrict__ loss, float* __restrict__ divisor) {
-  __shared__ double red[2 * kWaves];
-  double total = (int)threadIdx.x < n ? partial[2 * threadIdx.x] : 0.0;
-  double count = (int)threadIdx.x < n ? partial[2 * threadIdx.x + 1] : 0.0;
-  block_sum2(total, count, red);
+__global__ __launch_bounds__(kFinalThreads) void k_sum_final(const double* __restrict__ pairs, int64_t n, int reduction,
+                                                             float* __restrict__ loss, float* __restrict__ divisor) {
+  __shared__ double red[2 * (kFinalThreads / 64)];
+  double total = 0.0, count = 0.0;
+  for (int64_t i = threadIdx.x; i < n; i += kFinalThreads) {
+    total += pairs[2 * i];
+    count += pairs[2 * i + 1];
+  }
+  block_sum2<kFinalThreads / 64>(total, count, red);
   if (threadIdx.x == 0) finish_sum(total, count, reduction, loss, divisor);
 }
-static_assert(kSumBlocks <= kThreads, "one thread of k_sum_final per block of k_sum_rows");
 
 int sum_blocks(int64_t rows) {
   const int64_t b = ceil_div(rows, kSumRows);
@@ -80,13 +84,15 @@ int sum_blocks(int64_t rows) {
 
 size_t sum_workspace_bytes(int64_t rows) { return up256((size_t)sum_blocks(rows) * 2 * sizeof(double)); }
 
-void launch_sum(const float* row_loss, const float* weights, const int64_t* target, int64_t ignore_index, int64_t rows,
-                int reduction, void* partial, float* loss, float* divisor, hipStream_t s) {
+void launch_sum(const float* row_loss, const float* weights, int64_t rows, int reduction, void* partial, float* loss,
+                float* divisor, hipStream_t s) {
   const int n = sum_blocks(rows);
-  hipLaunchKernelGGL(k_sum_rows, dim3(n), dim3(kThreads), 0, s, row_loss, weights, target, ignore_index, rows,
-                     ceil_div(rows, n), reduction, (double*)partial, loss, divisor);
-  if (n > 1)
-    hipLaunchKernelGGL(k_sum_final, dim3(1), dim3(kThreads), 0, s, (const double*)partial, n, reduction, loss, divisor);
+  hipLaunchKernelGGL(k_sum_rows, dim3(n), dim3(kThreads), 0, s, row_loss, weights, rows, ceil_div(rows, n), reduction,
+                     (double*)partial, loss, divisor);
+  if (n > 1) launch_sum_pairs((const double*)partial, n, reduction, loss, divisor, s);
+}
+void launch_sum_pairs(const double* pairs, int64_t n, int reduction, float* loss, float* divisor, hipStream_t s) {
+  hipLaunchKernelGGL(k_sum_final, dim3(1), dim3(kFinalThreads), 0, s, pairs, n, reduction, loss, divisor);
 }
 
 namespace {
@@ -570,6 +576,7 @@ struct DistillArgs {
   float* row_loss;
   float* stats;        // [rows] of RowStats
   float* partial;      // [rows][segs][2], stream only
+  double* sums;        // [blocks][2] weighted losses and weights of a block's rows, short rows only; NULL: not wanted
   const float* divisor;  // backward: of the mean
   const float* g_loss;
   void* grad;
@@ -736,6 +743,7 @@ __global__ __launch_bounds__(kThreads) void k_distill_rows(DistillArgs a) {
   T* line = lines[group];
   const unsigned long long members = (~0ull >> (64 - L)) << (((threadIdx.x & 63) / L) * L);
   const int64_t step = (int64_t)gridDim.x * G;
+  double total = 0.0, count = 0.0;
   ShortRow<T, L, NV> next;
   next.template load<false>(a, (int64_t)blockIdx.x * G + group, lane);
   for (int64_t r0 = (int64_t)blockIdx.x * G; r0 < a.rows; r0 += step) {
@@ -845,8 +853,20 @@ __global__ __launch_bounds__(kThreads) void k_distill_rows(DistillArgs a) {
     }
     if (row < a.rows && lane == 0) {
       st.store(a, row);
-      a.row_loss[row] = loss;
+      if (a.sums) {
+        total += (double)loss;
+        count += (double)in.weight;
+      } else {
+        a.row_loss[row] = loss;
+      }
     }
+  }
+  if (!a.sums) return;
+  __shared__ double red[2 * kWaves];
+  block_sum2<kWaves>(total, count, red);
+  if (threadIdx.x == 0) {
+    a.sums[2 * blockIdx.x] = total;
+    a.sums[2 * blockIdx.x + 1] = count;
   }
 }
 
@@ -1177,35 +1197,35 @@ DistillArgs distill_args(const vsl_distill_desc* d) {
 }
 
 template <typename T, bool GRAD>
-void launch_distill(const DistillArgs& a, hipStream_t s) {
+int launch_distill(const DistillArgs& a, hipStream_t s) {  // returns the blocks
   const dim3 b(kThreads);
   if (a.V <= 256 * Vec<T>::E) {
     const int nv = (int)ceil_div(a.V, Vec<T>::E);
-    auto resident = [](int64_t blocks) { return dim3((unsigned)(blocks < kResident ? blocks : kResident)); };
-    const dim3 g8 = resident(ceil_div(a.rows, kThreads / 8));
-    const dim3 g16 = resident(ceil_div(a.rows, kThreads / 16)), g64 = resident(ceil_div(a.rows, kThreads / 64));
-    auto launch = [&](auto fwd, auto bwd, dim3 g) {
+    auto launch = [&](auto fwd, auto bwd, int lanes) {
+      const int64_t blocks = ceil_div(a.rows, kThreads / lanes);
+      const dim3 g((unsigned)(blocks < kResident ? blocks : kResident));
       if (GRAD) hipLaunchKernelGGL(bwd, g, b, 0, s, a);
       else hipLaunchKernelGGL(fwd, g, b, 0, s, a);
+      return (int)g.x;
     };
     // Fewer lanes a row share the work that every row costs among more rows: 8 lanes of two vectors against 16 of one, 128
     // bins in bfloat16, 146 against 232 us forward.
-    if (nv <= 8) launch(k_distill_rows<T, 8, 1>, k_distill_rows_grad<T, 8, 1>, g8);
-    else if (nv <= 16) launch(k_distill_rows<T, 8, 2>, k_distill_rows_grad<T, 8, 2>, g8);
-    else if (nv <= 32) launch(k_distill_rows<T, 16, 2>, k_distill_rows_grad<T, 16, 2>, g16);
-    else if (nv <= 64) launch(k_distill_rows<T, 16, 4>, k_distill_rows_grad<T, 16, 4>, g16);
-    else if (nv <= 128) launch(k_distill_rows<T, 64, 2>, k_distill_rows_grad<T, 64, 2>, g64);
-    else launch(k_distill_rows<T, 64, 4>, k_distill_rows_grad<T, 64, 4>, g64);
-    return;
+    if (nv <= 8) return launch(k_distill_rows<T, 8, 1>, k_distill_rows_grad<T, 8, 1>, 8);
+    if (nv <= 16) return launch(k_distill_rows<T, 8, 2>, k_distill_rows_grad<T, 8, 2>, 8);
+    if (nv <= 32) return launch(k_distill_rows<T, 16, 2>, k_distill_rows_grad<T, 16, 2>, 16);
+    if (nv <= 64) return launch(k_distill_rows<T, 16, 4>, k_distill_rows_grad<T, 16, 4>, 16);
+    if (nv <= 128) return launch(k_distill_rows<T, 64, 2>, k_distill_rows_grad<T, 64, 2>, 64);
+    return launch(k_distill_rows<T, 64, 4>, k_distill_rows_grad<T, 64, 4>, 64);
   }
   const dim3 g(grid_of(a.rows * a.segs));
   if (GRAD) {
     hipLaunchKernelGGL(k_distill_grad<T>, g, b, 0, s, a);
-    return;
+    return (int)g.x;
   }
   if (a.lse) hipLaunchKernelGGL((k_distill_stream<T, true>), g, b, 0, s, a);
   else hipLaunchKernelGGL((k_distill_stream<T, false>), g, b, 0, s, a);
   if (a.segs > 1) hipLaunchKernelGGL(k_distill_join<T>, dim3(grid_of(a.rows)), b, 0, s, a);
+  return (int)g.x;
 }
 
 int check_workspace(const char* what, const void* workspace, size_t have, size_t need) {
@@ -1262,6 +1282,7 @@ int vsl_top_logits(const vsl_top_desc* d, void* values, int32_t* indices, float*
 size_t vsl_distill_workspace_bytes(const vsl_distill_desc* d) {
   if (!d || d->rows < 0 || d->vocab < 1 || bad_type(d->type)) return 0;
   const Split sp = distill_split(d);
+  if (d->vocab <= short_row(d->type)) return up256(kResident * 2 * sizeof(double));
   return (sp.segs > 1 ? up256((size_t)d->rows * sp.segs * 8) : 0) + sum_workspace_bytes(d->rows);
 }
 
@@ -1275,15 +1296,16 @@ int vsl_distill_fwd(const vsl_distill_desc* d, float* row_loss, float* loss, flo
   DistillArgs a = distill_args(d);
   a.row_loss = row_loss;
   a.stats = stats;
+  const bool reduce = d->reduction != VSL_REDUCE_NONE, short_rows = d->vocab <= short_row(d->type);
   const size_t part = a.segs > 1 ? up256((size_t)d->rows * a.segs * 8) : 0;
   a.partial = (float*)workspace;
-  if (d->rows > 0) {
-    if (d->type == VSL_TYPE_F32) launch_distill<float, false>(a, s);
-    else if (d->type == VSL_TYPE_BF16) launch_distill<__bf16, false>(a, s);
-    else launch_distill<_Float16, false>(a, s);
-  }
-  if (d->reduction != VSL_REDUCE_NONE)
-    launch_sum(row_loss, d->weights, nullptr, 0, d->rows, d->reduction, (char*)workspace + part, loss, divisor, s);
+  a.sums = reduce && short_rows ? (double*)workspace : nullptr;
+  int blocks = 0;
+  if (d->rows > 0)
+    blocks = d->type == VSL_TYPE_F32 ? launch_distill<float, false>(a, s)
+             : d->type == VSL_TYPE_BF16 ? launch_distill<__bf16, false>(a, s) : launch_distill<_Float16, false>(a, s);
+  if (reduce && short_rows) launch_sum_pairs(a.sums, blocks, d->reduction, loss, divisor, s);
+  else if (reduce) launch_sum(row_loss, d->weights, d->rows, d->reduction, (char*)workspace + part, loss, divisor, s);
   return launch_status("distill");
 }
 

@@ -212,10 +212,11 @@ inline size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Reduced loss of `rows` row losses in a fixed order (float64 sums): *loss = sum or mean, *divisor = what the mean is
-// divided by: the sum of `weights`, the number of targets other than ignore_index, or the number of rows.
-// partial: sum_workspace_bytes(rows) bytes.
+// divided by: the sum of `weights`, or the number of rows.  partial: sum_workspace_bytes(rows) bytes.
 size_t sum_workspace_bytes(int64_t rows);
-void launch_sum(const float* row_loss, const float* weights, const int64_t* target, int64_t ignore_index, int64_t rows,
-                int reduction, void* partial, float* loss, float* divisor, hipStream_t s);
+void launch_sum(const float* row_loss, const float* weights, int64_t rows, int reduction, void* partial, float* loss,
+                float* divisor, hipStream_t s);
+// The same from n (sum, count) pairs of float64 that blocks of a kernel have left.
+void launch_sum_pairs(const double* pairs, int64_t n, int reduction, float* loss, float* divisor, hipStream_t s);
 
 }  // namespace vsl_vocab
