@@ -482,8 +482,8 @@ int vsl_distill_bwd(const vsl_distill_desc* desc, const float* stats, const floa
  * vsl_linear_ce_bwd: g_loss: one float, or [rows] for VSL_REDUCE_NONE; stats and divisor are the forward call's outputs.
  * grad_hidden [rows,dim], grad_weight [vocab,dim], grad_bias [vocab], contiguous, of the operands' type; each may be
  * NULL.  Workspaces: the matching *_workspace_bytes (grad_mask: bit 0 hidden, 1 weight, 2 bias), 256-byte aligned.
- * Further limits: rows < 2^28, 1 <= dim < 2^24, rows * vocab < 2^37, rows * dim < 2^36, vocab * dim < 2^36 (each size
- * rounded up to a multiple of 256).
+ * Further limits: rows < 2^28, 1 <= dim < 2^24, rows * vocab < 2^37, rows * dim < 2^34, vocab * dim < 2^34 (rows and
+ * vocab rounded up to a multiple of 256, dim of 64).
  */
 typedef struct vsl_linear_ce_desc {
   int64_t rows, vocab, dim, hidden_stride, weight_stride;

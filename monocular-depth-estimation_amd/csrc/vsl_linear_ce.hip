@@ -884,9 +884,10 @@ int check_ce(const vsl_linear_ce_desc* d) {
     return fail(VSL_ERR_INVALID_ARGUMENT, "linear_ce: unknown element type");
   if (d->rows < 0 || d->rows >= (1LL << 28) || d->vocab < 1 || d->vocab >= (1LL << 30) || d->dim < 1 || d->dim >= (1LL << 24))
     return fail(VSL_ERR_INVALID_ARGUMENT, "linear_ce: need 0 <= rows < 2^28, 1 <= vocab < 2^30, 1 <= dim < 2^24");
+  // a launch counts its threads in 32 bits: tiles of 128 x 64 by 256 threads, blocks of 64 x 64 laid out by 256
   if (round_up(d->rows, 256) * round_up(d->vocab, 256) >= (1LL << 37) ||
-      round_up(d->rows, 256) * round_up(d->dim, 256) >= (1LL << 36) || round_up(d->vocab, 256) * round_up(d->dim, 256) >= (1LL << 36))
-    return fail(VSL_ERR_INVALID_ARGUMENT, "linear_ce: need rows * vocab < 2^37, rows * dim < 2^36 and vocab * dim < 2^36");
+      round_up(d->rows, 256) * round_up(d->dim, 64) >= (1LL << 34) || round_up(d->vocab, 256) * round_up(d->dim, 64) >= (1LL << 34))
+    return fail(VSL_ERR_INVALID_ARGUMENT, "linear_ce: need rows * vocab < 2^37, rows * dim < 2^34 and vocab * dim < 2^34");
   if (d->hidden_stride < d->dim || d->weight_stride < d->dim || d->hidden_stride >= (1LL << 40) || d->weight_stride >= (1LL << 40))
     return fail(VSL_ERR_INVALID_ARGUMENT, "linear_ce: row strides must be at least dim");
   if (d->reduction < VSL_REDUCE_NONE || d->reduction > VSL_REDUCE_MEAN)
@@ -1333,6 +1334,9 @@ int vsl_linear_ce_bwd(const vsl_linear_ce_desc* d, const float* stats, const flo
   if (!stats || !g_loss || (d->reduction == VSL_REDUCE_MEAN && !divisor))
     return fail(VSL_ERR_INVALID_ARGUMENT, "linear_ce backward: NULL tensor");
   if (!grad_hidden && !grad_weight && !grad_bias) return VSL_OK;
+  const int size = size_of(d->type);
+  if ((uintptr_t)grad_hidden % size || (uintptr_t)grad_weight % size || (uintptr_t)grad_bias % size)
+    return fail(VSL_ERR_INVALID_ARGUMENT, "linear_ce backward: misaligned gradient");
   const uint32_t mask = (grad_hidden ? 1u : 0u) | (grad_weight ? 2u : 0u) | (grad_bias ? 4u : 0u);
   const Backward b = backward_workspace(d, mask, workspace);
   if (int rc = check_space(workspace, workspace_bytes, b.total)) return rc;

@@ -527,17 +527,20 @@ Split top_split(const vsl_top_desc* d) {
 
 bool bad_type(int t) { return t != VSL_TYPE_F32 && t != VSL_TYPE_BF16 && t != VSL_TYPE_F16; }
 
-int check_matrix(const char* what, int64_t rows, int64_t vocab, int64_t stride, int type) {
+int size_of(int type) { return type == VSL_TYPE_F32 ? 4 : 2; }
+
+int check_matrix(const char* what, const void* logits, int64_t rows, int64_t vocab, int64_t stride, int type) {
   if (bad_type(type)) return fail(VSL_ERR_INVALID_ARGUMENT, std::string(what) + ": unknown element type");
   if (rows < 0 || rows >= (1LL << 31) || vocab < 1 || vocab >= (1LL << 30))
     return fail(VSL_ERR_INVALID_ARGUMENT, std::string(what) + ": need 0 <= rows < 2^31 and 1 <= vocab < 2^30");
   if (stride < vocab || stride >= (1LL << 40))
     return fail(VSL_ERR_INVALID_ARGUMENT, std::string(what) + ": the row stride must be at least vocab");
+  if ((uintptr_t)logits % size_of(type)) return fail(VSL_ERR_INVALID_ARGUMENT, std::string(what) + ": misaligned logits");
   return VSL_OK;
 }
 int check_top(const vsl_top_desc* d) {
   if (!d) return fail(VSL_ERR_INVALID_ARGUMENT, "top_logits: descriptor is null");
-  if (int rc = check_matrix("top_logits", d->rows, d->vocab, d->stride, d->type)) return rc;
+  if (int rc = check_matrix("top_logits", d->logits, d->rows, d->vocab, d->stride, d->type)) return rc;
   if (d->k < 1 || d->k > VSL_MAX_TOP || d->k > d->vocab)
     return fail(VSL_ERR_INVALID_ARGUMENT, "top_logits: need 1 <= k <= min(vocab, 256)");
   if (!(d->temperature >= 1e-4f && d->temperature <= 1e4f))
@@ -1145,7 +1148,7 @@ __global__ __launch_bounds__(kThreads) void k_distill_grad(DistillArgs a) {
 
 int check_distill(const vsl_distill_desc* d) {
   if (!d) return fail(VSL_ERR_INVALID_ARGUMENT, "distill: descriptor is null");
-  if (int rc = check_matrix("distill", d->rows, d->vocab, d->stride, d->type)) return rc;
+  if (int rc = check_matrix("distill", d->logits, d->rows, d->vocab, d->stride, d->type)) return rc;
   if (d->k < 1 || d->k > VSL_MAX_TOP || d->k > d->vocab)
     return fail(VSL_ERR_INVALID_ARGUMENT, "distill: need 1 <= k <= min(vocab, 256)");
   if (bad_type(d->value_type)) return fail(VSL_ERR_INVALID_ARGUMENT, "distill: unknown type of the teacher's values");
@@ -1254,6 +1257,8 @@ int vsl_top_logits(const vsl_top_desc* d, void* values, int32_t* indices, float*
   if (int rc = check_top(d)) return rc;
   if (d->rows == 0) return VSL_OK;
   if (!d->logits || !values || !indices) return fail(VSL_ERR_INVALID_ARGUMENT, "top_logits: NULL tensor");
+  if ((uintptr_t)values % size_of(d->type) || (uintptr_t)indices % 4 || (uintptr_t)lse % 4)
+    return fail(VSL_ERR_INVALID_ARGUMENT, "top_logits: misaligned output");
   if (int rc = check_workspace("top_logits", workspace, workspace_bytes, vsl_top_logits_workspace_bytes(d))) return rc;
   const Split sp = top_split(d);
   TopArgs a{};
@@ -1291,6 +1296,7 @@ int vsl_distill_fwd(const vsl_distill_desc* d, float* row_loss, float* loss, flo
   if (int rc = check_distill(d)) return rc;
   if (d->reduction != VSL_REDUCE_NONE && (!loss || !divisor)) return fail(VSL_ERR_INVALID_ARGUMENT, "distill: NULL loss");
   if (d->rows > 0 && (!row_loss || !stats)) return fail(VSL_ERR_INVALID_ARGUMENT, "distill: NULL output");
+  if ((uintptr_t)stats % 16) return fail(VSL_ERR_INVALID_ARGUMENT, "distill: stats must be 16-byte aligned");
   if (int rc = check_workspace("distill", workspace, workspace_bytes, vsl_distill_workspace_bytes(d))) return rc;
   hipStream_t s = (hipStream_t)stream;
   DistillArgs a = distill_args(d);
@@ -1315,6 +1321,8 @@ int vsl_distill_bwd(const vsl_distill_desc* d, const float* stats, const float* 
   if (d->rows == 0) return VSL_OK;
   if (!stats || !g_loss || !grad || (d->reduction == VSL_REDUCE_MEAN && !divisor))
     return fail(VSL_ERR_INVALID_ARGUMENT, "distill backward: NULL tensor");
+  if ((uintptr_t)stats % 16 || (uintptr_t)grad % size_of(d->type))
+    return fail(VSL_ERR_INVALID_ARGUMENT, "distill backward: misaligned stats or gradient");
   if (grad_stride < d->vocab || grad_stride >= (1LL << 40))
     return fail(VSL_ERR_INVALID_ARGUMENT, "distill backward: the gradient's row stride must be at least vocab");
   DistillArgs a = distill_args(d);

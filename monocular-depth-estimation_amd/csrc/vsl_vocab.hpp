@@ -144,7 +144,8 @@ __device__ __forceinline__ float exp_ref(float m) { return m == ninf() ? 0.0f : 
 __device__ __forceinline__ float exp_of(float x, float ref, float c) { return __builtin_amdgcn_exp2f((x - ref) * c); }
 // The same for many x <= ref as one multiply-add and one exponential each.  Where ref * c is not finite (a row of lowest
 // values) the scale is so small that ref * c is, and still so large that the next value below ref gives 0: temperatures
-// are at least 1e-4, so |ref| is above 2^114 there and floats are at least 2^91 apart.
+// are at least 1e-4, so |ref| is above 2^114 there and floats are at least 2^91 apart.  The instruction gives 0 for results
+// below 2^-126, beside a largest term of 1: no sum feels them, a gradient loses at most 2^-126 of its factor.
 struct Exponent {
   float c, shift;
   __device__ __forceinline__ Exponent(float ref, float scale) {

@@ -82,6 +82,16 @@ def test_top_logits_of_ties_masks_and_specials(vocab, dtype):
     check_top(x.to(dtype).to(DEV), k)
 
 
+@pytest.mark.parametrize("temperature", [1e-4, 0.05, 1e4])
+def test_extreme_temperatures(temperature):
+    for vocab in (90, 700, 5000):
+        x = logits(4, vocab, 161, torch.float32)
+        check_top(x.to(DEV), 9, temperature)
+        if temperature >= 0.05:                             # 1e-4: logits / T of 1e5 leave the bound on a loss no digit
+            val, idx = teacher(4, vocab, 9, 162, torch.float32)
+            check_distill(x, val, idx, (torch.logsumexp(val.double() / temperature, 1) + 0.1).float(), temperature)
+
+
 def test_top_logits_of_strided_rows_leading_dimensions_and_no_rows():
     import mde_amd.vocab_losses as L
     base = logits(24, 400, 3, torch.bfloat16).to(DEV)
@@ -132,6 +142,11 @@ def check_distill(x, val, idx, lse=None, temperature=1.0, weights=None, upstream
     want = grad * upstream.double()[:, None]
     assert got.dtype == dtype and got.shape == a.shape
     tol = 4 * rel * size * upstream.double().abs()[:, None] + (O.HALF_STEP[dtype] + 4 * O.U) * want.abs() + O.TINY[dtype]
+    # An exponential below the smallest normal float, 2^-126, comes out as 0.  A class that is not the teacher's has one,
+    # times |total p_rest - q_rest| <= max(total, 1), a class of the teacher's one, times total; both times w t upstream.
+    # total = sum of q <= 1 for the lse of these tests, up to its rounding: 2^-126 (1 + 1) covers it.
+    flushed = 2.0 ** -125 * w.double()[:, None] * t
+    tol = tol + flushed * upstream.double().abs()[:, None]
     close(got, want, torch.nan_to_num(tol), "gradient")
     # the reductions
     total = L.topk_distillation_loss(a, *args, temperature=t, weights=dev(weights), reduction="sum")
@@ -142,7 +157,7 @@ def check_distill(x, val, idx, lse=None, temperature=1.0, weights=None, upstream
     close(mean.detach(), s / ws if ws else torch.zeros((), dtype=torch.float64), 4 * O.U * s.abs() / max(ws, 1e-30) if torch.isfinite(s) else 0.0, "mean")
     (gm,) = torch.autograd.grad(mean, a, torch.tensor(0.5, device=DEV))
     gw = grad * (0.5 / ws if ws else 0.0)
-    tol = 4 * rel * size * (0.5 / ws if ws else 0.0) + (O.HALF_STEP[dtype] + 8 * O.U) * gw.abs() + O.TINY[dtype]
+    tol = (4 * rel * size + flushed) * (0.5 / ws if ws else 0.0) + (O.HALF_STEP[dtype] + 8 * O.U) * gw.abs() + O.TINY[dtype]
     close(gm, gw, torch.nan_to_num(tol), "gradient of the mean")
     return rows_out, got
 

@@ -34,7 +34,7 @@ def test_mirrors_and_version():
 
 BAD_ROWS = [dict(rows=-1), dict(rows=1 << 31), dict(vocab=0, stride=9), dict(vocab=1 << 30, stride=1 << 30), dict(stride=4999),
             dict(type=3), dict(k=0), dict(k=257), dict(k=5, vocab=4), dict(temperature=0.0), dict(temperature=float("nan")),
-            dict(temperature=float("inf")), dict(logits=None)]
+            dict(temperature=float("inf")), dict(temperature=9e-5), dict(temperature=1.1e4), dict(logits=None), dict(logits=FAKE + 1)]
 
 
 @pytest.mark.parametrize("bad", BAD_ROWS)
@@ -54,6 +54,7 @@ def test_top_logits_outputs_and_workspace():
     assert call(FAKE, FAKE, FAKE * 16, need - 1) == -2 and b"workspace" in err(abi)
     assert call(FAKE, FAKE, FAKE * 16 + 8, need) == -1 and b"aligned" in err(abi)
     assert call(FAKE, FAKE, None, need) == -1
+    assert call(FAKE + 2, FAKE, FAKE * 16, need) == -1 and call(FAKE, FAKE + 2, FAKE * 16, need) == -1
     assert abi.lib.vsl_top_logits_workspace_bytes(ctypes.byref(top(abi, vocab=1000, stride=1000))) == 0   # short rows need none
     assert abi.lib.vsl_top_logits(None, FAKE, FAKE, None, None, 0, None) == -1
     assert abi.lib.vsl_top_logits(ctypes.byref(top(abi, rows=0, logits=None)), None, None, None, None, 0, None) == 0
@@ -84,6 +85,8 @@ def test_distill_outputs_and_workspace():
     assert bwd(None, FAKE, FAKE, FAKE, 5000) == -1 and bwd(FAKE, None, FAKE, FAKE, 5000) == -1
     assert bwd(FAKE, FAKE, None, FAKE, 5000) == -1 and bwd(FAKE, FAKE, FAKE, None, 5000) == -1
     assert bwd(FAKE, FAKE, FAKE, FAKE, 4999) == -1 and b"stride" in err(abi)
+    assert bwd(FAKE + 4, FAKE, FAKE, FAKE, 5000) == -1 and bwd(FAKE, FAKE, FAKE, FAKE + 1, 5000) == -1 and b"misaligned" in err(abi)
+    assert fwd(FAKE, FAKE, FAKE, FAKE + 4, FAKE * 16, need) == -1 and b"aligned" in err(abi)
     assert abi.lib.vsl_distill_fwd(None, FAKE, FAKE, FAKE, FAKE, FAKE, 1, None) == -1
 
 
@@ -119,6 +122,7 @@ def test_linear_ce_outputs_and_workspace():
     assert bwd(None, FAKE, FAKE, FAKE, FAKE * 16, sizes[0]) == -1 and bwd(FAKE, None, FAKE, FAKE, FAKE * 16, sizes[0]) == -1
     assert bwd(FAKE, FAKE, None, FAKE, FAKE * 16, sizes[0]) == -1
     assert bwd(FAKE, FAKE, FAKE, FAKE, FAKE * 16, sizes[0] - 1) == -2
+    assert bwd(FAKE, FAKE, FAKE, FAKE + 1, FAKE * 16, sizes[0]) == -1 and b"misaligned" in err(abi)
     assert bwd(FAKE, FAKE, FAKE, None, None, 0) == 0                       # no gradient is wanted
     # odd widths and rows that 16-byte loads cannot take are laid out anew: more workspace, never less
     for kw in (dict(dim=65, hidden_stride=65, weight_stride=65), dict(hidden=FAKE + 2), dict(hidden_stride=65)):
