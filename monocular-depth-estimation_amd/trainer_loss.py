@@ -19,6 +19,11 @@ disable_automasking, avg_reprojection, no_ssim, disparity_smoothness, pose_model
 
     pose_outputs(axisangle, translation) -> {("cam_T_cam",f), ...}   Trainer.py:388-393,408-414
     compute_depth_losses(inputs, outputs, losses) -> (sum, [7 metrics])   Trainer.py:622-662
+
+For decoders that answer with a distribution over depth bins (no counterpart in the reference):
+
+    compute_bin_cross_entropy(features, weight, target, bias)         the bins' 1x1 head and its cross entropy in one
+    compute_bin_distillation(logits, teacher_logits, k, temperature)  a student's bins against a teacher's k largest
 """
 from __future__ import annotations
 
@@ -32,6 +37,7 @@ from .layers import (BackprojectDepth, Project3D, SSIM, affinity_reprojection_lo
                      get_smooth_loss, grid_sample_border, mean_inverse_depth, poses_from_parameters, warp_features,
                      warp_features_multi)
 from .ops import fused_view_synthesis_loss, fused_view_synthesis_loss_heads
+from .vocab_losses import linear_cross_entropy, top_logits, topk_distillation_loss
 
 
 class ViewSynthesisLoss:
@@ -254,6 +260,23 @@ class ViewSynthesisLoss:
     def compute_losses_distillation(self, inputs, outputs, outputs_teacher=None, features=None, teacher_features=None,
                                     buffered_features=None, noise=None):
         return self.compute_losses(inputs, outputs, noise, photometric_scale=0.9)
+
+    # ------------------------------------------------------------------ decoders that answer with depth bins
+    def compute_bin_cross_entropy(self, features, weight, target, bias=None, ignore_index: int = -100):
+        """Mean cross entropy of a 1x1 classification head: ``features`` [B,D,H,W], ``weight`` [bins,D] or the
+        convolution's [bins,D,1,1], ``target`` [B,H,W] bins, ``ignore_index`` where a pixel has no ground truth.  The
+        bins' logits are never kept; gradients reach features, weight and bias."""
+        if weight.dim() == 4 and tuple(weight.shape[2:]) == (1, 1):
+            weight = weight.flatten(1)
+        return linear_cross_entropy(features.movedim(1, -1), weight, target, bias, ignore_index=ignore_index)
+
+    def compute_bin_distillation(self, logits, teacher_logits, k: int = 8, temperature: float = 1.0, weights=None):
+        """Mean over the pixels of temperature^2 * KL(teacher || student) from the teacher's ``k`` largest bins, its
+        other bins as one: ``logits``, ``teacher_logits`` [B,bins,H,W], ``weights`` [B,H,W] or None (a pixel of weight 0
+        is left out).  The gradient reaches ``logits``."""
+        top = top_logits(teacher_logits.movedim(1, -1), min(int(k), teacher_logits.shape[1]), temperature)
+        return topk_distillation_loss(logits.movedim(1, -1), top.values, top.indices, top.lse, temperature=temperature,
+                                      weights=weights)
 
     # ------------------------------------------------------------------ un-fused reference order, for cross-checks
     def compute_losses_unfused(self, inputs: Dict, outputs: Dict, noise: Optional[torch.Tensor] = None):

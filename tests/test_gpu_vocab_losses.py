@@ -476,6 +476,36 @@ def test_teacher_and_student_together():
         assert float((got.cpu().double() - ref).norm()) <= 1e-5 * float(ref.norm())
 
 
+@pytest.mark.parametrize("memory", [torch.contiguous_format, torch.channels_last])
+def test_trainer_surface_of_depth_bins(memory):
+    import types
+    from mde_amd.trainer_loss import ViewSynthesisLoss
+    vs = ViewSynthesisLoss(types.SimpleNamespace(height=12, width=20))
+    g = gen(151)
+    features, teacher_ = torch.randn(2, 32, 12, 20, generator=g), torch.randn(2, 48, 12, 20, generator=g) * 3
+    head = torch.nn.Conv2d(32, 48, 1)
+    target = torch.randint(48, (2, 12, 20), generator=g)
+    target[torch.rand(2, 12, 20, generator=g) < 0.3] = -100
+    valid = (target >= 0).float()
+    f = features.to(DEV).contiguous(memory_format=memory).requires_grad_(True)
+    w, b = (p.detach().to(DEV).requires_grad_(True) for p in (head.weight, head.bias))
+    ce = vs.compute_bin_cross_entropy(f, w, target.to(DEV), b)
+    z = torch.nn.functional.conv2d(f, w, b)
+    kd = vs.compute_bin_distillation(z, teacher_.to(DEV), k=5, temperature=2.0, weights=valid.to(DEV))
+    (ce + kd).backward()
+    f6, w6, b6 = (p.detach().double().requires_grad_(True) for p in (features, head.weight, head.bias))
+    z6 = torch.nn.functional.conv2d(f6, w6, b6)
+    want_ce = torch.nn.functional.cross_entropy(z6, target)
+    flat = lambda t: t.movedim(1, -1).reshape(-1, 48)
+    v, i, lse = O.top_logits(flat(teacher_), 5, 2.0)
+    loss, grad, _ = O.distill(flat(z6.detach()), v, i, lse.float(), 2.0, valid.reshape(-1))
+    count = float(valid.sum())
+    assert abs(float(ce.detach()) - float(want_ce.detach())) <= 1e-5 and abs(float(kd.detach()) - float(loss.sum()) / count) <= 1e-5
+    (want_ce + (z6 * (grad / count).reshape(2, 12, 20, 48).movedim(-1, 1)).sum()).backward()
+    for got, ref in ((f.grad, f6.grad), (w.grad, w6.grad), (b.grad, b6.grad)):
+        assert got.shape == ref.shape and float((got.cpu().double() - ref).norm()) <= 2e-5 * float(ref.norm())
+
+
 def both(L, s):
     top = L.top_logits(s["teacher"], 5)
     kd = L.topk_distillation_loss(s["x"], top.values, top.indices, top.lse)
