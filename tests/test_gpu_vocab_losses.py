@@ -506,6 +506,67 @@ def test_trainer_surface_of_depth_bins(memory):
         assert got.shape == ref.shape and float((got.cpu().double() - ref).norm()) <= 2e-5 * float(ref.norm())
 
 
+# ------------------------------------------------------------------ offsets past 2^31 elements
+@pytest.mark.parametrize("rows,vocab,k", [(16400, 131100, 20), (33600000, 65, 4)])
+def test_rows_behind_two_to_the_31_elements(rows, vocab, k):
+    """Long and short rows; the first and the last ones against the definition, every row's statistics finite."""
+    import mde_amd.vocab_losses as L
+    assert rows * vocab > 1 << 31
+    x = torch.empty(rows, vocab, dtype=torch.bfloat16, device=DEV)
+    for i in range(0, rows, rows // 8 + 1):
+        x[i:i + rows // 8 + 1].normal_(generator=torch.Generator(DEV).manual_seed(i + 1))
+    pick = [0, 1, rows // 2, rows - 2, rows - 1]
+    top = L.top_logits(x, k)
+    v, i, lse = O.top_logits(x[pick], k)
+    assert torch.equal(top.indices[pick].cpu().long(), i) and torch.equal(top.values[pick].cpu().double(), v)
+    close(top.lse[pick], lse, O.sum_error(vocab) + 16 * O.U * 16, "log sum")
+    assert bool(torch.isfinite(top.lse).all())
+    teach = (top.values, top.indices.roll(1, 1).contiguous(), top.lse)
+    x.requires_grad_(True)
+    out = L.topk_distillation_loss(x, *teach, reduction="none")
+    up = torch.ones(rows, device=DEV)
+    (grad,) = torch.autograd.grad(out, x, up)
+    x.requires_grad_(False)
+    loss, want, size = O.distill(x[pick], *(t[pick] for t in teach))
+    rel = 4 * (O.exponent_error(x[pick].float(), 1.0) * 2 + 2 * O.sum_error(vocab) + 16 * O.U * 17)
+    close(out[pick], loss, rel * (1 + 40 * 2 ** -4), "row losses")
+    close(grad[pick], want, rel * size + (2 ** -8 + 4 * O.U) * want.abs() + 2.0 ** -125, "gradient")
+    assert bool(torch.isfinite(grad).all())
+
+
+def test_linear_cross_entropy_behind_two_to_the_31_elements():
+    import mde_amd.vocab_losses as L
+    h, w, b, t = ce_inputs(520, 540, 72, torch.bfloat16, 171, bias=True)
+    far = torch.zeros(541, 1 << 22, dtype=torch.bfloat16, device=DEV)       # rows 2^22 apart, read in place and copied
+    for at in (0, 3):
+        far[:520, at:at + 72], far[:540, 1024 + at:1024 + at + 72] = h.to(DEV), w.to(DEV)
+        check_ce(h, w, b, t, on_device=(far[:520, at:at + 72], far[:540, 1024 + at:1024 + at + 72]))
+    del far
+    rows, vocab, dim = 4, 530000, 4100                                       # a weight of more than 2^31 elements
+    assert vocab * dim > 1 << 31
+    w = torch.empty(vocab, dim, dtype=torch.bfloat16, device=DEV).normal_(std=0.03, generator=torch.Generator(DEV).manual_seed(5))
+    h = torch.randn(rows, dim, generator=gen(172)).bfloat16().to(DEV)
+    t = torch.tensor([0, vocab - 1, 1000, vocab // 2], device=DEV)
+    h.requires_grad_(True), w.requires_grad_(True)
+    out = L.linear_cross_entropy(h, w, t, reduction="none")
+    gh, gw = torch.autograd.grad(out, (h, w), torch.ones(rows, device=DEV))
+    h, w = h.detach().double(), w.detach()
+    parts = w.split(1 << 16)
+    z = torch.cat([h @ p.double().T.contiguous() for p in parts], 1)
+    zerr = dim * O.U * 100                                                   # |h| |w| sums to below 100 a logit
+    lse = torch.logsumexp(z, 1)
+    close(out, lse - z.gather(1, t[:, None])[:, 0], 2 * zerr + O.sum_error(vocab) + 1e-5, "row losses")
+    ds = (z - lse[:, None]).exp()
+    ds[torch.arange(rows), t] -= 1
+    derr = (2 * zerr + 2 ** -8 + O.sum_error(vocab) + 16 * O.U) * ds.abs() + 4 * O.U * (ds < 0)
+    want = sum(d @ p.double() for d, p in zip(ds.split(1 << 16, 1), parts))
+    size = sum(d @ p.double().abs() for d, p in zip(derr.split(1 << 16, 1), parts))
+    close(gh, want, size + (2 ** -8 + 8 * O.U) * want.abs() + vocab * O.U * size * 2 ** 8, "grad hidden")
+    for a in (0, vocab // 2, vocab - 64):
+        want = ds[:, a:a + 64].T.contiguous() @ h
+        close(gw[a:a + 64], want, derr[:, a:a + 64].T.contiguous() @ h.abs() * (1 + 2 ** -8) + (2 ** -8 + 8 * O.U) * want.abs(), "grad weight")
+
+
 def both(L, s):
     top = L.top_logits(s["teacher"], 5)
     kd = L.topk_distillation_loss(s["x"], top.values, top.indices, top.lse)
