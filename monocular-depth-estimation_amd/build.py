@@ -1,4 +1,4 @@
-"""Builds libvsloss.so in-tree with hipcc for gfx950 (no GPU needed to compile)."""
+"""Builds libvsloss.so in-tree with hipcc for gfx950, and the torch binding of the class losses (no GPU needed to compile)."""
 from __future__ import annotations
 
 import os
@@ -11,6 +11,8 @@ CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libvsloss.so")
 RESOURCES = os.path.join(HERE, "libvsloss.resources.txt")
 SOURCES = ["vsl_loss.hip", "vsl_layers.hip", "vsl_pose.hip", "vsl_metrics.hip", "vsl_vocab.hip", "vsl_linear_ce.hip"]
+BINDING_SOURCE = os.path.join(CSRC, "vsl_vocab_binding.cpp")
+BINDING = os.path.join(HERE, "vsl_vocab_binding.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 
@@ -18,7 +20,8 @@ def needs_build() -> bool:
     if not os.path.exists(OUT):
         return True
     t = os.path.getmtime(OUT)
-    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(HERE, "..", "include", "vsloss.h")]
+    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if not f.endswith(".cpp")]
+    deps.append(os.path.join(HERE, "..", "include", "vsloss.h"))
     return any(os.path.getmtime(d) > t for d in deps if os.path.isfile(d))
 
 
@@ -64,6 +67,28 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return OUT
 
 
+def build_binding(force: bool = False) -> str:
+    """The extension module behind vocab_losses: include/vsloss_vocab_torch.h against the installed torch, with g++.  The
+    library's functions stay undefined in it; the package loads them first."""
+    include = os.path.join(HERE, "..", "include")
+    deps = [BINDING_SOURCE] + [os.path.join(include, f) for f in os.listdir(include)]
+    if not force and os.path.exists(BINDING) and all(os.path.getmtime(BINDING) >= os.path.getmtime(d) for d in deps):
+        return BINDING
+    import sysconfig
+
+    import torch
+    tdir = os.path.dirname(torch.__file__)
+    subprocess.check_call(
+        ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+         "-DTORCH_EXTENSION_NAME=vsl_vocab_binding", "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch.compiled_with_cxx11_abi()),
+         "-I", include, "-I", os.path.join(tdir, "include"),
+         "-I", os.path.join(tdir, "include", "torch", "csrc", "api", "include"), "-I", "/opt/rocm/include",
+         "-I", sysconfig.get_paths()["include"], BINDING_SOURCE, "-o", BINDING, "-L", os.path.join(tdir, "lib"),
+         "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip",
+         "-Wl,-rpath," + os.path.join(tdir, "lib")])
+    return BINDING
+
+
 def kernel_resources(remarks: str):
     """The compiler's per-kernel resource remarks as a list of dicts."""
     out, cur = [], None
@@ -84,3 +109,4 @@ def kernel_resources(remarks: str):
 
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose="-v" in sys.argv))
+    print(build_binding(force="--force" in sys.argv))

@@ -667,7 +667,16 @@ def test_refusals_on_the_device():
         with pytest.raises(ValueError):
             call()
             print("accepted: %d" % n)
+    import mde_amd._abi as abi
+    with pytest.raises(abi.VslError, match="2\\^30"):        # the library's own limits
+        L.top_logits(torch.empty(1 << 30, dtype=torch.float16, device=DEV), 1)
     with pytest.raises(RuntimeError):                       # no second derivatives
         y = x.clone().requires_grad_(True)
         (g,) = torch.autograd.grad(L.topk_distillation_loss(y, v, i), y, create_graph=True)
         g.sum().backward()
+    for i in range(3):
+        with pytest.raises(RuntimeError, match="once"):
+            leaves = [torch.ones(s, device=DEV, requires_grad=True) for s in ((4, 8), (20, 8), (20,))]
+            loss = L.linear_cross_entropy(leaves[0], leaves[1], torch.arange(4, device=DEV), leaves[2])
+            grads = torch.autograd.grad(loss, leaves, create_graph=True)
+            grads[i].sum().backward()
