@@ -105,6 +105,7 @@ __device__ __forceinline__ unsigned ordered32(unsigned b) {
   if (b == 0x80000000u) b = 0u;                             // -0 ties with +0
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+constexpr unsigned kOrderedLowest = 0x007FFFFFu;            // -infinity
 __device__ __forceinline__ unsigned unordered32(unsigned o) { return o & 0x80000000u ? o & 0x7FFFFFFFu : ~o; }
 
 // Short rows: a 16-bit value as a float has at least 13 zero bits at the end, so value and index share 32 bits; float32
@@ -294,10 +295,31 @@ __device__ __forceinline__ void sort_some(unsigned long long* buf, int count) {
   for (int r = 0; r < R; ++r) buf[r * kThreads + threadIdx.x] = key[r];
   __syncthreads();
 }
+// Up to 256 different keys: a key's place is the number of larger ones, which every thread counts for its own key over
+// LDS reads that all lanes share.  No step waits for the one before: 2 us less than the bitonic network for 50 keys, 1 us
+// for 200.
+__device__ __forceinline__ void sort_by_rank(unsigned long long* buf, int count) {
+  const int tid = threadIdx.x;
+  const unsigned long long key = tid < count ? buf[tid] : 0ull;
+  if (tid == 0 && (count & 1)) buf[count] = 0ull;
+  __syncthreads();
+  int place = 0;
+  if ((tid & ~63) < count) {
+    const u64x2* pairs = (const u64x2*)buf;
+#pragma unroll 4
+    for (int j = 0; j < (count + 1) / 2; ++j) {
+      const u64x2 two = pairs[j];
+      place += (int)(two.x > key) + (int)(two.y > key);
+    }
+  }
+  __syncthreads();
+  buf[tid < count ? place : tid] = key;
+  __syncthreads();
+}
 // Sorts the first `count` keys of an LDS buffer of kBuffer, larger first, zeros behind (as far as a power of two or 256).
 // Starts behind a barrier that made the keys visible; ends with one.
 __device__ __forceinline__ void sort_count(unsigned long long* buf, int count) {
-  if (count <= kThreads) return sort_some<1>(buf, count);
+  if (count <= kThreads) return sort_by_rank(buf, count);
   if (count <= 2 * kThreads) return sort_some<2>(buf, count);
   int n = 4 * kThreads;
   while (n < count) n <<= 1;
@@ -357,8 +379,9 @@ __device__ __forceinline__ float add_group(const float (&v)[N][Vec<T>::E], MaxSu
 template <typename T>
 __global__ __launch_bounds__(kThreads, 4) void k_top_stream(TopArgs a) {
   constexpr int E = Vec<T>::E, kSpan = kThreads * E * kGroup;
-  __shared__ unsigned long long buf[kBuffer];
+  __shared__ alignas(16) unsigned long long buf[kBuffer];
   __shared__ int count;
+  __shared__ unsigned found;
   __shared__ float red[2 * kWaves];
   const int tid = threadIdx.x;
   const int64_t items = a.rows * a.segs;
@@ -371,15 +394,12 @@ __global__ __launch_bounds__(kThreads, 4) void k_top_stream(TopArgs a) {
     unsigned long long bound = 0;
     float floor_value = ninf();
     int kept = 0;  // keys in the buffer, as every thread knows it
-    const int trigger = min(kTrigger, a.k + 128);  // sorting 256 keys is cheaper than collecting by a loose bound
-    auto key_of = [&](float v, int i) {
-      return (unsigned long long)ordered32(__float_as_uint(v)) << 32 | (0xFFFFFFFFu - (unsigned)i);
-    };
+    const int trigger = min(kTrigger, a.k + max(a.k, 64));  // sorting a few keys is cheaper than collecting by a loose bound
     auto collect = [&](const float (&v)[E], int i) {
 #pragma unroll
       for (int e = 0; e < E; ++e)
         if (!(v[e] < floor_value)) {  // few lanes, and soon hardly any
-          const unsigned long long key = key_of(v[e], i + e);
+          const unsigned long long key = RowKey<float>::make(v[e], i + e);
           if (key >= bound && i + e < e1) {
             const int at = atomicAdd(&count, 1);
             if (at < kBuffer) buf[at] = key;
@@ -409,18 +429,32 @@ __global__ __launch_bounds__(kThreads, 4) void k_top_stream(TopArgs a) {
       if (i0 + kSpan < probe_end) load_group(x, i0 + kSpan, e1, next);
       best = __builtin_elementwise_maximum(best, add_group<T>(v, t, a.c));
     }
-    load_group(x, e0, e1, next);
+    if (e1 - e0 > kSpan) load_group(x, e0, e1, next);  // else it is there still
     {
-      // the value alone: whatever equals it reaches the bound as well.  A thread without an element says -infinity.
-      unsigned long long key[1] = {(unsigned long long)ordered32(__float_as_uint(best)) << 32};
-      sort_registers<1>(key, buf);
+      // The k-th largest of the maxima, by ranks again, over maxima of `share` threads each as long as twice k of them are
+      // left: fewer to count through, for a bound that still no more than 1.4 k elements of random rows reach.  The value's
+      // upper 24 bits (an element that equals the maximum reaches that as well) over the thread, so that no two are the
+      // same.  A thread without an element says -infinity.
+      const int share = a.k <= kThreads / 8 ? 4 : a.k <= kThreads / 4 ? 2 : 1;
+      if (share >= 2) best = MaxF()(best, dpp<kXor1>(best));
+      if (share == 4) best = MaxF()(best, dpp<kXor2>(best));
+      unsigned* maxima = (unsigned*)buf;
+      const unsigned mine = (ordered32(__float_as_uint(best)) & ~255u) | (unsigned)((kThreads - 1 - tid) / share);
+      if (tid % share == 0) maxima[tid / share] = mine;
       __syncthreads();
-      buf[tid] = key[0];
+      int place = 0;
+      const u32x4* four = (const u32x4*)maxima;
+#pragma unroll 8
+      for (int j = 0; j < kThreads / 4 / share; ++j) {
+        const u32x4 m = four[j];
+        place += (int)(m.x > mine) + (int)(m.y > mine) + (int)(m.z > mine) + (int)(m.w > mine);
+      }
+      if (place == a.k - 1) found = mine & ~255u;
       if (tid == 0) count = 0;
       __syncthreads();
-      bound = buf[a.k - 1];
+      const unsigned low = found;
+      bound = (unsigned long long)(low < kOrderedLowest ? kOrderedLowest : low) << 32;
       floor_value = key_floor(bound);
-      __syncthreads();
     }
     for (int i0 = e0; i0 < e1; i0 += kSpan) {
       float v[kGroup][E];
@@ -462,9 +496,8 @@ __global__ __launch_bounds__(kThreads, 4) void k_top_stream(TopArgs a) {
       }
     } else {
       if (tid < a.k) {
-        const int at = (int)(0xFFFFFFFFu - (unsigned)buf[tid]);
-        ((T*)a.values)[row * a.k + tid] = x[at];
-        a.indices[row * a.k + tid] = at;
+        ((T*)a.values)[row * a.k + tid] = (T)RowKey<float>::value(buf[tid]);
+        a.indices[row * a.k + tid] = RowKey<float>::index(buf[tid]);
       }
       if (a.lse && tid == 0) a.lse[row] = log_sum(t, a.inv_t);
     }
@@ -472,27 +505,53 @@ __global__ __launch_bounds__(kThreads, 4) void k_top_stream(TopArgs a) {
   }
 }
 
-// Joins the segments of a row, at most kJoinKeys keys: what a block sorts in registers (800 keys through LDS took 21 us).
-constexpr int kJoinKeys = 2 * kThreads;
-static_assert(kJoinKeys <= kBuffer && kJoinKeys >= VSL_MAX_TOP, "segments of a row");
+// Joins the segments of a row, at most kJoinKeys keys in lists of k, larger first.  All segments but the last are longer
+// than k: the smallest of their q-th keys, q = ceil(k / lists), is reached by at least k keys, and so is the largest of all
+// lists' k-th.  What is below is left out; of random rows about 2 k keys stay.
+constexpr int kJoinKeys = kBuffer;
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_top_join(TopArgs a) {
-  __shared__ unsigned long long buf[kBuffer];
+  __shared__ alignas(16) unsigned long long buf[kJoinKeys];
+  __shared__ unsigned long long low[2];
+  __shared__ int count;
   __shared__ float red[2 * kWaves];
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lists = a.segs - 1, q = (a.k + lists - 1) / lists;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const unsigned long long* keys = a.keys + row * a.segs * a.k;
     const int n = a.segs * a.k;
-    for (int i = tid; i < n; i += kThreads) buf[i] = a.keys[row * n + i];
-    sort_count(buf, n);
+    if (tid == 0) {
+      low[0] = 0ull;
+      low[1] = ~0ull;
+      count = 0;
+    }
+    unsigned long long key[4];  // four at a time, the first ones under way while the bound is made
+    auto load_keys = [&](int i0) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) key[r] = keys[min(i0 + r * kThreads + tid, n - 1)];
+    };
+    load_keys(0);
+    MaxSum t{ninf(), 0.0f};
+    __syncthreads();
+    for (int s = tid; s < a.segs; s += kThreads) {
+      atomicMax(&low[0], keys[s * a.k + a.k - 1]);
+      if (s < lists) atomicMin(&low[1], keys[s * a.k + q - 1]);
+      if (a.lse) t = join(t, {a.stat[2 * (row * a.segs + s)], a.stat[2 * (row * a.segs + s) + 1]}, a.c);
+    }
+    __syncthreads();
+    const unsigned long long bound = low[0] > low[1] ? low[0] : low[1];
+    for (int i0 = 0; i0 < n; i0 += 4 * kThreads) {
+      if (i0 > 0) load_keys(i0);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (i0 + r * kThreads + tid < n && key[r] >= bound && key[r] != 0ull) buf[atomicAdd(&count, 1)] = key[r];
+    }
+    __syncthreads();
+    sort_count(buf, count);
     if (tid < a.k) {
-      const int at = (int)(0xFFFFFFFFu - (unsigned)buf[tid]);
-      ((T*)a.values)[row * a.k + tid] = ((const T*)a.logits)[row * a.stride + at];
-      a.indices[row * a.k + tid] = at;
+      ((T*)a.values)[row * a.k + tid] = (T)RowKey<float>::value(buf[tid]);
+      a.indices[row * a.k + tid] = RowKey<float>::index(buf[tid]);
     }
     if (a.lse) {
-      MaxSum t{ninf(), 0.0f};
-      for (int s = tid; s < a.segs; s += kThreads)
-        t = join(t, {a.stat[2 * (row * a.segs + s)], a.stat[2 * (row * a.segs + s) + 1]}, a.c);
       t = block_join<kWaves>(t, red, a.c);
       if (tid == 0) a.lse[row] = log_sum(t, a.inv_t);
     }
@@ -507,11 +566,12 @@ int64_t short_row(int type) { return 256 * vec_of(type); }
 struct Split {
   int segs, seg_len;
 };
-// Segments of a long row: enough blocks for the 256 CUs when there are few rows, whole tiles each, at most `most`.
-Split split_row(int64_t rows, int64_t V, int tile, int most) {
+// Segments of a long row: enough blocks for the 256 CUs when there are few rows, whole tiles each, `least` at least, and at
+// most `most` of them.
+Split split_row(int64_t rows, int64_t V, int tile, int least, int most) {
   const int64_t tiles = ceil_div(V, tile);
   int64_t segs = ceil_div(1024, rows < 1 ? 1 : rows);
-  if (segs > tiles) segs = tiles;
+  if (segs > tiles / least) segs = tiles / least;
   if (segs > most) segs = most;
   if (segs < 1) segs = 1;
   const int64_t per = ceil_div(tiles, segs);
@@ -522,7 +582,11 @@ int grid_of(int64_t items) { return (int)(items < 1 ? 1 : (items > kMaxBlocks ? 
 
 Split top_split(const vsl_top_desc* d) {
   if (d->vocab <= short_row(d->type)) return {1, (int)d->vocab};
-  return split_row(d->rows, d->vocab, kThreads * vec_of(d->type), kJoinKeys / d->k);
+  // Up to 16 tiles stay whole, a join costs more (200 x 20000 bf16: 10.0 us, in two segments 13.7), and a segment is no
+  // shorter than 4 (1 x 50021 bf16, k = 32: 14.7 us, with 2 27.9, with 8 16.4).
+  const int tile = kThreads * vec_of(d->type);
+  if (d->vocab <= 16 * tile) return {1, (int)ceil_div(d->vocab, tile) * tile};
+  return split_row(d->rows, d->vocab, tile, 4, kJoinKeys / d->k);
 }
 
 bool bad_type(int t) { return t != VSL_TYPE_F32 && t != VSL_TYPE_BF16 && t != VSL_TYPE_F16; }
@@ -1166,7 +1230,7 @@ int check_distill(const vsl_distill_desc* d) {
 Split distill_split(const vsl_distill_desc* d) {
   if (d->vocab <= short_row(d->type)) return {1, (int)d->vocab};
   const int tile = kThreads * vec_of(d->type);
-  Split s = split_row(d->rows, d->vocab, tile, 1 << 20);
+  Split s = split_row(d->rows, d->vocab, tile, 1, 1 << 20);
   if (s.seg_len > kMaxSegment) {
     s.seg_len = kMaxSegment;
     s.segs = (int)ceil_div(d->vocab, kMaxSegment);

@@ -20,6 +20,7 @@ constexpr float kLog2eLow = (float)(1.4426950408889634 - (double)1.4426950408889
 constexpr float kLn2 = 0.693147180559945309417f;
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
