@@ -168,9 +168,55 @@ __device__ __forceinline__ void sort_own(K (&key)[N]) {
           }
 }
 
-// Short rows: L lanes hold NV vectors each.  Every lane sorts its keys; every round takes the largest of the group's first
-// ones, and its lane moves on to its next.
-template <typename T, int L, int NV>
+// The sorted keys of the L lanes of a group, as one list, N to a lane: bitonic merges of twice as many lanes each, first
+// against the other half in reverse, then over half the distance and so on down to the lane's own keys.
+template <int S, typename K, int N>
+__device__ __forceinline__ void exchange(K (&key)[N]) {  // with lane ^ S (a power of two): the lower lane keeps the larger ones
+  const bool upper = threadIdx.x & S;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const K other = lane_xor<S>(key[e]);
+    key[e] = (other > key[e]) != upper ? other : key[e];
+  }
+}
+template <int S, typename K, int N>
+__device__ __forceinline__ void merge_lanes(K (&key)[N]) {  // two lists of S / 2 lanes each
+  const bool upper = threadIdx.x & (S / 2);
+  K other[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) other[e] = lane_xor<S - 1>(key[N - 1 - e]);
+#pragma unroll
+  for (int e = 0; e < N; ++e) key[e] = (other[e] > key[e]) != upper ? other[e] : key[e];
+  if (S >= 64) exchange<16>(key);
+  if (S >= 32) exchange<8>(key);
+  if (S >= 16) exchange<4>(key);
+  if (S >= 8) exchange<2>(key);
+  if (S >= 4) exchange<1>(key);
+#pragma unroll
+  for (int q = N / 2; q >= 1; q >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (!(i & q)) {
+        const K a = key[i], b = key[i + q];
+        key[i] = a > b ? a : b;
+        key[i + q] = a > b ? b : a;
+      }
+}
+template <int L, typename K, int N>
+__device__ __forceinline__ void merge_group(K (&key)[N]) {
+  merge_lanes<2>(key);
+  merge_lanes<4>(key);
+  merge_lanes<8>(key);
+  if (L > 8) merge_lanes<16>(key);
+  if (L > 16) {
+    merge_lanes<32>(key);
+    merge_lanes<64>(key);
+  }
+}
+
+// Short rows: L lanes hold NV vectors each.  Every lane sorts its keys.  For few keys every round takes the largest of the
+// group's first ones, and its lane moves on to its next; for many (SORT) the lanes' lists are merged.
+template <typename T, int L, int NV, bool SORT>
 __global__ __launch_bounds__(kThreads) void k_top_rows(TopArgs a) {
   constexpr int E = Vec<T>::E, G = kThreads / L;
   typedef typename RowKey<T>::K K;
@@ -213,6 +259,18 @@ __global__ __launch_bounds__(kThreads) void k_top_rows(TopArgs a) {
       if (live && lane == 0) a.lse[row] = log_sum(t, a.inv_t);
     }
     sort_own<NV * E>(key);
+    if (SORT) {
+      merge_group<L>(key);
+#pragma unroll
+      for (int e = 0; e < NV * E; ++e) {
+        const int j = lane * NV * E + e;
+        if (live && j < a.k) {
+          ((T*)a.values)[row * a.k + j] = RowKey<T>::value(key[e]);
+          a.indices[row * a.k + j] = RowKey<T>::index(key[e]);
+        }
+      }
+      continue;
+    }
     K mine = 0;
     for (int j = 0; j < a.k; ++j) {
       const K best = group_all<L>(key[0], MaxU());
@@ -612,19 +670,29 @@ int check_top(const vsl_top_desc* d) {
   return VSL_OK;
 }
 
+// Merging the lanes' lists takes the time of about 20 rounds, of 15 with the 64-bit keys of float32 (by rounds and merged:
+// 100000 x 60 bf16, k = 16: 13.0 and 12.0 us; 20000 x 500 bf16, k = 16: 24.3 and 26.5, k = 32: 40.2 and 27.7;
+// 20000 x 250 f32, k = 8: 24.1 and 24.9, k = 24: 50.3 and 25.7).
+template <typename T>
+constexpr int most_rounds() { return sizeof(T) == 4 ? 15 : 20; }
+template <typename T, bool SORT>
+void launch_rows(const TopArgs& a, int nv, hipStream_t s) {
+  const dim3 b(kThreads);
+  const dim3 g8(grid_of(ceil_div(a.rows, kThreads / 8)));
+  const dim3 g16(grid_of(ceil_div(a.rows, kThreads / 16))), g64(grid_of(ceil_div(a.rows, kThreads / 64)));
+  if (nv <= 8) hipLaunchKernelGGL((k_top_rows<T, 8, 1, SORT>), g8, b, 0, s, a);
+  else if (nv <= 16) hipLaunchKernelGGL((k_top_rows<T, 8, 2, SORT>), g8, b, 0, s, a);
+  else if (nv <= 32) hipLaunchKernelGGL((k_top_rows<T, 16, 2, SORT>), g16, b, 0, s, a);
+  else if (nv <= 64) hipLaunchKernelGGL((k_top_rows<T, 16, 4, SORT>), g16, b, 0, s, a);
+  else if (nv <= 128) hipLaunchKernelGGL((k_top_rows<T, 64, 2, SORT>), g64, b, 0, s, a);
+  else hipLaunchKernelGGL((k_top_rows<T, 64, 4, SORT>), g64, b, 0, s, a);
+}
 template <typename T>
 void launch_top(const TopArgs& a, bool rows_program, hipStream_t s) {
   if (rows_program) {
     const int nv = (int)ceil_div(a.V, Vec<T>::E);
-    const dim3 b(kThreads);
-    const dim3 g8(grid_of(ceil_div(a.rows, kThreads / 8)));
-    const dim3 g16(grid_of(ceil_div(a.rows, kThreads / 16))), g64(grid_of(ceil_div(a.rows, kThreads / 64)));
-    if (nv <= 8) hipLaunchKernelGGL((k_top_rows<T, 8, 1>), g8, b, 0, s, a);
-    else if (nv <= 16) hipLaunchKernelGGL((k_top_rows<T, 8, 2>), g8, b, 0, s, a);
-    else if (nv <= 32) hipLaunchKernelGGL((k_top_rows<T, 16, 2>), g16, b, 0, s, a);
-    else if (nv <= 64) hipLaunchKernelGGL((k_top_rows<T, 16, 4>), g16, b, 0, s, a);
-    else if (nv <= 128) hipLaunchKernelGGL((k_top_rows<T, 64, 2>), g64, b, 0, s, a);
-    else hipLaunchKernelGGL((k_top_rows<T, 64, 4>), g64, b, 0, s, a);
+    if (a.k > most_rounds<T>()) launch_rows<T, true>(a, nv, s);
+    else launch_rows<T, false>(a, nv, s);
     return;
   }
   hipLaunchKernelGGL(k_top_stream<T>, dim3(grid_of(a.rows * a.segs)), dim3(kThreads), 0, s, a);

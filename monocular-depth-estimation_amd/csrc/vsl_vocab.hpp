@@ -108,7 +108,19 @@ template <int CTRL>
 __device__ __forceinline__ unsigned long long dpp(unsigned long long v) {
   return ((unsigned long long)dpp<CTRL>((unsigned)(v >> 32)) << 32) | dpp<CTRL>((unsigned)v);
 }
-constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kMirror8 = 0x141, kMirror16 = 0x140;
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kMirror4 = 0x1B, kMirror8 = 0x141, kMirror16 = 0x140;
+// the value of lane ^ X, X a power of two or one less (a mirror)
+template <int X, typename V>
+__device__ __forceinline__ V lane_xor(V v) {
+  if (X == 1) return dpp<kXor1>(v);
+  if (X == 2) return dpp<kXor2>(v);
+  if (X == 3) return dpp<kMirror4>(v);
+  if (X == 4) return dpp<kMirror8>(dpp<kMirror4>(v));
+  if (X == 7) return dpp<kMirror8>(v);
+  if (X == 8) return dpp<kMirror16>(dpp<kMirror8>(v));
+  if (X == 15) return dpp<kMirror16>(v);
+  return (V)__shfl_xor(v, X, 64);
+}
 
 // all L lanes of a group (L = 8, 16 or 64, aligned) get op over the group
 template <int L, typename V, typename Op>
