@@ -425,6 +425,23 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
   }
 }
 
+// A row's loss and statistics from its joined maximum and sum; logit(t): the target's.
+template <typename F>
+__device__ __forceinline__ float close_row(MaxSum q, F logit, int64_t t, int64_t ignore_index, int64_t vocab, float z_loss,
+                                           int64_t row, int64_t rows, float* row_loss, float* stats, bool& counts) {
+  const float ls = log2_sum(q), lse = log_sum(q, 1.0f);
+  float m = q.m, loss = 0.0f;
+  counts = t != ignore_index;
+  if (counts) {
+    if (t < 0 || t >= vocab) loss = m = qnan();
+    else if (m != ninf()) loss = fmaf(ls, kLn2, m - logit(t)) + (z_loss == 0.0f ? 0.0f : z_loss * lse * lse);
+  }
+  row_loss[row] = loss;
+  stats[row] = m;
+  stats[rows + row] = ls;
+  return loss;
+}
+
 // R rows a block, THREADS / R lanes each: joins the tiles' maxima and sums, four of a lane's at a time.  A block also sums
 // its rows' losses: closes the reduced loss if it has all rows, leaves its sums in `pairs` otherwise.
 template <int R, int THREADS>
@@ -459,19 +476,9 @@ __global__ __launch_bounds__(THREADS) void k_ce_rows(const float2* __restrict__ 
   }
   float loss = 0.0f;
   bool counts = false;
-  if (g == 0 && row < rows) {
-    const float ls = log2_sum(q), lse = log_sum(q, 1.0f);
-    float m = q.m;
-    const int64_t t = target[row];
-    counts = t != ignore_index;
-    if (counts) {
-      if (t < 0 || t >= vocab) loss = m = qnan();
-      else if (m != ninf()) loss = fmaf(ls, kLn2, m - target_logit[row]) + (z_loss == 0.0f ? 0.0f : z_loss * lse * lse);
-    }
-    row_loss[row] = loss;
-    stats[row] = m;
-    stats[rows + row] = ls;
-  }
+  if (g == 0 && row < rows)
+    loss = close_row(q, [&](int64_t) { return target_logit[row]; }, target[row], ignore_index, vocab, z_loss, row, rows, row_loss,
+                     stats, counts);
   if (reduction == VSL_REDUCE_NONE) return;
   __shared__ double sum[2][R];
   __syncthreads();
@@ -873,6 +880,125 @@ __global__ __launch_bounds__(kThreads) void k_ce_bias(const void* __restrict__ d
 }
 
 // ------------------------------------------------------------------------------------------------------------------
+// Logits in parts of the features: few tiles over many features leave most CUs idle, so the product is cut along them
+// like the gradients' and leaves [splits][rows][classes] sums, from which these two take their logits.  12 x 1398 x 1944
+// float32 forward: 16 us, whole 69; 459 x 767 x 3722 with gradients: 210 and 503; 200 x 1000 x 4096 bfloat16 forward: 15 and
+// 40.  Both kernels are bound by the latency of their reads, which is why these go out 16 at a time.
+// ------------------------------------------------------------------------------------------------------------------
+struct Parts {
+  const float* sum;
+  int splits;
+  int64_t rows, vocab;
+  const void* bias;
+  // U logits `apart` elements apart, the first of them `row`, `v`; -infinity where `on` says no
+  template <typename T, int U, typename On>
+  __device__ __forceinline__ void logits(int64_t row, int64_t v, int64_t rows_apart, int64_t classes_apart, On on,
+                                         float (&z)[U]) const {
+    const int64_t all = rows * vocab;
+    const float* p[U];  // every one is read, so that the reads go out together
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      z[u] = 0.0f;
+      p[u] = sum + (on(u) ? (row + u * rows_apart) * vocab + v + u * classes_apart : 0);
+    }
+    int s = 0;
+    for (; s + 4 <= splits; s += 4) {
+      float x[4][U];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[i][u] = p[u][(s + i) * all];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int u = 0; u < U; ++u) z[u] += x[i][u];
+    }
+    for (; s < splits; ++s)
+#pragma unroll
+      for (int u = 0; u < U; ++u) z[u] += p[u][s * all];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float b = !on(u) ? ninf() : bias ? (float)((const T*)bias)[v + u * classes_apart] : 0.0f;
+      z[u] = b == ninf() ? b : z[u] + b;  // a masked class stays masked whatever its weights hold
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ float logit(int64_t row, int64_t v) const {
+    float z[1];
+    logits<T>(row, v, 0, 0, [](int) { return true; }, z);
+    return z[0];
+  }
+};
+
+// forward: a block per row
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_ce_parts_rows(Parts z, const int64_t* __restrict__ target, int64_t ignore_index,
+                                                           float z_loss, float* __restrict__ row_loss,
+                                                           float* __restrict__ stats, int reduction,
+                                                           double* __restrict__ pairs, float* __restrict__ loss_out,
+                                                           float* __restrict__ divisor) {
+  __shared__ float red[THREADS / 32];
+  const int64_t row = blockIdx.x;
+  MaxSum q{ninf(), 0.0f};
+  for (int64_t v = threadIdx.x; v < z.vocab; v += 4 * THREADS) {
+    float x[4];
+    z.logits<T>(row, v, 0, THREADS, [&](int u) { return v + u * THREADS < z.vocab; }, x);
+    float m = q.m;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) m = __builtin_elementwise_maximum(m, x[u]);
+    const Exponent ex(exp_ref(m), kLog2e);
+    float s = q.s * exp_of(q.m, exp_ref(m), kLog2e);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) s += ex(x[u]);
+    q = {m, s};
+  }
+  q = block_join<THREADS / 64>(q, red, kLog2e);
+  if (threadIdx.x) return;
+  bool counts;
+  const float loss = close_row(q, [&](int64_t t) { return z.logit<T>(row, t); }, target[row], ignore_index, z.vocab, z_loss, row,
+                               z.rows, row_loss, stats, counts);
+  if (reduction == VSL_REDUCE_NONE) return;
+  if (gridDim.x == 1) {
+    finish_sum((double)loss, counts ? 1.0 : 0.0, reduction, loss_out, divisor);
+  } else {
+    pairs[2 * row] = (double)loss;
+    pairs[2 * row + 1] = counts ? 1.0 : 0.0;
+  }
+}
+
+// backward: 16 rows x 64 classes a block, written as they are and transposed
+constexpr int kPartRows = 16;
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_ce_parts_delta(Parts z, LogitArgs a) {
+  __shared__ float tile[kPartRows][65];
+  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+  const int64_t r0 = (int64_t)blockIdx.y * kPartRows, v0 = (int64_t)blockIdx.x * 64, v = v0 + x;
+  float logit[4];
+  z.logits<T>(r0 + y, v, 4, 0, [&](int u) { return r0 + y + 4 * u < z.rows && v < z.vocab; }, logit);
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int64_t row = r0 + y + 4 * u;
+    const bool live = row < z.rows;
+    const int64_t target = live ? a.target[row] : -1;
+    const float top = live ? a.stats[row] : ninf(), ls = live ? a.stats[z.rows + row] : 0.0f;
+    const float scale = !live || top == ninf() || target == a.ignore_index ? 0.0f : a.row_scale ? a.row_scale[row] : a.unit;
+    float d = 0.0f;
+    if (scale != 0.0f) {
+      const Exponent ex(top, kLog2e);
+      d = scale * slope_of(a.z_loss, top, ls) * __builtin_amdgcn_exp2f(fmaf(logit[u], ex.c, ex.shift - ls));
+      if (v == target) d -= scale;
+    }
+    if (a.delta) ((T*)a.delta)[row * a.ldd + v] = (T)d;
+    tile[y + 4 * u][x] = d;
+  }
+  if (!a.delta_t) return;
+  __syncthreads();
+  const int r = threadIdx.x % kPartRows;
+#pragma unroll
+  for (int c = threadIdx.x / kPartRows; c < 64; c += kThreads / kPartRows) ((T*)a.delta_t)[(v0 + c) * a.ldt + r0 + r] = (T)tile[r][c];
+}
+
+// ------------------------------------------------------------------------------------------------------------------
 // host
 // ------------------------------------------------------------------------------------------------------------------
 int size_of(int type) { return type == VSL_TYPE_F32 ? 4 : 2; }
@@ -960,16 +1086,28 @@ struct Layout {
   int64_t rows_padded, dim_padded;
   bool copy_hidden, copy_weight;
   int tail;            // Operands::tail of the logits' products
+  Plan logits;         // of the logits of all classes; several splits: in parts
   int64_t steps(int64_t K) const { return (split ? kPairs : 1) * blocks_of(K, type); }
 };
+constexpr int64_t kMostParts = 1LL << 23;  // padded logits whose product may be cut: with more there are tiles enough
 Layout layout_of(const vsl_linear_ce_desc* d) {
   Layout l{};
   l.rows_padded = round_up(d->rows, kPad);
+  // Logits in parts cost a pass over the sums, forward and backward (5 us, and 0.5 for every
+  // turn of its block along a row).
+  auto plan_logits = [&](int type, int64_t steps, bool parts) {
+    const Plan whole = plan_of(d->vocab, d->rows, steps, type, false);
+    if (!parts || l.rows_padded * round_up(d->vocab, kPad) > kMostParts) return whole;
+    Plan cut = plan_of(d->vocab, d->rows, steps, type, true);
+    cut.time += 5.0 + 0.5 * (double)ceil_div(d->vocab, 4096);
+    return cut.splits > 1 && cut.time < whole.time ? cut : whole;
+  };
+  l.logits = plan_logits(d->type, blocks_of(d->dim, d->type), true);
   if (d->type == VSL_TYPE_F32) {
     // the planes are worth writing (10 bytes a value) where they save more on the logits than that
-    const double direct = plan_of(d->vocab, d->rows, blocks_of(d->dim, VSL_TYPE_F32), VSL_TYPE_F32, false).time;
-    const double planes = plan_of(d->vocab, d->rows, kPairs * blocks_of(d->dim, VSL_TYPE_BF16), VSL_TYPE_BF16, false).time;
-    l.split = planes + 10.0 + (double)(d->rows + d->vocab) * (double)d->dim * 10.0 / 4e6 < direct;
+    const Plan planes = plan_logits(VSL_TYPE_BF16, kPairs * blocks_of(d->dim, VSL_TYPE_BF16), false);
+    l.split = planes.time + 10.0 + (double)(d->rows + d->vocab) * (double)d->dim * 10.0 / 4e6 < l.logits.time;
+    if (l.split) l.logits = planes;
   }
   l.type = l.split ? VSL_TYPE_BF16 : d->type;
   l.size = size_of(l.type);
@@ -987,6 +1125,7 @@ struct Forward {
   void *hidden, *weight;
   float2* partial;
   float* target_logit;
+  float* parts;
   double* pairs;
   size_t total;
 };
@@ -997,6 +1136,12 @@ Forward forward_workspace(const vsl_linear_ce_desc* d, void* base) {
   Forward f{};
   f.hidden = l.copy_hidden ? a.take((size_t)d->rows * l.dim_padded * s) : nullptr;
   f.weight = l.copy_weight ? a.take((size_t)d->vocab * l.dim_padded * s) : nullptr;
+  if (l.logits.splits > 1) {
+    f.parts = (float*)a.take((size_t)l.logits.splits * d->rows * d->vocab * 4);
+    f.pairs = (double*)a.take((size_t)d->rows * 2 * sizeof(double));
+    f.total = a.used;
+    return f;
+  }
   f.partial = (float2*)a.take((size_t)ceil_div(d->vocab, Small::BM) * l.rows_padded * sizeof(float2));
   f.target_logit = (float*)a.take((size_t)d->rows * 4);
   f.pairs = (double*)a.take((size_t)ceil_div(d->rows, d->rows <= 2048 ? 4 : 16) * 2 * sizeof(double));
@@ -1008,6 +1153,7 @@ Forward forward_workspace(const vsl_linear_ce_desc* d, void* base) {
 // would stay in the last-level cache, but every piece reads and writes grad_hidden's sums: at 8192 x 131072 x 4096 in
 // bfloat16 2^26, 2^27 and 2^28 elements take 29.6, 29.3 and 29.3 ms.
 constexpr int64_t kPieceElements = 1LL << 27;
+static_assert(kMostParts <= kPieceElements && kMostParts / kPad / kPartRows < 65536, "logits in parts are one piece, their rows one grid");
 
 constexpr int64_t kBiasBlocks = 1024;
 
@@ -1016,7 +1162,7 @@ struct Backward {
   int64_t piece, pieces, vocab_padded;
   Plan plan_h, plan_w;
   void *hidden, *weight, *hidden_t, *weight_t, *delta, *delta_t;
-  float *sum_h, *sum_w, *sum_b, *row_scale, *out_scale, *largest;
+  float *sum_h, *sum_w, *sum_b, *row_scale, *out_scale, *largest, *parts;
   size_t total;
 };
 Backward backward_workspace(const vsl_linear_ce_desc* d, uint32_t mask, void* base) {
@@ -1044,6 +1190,7 @@ Backward backward_workspace(const vsl_linear_ce_desc* d, uint32_t mask, void* ba
   b.row_scale = (float*)a.take((size_t)b.l.rows_padded * 4);
   b.out_scale = (float*)a.take(4);
   b.largest = (float*)a.take(256 * 4);
+  b.parts = b.l.logits.splits > 1 ? (float*)a.take((size_t)b.l.logits.splits * d->rows * d->vocab * 4) : nullptr;
   b.total = a.used;
   return b;
 }
@@ -1130,6 +1277,16 @@ void launch_grad(GradArgs* g, const int* shape, int n, hipStream_t s) {
   launch_grad_as<T, Small, SPLIT>(g, n, s);
 }
 
+template <typename T>
+void launch_parts(const Operands& op, const Plan& plan, float* parts, hipStream_t s) {
+  GradArgs g{};
+  g.op = op;
+  g.sum = parts;
+  g.out = parts;
+  g.splits = plan.splits;
+  launch_grad<T, false>(&g, &plan.shape, 1, s);
+}
+
 template <typename T, bool SPLIT>
 void run_forward(const vsl_linear_ce_desc* d, const Layout& l, const Forward& f, float* row_loss, float* stats, float* loss,
                  float* divisor, hipStream_t s) {
@@ -1145,9 +1302,22 @@ void run_forward(const vsl_linear_ce_desc* d, const Layout& l, const Forward& f,
   a.bias = d->bias;
   a.target = d->target;
   a.rows_padded = l.rows_padded;
+  if constexpr (!SPLIT)
+    if (f.parts) {
+      launch_parts<T>(a.op, l.logits, f.parts, s);
+      auto rows = [&](auto kernel, int threads) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)d->rows), dim3(threads), 0, s,
+                           Parts{f.parts, l.logits.splits, d->rows, d->vocab, d->bias}, d->target, d->ignore_index, d->z_loss,
+                           row_loss, stats, d->reduction, f.pairs, loss, divisor);
+      };
+      if (d->vocab > 2048) rows(k_ce_parts_rows<T, 1024>, 1024);  // 10544 classes of two rows: 8.9 us, with 256 threads 17.6
+      else rows(k_ce_parts_rows<T, kThreads>, kThreads);
+      if (d->reduction != VSL_REDUCE_NONE && d->rows > 1) launch_sum_pairs(f.pairs, d->rows, d->reduction, loss, divisor, s);
+      return;
+    }
   a.partial = f.partial;
   a.target_logit = f.target_logit;
-  const int tiles = launch_logits<T, false, SPLIT>(a, plan_of(a.op.M, a.op.N, l.steps(d->dim), l.type, false).shape, s);
+  const int tiles = launch_logits<T, false, SPLIT>(a, l.logits.shape, s);
   // few rows: more lanes each, so that no lane walks many tiles (16 rows of 512 tiles: 14 us with 16 lanes a row); many rows:
   // more of them a block, so that fewer sums are left
   auto rows = [&](auto kernel, int per_block, int threads) {
@@ -1211,9 +1381,10 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
   const int64_t ldw = l.copy_weight ? l.planes * l.dim_padded : d->weight_stride;
   for (int64_t p = 0; p < b.pieces; ++p) {
     const int64_t v0 = p * b.piece, classes = d->vocab - v0 < b.piece ? d->vocab - v0 : b.piece;
-    const int shape = plan_of(classes, d->rows, l.steps(d->dim), l.type, false).shape;
+    const int shape = b.pieces == 1 ? l.logits.shape : plan_of(classes, d->rows, l.steps(d->dim), l.type, false).shape;
     // what the derivative kernel covers: whole steps of K for the two products that follow
-    const int64_t padded = round_up(classes, kShapes[shape].bm), rows_covered = round_up(d->rows, kShapes[shape].bn);
+    const int64_t padded = round_up(classes, b.parts ? 64 : kShapes[shape].bm);
+    const int64_t rows_covered = round_up(d->rows, b.parts ? 64 : kShapes[shape].bn);
     LogitArgs a{};
     a.op = {weight + v0 * ldw, hidden, ldw, ldh, (int)classes, (int)d->rows, (int)(l.dim_padded / Kind<O>::BK), l.dim_padded,
             l.dim_padded, l.tail};
@@ -1231,7 +1402,15 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
     a.plane_d = b.piece;
     a.ldt = l.planes * l.rows_padded;
     a.delta_t = grad_weight || grad_bias ? b.delta_t : nullptr;
-    launch_logits<T, true, SPLIT>(a, shape, s);
+    bool made = false;
+    if constexpr (!SPLIT)
+      if (b.parts) {
+        launch_parts<T>(a.op, l.logits, b.parts, s);
+        hipLaunchKernelGGL(k_ce_parts_delta<T>, dim3((unsigned)(padded / 64), (unsigned)(rows_covered / kPartRows)), dim3(kThreads),
+                           0, s, Parts{b.parts, l.logits.splits, d->rows, d->vocab, d->bias}, a);
+        made = true;
+      }
+    if (!made) launch_logits<T, true, SPLIT>(a, shape, s);
     GradArgs g[2] = {};
     int shapes[2], n = 0;
     FinishLaunch finish;

@@ -426,6 +426,33 @@ def test_linear_cross_entropy_tile_shapes(rows, vocab, dim, bias, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab,dim", [(1, 3, 4096), (12, 1398, 1944), (29, 71, 1537), (3, 9000, 2047), (200, 1001, 4095), (459, 767, 2000)])
+def test_linear_cross_entropy_in_parts_of_the_features(rows, vocab, dim, dtype):
+    """Few tiles over many features: the logits come from sums of parts."""
+    h, w, b, t = ce_inputs(rows, vocab, dim, dtype, rows + dim, bias=rows % 2 == 1)
+    if rows > 4:
+        t[torch.rand(rows, generator=gen(11)) < 0.2] = -100
+    check_ce(h, w, b, t, z_loss=1e-3 if rows % 4 == 0 else 0.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_cross_entropy_in_parts_masks_and_specials(dtype):
+    rows, vocab, dim = 40, 150, 3000
+    h, w, b, t = ce_inputs(rows, vocab, dim, dtype, 79, bias=True)
+    b[140:] = -INF
+    t[t >= 140] = 0
+    w[145:] = float("nan")
+    t[3], t[4], t[8] = 7, 7, 141                            # two rows that do not count, one whose target is masked out
+    h[3], h[4, 5] = float("nan"), INF
+    check_ce(h, w, b, t, ignore_index=7)
+    t[9] = vocab                                            # NaN, loudly
+    check_ce(h, w, b, t, ignore_index=7)
+    t[9], b[:] = 1, -INF
+    out, grads = check_ce(h, w, b, t, ignore_index=7)
+    assert not out.any() and not any(g.any() for g in grads)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_linear_cross_entropy_several_pieces_of_the_vocabulary(dtype):
     """rows * classes above one piece (2^27 derivatives): the pieces' sums join, the last one is ragged."""
     rows, vocab, dim = 2048, 70001, 64
