@@ -68,6 +68,15 @@ __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c, const float*) 
   return c;
 }
 
+// 16 bytes of a row that may start anywhere, zeros behind the last column
+template <typename T>
+__device__ __forceinline__ u32x4 load_columns(const T* p, int c, int cols) {
+  if (c + Kind<T>::E <= cols) return load16(p + c);
+  float v[Kind<T>::E];
+#pragma unroll
+  for (int e = 0; e < Kind<T>::E; ++e) v[e] = c + e < cols ? (float)p[c + e] : 0.0f;
+  return pack(v, (const T*)nullptr);
+}
 // Operands of a product: A [M, >= kblocks * BK], B [N, ...], rows `lda`, `ldb` elements apart; in the split form the
 // planes of a row are plane_a, plane_b elements apart.
 struct Operands {
@@ -77,6 +86,7 @@ struct Operands {
   int M, N, kblocks;
   int64_t plane_a, plane_b;
   int tail;  // 16-byte pieces of a row in the last block (8: it is whole); what follows them is not the row's
+  int dim;   // elements of a row, where rows lie at any address (STAGED)
 };
 // what the pieces behind a row's end are read from
 __device__ const u32x4 kZeros[1] = {{0u, 0u, 0u, 0u}};
@@ -98,8 +108,10 @@ struct Tile {
 // A step is four rounds; each round's fragments are read while the round before multiplies.  The barrier stands before the
 // last round, whose fragments are in registers by then: behind it the buffer is free for the step after next, and the
 // next step's first fragments are read under the last round's multiplications.
+// STAGED: rows that start anywhere or end inside a piece cannot go straight to LDS.  They go through registers, asked for a
+// step ahead of their store, which takes the place of the fetch.
 // T: the operands' type; steps [k0, k1) of kblocks, or of kPairs * kblocks in the split form.
-template <typename T, typename S, bool SPLIT>
+template <typename T, typename S, bool SPLIT, bool STAGED>
 __device__ __forceinline__ void tile_product(const Operands& op, int m0, int n0, int k0, int k1, char* lds, Tile<S>& t) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / S::WN, wn = wave % S::WN;
@@ -151,6 +163,21 @@ __device__ __forceinline__ void tile_product(const Operands& op, int m0, int n0,
       src[i] += i < S::kFetchA ? next_a : next_b;
     }
   };
+  u32x4 held[STAGED ? S::kFetch : 1];
+  int next_step = k0;
+  auto load = [&]() {
+    const int first = next_step * Kind<T>::BK + ((tid & 7) ^ ((tid >> 4) & 7)) * Kind<T>::E;  // column of a thread's pieces
+    const bool whole = (++next_step) * Kind<T>::BK <= op.dim;
+#pragma unroll
+    for (int i = 0; i < (STAGED ? S::kFetch : 0); ++i) {
+      held[i] = whole ? load16((const T*)src[i]) : load_columns((const T*)src[i], 0, op.dim - first);
+      src[i] += kBlockBytes;
+    }
+  };
+  auto store = [&](int buffer) {
+#pragma unroll
+    for (int i = 0; i < (STAGED ? S::kFetch : 0); ++i) *(u32x4*)(lds + buffer * S::kBuffer + (i * S::kThreads + tid) * 16) = held[i];
+  };
   auto wait = [&]() {  // this wave's pieces are in LDS and its reads are done; then everyone's are
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
@@ -183,9 +210,15 @@ __device__ __forceinline__ void tile_product(const Operands& op, int m0, int n0,
     __builtin_amdgcn_sched_group_barrier(0x008, kMma - kRead * kEach, 0);
     __builtin_amdgcn_sched_barrier(0);
   };
-  fetch(0);
+  if (STAGED) {
+    load();
+    store(0);
+    if (k0 + 1 < k1) load();
+  } else {
+    fetch(0);
+  }
   wait();
-  if (k0 + 1 < k1) fetch(1);
+  if (k0 + 1 < k1) STAGED ? store(1) : fetch(1);
   read(0, 0, 0);
   auto rounds = [&](int buffer) {  // the first three
 #pragma unroll
@@ -197,9 +230,10 @@ __device__ __forceinline__ void tile_product(const Operands& op, int m0, int n0,
   };
   for (int k = k0; k < k1 - 1; ++k) {
     const int buffer = (k - k0) & 1;
+    if (STAGED && k + 2 < k1) load();
     rounds(buffer);
     wait();
-    if (k + 2 < k1) fetch(buffer);
+    if (k + 2 < k1) STAGED ? store(buffer) : fetch(buffer);
     read(0, buffer ^ 1, 0);
     multiply(1);
     interleave();
@@ -288,7 +322,7 @@ __device__ __forceinline__ float take_plane(float& z) {
 }
 
 // T: the tensors' type; SPLIT: float32 by planes of bfloat16
-template <typename T, typename S, bool DELTA, bool SPLIT>
+template <typename T, typename S, bool DELTA, bool SPLIT, bool STAGED>
 __global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
   typedef std::conditional_t<SPLIT, __bf16, T> O;
   __shared__ __attribute__((aligned(16))) char lds[S::kLds];
@@ -297,7 +331,7 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
   tile_of(blockIdx.x, tm_count, tn_count, tm, tn);
   const int m0 = tm * S::BM, n0 = tn * S::BN;
   Tile<S> t;
-  tile_product<O, S, SPLIT>(a.op, m0, n0, 0, (SPLIT ? kPairs : 1) * a.op.kblocks, lds, t);
+  tile_product<O, S, SPLIT, STAGED>(a.op, m0, n0, 0, (SPLIT ? kPairs : 1) * a.op.kblocks, lds, t);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
   const int half = lane >> 5;
   const bool biased = a.bias || m0 + S::BM > a.op.M;
@@ -633,15 +667,6 @@ __device__ __forceinline__ void load8(const float* p, int c, int cols, float (&v
     for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? p[c + e] : 0.0f;
   }
 }
-// 16 bytes of a row that may start anywhere, zeros behind the last column
-template <typename T>
-__device__ __forceinline__ u32x4 load_columns(const T* p, int c, int cols) {
-  if (c + Kind<T>::E <= cols) return load16(p + c);
-  float v[Kind<T>::E];
-#pragma unroll
-  for (int e = 0; e < Kind<T>::E; ++e) v[e] = c + e < cols ? (float)p[c + e] : 0.0f;
-  return pack(v, (const T*)nullptr);
-}
 template <typename O>
 __device__ __forceinline__ void store_planes(O* out, int64_t width, const Planes& q) {
   *(u32x4*)out = q.h;
@@ -751,7 +776,7 @@ struct GradJobs {
   unsigned first;  // blocks of the first
 };
 
-template <typename T, typename S, bool SPLIT>
+template <typename T, typename S, bool SPLIT, bool STAGED>
 __global__ __launch_bounds__(S::kThreads) void k_ce_grad(GradJobs jobs) {
   const int which = blockIdx.x >= jobs.first ? 1 : 0;
   const GradArgs& a = jobs.job[which];
@@ -765,7 +790,7 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_grad(GradJobs jobs) {
   const int k0 = min(split * per, steps), k1 = min(k0 + per, steps);
   const int m0 = tm * S::BM, n0 = tn * S::BN;
   Tile<S> t;
-  tile_product<std::conditional_t<SPLIT, __bf16, T>, S, SPLIT>(a.op, m0, n0, k0, k1, lds, t);
+  tile_product<std::conditional_t<SPLIT, __bf16, T>, S, SPLIT, STAGED>(a.op, m0, n0, k0, k1, lds, t);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
   const float scale = a.sum ? 1.0f : a.scale.get();
 #pragma unroll
@@ -1056,15 +1081,18 @@ struct ShapeInfo {
 constexpr ShapeInfo kShapes[] = {{Large::BM, Large::BN, 256, 1.7f, 0.0f, 4.0f},
                                  {Small::BM, Small::BN, 512, 1.3f, 5.0f, 2.5f},
                                  {Narrow::BM, Narrow::BN, 768, 1.1f, 4.0f, 2.0f}};
+// A step through registers against one straight to LDS, its loads off their alignment.  7 x 96190 x 3653 bfloat16 forward
+// takes 161 us through registers and 420 copied first; 6439 x 736 x 2647 float16 with gradients 297 and 271.
+constexpr double kStaged = 1.5;
 // Shape of the tiles of a product M x N over `blocks` steps of K, and into how many parts K is cut: the least of the waves
 // of tiles times their length, plus the traffic of the partial sums.  float32 leaves out the large tile: its epilogue
 // does not fit the registers, and its matrix instructions are eight times slower, so that its loads never bind.
-Plan plan_of(int64_t M, int64_t N, int64_t blocks, int type, bool may_split) {
+Plan plan_of(int64_t M, int64_t N, int64_t blocks, int type, bool may_split, bool staged = false) {
   Plan best{kSmall, 1, 1e300};
-  for (int shape = type == VSL_TYPE_F32 ? kSmall : kLarge; shape <= kNarrow; ++shape) {
+  for (int shape = type == VSL_TYPE_F32 || staged ? kSmall : kLarge; shape <= kNarrow; ++shape) {
     const ShapeInfo& h = kShapes[shape];
     const double tiles = (double)(ceil_div(M, h.bm) * ceil_div(N, h.bn));
-    const double step = type == VSL_TYPE_F32 ? h.step32 : h.step16;
+    const double step = (type == VSL_TYPE_F32 ? h.step32 : h.step16) * (staged ? kStaged : 1.0);
     for (int s = 1; s <= 256 && (s == 1 || (may_split && blocks / s >= 4)); s = s < 16 ? s + 1 : s + s / 4) {
       // a CU that holds fewer tiles than it could runs each of them faster, though not in proportion
       const double full = (double)(int64_t)(tiles * s / h.slots), rest = tiles * s - full * h.slots;
@@ -1085,6 +1113,7 @@ struct Layout {
   int type, size, planes;
   int64_t rows_padded, dim_padded;
   bool copy_hidden, copy_weight;
+  bool staged;         // the logits' operands go through registers
   int tail;            // Operands::tail of the logits' products
   Plan logits;         // of the logits of all classes; several splits: in parts
   int64_t steps(int64_t K) const { return (split ? kPairs : 1) * blocks_of(K, type); }
@@ -1095,26 +1124,38 @@ Layout layout_of(const vsl_linear_ce_desc* d) {
   l.rows_padded = round_up(d->rows, kPad);
   // Logits in parts cost a pass over the sums, forward and backward (5 us, and 0.5 for every
   // turn of its block along a row).
-  auto plan_logits = [&](int type, int64_t steps, bool parts) {
-    const Plan whole = plan_of(d->vocab, d->rows, steps, type, false);
+  auto plan_logits = [&](int type, int64_t steps, bool parts, bool staged) {
+    const Plan whole = plan_of(d->vocab, d->rows, steps, type, false, staged);
     if (!parts || l.rows_padded * round_up(d->vocab, kPad) > kMostParts) return whole;
-    Plan cut = plan_of(d->vocab, d->rows, steps, type, true);
+    Plan cut = plan_of(d->vocab, d->rows, steps, type, true, staged);
     cut.time += 5.0 + 0.5 * (double)ceil_div(d->vocab, 4096);
     return cut.splits > 1 && cut.time < whole.time ? cut : whole;
   };
-  l.logits = plan_logits(d->type, blocks_of(d->dim, d->type), true);
+  l.logits = plan_logits(d->type, blocks_of(d->dim, d->type), true, false);
+  l.copy_hidden = !ready(d->hidden, d->hidden_stride, d->dim, d->type);
+  l.copy_weight = !ready(d->weight, d->weight_stride, d->dim, d->type);
+  if (l.copy_hidden || l.copy_weight) {
+    // Rows that the main loop cannot take as they are: copied (read and written), or through registers, without the large
+    // tile.
+    const int64_t elements = (l.copy_hidden ? d->rows : 0) + (l.copy_weight ? d->vocab : 0);
+    l.logits.time += 3.0 + (double)(elements * d->dim * size_of(d->type)) * 2.0 / 4e6;
+    const Plan staged = plan_logits(d->type, blocks_of(d->dim, d->type), true, true);
+    l.staged = staged.time < l.logits.time;
+    if (l.staged) l.logits = staged;
+  }
   if (d->type == VSL_TYPE_F32) {
     // the planes are worth writing (10 bytes a value) where they save more on the logits than that
-    const Plan planes = plan_logits(VSL_TYPE_BF16, kPairs * blocks_of(d->dim, VSL_TYPE_BF16), false);
+    const Plan planes = plan_logits(VSL_TYPE_BF16, kPairs * blocks_of(d->dim, VSL_TYPE_BF16), false, false);
     l.split = planes.time + 10.0 + (double)(d->rows + d->vocab) * (double)d->dim * 10.0 / 4e6 < l.logits.time;
     if (l.split) l.logits = planes;
   }
+  if (l.split) l.staged = false;
   l.type = l.split ? VSL_TYPE_BF16 : d->type;
   l.size = size_of(l.type);
   l.planes = l.split ? 3 : 1;
   l.dim_padded = round_up(d->dim, kBlockBytes / l.size);
-  l.copy_hidden = l.split || !ready(d->hidden, d->hidden_stride, d->dim, d->type);
-  l.copy_weight = l.split || !ready(d->weight, d->weight_stride, d->dim, d->type);
+  l.copy_hidden = l.split || (l.copy_hidden && !l.staged);
+  l.copy_weight = l.split || (l.copy_weight && !l.staged);
   // a copy is padded with zeros up to the block's end; beside an operand that is read in place only its pieces count
   l.tail = l.copy_hidden && l.copy_weight ? 8 : (int)((d->dim * l.size % kBlockBytes + 15) / 16);
   if (l.tail == 0) l.tail = 8;
@@ -1236,20 +1277,24 @@ struct FinishLaunch {
   }
 };
 
-template <typename T, typename S, bool DELTA, bool SPLIT>
+template <typename T, typename S, bool DELTA, bool SPLIT, bool STAGED>
 int launch_logits_as(const LogitArgs& a, hipStream_t s) {
   const int64_t tm = ceil_div(a.op.M, S::BM), tn = ceil_div(a.op.N, S::BN);
-  hipLaunchKernelGGL((k_ce_logits<T, S, DELTA, SPLIT>), dim3((unsigned)(tm * tn)), dim3(S::kThreads), 0, s, a);
+  hipLaunchKernelGGL((k_ce_logits<T, S, DELTA, SPLIT, STAGED>), dim3((unsigned)(tm * tn)), dim3(S::kThreads), 0, s, a);
   return (int)tm;
 }
 template <typename T, bool DELTA, bool SPLIT>
-int launch_logits(const LogitArgs& a, int shape, hipStream_t s) {  // returns the rows of tiles
+int launch_logits(const LogitArgs& a, int shape, bool staged, hipStream_t s) {  // returns the rows of tiles
+  if constexpr (!SPLIT)
+    if (staged)
+      return shape == kNarrow ? launch_logits_as<T, Narrow, DELTA, SPLIT, true>(a, s)
+                              : launch_logits_as<T, Small, DELTA, SPLIT, true>(a, s);
   if constexpr (sizeof(T) == 2 || SPLIT)
-    if (shape == kLarge) return launch_logits_as<T, Large, DELTA, SPLIT>(a, s);
-  if (shape == kNarrow) return launch_logits_as<T, Narrow, DELTA, SPLIT>(a, s);
-  return launch_logits_as<T, Small, DELTA, SPLIT>(a, s);
+    if (shape == kLarge) return launch_logits_as<T, Large, DELTA, SPLIT, false>(a, s);
+  if (shape == kNarrow) return launch_logits_as<T, Narrow, DELTA, SPLIT, false>(a, s);
+  return launch_logits_as<T, Small, DELTA, SPLIT, false>(a, s);
 }
-template <typename T, typename S, bool SPLIT>
+template <typename T, typename S, bool SPLIT, bool STAGED = false>
 void launch_grad_as(const GradArgs* g, int n, hipStream_t s) {
   GradJobs jobs{};
   unsigned blocks = 0;
@@ -1259,7 +1304,7 @@ void launch_grad_as(const GradArgs* g, int n, hipStream_t s) {
     blocks += (unsigned)(ceil_div(g[i].op.M, S::BM) * ceil_div(g[i].op.N, S::BN) * g[i].splits);
   }
   if (n == 1) jobs.first = blocks;
-  hipLaunchKernelGGL((k_ce_grad<T, S, SPLIT>), dim3(blocks), dim3(S::kThreads), 0, s, jobs);
+  hipLaunchKernelGGL((k_ce_grad<T, S, SPLIT, STAGED>), dim3(blocks), dim3(S::kThreads), 0, s, jobs);
 }
 // n products, one after the other in one launch where their tiles have one shape
 template <typename T, bool SPLIT>
@@ -1278,13 +1323,15 @@ void launch_grad(GradArgs* g, const int* shape, int n, hipStream_t s) {
 }
 
 template <typename T>
-void launch_parts(const Operands& op, const Plan& plan, float* parts, hipStream_t s) {
+void launch_parts(const Operands& op, const Layout& l, float* parts, hipStream_t s) {
   GradArgs g{};
   g.op = op;
   g.sum = parts;
-  g.out = parts;
-  g.splits = plan.splits;
-  launch_grad<T, false>(&g, &plan.shape, 1, s);
+  g.splits = l.logits.splits;
+  g.whole = op.M % 4 == 0;
+  if (l.staged && l.logits.shape == kNarrow) launch_grad_as<T, Narrow, false, true>(&g, 1, s);
+  else if (l.staged) launch_grad_as<T, Small, false, true>(&g, 1, s);
+  else launch_grad<T, false>(&g, &l.logits.shape, 1, s);
 }
 
 template <typename T, bool SPLIT>
@@ -1298,13 +1345,14 @@ void run_forward(const vsl_linear_ce_desc* d, const Layout& l, const Forward& f,
   lay.run<T, SPLIT>(s);
   a.op = {l.copy_weight ? f.weight : d->weight, l.copy_hidden ? f.hidden : d->hidden,
           l.copy_weight ? l.planes * l.dim_padded : d->weight_stride, l.copy_hidden ? l.planes * l.dim_padded : d->hidden_stride,
-          (int)d->vocab, (int)d->rows, (int)(l.dim_padded / Kind<O>::BK), l.dim_padded, l.dim_padded, l.tail};
+          (int)d->vocab, (int)d->rows, (int)(l.dim_padded / Kind<O>::BK), l.dim_padded, l.dim_padded, l.tail,
+          (int)d->dim};
   a.bias = d->bias;
   a.target = d->target;
   a.rows_padded = l.rows_padded;
   if constexpr (!SPLIT)
     if (f.parts) {
-      launch_parts<T>(a.op, l.logits, f.parts, s);
+      launch_parts<T>(a.op, l, f.parts, s);
       auto rows = [&](auto kernel, int threads) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)d->rows), dim3(threads), 0, s,
                            Parts{f.parts, l.logits.splits, d->rows, d->vocab, d->bias}, d->target, d->ignore_index, d->z_loss,
@@ -1317,7 +1365,7 @@ void run_forward(const vsl_linear_ce_desc* d, const Layout& l, const Forward& f,
     }
   a.partial = f.partial;
   a.target_logit = f.target_logit;
-  const int tiles = launch_logits<T, false, SPLIT>(a, l.logits.shape, s);
+  const int tiles = launch_logits<T, false, SPLIT>(a, l.logits.shape, l.staged, s);
   // few rows: more lanes each, so that no lane walks many tiles (16 rows of 512 tiles: 14 us with 16 lanes a row); many rows:
   // more of them a block, so that fewer sums are left
   auto rows = [&](auto kernel, int per_block, int threads) {
@@ -1381,13 +1429,13 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
   const int64_t ldw = l.copy_weight ? l.planes * l.dim_padded : d->weight_stride;
   for (int64_t p = 0; p < b.pieces; ++p) {
     const int64_t v0 = p * b.piece, classes = d->vocab - v0 < b.piece ? d->vocab - v0 : b.piece;
-    const int shape = b.pieces == 1 ? l.logits.shape : plan_of(classes, d->rows, l.steps(d->dim), l.type, false).shape;
+    const int shape = b.pieces == 1 ? l.logits.shape : plan_of(classes, d->rows, l.steps(d->dim), l.type, false, l.staged).shape;
     // what the derivative kernel covers: whole steps of K for the two products that follow
     const int64_t padded = round_up(classes, b.parts ? 64 : kShapes[shape].bm);
     const int64_t rows_covered = round_up(d->rows, b.parts ? 64 : kShapes[shape].bn);
     LogitArgs a{};
     a.op = {weight + v0 * ldw, hidden, ldw, ldh, (int)classes, (int)d->rows, (int)(l.dim_padded / Kind<O>::BK), l.dim_padded,
-            l.dim_padded, l.tail};
+            l.dim_padded, l.tail, (int)d->dim};
     a.bias = d->bias;
     a.target = d->target;
     a.class0 = v0;
@@ -1405,18 +1453,18 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
     bool made = false;
     if constexpr (!SPLIT)
       if (b.parts) {
-        launch_parts<T>(a.op, l.logits, b.parts, s);
+        launch_parts<T>(a.op, l, b.parts, s);
         hipLaunchKernelGGL(k_ce_parts_delta<T>, dim3((unsigned)(padded / 64), (unsigned)(rows_covered / kPartRows)), dim3(kThreads),
                            0, s, Parts{b.parts, l.logits.splits, d->rows, d->vocab, d->bias}, a);
         made = true;
       }
-    if (!made) launch_logits<T, true, SPLIT>(a, shape, s);
+    if (!made) launch_logits<T, true, SPLIT>(a, shape, l.staged, s);
     GradArgs g[2] = {};
     int shapes[2], n = 0;
     FinishLaunch finish;
     if (grad_hidden) {
       g[n].op = {(const O*)b.weight_t + v0, b.delta, l.planes * b.vocab_padded, l.planes * b.piece, (int)d->dim, (int)d->rows,
-                 (int)(padded / Kind<O>::BK), b.vocab_padded, b.piece, 8};
+                 (int)(padded / Kind<O>::BK), b.vocab_padded, b.piece, 8, 0};
       g[n].add = p > 0;
       g[n].sum = b.sum_h;
       g[n].out = grad_hidden;
@@ -1427,7 +1475,7 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
     }
     if (grad_weight) {
       g[n].op = {b.hidden_t, b.delta_t, l.planes * l.rows_padded, l.planes * l.rows_padded, (int)d->dim, (int)classes,
-                 (int)(rows_covered / Kind<O>::BK), l.rows_padded, l.rows_padded, 8};
+                 (int)(rows_covered / Kind<O>::BK), l.rows_padded, l.rows_padded, 8, 0};
       g[n].sum = b.sum_w;
       g[n].out = grad_weight + v0 * d->dim;
       g[n].scale = scale;
