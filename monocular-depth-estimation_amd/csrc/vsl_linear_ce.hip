@@ -764,7 +764,7 @@ struct GradArgs {
   Operands op;             // A: [M features, K], B: [N rows or classes, K]
   int splits;              // of K
   bool add;                // to what `sum` holds
-  bool whole;              // four features in a row are one aligned store
+  bool whole;              // four features in a row of `sum` are one aligned store
   float* sum;              // [splits][N][M], or NULL: straight to `out`
   void* out;               // [N][M] of the operands' type
   OutScale scale;
@@ -775,6 +775,56 @@ struct GradJobs {
   GradArgs job[2];
   unsigned first;  // blocks of the first
 };
+
+// A tile straight to `out`.  A lane holds four features of 32 rows each: stored from there, a row's line is written in
+// eight or sixteen pieces by as many stores.  So the tile goes through LDS first, whole rows leave it, 16 bytes a lane, at
+// any address.  Pieces of a row are turned by the row, so that neither side's 16 lanes meet in a bank.  A float32 tile that
+// is larger than the LDS goes in two halves of its features.
+template <typename T, typename S>
+__device__ __forceinline__ void store_tile(const GradArgs& a, int m0, int n0, const Tile<S>& t, char* lds) {
+  constexpr int kHalves = S::BM * S::BN * (int)sizeof(T) > S::kLds ? 2 : 1, kWide = S::BM / kHalves;
+  constexpr int E = Kind<T>::E, kPieces = kWide / E;  // of a row
+  static_assert(kWide * S::BN * (int)sizeof(T) <= S::kLds && kPieces >= 16 && S::WM % kHalves == 0, "tile through LDS");
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
+  const float scale = a.scale.get();
+#pragma unroll
+  for (int h = 0; h < kHalves; ++h) {
+    if (h) __syncthreads();
+    if (wm / (S::WM / kHalves) == h) {
+#pragma unroll
+      for (int j = 0; j < S::JN; ++j)
+#pragma unroll
+        for (int i = 0; i < S::IM; ++i)
+#pragma unroll
+          for (int r4 = 0; r4 < 4; ++r4) {
+            const int n = (wn * S::JN + j) * 32 + (lane & 31);
+            const int m = (wm * S::IM + i) * 32 - h * kWide + 8 * r4 + 4 * (lane >> 5);
+            float g[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) g[e] = scale * t.acc[i][j][4 * r4 + e];
+            char* p = lds + (n * kPieces + ((m / E) ^ (n & 15))) * 16;
+            if constexpr (sizeof(T) == 4) *(f32x4*)p = f32x4{g[0], g[1], g[2], g[3]};
+            else *(uint2*)(p + 8 * (lane >> 5)) = pack4<T>(g);
+          }
+    }
+    __syncthreads();
+    for (int at = threadIdx.x; at < S::BN * kPieces; at += S::kThreads) {
+      const int n = at / kPieces, piece = at % kPieces, m = m0 + h * kWide + piece * E;
+      if (n0 + n >= a.op.N || m >= a.op.M) continue;
+      const u32x4 v = *(const u32x4*)(lds + (n * kPieces + (piece ^ (n & 15))) * 16);
+      T* out = (T*)a.out + (int64_t)(n0 + n) * a.op.M + m;
+      if (m + E <= a.op.M) {
+        store16(out, v);
+      } else {
+        float x[E];
+        unpack(v, x, (const T*)nullptr);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (m + e < a.op.M) out[e] = (T)x[e];
+      }
+    }
+  }
+}
 
 template <typename T, typename S, bool SPLIT, bool STAGED>
 __global__ __launch_bounds__(S::kThreads) void k_ce_grad(GradJobs jobs) {
@@ -792,40 +842,26 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_grad(GradJobs jobs) {
   Tile<S> t;
   tile_product<std::conditional_t<SPLIT, __bf16, T>, S, SPLIT, STAGED>(a.op, m0, n0, k0, k1, lds, t);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
-  const float scale = a.sum ? 1.0f : a.scale.get();
+  if (!a.sum) return store_tile<T, S>(a, m0, n0, t, lds);
 #pragma unroll
   for (int j = 0; j < S::JN; ++j) {
     const int row = n0 + (wn * S::JN + j) * 32 + (lane & 31);
     if (row >= a.op.N) continue;
-    const int64_t at = (int64_t)row * a.op.M;
-    float* sum = a.sum ? a.sum + (int64_t)split * a.op.M * a.op.N + at : nullptr;
-    T* out = (T*)a.out + at;
+    float* sum = a.sum + (int64_t)split * a.op.M * a.op.N + (int64_t)row * a.op.M;
 #pragma unroll
     for (int i = 0; i < S::IM; ++i)
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4) {
         const int m = m0 + (wm * S::IM + i) * 32 + 8 * r4 + 4 * (lane >> 5);
-        float g[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) g[e] = scale * t.acc[i][j][4 * r4 + e];
         if (a.whole && m < a.op.M) {
-          if (sum) {
-            f32x4* p = (f32x4*)(sum + m);
-            f32x4 v{g[0], g[1], g[2], g[3]};
-            if (a.add) v += *p;
-            *p = v;
-          } else if constexpr (sizeof(T) == 4) {
-            *(f32x4*)(out + m) = f32x4{g[0], g[1], g[2], g[3]};
-          } else {
-            *(uint2*)(out + m) = pack4<T>(g);
-          }
+          f32x4* p = (f32x4*)(sum + m);
+          f32x4 v{t.acc[i][j][4 * r4], t.acc[i][j][4 * r4 + 1], t.acc[i][j][4 * r4 + 2], t.acc[i][j][4 * r4 + 3]};
+          if (a.add) v += *p;
+          *p = v;
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (m + e < a.op.M) {
-              if (sum) sum[m + e] = a.add ? sum[m + e] + g[e] : g[e];
-              else out[m + e] = (T)g[e];
-            }
+            if (m + e < a.op.M) sum[m + e] = a.add ? sum[m + e] + t.acc[i][j][4 * r4 + e] : t.acc[i][j][4 * r4 + e];
         }
       }
   }
@@ -878,28 +914,31 @@ __global__ __launch_bounds__(kThreads) void k_ce_finish(FinishJobs jobs) {
   }
 }
 
-// grad_bias: sums of the rows of d^T, the values that grad_weight is made of; a block per class and part of its row
-template <typename T, bool SPLIT>
+// grad_bias: sums of the rows of d^T, the values that grad_weight is made of; L lanes per class and part of its row
+template <typename T, bool SPLIT, int L>
 __global__ __launch_bounds__(kThreads) void k_ce_bias(const void* __restrict__ delta_t, int64_t ldt, int64_t rows_padded,
                                                       int64_t rows, int classes, int parts, float* __restrict__ sum,
                                                       OutScale out_scale, T* __restrict__ out) {
   typedef std::conditional_t<SPLIT, __bf16, T> O;
   __shared__ float red[4];
-  const int c = blockIdx.x % classes, part = blockIdx.x / classes;
+  const int item = blockIdx.x * (kThreads / L) + threadIdx.x / L, lane = threadIdx.x % L;
+  if (item >= classes * parts) return;  // whole groups of L
+  const int c = item % classes, part = item / classes;
   const int64_t vectors = rows / Kind<O>::E, per = (vectors + parts - 1) / parts;
   const int64_t end = min(vectors, (part + 1) * per);
   float s = 0.0f;
   for (int plane = SPLIT ? 2 : 0; plane >= 0; --plane) {
     const O* d = (const O*)delta_t + (int64_t)c * ldt + plane * rows_padded;
-    for (int64_t i = part * per + threadIdx.x; i < end; i += kThreads) {
+    for (int64_t i = part * per + lane; i < end; i += L) {
       float x[Kind<O>::E];
       unpack(load16(d + i * Kind<O>::E), x, (const O*)nullptr);
 #pragma unroll
       for (int e = 0; e < Kind<O>::E; ++e) s += x[e];
     }
   }
-  s = block_add<4>(s, red);
-  if (threadIdx.x) return;
+  if constexpr (L == kThreads) s = block_add<4>(s, red);
+  else s = group_all<L>(s, AddF());
+  if (lane) return;
   if (sum) sum[(int64_t)part * classes + c] = s;
   else out[c] = (T)(s * out_scale.get());
 }
@@ -1309,7 +1348,7 @@ void launch_grad_as(const GradArgs* g, int n, hipStream_t s) {
 // n products, one after the other in one launch where their tiles have one shape
 template <typename T, bool SPLIT>
 void launch_grad(GradArgs* g, const int* shape, int n, hipStream_t s) {
-  for (int i = 0; i < n; ++i) g[i].whole = g[i].op.M % 4 == 0 && (uintptr_t)g[i].out % 16 == 0;
+  for (int i = 0; i < n; ++i) g[i].whole = g[i].op.M % 4 == 0;
   if (n == 2 && shape[0] != shape[1]) {
     launch_grad<T, SPLIT>(g, shape, 1, s);
     launch_grad<T, SPLIT>(g + 1, shape + 1, 1, s);
@@ -1487,9 +1526,14 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
     if (grad_bias) {
       // few classes: their rows in parts, so that more than a block per class works on them
       const int parts = b.sum_b ? (int)(kBiasBlocks / classes < 1 ? 1 : kBiasBlocks / classes) : 1;
-      hipLaunchKernelGGL((k_ce_bias<T, SPLIT>), dim3((unsigned)(classes * parts)), dim3(kThreads), 0, s,
-                         (const void*)b.delta_t, l.planes * l.rows_padded, l.rows_padded, rows_covered, (int)classes, parts,
-                         parts > 1 ? b.sum_b : nullptr, scale, grad_bias + v0);
+      auto bias = [&](auto kernel, int per_block) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(classes * parts, per_block)), dim3(kThreads), 0, s,
+                           (const void*)b.delta_t, l.planes * l.rows_padded, l.rows_padded, rows_covered, (int)classes, parts,
+                           parts > 1 ? b.sum_b : nullptr, scale, grad_bias + v0);
+      };
+      // few rows: a block per class would have little to add up (57 rows, 90227 classes: 58 us, with 8 lanes 5)
+      if (rows_covered <= 1024) bias(k_ce_bias<T, SPLIT, 8>, kThreads / 8);
+      else bias(k_ce_bias<T, SPLIT, kThreads>, 1);
       if (parts > 1) finish.add(b.sum_b, parts, classes, grad_bias + v0);
     }
     finish.run<T>(scale, s);
