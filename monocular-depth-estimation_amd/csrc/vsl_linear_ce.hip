@@ -1161,13 +1161,13 @@ constexpr int64_t kMostParts = 1LL << 23;  // padded logits whose product may be
 Layout layout_of(const vsl_linear_ce_desc* d) {
   Layout l{};
   l.rows_padded = round_up(d->rows, kPad);
-  // Logits in parts cost a pass over the sums, forward and backward (5 us, and 0.5 for every
-  // turn of its block along a row).
+  // Logits in parts cost a pass over the sums, forward and backward (5 us, 3 more to launch
+  // it, and 0.5 for every turn of its block along a row).
   auto plan_logits = [&](int type, int64_t steps, bool parts, bool staged) {
     const Plan whole = plan_of(d->vocab, d->rows, steps, type, false, staged);
     if (!parts || l.rows_padded * round_up(d->vocab, kPad) > kMostParts) return whole;
     Plan cut = plan_of(d->vocab, d->rows, steps, type, true, staged);
-    cut.time += 5.0 + 0.5 * (double)ceil_div(d->vocab, 4096);
+    cut.time += 8.0 + 0.5 * (double)ceil_div(d->vocab, 4096);
     return cut.splits > 1 && cut.time < whole.time ? cut : whole;
   };
   l.logits = plan_logits(d->type, blocks_of(d->dim, d->type), true, false);
@@ -1202,6 +1202,7 @@ Layout layout_of(const vsl_linear_ce_desc* d) {
 }
 
 struct Forward {
+  Layout l;
   void *hidden, *weight;
   float2* partial;
   float* target_logit;
@@ -1210,10 +1211,11 @@ struct Forward {
   size_t total;
 };
 Forward forward_workspace(const vsl_linear_ce_desc* d, void* base) {
-  const Layout l = layout_of(d);
+  Forward f{};
+  f.l = layout_of(d);
+  const Layout& l = f.l;
   const int s = l.size * l.planes;
   Arena a{(char*)base};
-  Forward f{};
   f.hidden = l.copy_hidden ? a.take((size_t)d->rows * l.dim_padded * s) : nullptr;
   f.weight = l.copy_weight ? a.take((size_t)d->vocab * l.dim_padded * s) : nullptr;
   if (l.logits.splits > 1) {
@@ -1374,9 +1376,10 @@ void launch_parts(const Operands& op, const Layout& l, float* parts, hipStream_t
 }
 
 template <typename T, bool SPLIT>
-void run_forward(const vsl_linear_ce_desc* d, const Layout& l, const Forward& f, float* row_loss, float* stats, float* loss,
+void run_forward(const vsl_linear_ce_desc* d, const Forward& f, float* row_loss, float* stats, float* loss,
                  float* divisor, hipStream_t s) {
   typedef std::conditional_t<SPLIT, __bf16, T> O;
+  const Layout& l = f.l;
   LogitArgs a{};
   LayoutLaunch lay;
   if (l.copy_hidden) lay.copy(d->hidden, d->hidden_stride, d->rows, d->dim, l.dim_padded, f.hidden);
@@ -1581,10 +1584,9 @@ int vsl_linear_ce_fwd(const vsl_linear_ce_desc* d, float* row_loss, float* stats
   if (d->rows == 0) {
     if (d->reduction != VSL_REDUCE_NONE) launch_sum_pairs(f.pairs, 0, d->reduction, loss, divisor, s);
   } else {
-    const Layout l = layout_of(d);
     auto run = d->type == VSL_TYPE_BF16 ? run_forward<__bf16, false> : d->type == VSL_TYPE_F16 ? run_forward<_Float16, false>
-               : l.split ? run_forward<float, true> : run_forward<float, false>;
-    run(d, l, f, row_loss, stats, loss, divisor, s);
+               : f.l.split ? run_forward<float, true> : run_forward<float, false>;
+    run(d, f, row_loss, stats, loss, divisor, s);
   }
   return launch_status("linear_ce");
 }

@@ -46,9 +46,9 @@ def test_top_logits_refuses(bad):
 
 def test_top_logits_outputs_and_workspace():
     import mde_amd._abi as abi
-    d = top(abi)
+    d = top(abi, vocab=50000, stride=50000)
     need = abi.lib.vsl_top_logits_workspace_bytes(ctypes.byref(d))
-    assert need >= 8 * 2 * 4 * 8 and need % 256 == 0         # few long rows are split
+    assert need >= 8 * 2 * 4 * 8 and need % 256 == 0         # few long rows are split, by 16384 classes at least
     call = lambda v, i, ws, n: abi.lib.vsl_top_logits(ctypes.byref(d), v, i, None, ws, n, None)
     assert call(None, FAKE, FAKE * 16, need) == -1 and call(FAKE, None, FAKE * 16, need) == -1
     assert call(FAKE, FAKE, FAKE * 16, need - 1) == -2 and b"workspace" in err(abi)
@@ -124,9 +124,9 @@ def test_linear_ce_outputs_and_workspace():
     assert bwd(FAKE, FAKE, FAKE, FAKE, FAKE * 16, sizes[0] - 1) == -2
     assert bwd(FAKE, FAKE, FAKE, FAKE + 1, FAKE * 16, sizes[0]) == -1 and b"misaligned" in err(abi)
     assert bwd(FAKE, FAKE, FAKE, None, None, 0) == 0                       # no gradient is wanted
-    # odd widths and rows that 16-byte loads cannot take are laid out anew: more workspace, never less
+    # odd widths and rows that 16-byte loads cannot take: through registers, or laid out anew, which takes more workspace
     for kw in (dict(dim=65, hidden_stride=65, weight_stride=65), dict(hidden=FAKE + 2), dict(hidden_stride=65)):
-        assert abi.lib.vsl_linear_ce_fwd_workspace_bytes(ctypes.byref(linear(abi, **kw))) > need
+        assert abi.lib.vsl_linear_ce_fwd_workspace_bytes(ctypes.byref(linear(abi, **kw))) >= need
     # one size for every extent of the documented limits, without overflow
     for rows, vocab, dim in ((1, 1, 1), (1, (1 << 27) - 1, 1), ((1 << 27) - 1, 100, 8), (1 << 18, 1 << 18, 64), (3, 3, (1 << 24) - 1)):
         d = linear(abi, rows=rows, vocab=vocab, dim=dim, hidden_stride=dim, weight_stride=dim)
