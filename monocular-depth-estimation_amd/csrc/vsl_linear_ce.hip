@@ -45,6 +45,7 @@ struct Shape {
 typedef Shape<256, 256, 2, 4> Large;
 typedef Shape<128, 128, 2, 2> Small;
 typedef Shape<128, 64, 4, 1> Narrow;  // few columns: rows of the loss
+typedef Shape<128, 32, 4, 1> Thin;    // 32 at most
 
 template <typename T>
 struct Kind {
@@ -86,8 +87,11 @@ struct Operands {
   int M, N, kblocks;
   int64_t plane_a, plane_b;
   int tail;  // 16-byte pieces of a row in the last block (8: it is whole); what follows them is not the row's
-  int dim;   // elements of a row, where rows lie at any address (STAGED)
+  int dim;   // elements of a row, where rows lie at any address (kStagedRows)
+  int rows_of_k;     // kStagedColumns: rows of A
+  const void* bias;  // kStagedColumns: rows of A at -infinity here count as zeros, or NULL
 };
+enum { kDirect, kStagedRows, kStagedColumns };  // ways of the operands to LDS
 // what the pieces behind a row's end are read from
 __device__ const u32x4 kZeros[1] = {{0u, 0u, 0u, 0u}};
 constexpr int kPairs = 6;
@@ -108,11 +112,15 @@ struct Tile {
 // A step is four rounds; each round's fragments are read while the round before multiplies.  The barrier stands before the
 // last round, whose fragments are in registers by then: behind it the buffer is free for the step after next, and the
 // next step's first fragments are read under the last round's multiplications.
-// STAGED: rows that start anywhere or end inside a piece cannot go straight to LDS.  They go through registers, asked for a
-// step ahead of their store, which takes the place of the fetch.
+// kStagedRows: rows that start anywhere or end inside a piece cannot go straight to LDS.  They go through registers, asked for
+// a step ahead of their store, which takes the place of the fetch.
+// kStagedColumns: so does an A that lies as [K, M]: BM elements of every row of a step, whose fragments are gathered from LDS
+// element by element; the two halves of the wave, E rows apart, read 32 elements apart as well, from other banks.
 // T: the operands' type; steps [k0, k1) of kblocks, or of kPairs * kblocks in the split form.
-template <typename T, typename S, bool SPLIT, bool STAGED>
+template <typename T, typename S, bool SPLIT, int FORM>
 __device__ __forceinline__ void tile_product(const Operands& op, int m0, int n0, int k0, int k1, char* lds, Tile<S>& t) {
+  constexpr bool STAGED = FORM != kDirect, COLUMNS = FORM == kStagedColumns;
+  constexpr int E = Kind<T>::E, kWide = S::BM / E;  // COLUMNS: pieces of A's BM elements of a row
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / S::WN, wn = wave % S::WN;
 #pragma unroll
@@ -170,8 +178,16 @@ __device__ __forceinline__ void tile_product(const Operands& op, int m0, int n0,
     const bool whole = (++next_step) * Kind<T>::BK <= op.dim;
 #pragma unroll
     for (int i = 0; i < (STAGED ? S::kFetch : 0); ++i) {
-      held[i] = whole ? load16((const T*)src[i]) : load_columns((const T*)src[i], 0, op.dim - first);
-      src[i] += kBlockBytes;
+      if (COLUMNS && i < S::kFetchA) {
+        const int at = i * S::kThreads + tid, k = at / kWide, row = (next_step - 1) * Kind<T>::BK + k;
+        const int m = m0 + (at % kWide * E ^ (k / E & 1) * 32);
+        held[i] = u32x4{0u, 0u, 0u, 0u};
+        if (row < op.rows_of_k && !(op.bias && (float)((const T*)op.bias)[row] == ninf()))
+          held[i] = load_columns((const T*)op.A + (int64_t)row * op.lda, m, op.M);
+      } else {
+        held[i] = COLUMNS || whole ? load16((const T*)src[i]) : load_columns((const T*)src[i], 0, op.dim - first);
+        src[i] += kBlockBytes;
+      }
     }
   };
   auto store = [&](int buffer) {
@@ -188,8 +204,23 @@ __device__ __forceinline__ void tile_product(const Operands& op, int m0, int n0,
   u32x4 fa[2][S::IM], fb[2][S::JN];
   auto read = [&](int set, int buffer, int round) {
     const int piece = ((2 * round + (lane >> 5)) ^ ((lane >> 1) & 7)) * 16 + buffer * S::kBuffer;
+    if constexpr (COLUMNS) {
+      const T* column = (const T*)(lds + buffer * S::kBuffer) + (2 * round + (lane >> 5)) * E * S::BM;
 #pragma unroll
-    for (int i = 0; i < S::IM; ++i) fa[set][i] = *(const u32x4*)(a + i * 32 * kBlockBytes + piece);
+      for (int i = 0; i < S::IM; ++i) {
+        const int m = ((wm * S::IM + i) * 32 + (lane & 31)) ^ (lane & 32);
+        union {
+          T t[E];
+          u32x4 u;
+        } f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) f.t[e] = column[e * S::BM + m];
+        fa[set][i] = f.u;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < S::IM; ++i) fa[set][i] = *(const u32x4*)(a + i * 32 * kBlockBytes + piece);
+    }
 #pragma unroll
     for (int j = 0; j < S::JN; ++j) fb[set][j] = *(const u32x4*)(b + j * 32 * kBlockBytes + piece);
   };
@@ -202,6 +233,7 @@ __device__ __forceinline__ void tile_product(const Operands& op, int m0, int n0,
   auto interleave = [&]() {  // a round's reads go out one by one behind its multiplications, and stay in their round
     constexpr int kMma = S::IM * S::JN * (sizeof(T) == 4 ? 4 : 1), kRead = S::IM + S::JN;
     constexpr int kEach = kMma / (kRead + 2) < 1 ? 1 : kMma / (kRead + 2);
+    if (COLUMNS) return;  // bound by its reads of A from memory
 #pragma unroll
     for (int i = 0; i < kRead; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);
@@ -322,7 +354,7 @@ __device__ __forceinline__ float take_plane(float& z) {
 }
 
 // T: the tensors' type; SPLIT: float32 by planes of bfloat16
-template <typename T, typename S, bool DELTA, bool SPLIT, bool STAGED>
+template <typename T, typename S, bool DELTA, bool SPLIT, int FORM>
 __global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
   typedef std::conditional_t<SPLIT, __bf16, T> O;
   __shared__ __attribute__((aligned(16))) char lds[S::kLds];
@@ -331,7 +363,7 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
   tile_of(blockIdx.x, tm_count, tn_count, tm, tn);
   const int m0 = tm * S::BM, n0 = tn * S::BN;
   Tile<S> t;
-  tile_product<O, S, SPLIT, STAGED>(a.op, m0, n0, 0, (SPLIT ? kPairs : 1) * a.op.kblocks, lds, t);
+  tile_product<O, S, SPLIT, FORM>(a.op, m0, n0, 0, (SPLIT ? kPairs : 1) * a.op.kblocks, lds, t);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
   const int half = lane >> 5;
   const bool biased = a.bias || m0 + S::BM > a.op.M;
@@ -826,7 +858,7 @@ __device__ __forceinline__ void store_tile(const GradArgs& a, int m0, int n0, co
   }
 }
 
-template <typename T, typename S, bool SPLIT, bool STAGED>
+template <typename T, typename S, bool SPLIT, int FORM>
 __global__ __launch_bounds__(S::kThreads) void k_ce_grad(GradJobs jobs) {
   const int which = blockIdx.x >= jobs.first ? 1 : 0;
   const GradArgs& a = jobs.job[which];
@@ -840,7 +872,7 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_grad(GradJobs jobs) {
   const int k0 = min(split * per, steps), k1 = min(k0 + per, steps);
   const int m0 = tm * S::BM, n0 = tn * S::BN;
   Tile<S> t;
-  tile_product<std::conditional_t<SPLIT, __bf16, T>, S, SPLIT, STAGED>(a.op, m0, n0, k0, k1, lds, t);
+  tile_product<std::conditional_t<SPLIT, __bf16, T>, S, SPLIT, FORM>(a.op, m0, n0, k0, k1, lds, t);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
   if (!a.sum) return store_tile<T, S>(a, m0, n0, t, lds);
 #pragma unroll
@@ -893,10 +925,10 @@ __global__ __launch_bounds__(kThreads) void k_ce_finish(FinishJobs jobs) {
   for (int64_t i0 = block * 256; i0 < j.n; i0 += j.blocks * 256) {
     const int64_t i = i0 + 4 * lane;
     f32x4 v{0.0f, 0.0f, 0.0f, 0.0f};
-    if (j.n % 4 == 0) {
-      if (i < j.n)
-        for (int s = s0; s < s1; ++s) v += *(const f32x4*)(j.sum + s * j.n + i);
-    } else {
+    if (i + 4 <= j.n) {
+#pragma unroll 8
+      for (int s = s0; s < s1; ++s) v += __builtin_bit_cast(f32x4, load16(j.sum + s * j.n + i));
+    } else if (i < j.n) {
       for (int s = s0; s < s1; ++s)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -1110,7 +1142,7 @@ struct Plan {
   int shape, splits;  // of the tiles of a product, and of its K
   double time;        // estimated, microseconds
 };
-enum { kLarge, kSmall, kNarrow };
+enum { kLarge, kSmall, kNarrow, kThin };
 struct ShapeInfo {
   int bm, bn, slots;             // tile, and how many of it the 256 CUs hold at once
   float step16, step32, around;  // microseconds of a step of K with all slots taken (16-bit types, float32), and of a tile's
@@ -1119,7 +1151,8 @@ struct ShapeInfo {
 // Measured on products of 2048..8192 rows (large: 1240 TFLOP/s in bfloat16, small: 850; float32: 105).
 constexpr ShapeInfo kShapes[] = {{Large::BM, Large::BN, 256, 1.7f, 0.0f, 4.0f},
                                  {Small::BM, Small::BN, 512, 1.3f, 5.0f, 2.5f},
-                                 {Narrow::BM, Narrow::BN, 768, 1.1f, 4.0f, 2.0f}};
+                                 {Narrow::BM, Narrow::BN, 768, 1.1f, 4.0f, 2.0f},
+                                 {Thin::BM, Thin::BN, 1024, 1.0f, 3.0f, 1.5f}};
 // A step through registers against one straight to LDS, its loads off their alignment.  7 x 96190 x 3653 bfloat16 forward
 // takes 161 us through registers and 420 copied first; 6439 x 736 x 2647 float16 with gradients 297 and 271.
 constexpr double kStaged = 1.5;
@@ -1128,7 +1161,7 @@ constexpr double kStaged = 1.5;
 // does not fit the registers, and its matrix instructions are eight times slower, so that its loads never bind.
 Plan plan_of(int64_t M, int64_t N, int64_t blocks, int type, bool may_split, bool staged = false) {
   Plan best{kSmall, 1, 1e300};
-  for (int shape = type == VSL_TYPE_F32 || staged ? kSmall : kLarge; shape <= kNarrow; ++shape) {
+  for (int shape = type == VSL_TYPE_F32 || staged ? kSmall : kLarge; shape <= (N <= Thin::BN ? kThin : kNarrow); ++shape) {
     const ShapeInfo& h = kShapes[shape];
     const double tiles = (double)(ceil_div(M, h.bm) * ceil_div(N, h.bn));
     const double step = (type == VSL_TYPE_F32 ? h.step32 : h.step16) * (staged ? kStaged : 1.0);
@@ -1239,8 +1272,15 @@ static_assert(kMostParts <= kPieceElements && kMostParts / kPad / kPartRows < 65
 
 constexpr int64_t kBiasBlocks = 1024;
 
+// grad_hidden of few rows takes a large weight as it lies: transposing it first reads and writes it once more.
+// 5 x 60478 x 1627 float32 with gradients takes 677 us, transposed 866; 57 x 90227 x 1024 float16 271 and 295; above 128 rows
+// the gathers bind (346 x 30813 x 1495 float16: 552 and 394), below 16 MB the further launch (19 x 56371 x 54 bfloat16: 104
+// and 90).
+constexpr int64_t kColumnsRows = 128, kColumnsBytes = 16 << 20;
+
 struct Backward {
   Layout l;
+  bool columns;
   int64_t piece, pieces, vocab_padded;
   Plan plan_h, plan_w;
   void *hidden, *weight, *hidden_t, *weight_t, *delta, *delta_t;
@@ -1261,10 +1301,11 @@ Backward backward_workspace(const vsl_linear_ce_desc* d, uint32_t mask, void* ba
   b.hidden = b.l.copy_hidden ? a.take((size_t)d->rows * b.l.dim_padded * s) : nullptr;
   b.weight = b.l.copy_weight ? a.take((size_t)d->vocab * b.l.dim_padded * s) : nullptr;
   b.hidden_t = gw ? a.take((size_t)d->dim * b.l.rows_padded * s) : nullptr;
-  b.weight_t = gh ? a.take((size_t)d->dim * b.vocab_padded * s) : nullptr;
+  b.columns = gh && !b.l.split && d->rows <= kColumnsRows && d->vocab * d->dim * size_of(d->type) >= kColumnsBytes;
+  b.weight_t = gh && !b.columns ? a.take((size_t)d->dim * b.vocab_padded * s) : nullptr;
   b.delta = gh ? a.take((size_t)b.l.rows_padded * b.piece * s) : nullptr;
   b.delta_t = gw || gb ? a.take((size_t)b.l.rows_padded * b.piece * s) : nullptr;
-  b.plan_h = plan_of(d->dim, d->rows, b.l.steps(b.piece), b.l.type, true);
+  b.plan_h = plan_of(d->dim, d->rows, b.l.steps(b.piece), b.l.type, true, b.columns);
   b.plan_w = plan_of(d->dim, d->vocab < b.piece ? d->vocab : b.piece, b.l.steps(d->rows), b.l.type, true);
   b.sum_h = gh && (b.pieces > 1 || b.plan_h.splits > 1) ? (float*)a.take((size_t)b.plan_h.splits * d->rows * d->dim * 4) : nullptr;
   b.sum_w = gw && b.plan_w.splits > 1 ? (float*)a.take((size_t)b.plan_w.splits * b.piece * d->dim * 4) : nullptr;
@@ -1318,24 +1359,26 @@ struct FinishLaunch {
   }
 };
 
-template <typename T, typename S, bool DELTA, bool SPLIT, bool STAGED>
+template <typename T, typename S, bool DELTA, bool SPLIT, int FORM>
 int launch_logits_as(const LogitArgs& a, hipStream_t s) {
   const int64_t tm = ceil_div(a.op.M, S::BM), tn = ceil_div(a.op.N, S::BN);
-  hipLaunchKernelGGL((k_ce_logits<T, S, DELTA, SPLIT, STAGED>), dim3((unsigned)(tm * tn)), dim3(S::kThreads), 0, s, a);
+  hipLaunchKernelGGL((k_ce_logits<T, S, DELTA, SPLIT, FORM>), dim3((unsigned)(tm * tn)), dim3(S::kThreads), 0, s, a);
   return (int)tm;
 }
 template <typename T, bool DELTA, bool SPLIT>
 int launch_logits(const LogitArgs& a, int shape, bool staged, hipStream_t s) {  // returns the rows of tiles
   if constexpr (!SPLIT)
     if (staged)
-      return shape == kNarrow ? launch_logits_as<T, Narrow, DELTA, SPLIT, true>(a, s)
-                              : launch_logits_as<T, Small, DELTA, SPLIT, true>(a, s);
+      return shape == kThin     ? launch_logits_as<T, Thin, DELTA, SPLIT, kStagedRows>(a, s)
+             : shape == kNarrow ? launch_logits_as<T, Narrow, DELTA, SPLIT, kStagedRows>(a, s)
+                                : launch_logits_as<T, Small, DELTA, SPLIT, kStagedRows>(a, s);
   if constexpr (sizeof(T) == 2 || SPLIT)
-    if (shape == kLarge) return launch_logits_as<T, Large, DELTA, SPLIT, false>(a, s);
-  if (shape == kNarrow) return launch_logits_as<T, Narrow, DELTA, SPLIT, false>(a, s);
-  return launch_logits_as<T, Small, DELTA, SPLIT, false>(a, s);
+    if (shape == kLarge) return launch_logits_as<T, Large, DELTA, SPLIT, kDirect>(a, s);
+  if (shape == kThin) return launch_logits_as<T, Thin, DELTA, SPLIT, kDirect>(a, s);
+  if (shape == kNarrow) return launch_logits_as<T, Narrow, DELTA, SPLIT, kDirect>(a, s);
+  return launch_logits_as<T, Small, DELTA, SPLIT, kDirect>(a, s);
 }
-template <typename T, typename S, bool SPLIT, bool STAGED = false>
+template <typename T, typename S, bool SPLIT, int FORM = kDirect>
 void launch_grad_as(const GradArgs* g, int n, hipStream_t s) {
   GradJobs jobs{};
   unsigned blocks = 0;
@@ -1345,7 +1388,7 @@ void launch_grad_as(const GradArgs* g, int n, hipStream_t s) {
     blocks += (unsigned)(ceil_div(g[i].op.M, S::BM) * ceil_div(g[i].op.N, S::BN) * g[i].splits);
   }
   if (n == 1) jobs.first = blocks;
-  hipLaunchKernelGGL((k_ce_grad<T, S, SPLIT, STAGED>), dim3(blocks), dim3(S::kThreads), 0, s, jobs);
+  hipLaunchKernelGGL((k_ce_grad<T, S, SPLIT, FORM>), dim3(blocks), dim3(S::kThreads), 0, s, jobs);
 }
 // n products, one after the other in one launch where their tiles have one shape
 template <typename T, bool SPLIT>
@@ -1359,6 +1402,7 @@ void launch_grad(GradArgs* g, const int* shape, int n, hipStream_t s) {
   if (!n) return;
   if constexpr (sizeof(T) == 2 || SPLIT)
     if (shape[0] == kLarge) return launch_grad_as<T, Large, SPLIT>(g, n, s);
+  if (shape[0] == kThin) return launch_grad_as<T, Thin, SPLIT>(g, n, s);
   if (shape[0] == kNarrow) return launch_grad_as<T, Narrow, SPLIT>(g, n, s);
   launch_grad_as<T, Small, SPLIT>(g, n, s);
 }
@@ -1370,8 +1414,9 @@ void launch_parts(const Operands& op, const Layout& l, float* parts, hipStream_t
   g.sum = parts;
   g.splits = l.logits.splits;
   g.whole = op.M % 4 == 0;
-  if (l.staged && l.logits.shape == kNarrow) launch_grad_as<T, Narrow, false, true>(&g, 1, s);
-  else if (l.staged) launch_grad_as<T, Small, false, true>(&g, 1, s);
+  if (l.staged && l.logits.shape == kThin) launch_grad_as<T, Thin, false, kStagedRows>(&g, 1, s);
+  else if (l.staged && l.logits.shape == kNarrow) launch_grad_as<T, Narrow, false, kStagedRows>(&g, 1, s);
+  else if (l.staged) launch_grad_as<T, Small, false, kStagedRows>(&g, 1, s);
   else launch_grad<T, false>(&g, &l.logits.shape, 1, s);
 }
 
@@ -1461,7 +1506,7 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
   if (grad_weight)
     lay.transpose(d->hidden, d->hidden_stride, d->rows, d->dim, l.rows_padded,
                   Contributes{d->target, stats, row_scale, nullptr, d->ignore_index}, b.hidden_t);
-  if (grad_hidden)
+  if (grad_hidden && !b.columns)
     lay.transpose(d->weight, d->weight_stride, d->vocab, d->dim, b.vocab_padded, Contributes{nullptr, nullptr, nullptr, d->bias, 0},
                   b.weight_t);
   lay.run<T, SPLIT>(s);
@@ -1471,8 +1516,9 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
   const int64_t ldw = l.copy_weight ? l.planes * l.dim_padded : d->weight_stride;
   for (int64_t p = 0; p < b.pieces; ++p) {
     const int64_t v0 = p * b.piece, classes = d->vocab - v0 < b.piece ? d->vocab - v0 : b.piece;
-    const int shape = b.pieces == 1 ? l.logits.shape : plan_of(classes, d->rows, l.steps(d->dim), l.type, false, l.staged).shape;
-    // what the derivative kernel covers: whole steps of K for the two products that follow
+    int shape = b.pieces == 1 ? l.logits.shape : plan_of(classes, d->rows, l.steps(d->dim), l.type, false, l.staged).shape;
+    if (sizeof(O) == 2 && shape == kThin) shape = kNarrow;
+    // what the derivative kernel covers: whole steps of K (32 float32, 64 in 16 bits) for the two products that follow
     const int64_t padded = round_up(classes, b.parts ? 64 : kShapes[shape].bm);
     const int64_t rows_covered = round_up(d->rows, b.parts ? 64 : kShapes[shape].bn);
     LogitArgs a{};
@@ -1513,6 +1559,13 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
       g[n].scale = scale;
       g[n].splits = b.plan_h.splits;
       shapes[n++] = b.plan_h.shape;
+      if (b.columns) {
+        g[0].op.A = (const T*)d->weight + v0 * d->weight_stride;
+        g[0].op.lda = d->weight_stride;
+        g[0].op.rows_of_k = (int)classes;
+        g[0].whole = d->dim % 4 == 0;
+        g[0].op.bias = d->bias ? (const T*)d->bias + v0 : nullptr;
+      }
       if (b.sum_h && p == b.pieces - 1) finish.add(b.sum_h, b.plan_h.splits, d->rows * d->dim, grad_hidden);
     }
     if (grad_weight) {
@@ -1525,7 +1578,15 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
       shapes[n++] = b.plan_w.shape;
       if (b.sum_w) finish.add(b.sum_w, b.plan_w.splits, classes * d->dim, grad_weight + v0 * d->dim);
     }
-    launch_grad<T, SPLIT>(g, shapes, n, s);
+    int first = 0;
+    if constexpr (!SPLIT)
+      if (b.columns) {
+        if (shapes[0] == kThin) launch_grad_as<T, Thin, false, kStagedColumns>(g, 1, s);
+        else if (shapes[0] == kNarrow) launch_grad_as<T, Narrow, false, kStagedColumns>(g, 1, s);
+        else launch_grad_as<T, Small, false, kStagedColumns>(g, 1, s);
+        first = 1;
+      }
+    launch_grad<T, SPLIT>(g + first, shapes + first, n - first, s);
     if (grad_bias) {
       // few classes: their rows in parts, so that more than a block per class works on them
       const int parts = b.sum_b ? (int)(kBiasBlocks / classes < 1 ? 1 : kBiasBlocks / classes) : 1;
