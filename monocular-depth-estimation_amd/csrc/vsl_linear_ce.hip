@@ -176,14 +176,20 @@ __device__ __forceinline__ void tile_product(const Operands& op, int m0, int n0,
   auto load = [&]() {
     const int first = next_step * Kind<T>::BK + ((tid & 7) ^ ((tid >> 4) & 7)) * Kind<T>::E;  // column of a thread's pieces
     const bool whole = (++next_step) * Kind<T>::BK <= op.dim;
+    // a piece that runs over the end of its row reads on in the next one (of 8 elements or more): those columns of the tile
+    // are nobody's
+    const bool followed = COLUMNS && next_step * Kind<T>::BK < op.rows_of_k;
 #pragma unroll
     for (int i = 0; i < (STAGED ? S::kFetch : 0); ++i) {
       if (COLUMNS && i < S::kFetchA) {
         const int at = i * S::kThreads + tid, k = at / kWide, row = (next_step - 1) * Kind<T>::BK + k;
         const int m = m0 + (at % kWide * E ^ (k / E & 1) * 32);
-        held[i] = u32x4{0u, 0u, 0u, 0u};
-        if (row < op.rows_of_k && !(op.bias && (float)((const T*)op.bias)[row] == ninf()))
-          held[i] = load_columns((const T*)op.A + (int64_t)row * op.lda, m, op.M);
+        if (followed) {
+          held[i] = load16((const T*)op.A + (int64_t)row * op.lda + min(m, op.M - 1));
+        } else {
+          held[i] = u32x4{0u, 0u, 0u, 0u};
+          if (row < op.rows_of_k) held[i] = load_columns((const T*)op.A + (int64_t)row * op.lda, m, op.M);
+        }
       } else {
         held[i] = COLUMNS || whole ? load16((const T*)src[i]) : load_columns((const T*)src[i], 0, op.dim - first);
         src[i] += kBlockBytes;
@@ -191,6 +197,12 @@ __device__ __forceinline__ void tile_product(const Operands& op, int m0, int n0,
     }
   };
   auto store = [&](int buffer) {
+    if (COLUMNS && op.bias)  // rows of the step that is held
+#pragma unroll
+      for (int i = 0; i < S::kFetchA; ++i) {
+        const int row = (next_step - 1) * Kind<T>::BK + (i * S::kThreads + tid) / kWide;
+        if ((float)((const T*)op.bias)[min(row, op.rows_of_k - 1)] == ninf()) held[i] = u32x4{0u, 0u, 0u, 0u};
+      }
 #pragma unroll
     for (int i = 0; i < (STAGED ? S::kFetch : 0); ++i) *(u32x4*)(lds + buffer * S::kBuffer + (i * S::kThreads + tid) * 16) = held[i];
   };
@@ -1161,7 +1173,10 @@ constexpr double kStaged = 1.5;
 // does not fit the registers, and its matrix instructions are eight times slower, so that its loads never bind.
 Plan plan_of(int64_t M, int64_t N, int64_t blocks, int type, bool may_split, bool staged = false) {
   Plan best{kSmall, 1, 1e300};
-  for (int shape = type == VSL_TYPE_F32 || staged ? kSmall : kLarge; shape <= (N <= Thin::BN ? kThin : kNarrow); ++shape) {
+  // the thin tile: float32 is bound by its multiplications, of which up to three of it waste fewer (67 x 113867 x 1013
+  // forward: 245 us, with two of the narrow one 270); 16-bit types by reading A
+  const int last = N <= (type == VSL_TYPE_F32 ? 3 : 1) * Thin::BN ? kThin : kNarrow;
+  for (int shape = type == VSL_TYPE_F32 || staged ? kSmall : kLarge; shape <= last; ++shape) {
     const ShapeInfo& h = kShapes[shape];
     const double tiles = (double)(ceil_div(M, h.bm) * ceil_div(N, h.bn));
     const double step = (type == VSL_TYPE_F32 ? h.step32 : h.step16) * (staged ? kStaged : 1.0);
@@ -1273,7 +1288,7 @@ static_assert(kMostParts <= kPieceElements && kMostParts / kPad / kPartRows < 65
 constexpr int64_t kBiasBlocks = 1024;
 
 // grad_hidden of few rows takes a large weight as it lies: transposing it first reads and writes it once more.
-// 5 x 60478 x 1627 float32 with gradients takes 677 us, transposed 866; 57 x 90227 x 1024 float16 271 and 295; above 128 rows
+// 5 x 60478 x 1627 float32 with gradients takes 481 us, transposed 746; 57 x 90227 x 1024 float16 263 and 295; above 128 rows
 // the gathers bind (346 x 30813 x 1495 float16: 552 and 394), below 16 MB the further launch (19 x 56371 x 54 bfloat16: 104
 // and 90).
 constexpr int64_t kColumnsRows = 128, kColumnsBytes = 16 << 20;
@@ -1301,7 +1316,8 @@ Backward backward_workspace(const vsl_linear_ce_desc* d, uint32_t mask, void* ba
   b.hidden = b.l.copy_hidden ? a.take((size_t)d->rows * b.l.dim_padded * s) : nullptr;
   b.weight = b.l.copy_weight ? a.take((size_t)d->vocab * b.l.dim_padded * s) : nullptr;
   b.hidden_t = gw ? a.take((size_t)d->dim * b.l.rows_padded * s) : nullptr;
-  b.columns = gh && !b.l.split && d->rows <= kColumnsRows && d->vocab * d->dim * size_of(d->type) >= kColumnsBytes;
+  // dim: a piece that runs over the end of a row has to end in the next one (kStagedColumns)
+  b.columns = gh && !b.l.split && d->rows <= kColumnsRows && d->dim >= 8 && d->vocab * d->dim * size_of(d->type) >= kColumnsBytes;
   b.weight_t = gh && !b.columns ? a.take((size_t)d->dim * b.vocab_padded * s) : nullptr;
   b.delta = gh ? a.take((size_t)b.l.rows_padded * b.piece * s) : nullptr;
   b.delta_t = gw || gb ? a.take((size_t)b.l.rows_padded * b.piece * s) : nullptr;

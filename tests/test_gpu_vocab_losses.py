@@ -436,6 +436,25 @@ def test_linear_cross_entropy_in_parts_of_the_features(rows, vocab, dim, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab,dim", [(1, 9001, 1003), (33, 8192, 1024), (70, 9001, 1003), (128, 9003, 1001), (96, 40000, 250),
+                                            (20, 1100000, 9)])
+def test_linear_cross_entropy_of_few_rows_and_a_large_weight(rows, vocab, dim, dtype):
+    """grad_hidden from the weight as it lies, 32 or 64 rows a tile, rows that end inside a 16-byte piece, masked classes
+    whatever their weights hold, the last ones among them."""
+    h, w, b, t = ce_inputs(rows, vocab, dim, dtype, rows + dim, bias=rows % 2 == 0)
+    if b is not None:
+        masked = torch.cat([torch.arange(vocab - 40, vocab), torch.arange(3, vocab, 97)])
+        b[masked], w[masked] = -INF, float("nan")
+        t = torch.where(torch.isin(t, masked), torch.ones_like(t), t)
+    if rows > 4:
+        t[torch.rand(rows, generator=gen(12)) < 0.2] = -100
+    check_ce(h, w, b, t)
+    wide = torch.zeros(vocab, dim + 5, dtype=dtype, device=DEV)          # the same in a larger tensor's columns
+    wide[:, 2:dim + 2] = w.to(DEV)
+    check_ce(h, w, b, t, on_device=(h.to(DEV), wide[:, 2:dim + 2]))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_linear_cross_entropy_in_parts_masks_and_specials(dtype):
     rows, vocab, dim = 40, 150, 3000
     h, w, b, t = ce_inputs(rows, vocab, dim, dtype, 79, bias=True)
