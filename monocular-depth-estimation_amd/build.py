@@ -5,6 +5,8 @@ import os
 import re
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -33,15 +35,23 @@ def build(force: bool = False, verbose: bool = False) -> str:
     # reference's float32 results (1.5e-5 instead of 1e-6 relative on the golden fixtures).
     # -fno-slp-vectorize: packed f32 math has no rate advantage on gfx950 and its operand pairing costs
     # register moves (measured 3 % slower with it).  -packed-fp32-ops keeps the compiler from forming it in other passes.
-    cmd = [HIPCC, "-Rpass-analysis=kernel-resource-usage", "-O3", "--offload-arch=gfx950", "-std=c++17", "-ffp-contract=on",
-           "-fno-slp-vectorize", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-shared", "-fPIC",
-           "-I", os.path.join(HERE, "..", "include"), "-o", OUT] + [os.path.join(CSRC, s) for s in SOURCES]
-    if verbose:
-        print(" ".join(cmd), file=sys.stderr)
-    proc = subprocess.run(cmd, stderr=subprocess.PIPE, text=True)
-    table = kernel_resources(proc.stderr)
+    flags = ["-Rpass-analysis=kernel-resource-usage", "-O3", "--offload-arch=gfx950", "-std=c++17", "-ffp-contract=on",
+             "-fno-slp-vectorize", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-fPIC",
+             "-I", os.path.join(HERE, "..", "include")]
+    with tempfile.TemporaryDirectory() as tmp:  # the sources side by side, the longest takes 80 s
+        objects = [os.path.join(tmp, s + ".o") for s in SOURCES]
+        compile_ = [[HIPCC] + flags + ["-c", os.path.join(CSRC, s), "-o", o] for s, o in zip(SOURCES, objects)]
+        link = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", OUT] + objects
+        if verbose:
+            print("\n".join(" ".join(c) for c in compile_ + [link]), file=sys.stderr)
+        with ThreadPoolExecutor(len(SOURCES)) as pool:
+            done = list(pool.map(lambda c: subprocess.run(c, stderr=subprocess.PIPE, text=True), compile_))
+        if all(p.returncode == 0 for p in done):
+            done.append(subprocess.run(link, stderr=subprocess.PIPE, text=True))
+    text = "".join(p.stderr for p in done)
+    table = kernel_resources(text)
     other, after_remark = [], False  # everything but the remarks and the source excerpts printed under them
-    for ln in proc.stderr.splitlines():
+    for ln in text.splitlines():
         if "-Rpass-analysis=kernel-resource-usage" in ln:
             after_remark = True
         elif not (after_remark and re.match(r"\s*\d*\s*\|", ln)):
@@ -49,8 +59,9 @@ def build(force: bool = False, verbose: bool = False) -> str:
             other.append(ln)
     if other:
         print("\n".join(other), file=sys.stderr)
-    if proc.returncode != 0:
-        raise subprocess.CalledProcessError(proc.returncode, cmd)
+    for proc in done:
+        if proc.returncode != 0:
+            raise subprocess.CalledProcessError(proc.returncode, proc.args)
     with open(RESOURCES, "w") as f:
         f.write("# kernel  VGPRs  SGPR-spills  VGPR-spills  scratch-bytes-per-lane  LDS-bytes\n")
         for k in table:
