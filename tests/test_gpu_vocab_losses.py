@@ -673,6 +673,30 @@ def test_captured_and_replayed():
             assert all(torch.equal(a, b) for a, b in zip(out, both(L, s)))
 
 
+@pytest.mark.parametrize("rows,vocab,dim,dtype", [(12, 500, 3000, torch.float32), (16, 9001, 1003, torch.float32), (40, 90, 2048, torch.float16)])
+def test_captured_and_replayed_in_parts_and_by_columns(rows, vocab, dim, dtype):
+    import mde_amd.vocab_losses as L
+    h, w, b, t = ce_inputs(rows, vocab, dim, dtype, 181, bias=True)
+    leaves = [x.to(DEV).requires_grad_(True) for x in (h, w, b)]
+    t = t.to(DEV)
+    step = lambda: torch.autograd.grad(L.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2]), leaves)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for turn in range(4):
+        with torch.no_grad():
+            leaves[turn % 3].mul_(0.9).add_(0.01)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(out, step()))
+
+
 def test_saved_tensors_may_move_between_forward_and_backward():
     import mde_amd.vocab_losses as L
     s = state(20, 3000, 64, torch.float32, 131)
@@ -684,6 +708,35 @@ def test_saved_tensors_may_move_between_forward_and_backward():
     filler = [torch.full((20, 3000), float("nan"), device=DEV) for _ in range(4)]   # over anything that was given back
     got = torch.autograd.grad(loss, (s["x"], s["h"], s["w"]))
     assert all(torch.equal(a, b) for a, b in zip(want[2:], got)) and len(filler) == 4
+
+
+def test_changed_tensors_and_two_threads():
+    """A tensor changed between forward and backward is refused; two threads' calls do not meet."""
+    import threading
+    import mde_amd.vocab_losses as L
+    s = state(30, 700, 64, torch.float32, 141)
+    for name in ("x", "w"):
+        top = L.top_logits(s["teacher"], 5)
+        loss = L.topk_distillation_loss(s["x"], top.values, top.indices, top.lse) + L.linear_cross_entropy(s["h"], s["w"], s["t"])
+        with torch.no_grad():
+            s[name].mul_(0.5)
+        with pytest.raises(RuntimeError, match="modified"):
+            torch.autograd.grad(loss, (s["x"], s["w"]))
+    states, outs = [state(30, 700, 64, torch.bfloat16, 150 + i) for i in range(2)], [None, None]
+    want = [both(L, s) for s in states]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                outs[i] = both(L, states[i])
+            torch.cuda.current_stream().synchronize()
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    for a, b in zip(want, outs):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
 def test_refusals_on_the_device():
