@@ -915,8 +915,9 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_grad(GradJobs jobs) {
   }
 }
 
-// out = scale * the sum of the splits, in their order: four elements a thread, the splits dealt to the four waves; up to
-// three sums in one launch.  8192 x 4096 float32 to bfloat16: 88 us.
+// out = scale * the sum of the splits, in their order: four elements a thread; many splits are dealt to the four waves; up to
+// three sums in one launch.  8192 x 4096 float32 to bfloat16: 53 us, 3.8 TB/s.
+constexpr int kDealtSplits = 8;  // at least
 struct FinishJob {
   const float* sum;
   void* out;
@@ -937,9 +938,7 @@ __global__ __launch_bounds__(kThreads) void k_ce_finish(FinishJobs jobs) {
   const FinishJob& j = jobs.job[which];
   const float scale = jobs.scale.get();
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int per = (j.splits + 3) / 4, s0 = wave * per, s1 = min(j.splits, s0 + per);
-  for (int64_t i0 = block * 256; i0 < j.n; i0 += j.blocks * 256) {
-    const int64_t i = i0 + 4 * lane;
+  auto sum = [&](int64_t i, int s0, int s1) {
     f32x4 v{0.0f, 0.0f, 0.0f, 0.0f};
     if (i + 4 <= j.n) {
 #pragma unroll 8
@@ -950,15 +949,28 @@ __global__ __launch_bounds__(kThreads) void k_ce_finish(FinishJobs jobs) {
         for (int e = 0; e < 4; ++e)
           if (i + e < j.n) v[e] += j.sum[s * j.n + i + e];
     }
+    return v;
+  };
+  auto store = [&](int64_t i, const f32x4& v) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (i + e < j.n) ((T*)j.out)[i + e] = (T)(scale * v[e]);
+  };
+  if (j.splits < kDealtSplits) {
+    for (int64_t i = (block * kThreads + threadIdx.x) * 4; i < j.n; i += j.blocks * kThreads * 4) store(i, sum(i, 0, j.splits));
+    return;
+  }
+  const int per = (j.splits + 3) / 4, s0 = min(j.splits, wave * per), s1 = min(j.splits, s0 + per);
+  for (int64_t i0 = block * 256; i0 < j.n; i0 += j.blocks * 256) {
+    const int64_t i = i0 + 4 * lane;
+    f32x4 v = sum(i, s0, s1);
     __syncthreads();
     if (wave) part[wave - 1][lane] = v;
     __syncthreads();
     if (wave) continue;
 #pragma unroll
     for (int w = 0; w < 3; ++w) v += part[w][lane];
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (i + e < j.n) ((T*)j.out)[i + e] = (T)(scale * v[e]);
+    store(i, v);
   }
 }
 
@@ -1368,7 +1380,7 @@ struct FinishLaunch {
   int n = 0;
   int64_t blocks = 0;
   void add(const float* sum, int splits, int64_t elements, void* out) {
-    const int64_t b = ceil_div(elements, 256);
+    const int64_t b = ceil_div(elements, splits < kDealtSplits ? 4 * kThreads : kThreads);
     jobs.job[n++] = {sum, out, splits, elements, b < 65536 ? b : 65536};
     blocks += jobs.job[n - 1].blocks;
   }
