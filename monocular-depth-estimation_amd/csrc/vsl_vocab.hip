@@ -215,10 +215,60 @@ __device__ __forceinline__ void merge_group(K (&key)[N]) {
   }
 }
 
-// Short rows: L lanes hold NV vectors each.  Every lane sorts its keys.  For few keys every round takes the largest of the
-// group's first ones, and its lane moves on to its next; for many (SORT) the lanes' lists are merged.
-// 368640 x 96 float16, k = 8: 44 us, 2.0 TB/s; bound by the vector instructions of the sorts.
-template <typename T, int L, int NV, bool SORT>
+// The eight largest of a lane's keys, larger first, and of a group's, which every lane gets: of two sorted lists the larger
+// of each place and its mirror are the largest eight, in bitonic order.
+template <typename K>
+__device__ __forceinline__ void clean8(K (&key)[8]) {
+#pragma unroll
+  for (int q = 4; q >= 1; q >>= 1)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (!(i & q)) {
+        const K a = key[i], b = key[i + q];
+        key[i] = a > b ? a : b;
+        key[i + q] = a > b ? b : a;
+      }
+}
+template <int N, typename K>
+__device__ __forceinline__ void own_top8(const K (&key)[N], K (&best)[8]) {
+#pragma unroll
+  for (int c = 0; c < (N + 7) / 8; ++c) {
+    K part[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) part[e] = 8 * c + e < N ? key[8 * c + e] : (K)0;
+    sort_own<8>(part);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) best[e] = c == 0 || part[7 - e] > best[e] ? part[c == 0 ? e : 7 - e] : best[e];
+    if (c > 0) clean8(best);
+  }
+}
+template <int X, typename K>
+__device__ __forceinline__ void join_top8(K (&best)[8]) {
+  K other[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) other[e] = lane_xor<X>(best[7 - e]);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) best[e] = other[e] > best[e] ? other[e] : best[e];
+  clean8(best);
+}
+template <int L, typename K>
+__device__ __forceinline__ void group_top8(K (&best)[8]) {  // mirrors: after every step all lanes of a half hold the same
+  join_top8<1>(best);
+  join_top8<3>(best);
+  join_top8<7>(best);
+  if (L > 8) join_top8<15>(best);
+  if (L > 16) {
+    join_top8<31>(best);
+    join_top8<63>(best);
+  }
+}
+
+// Short rows: L lanes hold NV vectors each.  Up to eight keys (kEight): lists of eight are joined over the lanes.  Else every
+// lane sorts its keys; every round takes the largest of the group's first ones, and its lane moves on to its next (kRounds),
+// or, for many keys, the lanes' lists are merged (kMerge).
+// 368640 x 96 float16, k = 8: 34 us, 2.6 TB/s; bound by the vector instructions of the sorts.
+enum { kEight, kRounds, kMerge };
+template <typename T, int L, int NV, int FORM>
 __global__ __launch_bounds__(kThreads) void k_top_rows(TopArgs a) {
   constexpr int E = Vec<T>::E, G = kThreads / L;
   typedef typename RowKey<T>::K K;
@@ -260,8 +310,21 @@ __global__ __launch_bounds__(kThreads) void k_top_rows(TopArgs a) {
       t.s = group_all<L>(t.s, AddF());
       if (live && lane == 0) a.lse[row] = log_sum(t, a.inv_t);
     }
+    if (FORM == kEight) {
+      K best[8];
+      own_top8<NV * E>(key, best);
+      group_top8<L>(best);
+      if (live && lane < a.k) {
+        K mine = best[0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) mine = lane == e ? best[e] : mine;
+        ((T*)a.values)[row * a.k + lane] = RowKey<T>::value(mine);
+        a.indices[row * a.k + lane] = RowKey<T>::index(mine);
+      }
+      continue;
+    }
     sort_own<NV * E>(key);
-    if (SORT) {
+    if (FORM == kMerge) {
       merge_group<L>(key);
 #pragma unroll
       for (int e = 0; e < NV * E; ++e) {
@@ -678,24 +741,29 @@ int check_top(const vsl_top_desc* d) {
 // 20000 x 250 f32, k = 8: 24.1 and 24.9, k = 24: 50.3 and 25.7).
 template <typename T>
 constexpr int most_rounds() { return sizeof(T) == 4 ? 15 : 20; }
-template <typename T, bool SORT>
+template <typename T, int FORM>
 void launch_rows(const TopArgs& a, int nv, hipStream_t s) {
   const dim3 b(kThreads);
   const dim3 g8(grid_of(ceil_div(a.rows, kThreads / 8)));
   const dim3 g16(grid_of(ceil_div(a.rows, kThreads / 16))), g64(grid_of(ceil_div(a.rows, kThreads / 64)));
-  if (nv <= 8) hipLaunchKernelGGL((k_top_rows<T, 8, 1, SORT>), g8, b, 0, s, a);
-  else if (nv <= 16) hipLaunchKernelGGL((k_top_rows<T, 8, 2, SORT>), g8, b, 0, s, a);
-  else if (nv <= 32) hipLaunchKernelGGL((k_top_rows<T, 16, 2, SORT>), g16, b, 0, s, a);
-  else if (nv <= 64) hipLaunchKernelGGL((k_top_rows<T, 16, 4, SORT>), g16, b, 0, s, a);
-  else if (nv <= 128) hipLaunchKernelGGL((k_top_rows<T, 64, 2, SORT>), g64, b, 0, s, a);
-  else hipLaunchKernelGGL((k_top_rows<T, 64, 4, SORT>), g64, b, 0, s, a);
+  if (nv <= 8) hipLaunchKernelGGL((k_top_rows<T, 8, 1, FORM>), g8, b, 0, s, a);
+  else if (nv <= 16) hipLaunchKernelGGL((k_top_rows<T, 8, 2, FORM>), g8, b, 0, s, a);
+  else if (nv <= 32) hipLaunchKernelGGL((k_top_rows<T, 16, 2, FORM>), g16, b, 0, s, a);
+  else if (nv <= 64) hipLaunchKernelGGL((k_top_rows<T, 16, 4, FORM>), g16, b, 0, s, a);
+  else if (nv <= 128) hipLaunchKernelGGL((k_top_rows<T, 64, 2, FORM>), g64, b, 0, s, a);
+  else hipLaunchKernelGGL((k_top_rows<T, 64, 4, FORM>), g64, b, 0, s, a);
 }
 template <typename T>
 void launch_top(const TopArgs& a, bool rows_program, hipStream_t s) {
   if (rows_program) {
     const int nv = (int)ceil_div(a.V, Vec<T>::E);
-    if (a.k > most_rounds<T>()) launch_rows<T, true>(a, nv, s);
-    else launch_rows<T, false>(a, nv, s);
+    // The join of eights takes the time of about five rounds (by rounds and joined: 368640 x 96 float16, k = 8: 41.2 and 33.9
+    // us; 100000 x 60 bfloat16, k = 4: 7.7 and 8.5; 20000 x 250 float32, k = 8: 24.1 and 12.8), of more where 64 lanes trade
+    // 64-bit keys and hold few (11261 x 288 float32, k = 7: 16.3 and 20.3).
+    const bool eight = a.k >= 5 && a.k <= 8 && !(sizeof(T) == 4 && nv > 64 && nv <= 128);
+    if (eight) launch_rows<T, kEight>(a, nv, s);
+    else if (a.k > most_rounds<T>()) launch_rows<T, kMerge>(a, nv, s);
+    else launch_rows<T, kRounds>(a, nv, s);
     return;
   }
   hipLaunchKernelGGL(k_top_stream<T>, dim3(grid_of(a.rows * a.segs)), dim3(kThreads), 0, s, a);

@@ -82,6 +82,18 @@ def test_top_logits_of_ties_masks_and_specials(vocab, dtype):
     check_top(x.to(dtype).to(DEV), k)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [23, 60, 100, 120, 250, 300, 500, 900, 1024, 1500, 2048])
+def test_top_logits_short_rows_by_every_form(vocab, dtype):
+    """Joined eights, rounds and merged lists over 8, 16 and 64 lanes; masked rows and ties that cross lanes."""
+    x = logits(37, vocab, vocab, dtype)
+    x[3:9] = (x[3:9] * 2).round()                           # many ties
+    x[10, :] = -INF
+    x[11, 5:] = -INF
+    for k in (1, 4, 5, 7, 8, 9, 15, 16, 20, 21):
+        check_top(x.to(DEV), k)
+
+
 @pytest.mark.parametrize("temperature", [1e-4, 0.05, 1e4])
 def test_extreme_temperatures(temperature):
     for vocab in (90, 700, 5000):
