@@ -664,8 +664,11 @@ struct Contributes {
   int64_t ignore_index;
   template <typename T>
   __device__ __forceinline__ bool row(int64_t r) const {
-    if (target && (target[r] == ignore_index || stats[r] == ninf())) return false;
-    return !(scale && scale[r] == 0.0f) && !(bias && (float)((const T*)bias)[r] == ninf());
+    bool on = true;
+    if (target) on = (int)(target[r] != ignore_index) & (int)(stats[r] != ninf());
+    if (scale) on &= scale[r] != 0.0f;
+    if (bias) on &= (float)((const T*)bias)[r] != ninf();
+    return on;
   }
 };
 struct LayoutJob {
@@ -772,8 +775,16 @@ __device__ __forceinline__ void transpose_job(const LayoutJob& j, int64_t block,
   } else {
     float(*tile)[65] = (float(*)[65])lds;
     const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
-    for (int i = y; i < 64; i += 4)
-      tile[i][x] = c0 + x < j.cols && r0 + i < j.rows && j.with.row<T>(r0 + i) ? in[(r0 + i) * j.stride + c0 + x] : 0.0f;
+    float v[16];
+    bool on[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {  // clamped into the matrix, so that all reads go out together
+      const int64_t r = min(r0 + y + 4 * i, j.rows - 1);
+      on[i] = j.with.row<T>(r);
+      v[i] = in[r * j.stride + min(c0 + x, j.cols - 1)];
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) tile[y + 4 * i][x] = on[i] && c0 + x < j.cols && r0 + y + 4 * i < j.rows ? v[i] : 0.0f;
     __syncthreads();
     if constexpr (SPLIT) {
 #pragma unroll
@@ -1187,12 +1198,13 @@ constexpr double kStaged = 1.5;
 // Shape of the tiles of a product M x N over `blocks` steps of K, and into how many parts K is cut: the least of the waves
 // of tiles times their length, plus the traffic of the partial sums.  float32 leaves out the large tile: its epilogue
 // does not fit the registers, and its matrix instructions are eight times slower, so that its loads never bind.
-Plan plan_of(int64_t M, int64_t N, int64_t blocks, int type, bool may_split, bool staged = false) {
+Plan plan_of(int64_t M, int64_t N, int64_t blocks, int type, bool may_split, bool staged = false, int only = -1) {
   Plan best{kSmall, 1, 1e300};
   // the thin tile: float32 is bound by its multiplications, of which up to three of it waste fewer (67 x 113867 x 1013
   // forward: 245 us, with two of the narrow one 270); 16-bit types by reading A
   const int last = N <= (type == VSL_TYPE_F32 ? 3 : 1) * Thin::BN ? kThin : kNarrow;
   for (int shape = type == VSL_TYPE_F32 || staged ? kSmall : kLarge; shape <= last; ++shape) {
+    if (only >= 0 && shape != only) continue;
     const ShapeInfo& h = kShapes[shape];
     const double tiles = (double)(ceil_div(M, h.bm) * ceil_div(N, h.bn));
     const double step = (type == VSL_TYPE_F32 ? h.step32 : h.step16) * (staged ? kStaged : 1.0);
@@ -1333,12 +1345,20 @@ Backward backward_workspace(const vsl_linear_ce_desc* d, uint32_t mask, void* ba
   b.weight = b.l.copy_weight ? a.take((size_t)d->vocab * b.l.dim_padded * s) : nullptr;
   b.hidden_t = gw ? a.take((size_t)d->dim * b.l.rows_padded * s) : nullptr;
   // dim: a piece that runs over the end of a row has to end in the next one (kStagedColumns)
-  b.columns = gh && !b.l.split && d->rows <= kColumnsRows && d->dim >= 8 && d->vocab * d->dim * size_of(d->type) >= kColumnsBytes;
+  const bool columns = !b.l.split && d->rows <= kColumnsRows && d->dim >= 8 && d->vocab * d->dim * size_of(d->type) >= kColumnsBytes;
+  b.columns = gh && columns;
   b.weight_t = gh && !b.columns ? a.take((size_t)d->dim * b.vocab_padded * s) : nullptr;
   b.delta = gh ? a.take((size_t)b.l.rows_padded * b.piece * s) : nullptr;
   b.delta_t = gw || gb ? a.take((size_t)b.l.rows_padded * b.piece * s) : nullptr;
-  b.plan_h = plan_of(d->dim, d->rows, b.l.steps(b.piece), b.l.type, true, b.columns);
+  b.plan_h = plan_of(d->dim, d->rows, b.l.steps(b.piece), b.l.type, true, columns);
   b.plan_w = plan_of(d->dim, d->vocab < b.piece ? d->vocab : b.piece, b.l.steps(d->rows), b.l.type, true);
+  if (!columns) {  // tiles of one shape go in one launch, which is worth 4 us; the same where one gradient is asked for alone
+    for (int shape = kLarge; shape <= kNarrow && b.plan_h.shape != b.plan_w.shape; ++shape) {
+      const Plan h = plan_of(d->dim, d->rows, b.l.steps(b.piece), b.l.type, true, false, shape);
+      const Plan w = plan_of(d->dim, d->vocab < b.piece ? d->vocab : b.piece, b.l.steps(d->rows), b.l.type, true, false, shape);
+      if (h.time + w.time < b.plan_h.time + b.plan_w.time + 4.0) b.plan_h = h, b.plan_w = w;
+    }
+  }
   b.sum_h = gh && (b.pieces > 1 || b.plan_h.splits > 1) ? (float*)a.take((size_t)b.plan_h.splits * d->rows * d->dim * 4) : nullptr;
   b.sum_w = gw && b.plan_w.splits > 1 ? (float*)a.take((size_t)b.plan_w.splits * b.piece * d->dim * 4) : nullptr;
   b.sum_b = gb && d->rows >= 8192 && d->vocab <= kBiasBlocks / 2 ? (float*)a.take(kBiasBlocks * 4) : nullptr;
