@@ -418,16 +418,15 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
           s += ex(t.acc[i][j][r]);
           s2 += ex(t.acc[i][j][r + 1]);
         }
-      MaxSum q{m, s + s2};
+      MaxSum q{m, (s + s2) * ex.factor()};
       q = join(q, {__shfl_xor(q.m, 32, 64), __shfl_xor(q.s, 32, 64)}, kLog2e);
       if (half == 0) ((float2*)lds)[wm * S::BN + col] = make_float2(q.m, q.s);
     } else {
       const float top = live ? a.stats[row] : ninf(), ls = live ? a.stats[a.op.N + row] : 0.0f;
       const float scale = !live || top == ninf() || target + a.class0 == a.ignore_index ? 0.0f
                           : a.row_scale ? a.row_scale[row] : a.unit;
-      const float factor = scale * slope_of(a.z_loss, top, ls);
       const Exponent ex(top, kLog2e);
-      const float shift = ex.shift - ls;
+      const float factor = scale * slope_of(a.z_loss, top, ls) * ex.factor(ls);
       O* d = (O*)a.delta + (int64_t)row * a.ldd;
 #pragma unroll
       for (int i = 0; i < S::IM; ++i) {
@@ -435,7 +434,7 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
         f32x16& z = t.acc[i][j];
         if (biased) add_bias(z, bias + v32 - m0 + 4 * half);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) z[r] = factor * __builtin_amdgcn_exp2f(fmaf(z[r], ex.c, shift));
+        for (int r = 0; r < 16; ++r) z[r] = factor * ex(z[r]);
         if (target >= v32 && target < v32 + 32) {
 #pragma unroll
           for (int r = 0; r < 16; ++r)
@@ -1074,20 +1073,18 @@ __global__ __launch_bounds__(THREADS) void k_ce_parts_rows(Parts z, const int64_
                                                            float* __restrict__ divisor) {
   __shared__ float red[THREADS / 32];
   const int64_t row = blockIdx.x;
-  MaxSum q{ninf(), 0.0f};
+  RunSum run;
   for (int64_t v = threadIdx.x; v < z.vocab; v += 4 * THREADS) {
     float x[4];
     z.logits<T>(row, v, 0, THREADS, [&](int u) { return v + u * THREADS < z.vocab; }, x);
-    float m = q.m;
+    float m = run.m;
 #pragma unroll
     for (int u = 0; u < 4; ++u) m = __builtin_elementwise_maximum(m, x[u]);
-    const Exponent ex(exp_ref(m), kLog2e);
-    float s = q.s * exp_of(q.m, exp_ref(m), kLog2e);
+    const Exponent ex = run.move(m, kLog2e);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) s += ex(x[u]);
-    q = {m, s};
+    for (int u = 0; u < 4; ++u) run.s += ex(x[u]);
   }
-  q = block_join<THREADS / 64>(q, red, kLog2e);
+  const MaxSum q = block_join<THREADS / 64>(run.get(), red, kLog2e);
   if (threadIdx.x) return;
   bool counts;
   const float loss = close_row(q, [&](int64_t t) { return z.logit<T>(row, t); }, target[row], ignore_index, z.vocab, z_loss, row,
@@ -1120,7 +1117,7 @@ __global__ __launch_bounds__(kThreads) void k_ce_parts_delta(Parts z, LogitArgs 
     float d = 0.0f;
     if (scale != 0.0f) {
       const Exponent ex(top, kLog2e);
-      d = scale * slope_of(a.z_loss, top, ls) * __builtin_amdgcn_exp2f(fmaf(logit[u], ex.c, ex.shift - ls));
+      d = scale * slope_of(a.z_loss, top, ls) * ex.factor(ls) * ex(logit[u]);
       if (v == target) d -= scale;
     }
     if (a.delta) ((T*)a.delta)[row * a.ldd + v] = (T)d;

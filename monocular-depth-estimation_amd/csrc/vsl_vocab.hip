@@ -307,7 +307,7 @@ __global__ __launch_bounds__(kThreads) void k_top_rows(TopArgs a) {
       for (int v = 0; v < NV; ++v)
 #pragma unroll
         for (int e = 0; e < E; ++e) t.s += ex(xs[v][e]);
-      t.s = group_all<L>(t.s, AddF());
+      t.s = group_all<L>(t.s, AddF()) * ex.factor();
       if (live && lane == 0) a.lse[row] = log_sum(t, a.inv_t);
     }
     if (FORM == kEight) {
@@ -480,23 +480,22 @@ __device__ __forceinline__ void load_group(const T* x, int i0, int end, u32x4 (&
 }
 // running maximum and sum over a group; returns the group's maximum
 template <typename T, int N>
-__device__ __forceinline__ float add_group(const float (&v)[N][Vec<T>::E], MaxSum& t, float c) {
+__device__ __forceinline__ float add_group(const float (&v)[N][Vec<T>::E], RunSum& t, float c) {
   float top = v[0][0];
 #pragma unroll
   for (int u = 0; u < N; ++u)
 #pragma unroll
     for (int e = 0; e < Vec<T>::E; ++e) top = __builtin_elementwise_maximum(top, v[u][e]);
-  const float m = __builtin_elementwise_maximum(t.m, top), ref = exp_ref(m);
-  const Exponent ex(ref, c);
-  float s = t.s * exp_of(t.m, ref, c), s2 = 0.0f;
+  const Exponent ex = t.move(__builtin_elementwise_maximum(t.m, top), c);
+  float s2 = 0.0f;
 #pragma unroll
   for (int u = 0; u < N; ++u)
 #pragma unroll
     for (int e = 0; e < Vec<T>::E; e += 2) {
-      s += ex(v[u][e]);
+      t.s += ex(v[u][e]);
       s2 += ex(v[u][e + 1]);
     }
-  t = {m, s + s2};
+  t.s += s2;
   return top;
 }
 
@@ -514,7 +513,7 @@ __global__ __launch_bounds__(kThreads, 4) void k_top_stream(TopArgs a) {
     const int seg = (int)(item % a.segs);
     const T* x = (const T*)a.logits + row * a.stride;
     const int e0 = seg * a.seg_len, e1 = min(a.V, e0 + a.seg_len);  // a segment never starts behind the row
-    MaxSum t{ninf(), 0.0f};
+    RunSum run;
     unsigned long long bound = 0;
     float floor_value = ninf();
     int kept = 0;  // keys in the buffer, as every thread knows it
@@ -551,7 +550,7 @@ __global__ __launch_bounds__(kThreads, 4) void k_top_stream(TopArgs a) {
 #pragma unroll
       for (int u = 0; u < kGroup; ++u) unpack(next[u], v[u], (const T*)nullptr);
       if (i0 + kSpan < probe_end) load_group(x, i0 + kSpan, e1, next);
-      best = __builtin_elementwise_maximum(best, add_group<T>(v, t, a.c));
+      best = __builtin_elementwise_maximum(best, add_group<T>(v, run, a.c));
     }
     if (e1 - e0 > kSpan) load_group(x, e0, e1, next);  // else it is there still
     {
@@ -592,7 +591,7 @@ __global__ __launch_bounds__(kThreads, 4) void k_top_stream(TopArgs a) {
 #pragma unroll
           for (int e = 0; e < E; ++e) top = __builtin_elementwise_maximum(top, v[u][e]);
       } else {
-        top = add_group<T>(v, t, a.c);
+        top = add_group<T>(v, run, a.c);
       }
       const int before = kept;
       if (__any(!(top < floor_value)))
@@ -611,7 +610,8 @@ __global__ __launch_bounds__(kThreads, 4) void k_top_stream(TopArgs a) {
     }
     const int n = kept;
     sort_count(buf, n);
-    if (a.lse || a.segs > 1) t = block_join<kWaves>(t, red, a.c);
+    MaxSum t{ninf(), 0.0f};
+    if (a.lse || a.segs > 1) t = block_join<kWaves>(run.get(), red, a.c);
     if (a.segs > 1) {
       if (tid < a.k) a.keys[item * a.k + tid] = tid < n ? buf[tid] : 0ull;
       if (tid == 0) {
@@ -1026,7 +1026,7 @@ __global__ __launch_bounds__(kThreads) void k_distill_rows(DistillArgs a) {
           s += ex(xs[v][e]);
           s2 += ex(xs[v][e + 1]);
         }
-      return group_all<L>(s + s2, AddF());
+      return group_all<L>(s + s2, AddF()) * ex.factor();
     };
     const float s = sum_from(ref);
     if (a.lse) {
@@ -1103,9 +1103,8 @@ __global__ __launch_bounds__(kThreads) void k_distill_rows_grad(DistillArgs a) {
     const RowStats& st = in.st;
     const bool skip = in.weight == 0.0f || st.dead();
     const float g = skip || divisor == 0.0f ? 0.0f : in.g / divisor * in.weight * a.temperature;
-    const float co = g * st.coefficient(a.c);
     const Exponent ex(st.base(), a.c);
-    const float shift = ex.shift - st.base_log();
+    const float co = g * st.coefficient(a.c) * ex.factor(st.base_log());
     clear_marks<L, W / 32>(marks, lane);
 #pragma unroll
     for (int v = 0; v < NV; ++v) *(u32x4*)(line + (v * L + lane) * E) = in.x[v];
@@ -1118,7 +1117,7 @@ __global__ __launch_bounds__(kThreads) void k_distill_rows_grad(DistillArgs a) {
       float d[E];
       unpack(in.x[v], d, (const T*)nullptr);
 #pragma unroll
-      for (int e = 0; e < E; ++e) d[e] = co * __builtin_amdgcn_exp2f(fmaf(d[e], ex.c, shift));
+      for (int e = 0; e < E; ++e) d[e] = co * ex(d[e]);
       if (skip) {
 #pragma unroll
         for (int e = 0; e < E; ++e) d[e] = 0.0f;
@@ -1246,7 +1245,7 @@ __global__ __launch_bounds__(kThreads) void k_distill_stream(DistillArgs a) {
       }
       __syncthreads();
     }
-    MaxSum t{ninf(), 0.0f};
+    RunSum run;
     u32x4 next[kWide];
     load_group(x, e0, e1, next);
     for (int i0 = e0; i0 < e1; i0 += kSpan) {
@@ -1266,9 +1265,9 @@ __global__ __launch_bounds__(kThreads) void k_distill_stream(DistillArgs a) {
               if (own >> e & 1) v[u][e] = ninf();
         }
       }
-      add_group<T>(v, t, a.c);
+      add_group<T>(v, run, a.c);
     }
-    t = block_join<kWaves>(t, red, a.c);
+    const MaxSum t = block_join<kWaves>(run.get(), red, a.c);
     if (a.segs == 1) {
       close_row<T>(a, row, w, t, index, red);
     } else if (tid == 0) {
@@ -1317,9 +1316,8 @@ __global__ __launch_bounds__(kThreads) void k_distill_grad(DistillArgs a) {
     T* out = (T*)a.grad + row * a.grad_stride;
     const int e0 = seg * a.seg_len, e1 = min(a.V, e0 + a.seg_len);
     const float g = skip ? 0.0f : row_scale(a, row, w);
-    const float co = g * st.coefficient(a.c);
     const Exponent ex(st.base(), a.c);
-    const float shift = ex.shift - st.base_log();
+    const float co = g * st.coefficient(a.c) * ex.factor(st.base_log());
     int at = -1;
     if (!skip && tid < a.k) {
       at = teacher_index(a, row * a.k + tid);
@@ -1336,7 +1334,7 @@ __global__ __launch_bounds__(kThreads) void k_distill_grad(DistillArgs a) {
       } else {
         unpack(load_row(x, i, e1), d, (const T*)nullptr);
 #pragma unroll
-        for (int e = 0; e < E; ++e) d[e] = co * __builtin_amdgcn_exp2f(fmaf(d[e], ex.c, shift));
+        for (int e = 0; e < E; ++e) d[e] = co * ex(d[e]);
       }
       if (i + E <= e1) {
         store16(out + i, pack(d, (const T*)nullptr));

@@ -155,17 +155,36 @@ struct MaxSum {
 };
 __device__ __forceinline__ float exp_ref(float m) { return m == ninf() ? 0.0f : m; }  // keeps -inf - -inf out of exponents
 __device__ __forceinline__ float exp_of(float x, float ref, float c) { return __builtin_amdgcn_exp2f((x - ref) * c); }
-// The same for many x <= ref as one multiply-add and one exponential each.  Where ref * c is not finite (a row of lowest
-// values) the scale is so small that ref * c is, and still so large that the next value below ref gives 0: temperatures
-// are at least 1e-4, so |ref| is above 2^114 there and floats are at least 2^91 apart.  The instruction gives 0 for results
-// below 2^-126, beside a largest term of 1: no sum feels them, a gradient loses at most 2^-126 of its factor.
+// The same for many x <= ref as one multiply-add and one exponential each: 2^(x c - round(ref c)), which is 2^((x - ref) c) times
+// a factor that all terms of one ref share, 2^rest, rest = ref c - round(ref c).  Half a step of ref c is little beside 1 only
+// while the logits are small (a relative error of 4e-5 at 1000, and at -1e9, which masks are made of, 2^64), so whoever uses
+// the terms multiplies by factor(): once a row, a thread or a tile; the multiply-add that gives `rest` is exact.  From 2^31 on
+// ref c would leave float's range or `rest` the range of the exponential; there floats are so far apart that every other x
+// gives 0 (next * c is at least 2^7 away), as it also does with c a power of two that puts them 2^8 apart; with it ref c is
+// exact and `rest` 0.  The instruction gives 0 for results below 2^-126, beside a largest term of 2^rest: no sum feels them, a
+// gradient loses at most 2^-62 of its factor at rest = -64, 2^-125 in ordinary rows.
 struct Exponent {
-  float c, shift;
+  float c, shift, rest;
   __device__ __forceinline__ Exponent(float ref, float scale) {
-    c = fabsf(ref * scale) < __uint_as_float(0x7F800000u) ? scale : 0x1p-80f;
+    const unsigned far = (286u - (__float_as_uint(ref) >> 23 & 255u)) << 23;  // 2^(32 - exponent of ref)
+    c = fabsf(ref * scale) < 0x1p31f ? scale : __uint_as_float(far);
     shift = -(ref * c);
+    rest = fmaf(ref, c, shift);
   }
   __device__ __forceinline__ float operator()(float x) const { return __builtin_amdgcn_exp2f(fmaf(x, c, shift)); }
+  __device__ __forceinline__ float factor(float log2_divisor = 0.0f) const { return __builtin_amdgcn_exp2f(-(rest + log2_divisor)); }
+};
+// A thread's running sum: of terms as an Exponent of its maximum gives them, times 2^-rest only at the end.
+struct RunSum {
+  float m = ninf(), s = 0.0f, rest = 0.0f;
+  __device__ __forceinline__ Exponent move(float to, float c) {  // to >= m; the terms that follow are those of the result
+    const Exponent ex(exp_ref(to), c);
+    s *= __builtin_amdgcn_exp2f(fmaf(m, ex.c, ex.shift) - rest);  // 1 where the maximum stays
+    m = to;
+    rest = ex.rest;
+    return ex;
+  }
+  __device__ __forceinline__ MaxSum get() const { return {m, s * __builtin_amdgcn_exp2f(-rest)}; }
 };
 __device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, float c) {
   const float m = __builtin_elementwise_maximum(a.m, b.m), r = exp_ref(m);

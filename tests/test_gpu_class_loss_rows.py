@@ -1,0 +1,128 @@
+"""The losses over a set of classes, row by row: bounds that know the distances within a row and not its size
+(tests/class_loss_bounds.py), rows that do not feel their neighbours, and calls that are refused."""
+import math
+
+import pytest
+import torch
+
+import class_loss_bounds as B
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+INF = float("inf")
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def spacing(offset, dtype):
+    """Distance of the type's values on either side of `offset`, the wider one."""
+    return 2.0 ** math.floor(math.log2(abs(offset) * (1 - 1e-9))) * torch.finfo(dtype).eps * 2 if offset else 0.0
+
+
+def shifted(rows, vocab, offset, dtype, seed):
+    """Logits around `offset` that the type holds exactly."""
+    step = max(2.0 ** -6, spacing(offset, dtype))
+    x = torch.round(torch.randn(rows, vocab, generator=gen(seed), dtype=torch.float64) * 2.5 / step).clamp(-50, 50) * step
+    got = (x + offset).to(dtype)
+    assert torch.equal(got.double(), x + offset) or dtype != torch.float32 or step > 64
+    return got
+
+
+def teacher(rows, vocab, k, seed, dtype, offset=0.0):
+    g = gen(seed)
+    at = torch.stack([torch.randperm(vocab, generator=g)[:k] for _ in range(rows)])
+    step = max(2.0 ** -6, spacing(offset, dtype))
+    v = torch.round(torch.randn(rows, k, generator=g, dtype=torch.float64) * 1.5 / step) * step + offset
+    return v.to(dtype), at
+
+
+def check_distill(x, val, idx, lse, t):
+    import mde_amd.vocab_losses as L
+    loss, ltol, grad, gtol = B.distill(x, val, idx, lse, t)
+    a = x.to(DEV).requires_grad_(True)
+    out = L.topk_distillation_loss(a, val.to(DEV), idx.to(DEV), None if lse is None else lse.to(DEV), temperature=t, reduction="none")
+    B.close(out, loss, ltol, "row losses")
+    up = torch.randn(x.shape[0], generator=gen(7))
+    (got,) = torch.autograd.grad(out, a, up.to(DEV))
+    want = grad * up.double()[:, None]
+    flushed = 2.0 ** -125 * t * up.double().abs()[:, None]     # exponentials below 2^-126 come out as 0
+    B.close(got, want, gtol * up.double().abs()[:, None] + (B.HALF_STEP[x.dtype] + 4 * B.U) * want.abs() + B.TINY[x.dtype] + flushed,
+            "gradient")
+
+
+# ------------------------------------------------------------------ a softmax does not feel its row's offset
+SHIFTS = [(0.0, 1.0), (1000.0, 1.0), (-10000.0, 1.0), (0.0, 0.01), (-1.0e9, 1.0), (-1.0e9, 40.0), (-1e30, 1.0)]
+SHAPES = [(5, 9, 4), (7, 128, 8), (6, 200, 20), (5, 300, 12), (4, 900, 33), (3, 2048, 9), (3, 5000, 16), (2, 70001, 64)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("offset,t", SHIFTS)
+@pytest.mark.parametrize("tail", [False, True])
+def test_distillation_does_not_feel_an_offset_of_the_students_logits(offset, t, tail, dtype):
+    if dtype == torch.float16 and abs(offset) > 6e4:
+        offset = math.copysign(6e4, offset)
+    for rows, vocab, k in SHAPES:
+        x = shifted(rows, vocab, offset, dtype, vocab)
+        val, idx = teacher(rows, vocab, k, vocab + k, torch.float32)
+        val = val * min(t, 1.0)
+        lse = (torch.logsumexp(val.double() / t, 1) + 0.1).float() if tail else None
+        check_distill(x, val, idx, lse, t)
+
+
+def exact_operands(rows, vocab, dim, offset, dtype, seed):
+    """hidden, weight, bias whose logits float32 holds exactly whatever the order of the sums: small whole numbers times a power
+    of two, few of a row's features not zero."""
+    g = gen(seed)
+    step = max(0.25, spacing(offset, torch.float32))
+    live = torch.rand(dim, generator=g) < 40.0 / dim
+    h = torch.randint(-1, 2, (rows, dim), generator=g).double() * live
+    w = torch.randint(-3, 4, (vocab, dim), generator=g).double() * step
+    b = torch.full((vocab,), offset, dtype=torch.float64)
+    bias = b.to(dtype)
+    z = h @ w.T + bias.double()
+    assert torch.equal(z.float().double(), z)
+    return h.to(dtype), w.to(dtype), bias, z, torch.randint(vocab, (rows,), generator=g)
+
+
+def check_linear_ce(h, w, b, t, z, z_loss=0.0):
+    import mde_amd.vocab_losses as L
+    dtype, rows, vocab = h.dtype, h.shape[0], w.shape[0]
+    loss, ltol, ds, dtol = B.linear_ce(z, t, z_loss)
+    leaves = [x.to(DEV).requires_grad_(True) for x in (h, w, b)]
+    out = L.linear_cross_entropy(leaves[0], leaves[1], t.to(DEV), leaves[2], z_loss=z_loss, reduction="none")
+    B.close(out, loss, ltol, "row losses")
+    up = torch.randn(rows, generator=gen(8)).double()
+    got = torch.autograd.grad(out, leaves, up.float().to(DEV), retain_graph=True)
+    mean = L.linear_cross_entropy(leaves[0], leaves[1], t.to(DEV), leaves[2], z_loss=z_loss)
+    total = float(loss.sum())
+    assert abs(float(mean.detach()) - total / rows) <= float(ltol.sum()) / rows + 4 * B.U * abs(total) / rows
+    got_mean = torch.autograd.grad(mean, leaves, torch.tensor(3.0, device=DEV))
+    for grads, u in ((got, up.float().double()), (got_mean, torch.full((rows,), 3.0 / rows, dtype=torch.float64))):
+        u = u[:, None]
+        d, half = ds * u, B.HALF_STEP[dtype]
+        largest = float(u.abs().max()) * (1 + 2 * z_loss * float(B.log_sum(z).abs().max()))
+        floor = largest * 2.0 ** -36 if dtype == torch.float16 else 0.0     # its smallest step under a scale of 2^11 at least
+        err = dtol * u.abs() + d.abs() * half * 1.01 + floor
+        n = max(rows, vocab) + 4
+        h6, w6 = h.double(), w.double()
+        for name, g, want, tol in (
+                ("grad hidden", grads[0], d @ w6, err @ w6.abs() + n * B.U * (d.abs() @ w6.abs())),
+                ("grad weight", grads[1], d.T @ h6, err.T @ h6.abs() + n * B.U * (d.abs().T @ h6.abs())),
+                ("grad bias", grads[2], d.sum(0), err.sum(0) + n * B.U * d.abs().sum(0))):
+            B.close(g, want, tol + (half + 8 * B.U) * want.abs() + B.TINY[dtype], name)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("offset", [0.0, 1024.0, -8192.0, -2.0 ** 30, -2.0 ** 100])
+@pytest.mark.parametrize("rows,vocab,dim", [
+    (5, 40, 24), (12, 500, 3000), (40, 3000, 64), (64, 700, 200), (200, 300, 96), (130, 1000, 40), (1030, 4000, 330),
+    (70, 9001, 1003), (2100, 8200, 128)])
+def test_linear_cross_entropy_does_not_feel_an_offset_of_the_logits(rows, vocab, dim, offset, dtype):
+    """Latency sizes, logits in parts of the features, thin, narrow, small and large tiles, float32 directly and by planes."""
+    if dtype == torch.float16 and abs(offset) > 6e4:
+        offset = -2.0 ** 15
+    h, w, b, z, t = exact_operands(rows, vocab, dim, offset, dtype, rows + vocab)
+    check_linear_ce(h, w, b, t, z)
