@@ -804,8 +804,8 @@ __device__ __forceinline__ int teacher_index(const DistillArgs& a, int64_t at) {
   return i < 0 || i >= a.V ? -1 : (int)i;
 }
 
-// log q = v / T - base - log_sum.  The exponent is kept in two floats: rounded to one it would be off by half an ulp of its
-// size, and that error of every q would land in q_t = 1 - sum q, which is small.
+// log q, kept in two floats: rounded to one it would be off by half an ulp of its size, and that error of every q would land
+// in q_t = 1 - sum q, which is small.
 struct LogQ {
   float hi, lo;
   __device__ __forceinline__ float log() const { return hi + lo; }
@@ -817,16 +817,19 @@ struct LogQ {
   }
 };
 struct TeacherSum {
-  float base, log_sum;  // lse and 0 where it is given; the largest value / T and the log of the sum above it otherwise
+  float base, log_sum;  // lse and kWhole where it is given; the largest value itself and the log of the sum above it otherwise
 };
+constexpr float kWhole = -1.0f;  // a log of a sum whose largest term is 1 is not negative
+// v / T - lse, or (v - largest) / T - log_sum: the difference comes first where there is one, since the largest value / T,
+// rounded, would be off by half an ulp of its own size in every q
 __device__ __forceinline__ LogQ log_q(const DistillArgs& a, float v, TeacherSum t) {
   if (v == ninf()) return {ninf(), 0.0f};
-  const float p = __fmul_rn(v, a.ih);
-  const float pe = fmaf(v, a.il, fmaf(v, a.ih, -p));
-  const float s = __fsub_rn(p, t.base), b = __fsub_rn(s, p);
-  const float err = __fadd_rn(__fsub_rn(p, __fsub_rn(s, b)), __fsub_rn(-t.base, b));
-  const float h = __fsub_rn(s, t.log_sum), g = __fsub_rn(h, s);
-  return {h, pe + err + __fadd_rn(__fsub_rn(s, __fsub_rn(h, g)), __fsub_rn(-t.log_sum, g))};
+  const bool whole = t.log_sum < 0.0f;
+  const float x = whole ? v : v - t.base, base = whole ? t.base : t.log_sum;
+  const float p = __fmul_rn(x, a.ih);
+  const float pe = fmaf(x, a.il, fmaf(x, a.ih, -p));
+  const float s = __fsub_rn(p, base), b = __fsub_rn(s, p);
+  return {s, pe + __fadd_rn(__fsub_rn(p, __fsub_rn(s, b)), __fsub_rn(-base, b))};
 }
 
 // weight of a row, its share of the upstream gradient and the factor T of the derivative
@@ -973,7 +976,7 @@ __global__ __launch_bounds__(kThreads) void k_distill_rows(DistillArgs a) {
       for (int e = 0; e < E; ++e) all.m = __builtin_elementwise_maximum(all.m, xs[v][e]);
     }
     __builtin_amdgcn_wave_barrier();
-    TeacherSum teacher{in.lse, 0.0f};
+    TeacherSum teacher{in.lse, kWhole};
     if (!a.lse) {
       MaxSum t{ninf(), 0.0f};
       in.each(a, row, lane, k, [&](int, int, float v) { t.m = __builtin_elementwise_maximum(t.m, v); });
@@ -981,7 +984,7 @@ __global__ __launch_bounds__(kThreads) void k_distill_rows(DistillArgs a) {
       const float ref = exp_ref(t.m);
       in.each(a, row, lane, k, [&](int, int, float v) { t.s += exp_of(v, ref, a.c); });
       t.s = group_all<L>(t.s, AddF());
-      teacher = {t.m * a.ih, log2_sum(t) * kLn2};
+      teacher = {t.m, log2_sum(t) * kLn2};
     }
     all.m = group_all<L>(all.m, MaxF());
     const float ref = exp_ref(all.m);
@@ -1171,10 +1174,10 @@ __device__ __forceinline__ void close_row(const DistillArgs& a, int64_t row, flo
   if (mine) index[tid] = at;
   TeacherSum teacher;
   if (a.lse) {
-    teacher = {a.lse[row], 0.0f};
+    teacher = {a.lse[row], kWhole};
   } else {
     const MaxSum t = block_join<kWaves>({value, value == ninf() ? 0.0f : 1.0f}, red, a.c);
-    teacher = {t.m * a.ih, log2_sum(t) * kLn2};
+    teacher = {t.m, log2_sum(t) * kLn2};
   }
   const bool bad = __syncthreads_or(mine && at < 0);
   bool first = mine && at >= 0;

@@ -75,7 +75,8 @@ def distill(x, values, indices, lse=None, temperature=1.0):
     logp = torch.log_softmax(z, 1)
     p = logp.exp()
     e_all = log_sum_error(z, stream_sum(vocab))[:, None]
-    logq = v - (torch.logsumexp(v, 1, keepdim=True) if lse is None else lse.double()[:, None])
+    # (float64 has no room for the logarithm of k beside a value of 1e30)
+    logq = torch.log_softmax(v - v.max(1, keepdim=True).values, 1) if lse is None else v - lse.double()[:, None]
     q = logq.exp()
     mass = q.sum(1, keepdim=True)
     k = values.shape[1]

@@ -54,7 +54,8 @@ def check_distill(x, val, idx, lse, t):
 
 
 # ------------------------------------------------------------------ a softmax does not feel its row's offset
-SHIFTS = [(0.0, 1.0), (1000.0, 1.0), (-10000.0, 1.0), (0.0, 0.01), (-1.0e9, 1.0), (-1.0e9, 40.0), (-1e30, 1.0)]
+SMALL = torch.tensor(0.01).item()                           # a temperature is a float32 in the library
+SHIFTS = [(0.0, 1.0), (1000.0, 1.0), (-10000.0, 1.0), (0.0, SMALL), (-1.0e9, 1.0), (-1.0e9, 40.0), (-1e30, 1.0)]
 SHAPES = [(5, 9, 4), (7, 128, 8), (6, 200, 20), (5, 300, 12), (4, 900, 33), (3, 2048, 9), (3, 5000, 16), (2, 70001, 64)]
 
 
@@ -70,6 +71,19 @@ def test_distillation_does_not_feel_an_offset_of_the_students_logits(offset, t, 
         val = val * min(t, 1.0)
         lse = (torch.logsumexp(val.double() / t, 1) + 0.1).float() if tail else None
         check_distill(x, val, idx, lse, t)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("offset,t", SHIFTS)
+def test_distillation_does_not_feel_an_offset_of_the_teachers_values(offset, t, dtype):
+    if dtype == torch.float16 and abs(offset) > 6e4:
+        offset = math.copysign(6e4, offset)
+    for rows, vocab, k in SHAPES:
+        x = shifted(rows, vocab, 0.0, torch.float32, vocab) * min(t, 1.0)
+        val, idx = teacher(rows, vocab, k, vocab + k, dtype, offset)
+        check_distill(x, val, idx, None, t)
+        if abs(offset) <= 1e4:                              # above, a float32 log sum holds no digit of the teacher's rest
+            check_distill(x, val, idx, (torch.logsumexp(val.double() / t, 1) + 0.1).float(), t)
 
 
 def exact_operands(rows, vocab, dim, offset, dtype, seed):
