@@ -1035,14 +1035,15 @@ __global__ __launch_bounds__(kThreads) void k_distill_rows(DistillArgs a) {
     if (a.lse) {
       all.s = group_all<L>(seen, AddF()) + s;
       rest = {s == 0.0f ? ninf() : all.m, s};
-      if (__any(s < 1e-20f)) {  // far below the teacher's classes: their sum from their own maximum
+      if (__any(s < 1e-20f)) {  // far below the teacher's classes: their sum from their own maximum, in the rows concerned
         float m = ninf();
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
           for (int e = 0; e < E; ++e) m = __builtin_elementwise_maximum(m, xs[v][e]);
-        rest.m = group_all<L>(m, MaxF());
-        rest.s = sum_from(exp_ref(rest.m));
+        m = group_all<L>(m, MaxF());
+        const float own = sum_from(exp_ref(m));
+        if (s < 1e-20f) rest = {m, own};  // the row's bits do not depend on the rows that share its wave
       }
     } else {
       all.s = s;

@@ -140,3 +140,42 @@ def test_linear_cross_entropy_does_not_feel_an_offset_of_the_logits(rows, vocab,
         offset = -2.0 ** 15
     h, w, b, z, t = exact_operands(rows, vocab, dim, offset, dtype, rows + vocab)
     check_linear_ce(h, w, b, t, z)
+
+
+# ------------------------------------------------------------------ rows beside other rows
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [12, 60, 128, 250, 500, 1000])
+def test_a_row_has_the_same_bits_alone_and_beside_any_other(vocab, dtype):
+    """Up to eight rows share a wave: ordinary ones beside rows whose rest class vanishes, is empty or masked, that are not
+    looked at, repeat an index or hold a NaN."""
+    import mde_amd.vocab_losses as L
+    rows, k = 16, 5
+    x = shifted(rows, vocab, 0.0, dtype, vocab + 1)
+    val, idx = teacher(rows, vocab, k, vocab + 2, torch.float32)
+    lse = (torch.logsumexp(val.double(), 1) + 0.1).float()
+    weights = torch.ones(rows)
+    at = torch.arange(rows)[:, None]
+    x[at, idx[:, :1]] += 3                                  # the student follows: the largest logit is not the rest's
+    x[at[1::8], idx[1::8]] += 60                            # the rest class vanishes
+    keep = torch.zeros(rows, vocab, dtype=torch.bool).scatter_(1, idx, True)
+    x[2::8] = torch.where(keep[2::8], x[2::8], torch.full_like(x[2::8], -INF))     # is empty
+    weights[3::8] = 0.0
+    x[4::8] = -INF
+    idx[5::8, 1] = idx[5::8, 0]
+    x[6::8, 0] = float("nan")
+
+    def step(pick):
+        for tail in (lse[pick].to(DEV), None):
+            a = x[pick].to(DEV).requires_grad_(True)
+            out = L.topk_distillation_loss(a, val[pick].to(DEV), idx[pick].to(DEV), tail, weights=weights[pick].to(DEV),
+                                           reduction="none")
+            (g,) = torch.autograd.grad(out, a, torch.ones(len(pick), device=DEV))
+            yield out.detach().cpu(), g.cpu()
+        top = L.top_logits(x[pick].to(DEV), k)
+        yield top.lse.cpu(), top.values.cpu()
+
+    together = list(step(list(range(rows))))
+    for r in range(rows):
+        for (loss, grad), (loss1, grad1) in zip(together, step([r])):
+            for name, a, b in (("loss", loss[r], loss1[0]), ("gradient", grad[r], grad1[0])):
+                assert torch.equal(torch.nan_to_num(a.float(), nan=7e4), torch.nan_to_num(b.float(), nan=7e4)), (name, r)
