@@ -473,7 +473,8 @@ int vsl_distill_bwd(const vsl_distill_desc* desc, const float* stats, const floa
  *   row loss = lse - z[target] + z_loss * lse^2,  lse = log sum exp z;  rows with target == ignore_index count nothing.
  * hidden [rows,dim], weight [vocab,dim], bias [vocab] or NULL, all of one type; target [rows].  Products run on the
  * matrix cores with float32 accumulation; in the backward call the derivative of a logit is rounded to the operands'
- * type before it meets weight and hidden (scaled by its largest value, so that float16 keeps it).
+ * type before it meets weight and hidden (scaled, so that float16 keeps it: by the row's largest for grad_hidden, by the
+ * largest of all for grad_weight and grad_bias).  grad_hidden of a row depends on nothing but that row.
  * A class whose bias is -infinity is masked out, whatever its weights hold.
  *
  * vsl_linear_ce_fwd: row_loss [rows] (scratch unless VSL_REDUCE_NONE); stats [2][rows], the maximum of a row's logits and the log2 of its sum of

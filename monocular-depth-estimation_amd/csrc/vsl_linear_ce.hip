@@ -311,7 +311,9 @@ struct LogitArgs {
   float* target_logit; // [rows]
   // backward
   const float* stats;  // [2][rows] maximum and log2 of the sum above it
-  const float* row_scale;  // NULL: `unit` for every row that counts
+  const float* row_scale;  // kRowDerivatives; otherwise `unit` for every row that counts
+  const float* row_size;   // what the row's scale was divided by; out_scale: the largest of them
+  const float* out_scale;
   float unit;
   int64_t ignore_index;
   float z_loss;
@@ -368,8 +370,10 @@ __device__ __forceinline__ float take_plane(float& z) {
 // T: the tensors' type; SPLIT: float32 by planes of bfloat16.  8192 x 131072 x 4096 bfloat16: forward 6.7 ms, 1305 TFLOP/s,
 // derivatives 8 x 0.99 ms, 1110; bound by the matrix instructions at the power the card allows, then by the epilogue's
 // exponentials, which no other tile's products cover (a large tile fills its CU).  2011 x 32003 x 1000 float16: 165 and 206 us.
-template <typename T, typename S, bool DELTA, bool SPLIT, int FORM>
+enum { kStatistics, kDerivatives, kRowDerivatives };  // of the logits; derivatives of one gradient, or of one per row
+template <typename T, typename S, int WHAT, bool SPLIT, int FORM>
 __global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
+  constexpr bool DELTA = WHAT != kStatistics, ROWS = WHAT == kRowDerivatives;
   typedef std::conditional_t<SPLIT, __bf16, T> O;
   __shared__ __attribute__((aligned(16))) char lds[S::kLds];
   const int tm_count = (a.op.M + S::BM - 1) / S::BM, tn_count = (a.op.N + S::BN - 1) / S::BN;
@@ -424,9 +428,10 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
     } else {
       const float top = live ? a.stats[row] : ninf(), ls = live ? a.stats[a.op.N + row] : 0.0f;
       const float scale = !live || top == ninf() || target + a.class0 == a.ignore_index ? 0.0f
-                          : a.row_scale ? a.row_scale[row] : a.unit;
+                          : ROWS ? a.row_scale[row] : a.unit;
       const Exponent ex(top, kLog2e);
       const float factor = scale * slope_of(a.z_loss, top, ls) * ex.factor(ls);
+      const float ratio = ROWS && live ? a.row_size[row] / *a.out_scale : 1.0f;  // a power of two
       O* d = (O*)a.delta + (int64_t)row * a.ldd;
 #pragma unroll
       for (int i = 0; i < S::IM; ++i) {
@@ -453,7 +458,7 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
               if (a.delta) *(f32x4*)(d + v0) = f32x4{z[r], z[r + 1], z[r + 2], z[r + 3]};
               if (a.delta_t)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) ((O*)a.delta_t)[(int64_t)(v0 + e) * a.ldt + row] = z[r + e];
+                for (int e = 0; e < 4; ++e) ((O*)a.delta_t)[(int64_t)(v0 + e) * a.ldt + row] = z[r + e] * ratio;
             }
           } else {
 #pragma unroll
@@ -475,10 +480,19 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
                 *(u32x4*)(d + plane * a.plane_d + v32 + 16 * r8 + 8 * half) = u32x4{x[0], y[0], x[1], y[1]};
               }
               if (a.delta_t) {
+                uint2 t[2] = {p0, p1};
+                if (ROWS) {
+#pragma unroll
+                  for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) g[u][e] *= ratio;
+                    t[u] = pack4<O>(g[u]);
+                  }
+                }
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                   const int v = v32 + 16 * r8 + 8 * u + 4 * half + (lane & 3);
-                  *(uint2*)((O*)a.delta_t + (int64_t)v * a.ldt + plane * a.rows_padded + (row & ~3)) = transpose4(u ? p1 : p0);
+                  *(uint2*)((O*)a.delta_t + (int64_t)v * a.ldt + plane * a.rows_padded + (row & ~3)) = transpose4(t[u]);
                 }
               }
             }
@@ -585,12 +599,15 @@ __global__ __launch_bounds__(THREADS) void k_ce_rows(const float2* __restrict__ 
 // backward: scales of the rows
 // ------------------------------------------------------------------------------------------------------------------
 // What the products are multiplied by at the end.  Where every row has the same gradient g, the derivatives are made for
-// a gradient of `unit` and this is g / unit; where they differ (one per row, or by z_loss) the derivatives are made for
-// gradients scaled so that the largest becomes `unit`, and this is that largest / unit.
+// a gradient of `unit` and this is g / unit.  Where they differ (one per row, or by z_loss) a row's derivatives are made for
+// its own gradient over a power of two, its size, which puts the largest of them between unit and 2 unit.  grad_hidden's rows
+// are multiplied by their sizes again: nothing of a row, however small its gradient, infinite or NaN, meets another's.  The
+// other two gradients add up rows: there the derivatives are scaled to the largest size of all, and this is that size.
 struct OutScale {
   const float* g_loss;    // NULL: `given` holds the scale
   const float* divisor;   // NULL: 1
   const float* given;
+  const float* rows;      // not NULL: one for every row of the output
   float unit;
   __device__ __forceinline__ float gradient() const {
     if (!divisor) return *g_loss;
@@ -606,17 +623,26 @@ struct ScaleArgs {
   const int64_t* target;
   int64_t ignore_index, rows, rows_padded;
   bool per_row;          // g_loss holds one gradient per row
-  float z_loss, unit;    // unit: what the largest derivative is scaled to
+  float z_loss, unit;
   float* partial;        // maxima of the blocks of k_ce_largest
   int partials;
   float* row_scale;      // [rows_padded]
+  float* row_size;       // [rows_padded]
   float* out_scale;      // one float
 };
 __device__ __forceinline__ float row_gradient(const ScaleArgs& a, int64_t row) {
   if (a.target[row] == a.ignore_index || a.stats[row] == ninf()) return 0.0f;
-  const OutScale g{a.g_loss + (a.per_row ? row : 0), a.divisor, nullptr, 1.0f};
+  const OutScale g{a.g_loss + (a.per_row ? row : 0), a.divisor, nullptr, nullptr, 1.0f};
   return g.gradient();
 }
+// size of a row's largest derivative, 0 where it has none that is finite
+__device__ __forceinline__ float row_largest(const ScaleArgs& a, int64_t row, float g) {
+  if (!(fabsf(g) < __uint_as_float(0x7F800000u))) return 0.0f;
+  const float slope = fabsf(slope_of(a.z_loss, a.stats[row], a.stats[a.rows + row]));  // NaN in a row of NaN
+  return fminf(fabsf(g) * fmaxf(1.0f, slope), __uint_as_float(0x7F7FFFFFu));
+}
+// (below 2^-100 sizes stay there: a gradient of 2^-149 still keeps its bits, and sizes over unit stay normal numbers)
+__device__ __forceinline__ int exponent_of(float x) { return x == 0.0f ? 0 : max(ilogbf(x), -100); }
 __device__ __forceinline__ float block_max(float v, float* red) {
   v = group_all<64>(v, MaxF());
   __syncthreads();
@@ -628,23 +654,23 @@ __device__ __forceinline__ float block_max(float v, float* red) {
 __global__ __launch_bounds__(kThreads) void k_ce_largest(ScaleArgs a) {
   __shared__ float red[4];
   float m = 0.0f;
-  for (int64_t r = (int64_t)blockIdx.x * kThreads + threadIdx.x; r < a.rows; r += (int64_t)gridDim.x * kThreads) {
-    const float g = row_gradient(a, r);
-    if (g != 0.0f)
-      m = __builtin_elementwise_maximum(m, fabsf(g) * fmaxf(1.0f, fabsf(slope_of(a.z_loss, a.stats[r], a.stats[a.rows + r]))));
-  }
+  for (int64_t r = (int64_t)blockIdx.x * kThreads + threadIdx.x; r < a.rows; r += (int64_t)gridDim.x * kThreads)
+    m = fmaxf(m, row_largest(a, r, row_gradient(a, r)));
   m = block_max(m, red);
   if (threadIdx.x == 0) a.partial[blockIdx.x] = m;
 }
 __global__ __launch_bounds__(kThreads) void k_ce_scale(ScaleArgs a) {
   __shared__ float red[4];
-  const float largest = block_max((int)threadIdx.x < a.partials ? a.partial[threadIdx.x] : 0.0f, red);
+  const int all = exponent_of(block_max((int)threadIdx.x < a.partials ? a.partial[threadIdx.x] : 0.0f, red));
   const int64_t r = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   if (r < a.rows_padded) {
     const float g = r < a.rows ? row_gradient(a, r) : 0.0f;
-    a.row_scale[r] = g == 0.0f ? 0.0f : g / largest * a.unit;
+    const float largest = r < a.rows ? row_largest(a, r, g) : 0.0f;
+    const int own = largest == 0.0f ? all : exponent_of(largest);
+    a.row_scale[r] = ldexpf(g, -own) * a.unit;
+    a.row_size[r] = ldexpf(1.0f, own) / a.unit;
   }
-  if (r == 0) *a.out_scale = largest / a.unit;
+  if (r == 0) *a.out_scale = ldexpf(1.0f, all) / a.unit;
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -843,7 +869,10 @@ __device__ __forceinline__ void store_tile(const GradArgs& a, int m0, int n0, co
   constexpr int E = Kind<T>::E, kPieces = kWide / E;  // of a row
   static_assert(kWide * S::BN * (int)sizeof(T) <= S::kLds && kPieces >= 16 && S::WM % kHalves == 0, "tile through LDS");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
-  const float scale = a.scale.get();
+  float scale[S::JN];
+#pragma unroll
+  for (int j = 0; j < S::JN; ++j)
+    scale[j] = a.scale.rows ? a.scale.rows[min(n0 + (wn * S::JN + j) * 32 + (lane & 31), a.op.N - 1)] : a.scale.get();
 #pragma unroll
   for (int h = 0; h < kHalves; ++h) {
     if (h) __syncthreads();
@@ -858,7 +887,7 @@ __device__ __forceinline__ void store_tile(const GradArgs& a, int m0, int n0, co
             const int m = (wm * S::IM + i) * 32 - h * kWide + 8 * r4 + 4 * (lane >> 5);
             float g[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) g[e] = scale * t.acc[i][j][4 * r4 + e];
+            for (int e = 0; e < 4; ++e) g[e] = scale[j] * t.acc[i][j][4 * r4 + e];
             char* p = lds + (n * kPieces + ((m / E) ^ (n & 15))) * 16;
             if constexpr (sizeof(T) == 4) *(f32x4*)p = f32x4{g[0], g[1], g[2], g[3]};
             else *(uint2*)(p + 8 * (lane >> 5)) = pack4<T>(g);
@@ -934,19 +963,21 @@ struct FinishJob {
   int splits;
   int64_t n;
   int64_t blocks;
+  const float* row_scale;  // ROWS: of rows of `width` elements, otherwise jobs' scale
+  int64_t width;
 };
 struct FinishJobs {
   FinishJob job[3];
   OutScale scale;
 };
-template <typename T>
+template <typename T, bool ROWS>
 __global__ __launch_bounds__(kThreads) void k_ce_finish(FinishJobs jobs) {
   __shared__ f32x4 part[3][64];
   int64_t block = blockIdx.x;
   int which = 0;
   while (block >= jobs.job[which].blocks) block -= jobs.job[which++].blocks;  // the grid is the sum of the jobs' blocks
   const FinishJob& j = jobs.job[which];
-  const float scale = jobs.scale.get();
+  const float scale = ROWS ? 0.0f : jobs.scale.get();
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   auto sum = [&](int64_t i, int s0, int s1) {
     f32x4 v{0.0f, 0.0f, 0.0f, 0.0f};
@@ -964,7 +995,7 @@ __global__ __launch_bounds__(kThreads) void k_ce_finish(FinishJobs jobs) {
   auto store = [&](int64_t i, const f32x4& v) {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (i + e < j.n) ((T*)j.out)[i + e] = (T)(scale * v[e]);
+      if (i + e < j.n) ((T*)j.out)[i + e] = (T)((ROWS ? j.row_scale[(i + e) / j.width] : scale) * v[e]);
   };
   if (j.splits < kDealtSplits) {
     for (int64_t i = (block * kThreads + threadIdx.x) * 4; i < j.n; i += j.blocks * kThreads * 4) store(i, sum(i, 0, j.splits));
@@ -1121,7 +1152,7 @@ __global__ __launch_bounds__(kThreads) void k_ce_parts_delta(Parts z, LogitArgs 
       if (v == target) d -= scale;
     }
     if (a.delta) ((T*)a.delta)[row * a.ldd + v] = (T)d;
-    tile[y + 4 * u][x] = d;
+    tile[y + 4 * u][x] = live && a.row_scale ? d * (a.row_size[row] / *a.out_scale) : d;
   }
   if (!a.delta_t) return;
   __syncthreads();
@@ -1324,7 +1355,7 @@ struct Backward {
   int64_t piece, pieces, vocab_padded;
   Plan plan_h, plan_w;
   void *hidden, *weight, *hidden_t, *weight_t, *delta, *delta_t;
-  float *sum_h, *sum_w, *sum_b, *row_scale, *out_scale, *largest, *parts;
+  float *sum_h, *sum_w, *sum_b, *row_scale, *row_size, *out_scale, *largest, *parts;
   size_t total;
 };
 Backward backward_workspace(const vsl_linear_ce_desc* d, uint32_t mask, void* base) {
@@ -1360,6 +1391,7 @@ Backward backward_workspace(const vsl_linear_ce_desc* d, uint32_t mask, void* ba
   b.sum_w = gw && b.plan_w.splits > 1 ? (float*)a.take((size_t)b.plan_w.splits * b.piece * d->dim * 4) : nullptr;
   b.sum_b = gb && d->rows >= 8192 && d->vocab <= kBiasBlocks / 2 ? (float*)a.take(kBiasBlocks * 4) : nullptr;
   b.row_scale = (float*)a.take((size_t)b.l.rows_padded * 4);
+  b.row_size = (float*)a.take((size_t)b.l.rows_padded * 4);
   b.out_scale = (float*)a.take(4);
   b.largest = (float*)a.take(256 * 4);
   b.parts = b.l.logits.splits > 1 ? (float*)a.take((size_t)b.l.logits.splits * d->rows * d->vocab * 4) : nullptr;
@@ -1396,36 +1428,36 @@ struct FinishLaunch {
   FinishJobs jobs{};
   int n = 0;
   int64_t blocks = 0;
-  void add(const float* sum, int splits, int64_t elements, void* out) {
+  void add(const float* sum, int splits, int64_t elements, void* out, const float* row_scale = nullptr, int64_t width = 1) {
     const int64_t b = ceil_div(elements, splits < kDealtSplits ? 4 * kThreads : kThreads);
-    jobs.job[n++] = {sum, out, splits, elements, b < 65536 ? b : 65536};
+    jobs.job[n++] = {sum, out, splits, elements, b < 65536 ? b : 65536, row_scale, width};
     blocks += jobs.job[n - 1].blocks;
   }
-  template <typename T>
+  template <typename T, bool ROWS = false>
   void run(const OutScale& scale, hipStream_t s) {
     jobs.scale = scale;
-    if (n) hipLaunchKernelGGL(k_ce_finish<T>, dim3((unsigned)blocks), dim3(kThreads), 0, s, jobs);
+    if (n) hipLaunchKernelGGL((k_ce_finish<T, ROWS>), dim3((unsigned)blocks), dim3(kThreads), 0, s, jobs);
   }
 };
 
-template <typename T, typename S, bool DELTA, bool SPLIT, int FORM>
+template <typename T, typename S, int WHAT, bool SPLIT, int FORM>
 int launch_logits_as(const LogitArgs& a, hipStream_t s) {
   const int64_t tm = ceil_div(a.op.M, S::BM), tn = ceil_div(a.op.N, S::BN);
-  hipLaunchKernelGGL((k_ce_logits<T, S, DELTA, SPLIT, FORM>), dim3((unsigned)(tm * tn)), dim3(S::kThreads), 0, s, a);
+  hipLaunchKernelGGL((k_ce_logits<T, S, WHAT, SPLIT, FORM>), dim3((unsigned)(tm * tn)), dim3(S::kThreads), 0, s, a);
   return (int)tm;
 }
-template <typename T, bool DELTA, bool SPLIT>
+template <typename T, int WHAT, bool SPLIT>
 int launch_logits(const LogitArgs& a, int shape, bool staged, hipStream_t s) {  // returns the rows of tiles
   if constexpr (!SPLIT)
     if (staged)
-      return shape == kThin     ? launch_logits_as<T, Thin, DELTA, SPLIT, kStagedRows>(a, s)
-             : shape == kNarrow ? launch_logits_as<T, Narrow, DELTA, SPLIT, kStagedRows>(a, s)
-                                : launch_logits_as<T, Small, DELTA, SPLIT, kStagedRows>(a, s);
+      return shape == kThin     ? launch_logits_as<T, Thin, WHAT, SPLIT, kStagedRows>(a, s)
+             : shape == kNarrow ? launch_logits_as<T, Narrow, WHAT, SPLIT, kStagedRows>(a, s)
+                                : launch_logits_as<T, Small, WHAT, SPLIT, kStagedRows>(a, s);
   if constexpr (sizeof(T) == 2 || SPLIT)
-    if (shape == kLarge) return launch_logits_as<T, Large, DELTA, SPLIT, kDirect>(a, s);
-  if (shape == kThin) return launch_logits_as<T, Thin, DELTA, SPLIT, kDirect>(a, s);
-  if (shape == kNarrow) return launch_logits_as<T, Narrow, DELTA, SPLIT, kDirect>(a, s);
-  return launch_logits_as<T, Small, DELTA, SPLIT, kDirect>(a, s);
+    if (shape == kLarge) return launch_logits_as<T, Large, WHAT, SPLIT, kDirect>(a, s);
+  if (shape == kThin) return launch_logits_as<T, Thin, WHAT, SPLIT, kDirect>(a, s);
+  if (shape == kNarrow) return launch_logits_as<T, Narrow, WHAT, SPLIT, kDirect>(a, s);
+  return launch_logits_as<T, Small, WHAT, SPLIT, kDirect>(a, s);
 }
 template <typename T, typename S, bool SPLIT, int FORM = kDirect>
 void launch_grad_as(const GradArgs* g, int n, hipStream_t s) {
@@ -1501,7 +1533,7 @@ void run_forward(const vsl_linear_ce_desc* d, const Forward& f, float* row_loss,
     }
   a.partial = f.partial;
   a.target_logit = f.target_logit;
-  const int tiles = launch_logits<T, false, SPLIT>(a, l.logits.shape, l.staged, s);
+  const int tiles = launch_logits<T, kStatistics, SPLIT>(a, l.logits.shape, l.staged, s);
   // few rows: more lanes each, so that no lane walks many tiles (16 rows of 512 tiles: 14 us with 16 lanes a row); many rows:
   // more of them a block, so that fewer sums are left
   auto rows = [&](auto kernel, int per_block, int threads) {
@@ -1528,7 +1560,8 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
   const float* mean_of = d->reduction == VSL_REDUCE_MEAN ? divisor : nullptr;
   const bool uniform = d->reduction != VSL_REDUCE_NONE && d->z_loss == 0.0f;
   const float* row_scale = uniform ? nullptr : b.row_scale;
-  const OutScale scale = uniform ? OutScale{g_loss, mean_of, nullptr, unit} : OutScale{nullptr, nullptr, b.out_scale, unit};
+  const float* row_size = uniform ? nullptr : b.row_size;
+  const OutScale scale = uniform ? OutScale{g_loss, mean_of, nullptr, nullptr, unit} : OutScale{nullptr, nullptr, b.out_scale, nullptr, unit};
   if (!uniform) {
     ScaleArgs sc{};
     sc.g_loss = g_loss;
@@ -1542,6 +1575,7 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
     sc.z_loss = d->z_loss;
     sc.unit = unit;
     sc.row_scale = b.row_scale;
+    sc.row_size = b.row_size;
     sc.out_scale = b.out_scale;
     const int64_t n = ceil_div(d->rows, kThreads);
     sc.partial = b.largest;
@@ -1579,6 +1613,8 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
     a.rows_padded = l.rows_padded;
     a.stats = stats;
     a.row_scale = row_scale;
+    a.row_size = row_size;
+    a.out_scale = b.out_scale;
     a.unit = unit;
     a.ignore_index = d->ignore_index;
     a.z_loss = d->z_loss;
@@ -1595,10 +1631,13 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
                            0, s, Parts{b.parts, l.logits.splits, d->rows, d->vocab, d->bias}, a);
         made = true;
       }
-    if (!made) launch_logits<T, true, SPLIT>(a, shape, l.staged, s);
+    if (!made) {
+      if (uniform) launch_logits<T, kDerivatives, SPLIT>(a, shape, l.staged, s);
+      else launch_logits<T, kRowDerivatives, SPLIT>(a, shape, l.staged, s);
+    }
     GradArgs g[2] = {};
     int shapes[2], n = 0;
-    FinishLaunch finish;
+    FinishLaunch finish, finish_rows;
     if (grad_hidden) {
       g[n].op = {(const O*)b.weight_t + v0, b.delta, l.planes * b.vocab_padded, l.planes * b.piece, (int)d->dim, (int)d->rows,
                  (int)(padded / Kind<O>::BK), b.vocab_padded, b.piece, 8, 0};
@@ -1606,6 +1645,7 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
       g[n].sum = b.sum_h;
       g[n].out = grad_hidden;
       g[n].scale = scale;
+      g[n].scale.rows = row_size;
       g[n].splits = b.plan_h.splits;
       shapes[n++] = b.plan_h.shape;
       if (b.columns) {
@@ -1615,7 +1655,8 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
         g[0].whole = d->dim % 4 == 0;
         g[0].op.bias = d->bias ? (const T*)d->bias + v0 : nullptr;
       }
-      if (b.sum_h && p == b.pieces - 1) finish.add(b.sum_h, b.plan_h.splits, d->rows * d->dim, grad_hidden);
+      if (b.sum_h && p == b.pieces - 1)
+        (uniform ? finish : finish_rows).add(b.sum_h, b.plan_h.splits, d->rows * d->dim, grad_hidden, row_size, d->dim);
     }
     if (grad_weight) {
       g[n].op = {b.hidden_t, b.delta_t, l.planes * l.rows_padded, l.planes * l.rows_padded, (int)d->dim, (int)classes,
@@ -1650,6 +1691,7 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
       if (parts > 1) finish.add(b.sum_b, parts, classes, grad_bias + v0);
     }
     finish.run<T>(scale, s);
+    finish_rows.run<T, true>(scale, s);
   }
 }
 

@@ -179,3 +179,56 @@ def test_a_row_has_the_same_bits_alone_and_beside_any_other(vocab, dtype):
         for (loss, grad), (loss1, grad1) in zip(together, step([r])):
             for name, a, b in (("loss", loss[r], loss1[0]), ("gradient", grad[r], grad1[0])):
                 assert torch.equal(torch.nan_to_num(a.float(), nan=7e4), torch.nan_to_num(b.float(), nan=7e4)), (name, r)
+
+
+SIZES = [(5, 40, 24, False), (12, 500, 3000, True), (40, 3000, 64, True), (200, 300, 96, False), (1030, 4000, 330, True),
+         (70, 9001, 1003, True), (2100, 8200, 128, False)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab,dim,bias", SIZES)
+@pytest.mark.parametrize("bad", [INF, -INF, float("nan")])
+def test_a_gradient_that_is_not_finite_stays_in_its_row(rows, vocab, dim, bias, bad, dtype):
+    import mde_amd.vocab_losses as L
+    h, w, b, _, t = exact_operands(rows, vocab, dim, 0.0, dtype, 5)
+    leaves = [x.to(DEV).requires_grad_(True) for x in ((h, w, b) if bias else (h, w))]
+    for z_loss in (0.0, 1e-2):
+        out = L.linear_cross_entropy(leaves[0], leaves[1], t.to(DEV), leaves[2] if bias else None, z_loss=z_loss, reduction="none")
+        up = torch.randn(rows, generator=gen(3)).to(DEV)
+        want = torch.autograd.grad(out, leaves, up, retain_graph=True)
+        worse = up.clone()
+        worse[2] = bad
+        got = torch.autograd.grad(out, leaves, worse)
+        others = torch.arange(rows, device=DEV) != 2
+        assert bool(torch.isfinite(want[0]).all()) and torch.equal(got[0][others], want[0][others])
+        assert not torch.isfinite(got[0][2]).any()
+        assert not any(torch.isfinite(g).any() for g in got[1:])      # sums over all rows
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab,dim,bias", SIZES)
+def test_rows_of_very_different_gradients_keep_their_digits(rows, vocab, dim, bias, dtype):
+    """Powers of two between 2^-30 and 2^15 (float16: results down to its subnormal numbers), 2^-110 and 2^15: a row's
+    grad_hidden is the one of a gradient of 1, times its own."""
+    import mde_amd.vocab_losses as L
+    h, w, b, _, t = exact_operands(rows, vocab, dim, 0.0, dtype, 6)
+    leaves = [x.to(DEV).requires_grad_(True) for x in ((h, w, b) if bias else (h, w))]
+    out = L.linear_cross_entropy(leaves[0], leaves[1], t.to(DEV), leaves[2] if bias else None, reduction="none")
+    (ones,) = torch.autograd.grad(out, leaves[:1], torch.ones(rows, device=DEV), retain_graph=True)
+    low = -30 if dtype == torch.float16 else -110
+    power = torch.randint(low, 16, (rows,), generator=gen(4))
+    power[0], power[1] = 15, low
+    up = torch.tensor([2.0 ** p for p in power.tolist()], device=DEV)      # exactly (torch.ldexp is off by a step there)
+    got = torch.autograd.grad(out, leaves, up)
+    want = ones.double() * up.double()[:, None]
+    if dtype != torch.float16:
+        # a power of two changes no digit of a normal number; below 2^-126 the type's step is fixed and a result is rounded to
+        # it (float32: half a step; bfloat16: after float32's, half a step of its own and 2^-150), less than one step
+        small = want.abs() < 2.0 ** -126
+        assert torch.equal(got[0].double()[~small], want[~small])
+        B.close(got[0].double()[small], want[small], B.TINY[dtype], "subnormal results")
+        return
+    # both are rounded to float16: by half a step of the value, below 2^-14 by half its fixed step of 2^-24, which the comparison
+    # multiplies by the gradient where it is that of 1 which was rounded
+    fixed = B.TINY[dtype] / 2 * (1 + up.double()[:, None].cpu())
+    B.close(got[0], want, 2 * B.HALF_STEP[dtype] * want.abs().cpu() + fixed, "grad hidden")
