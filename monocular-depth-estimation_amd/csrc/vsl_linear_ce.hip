@@ -1446,16 +1446,22 @@ int launch_logits_as(const LogitArgs& a, hipStream_t s) {
   hipLaunchKernelGGL((k_ce_logits<T, S, WHAT, SPLIT, FORM>), dim3((unsigned)(tm * tn)), dim3(S::kThreads), 0, s, a);
   return (int)tm;
 }
+// The thin tile: not for derivatives in 16 bits, whose steps of K are 64 rows (run_backward takes the narrow one), nor by planes,
+// whose time on it is the direct form's and the layouts' on top.
 template <typename T, int WHAT, bool SPLIT>
 int launch_logits(const LogitArgs& a, int shape, bool staged, hipStream_t s) {  // returns the rows of tiles
+  constexpr bool kHasThin = !SPLIT && (WHAT == kStatistics || sizeof(T) == 4);
   if constexpr (!SPLIT)
-    if (staged)
-      return shape == kThin     ? launch_logits_as<T, Thin, WHAT, SPLIT, kStagedRows>(a, s)
-             : shape == kNarrow ? launch_logits_as<T, Narrow, WHAT, SPLIT, kStagedRows>(a, s)
-                                : launch_logits_as<T, Small, WHAT, SPLIT, kStagedRows>(a, s);
+    if (staged) {
+      if constexpr (kHasThin)
+        if (shape == kThin) return launch_logits_as<T, Thin, WHAT, SPLIT, kStagedRows>(a, s);
+      if (shape == kNarrow) return launch_logits_as<T, Narrow, WHAT, SPLIT, kStagedRows>(a, s);
+      return launch_logits_as<T, Small, WHAT, SPLIT, kStagedRows>(a, s);
+    }
   if constexpr (sizeof(T) == 2 || SPLIT)
     if (shape == kLarge) return launch_logits_as<T, Large, WHAT, SPLIT, kDirect>(a, s);
-  if (shape == kThin) return launch_logits_as<T, Thin, WHAT, SPLIT, kDirect>(a, s);
+  if constexpr (kHasThin)
+    if (shape == kThin) return launch_logits_as<T, Thin, WHAT, SPLIT, kDirect>(a, s);
   if (shape == kNarrow) return launch_logits_as<T, Narrow, WHAT, SPLIT, kDirect>(a, s);
   return launch_logits_as<T, Small, WHAT, SPLIT, kDirect>(a, s);
 }
