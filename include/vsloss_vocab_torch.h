@@ -1,7 +1,7 @@
 /*
  * vsloss_vocab_torch.h -- header-only libtorch (C++) binding of the losses over a set of classes (vsloss.h):
  * vsl::top_logits(), vsl::topk_distillation_loss(), vsl::linear_cross_entropy().  torch::Tensor in, torch::Tensor out,
- * differentiable once, stream-ordered on the current HIP stream of the tensors' device, no host synchronisation.  The
+ * differentiable once (backwards only), stream-ordered on the current HIP stream of the tensors' device, no host synchronisation.  The
  * Python package's vocab_losses module calls these functions: a loss of a few rows takes some ten microseconds on the
  * device, and an autograd node that runs without the interpreter is half of what such a call costs the host.
  *
@@ -67,7 +67,11 @@ inline int reduction_of(const std::string& name) {
   return VSL_REDUCE_NONE;
 }
 
+/* Whether a call needs an autograd node.  A tangent of torch's forward mode would be lost without a word: it is refused. */
 inline bool differentiable(std::initializer_list<const torch::Tensor*> tensors) {
+  for (const torch::Tensor* t : tensors)
+    if (t->defined() && t->_fw_grad(/*level=*/0).defined())
+      throw std::runtime_error("libvsloss: the losses over a set of classes have no forward-mode derivative");
   if (!torch::GradMode::is_enabled()) return false;
   for (const torch::Tensor* t : tensors)
     if (t->defined() && t->requires_grad()) return true;

@@ -12,7 +12,7 @@ else is made contiguous.  Losses and statistics are float32, gradients have thei
 
 A logit of -infinity is a masked class.  A row in which nothing is left adds nothing and gets a zero gradient; NaN or
 +infinity in a row, and a target or index outside the vocabulary, make that row's results NaN.  ``"mean"`` over no rows is
-0.  Results are deterministic.  No host synchronisation: every call can be captured into a graph, its backward pass too
+0.  Derivatives are first ones and backward ones; forward mode is refused.  Results are deterministic.  No host synchronisation: every call can be captured into a graph, its backward pass too
 once no earlier result of the same leaves is alive (torch ends the process otherwise).
 
 The functions are those of ``include/vsloss_vocab_torch.h``, where their arguments are checked, behind a small extension

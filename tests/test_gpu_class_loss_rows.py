@@ -232,3 +232,30 @@ def test_rows_of_very_different_gradients_keep_their_digits(rows, vocab, dim, bi
     # multiplies by the gradient where it is that of 1 which was rounded
     fixed = B.TINY[dtype] / 2 * (1 + up.double()[:, None].cpu())
     B.close(got[0], want, 2 * B.HALF_STEP[dtype] * want.abs().cpu() + fixed, "grad hidden")
+
+
+# ------------------------------------------------------------------ calls that are refused
+def test_forward_mode_tangents_are_refused():
+    import torch.autograd.forward_ad as fwad
+
+    import mde_amd._abi as abi
+    import mde_amd.vocab_losses as L
+    x, w, b = (torch.randn(s, generator=gen(1)).to(DEV) for s in ((6, 20), (30, 20), (30,)))
+    v, i = L.top_logits(x, 3)[:2]
+    t = torch.arange(6, device=DEV)
+    with fwad.dual_level():
+        for needs in (False, True):
+            dual = [fwad.make_dual(a.clone().requires_grad_(needs), torch.ones_like(a)) for a in (x, w, b)]
+            calls = [lambda: L.topk_distillation_loss(dual[0], v, i), lambda: L.topk_distillation_loss(dual[0][:, ::2], v, i // 2),
+                     lambda: L.linear_cross_entropy(dual[0], w, t, b), lambda: L.linear_cross_entropy(x, dual[1], t, b),
+                     lambda: L.linear_cross_entropy(x, w, t, dual[2])]
+            for call in calls:
+                with pytest.raises(abi.VslError, match="forward-mode"):
+                    call()
+                with torch.no_grad(), pytest.raises(abi.VslError, match="forward-mode"):
+                    call()
+        # what carries no gradient backwards carries none forwards
+        assert fwad.unpack_dual(L.top_logits(dual[0], 3).values).tangent is None
+        loss = L.topk_distillation_loss(x, fwad.make_dual(v, torch.ones_like(v)), i)
+        assert fwad.unpack_dual(loss).tangent is None
+    assert bool(torch.isfinite(L.topk_distillation_loss(x, v, i)))
