@@ -37,7 +37,6 @@ from .layers import (BackprojectDepth, Project3D, SSIM, affinity_reprojection_lo
                      get_smooth_loss, grid_sample_border, mean_inverse_depth, poses_from_parameters, warp_features,
                      warp_features_multi)
 from .ops import fused_view_synthesis_loss, fused_view_synthesis_loss_heads
-from .vocab_losses import linear_cross_entropy, top_logits, topk_distillation_loss
 
 
 class ViewSynthesisLoss:
@@ -266,6 +265,7 @@ class ViewSynthesisLoss:
         """Mean cross entropy of a 1x1 classification head: ``features`` [B,D,H,W], ``weight`` [bins,D] or the
         convolution's [bins,D,1,1], ``target`` [B,H,W] bins, ``ignore_index`` where a pixel has no ground truth.  The
         bins' logits are never kept; gradients reach features, weight and bias."""
+        from .vocab_losses import linear_cross_entropy   # its binding is this torch's; the photometric losses need none
         if weight.dim() == 4 and tuple(weight.shape[2:]) == (1, 1):
             weight = weight.flatten(1)
         return linear_cross_entropy(features.movedim(1, -1), weight, target, bias, ignore_index=ignore_index)
@@ -274,6 +274,7 @@ class ViewSynthesisLoss:
         """Mean over the pixels of temperature^2 * KL(teacher || student) from the teacher's ``k`` largest bins, its
         other bins as one: ``logits``, ``teacher_logits`` [B,bins,H,W], ``weights`` [B,H,W] or None (a pixel of weight 0
         is left out).  The gradient reaches ``logits``."""
+        from .vocab_losses import top_logits, topk_distillation_loss
         top = top_logits(teacher_logits.movedim(1, -1), min(int(k), teacher_logits.shape[1]), temperature)
         return topk_distillation_loss(logits.movedim(1, -1), top.values, top.indices, top.lse, temperature=temperature,
                                       weights=weights)
