@@ -264,10 +264,13 @@ class ViewSynthesisLoss:
     def compute_bin_cross_entropy(self, features, weight, target, bias=None, ignore_index: int = -100):
         """Mean cross entropy of a 1x1 classification head: ``features`` [B,D,H,W], ``weight`` [bins,D] or the
         convolution's [bins,D,1,1], ``target`` [B,H,W] bins, ``ignore_index`` where a pixel has no ground truth.  The
-        bins' logits are never kept; gradients reach features, weight and bias."""
+        bins' logits are never kept; gradients reach features, weight and bias.  Under autocast the features are 16-bit and the
+        parameters float32: as in the convolution that this stands for, they are rounded to the features' type, and their
+        gradients come back in float32."""
         from .vocab_losses import linear_cross_entropy   # its binding is this torch's; the photometric losses need none
         if weight.dim() == 4 and tuple(weight.shape[2:]) == (1, 1):
             weight = weight.flatten(1)
+        weight, bias = weight.to(features.dtype), None if bias is None else bias.to(features.dtype)
         return linear_cross_entropy(features.movedim(1, -1), weight, target, bias, ignore_index=ignore_index)
 
     def compute_bin_distillation(self, logits, teacher_logits, k: int = 8, temperature: float = 1.0, weights=None):

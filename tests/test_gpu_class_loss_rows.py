@@ -234,6 +234,58 @@ def test_rows_of_very_different_gradients_keep_their_digits(rows, vocab, dim, bi
     B.close(got[0], want, 2 * B.HALF_STEP[dtype] * want.abs().cpu() + fixed, "grad hidden")
 
 
+# ------------------------------------------------------------------ the trainer's surface
+@pytest.mark.parametrize("low", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bias", [True, False])
+def test_depth_bins_under_autocast(low, bias):
+    """A 16-bit decoder with float32 parameters: the head's cross entropy beside the convolution's own, gradients in float32."""
+    import types
+    from mde_amd.trainer_loss import ViewSynthesisLoss
+    vs = ViewSynthesisLoss(types.SimpleNamespace(height=12, width=20))
+    g = gen(31)
+    image = torch.randn(2, 8, 12, 20, generator=g).to(DEV)
+    body, head = torch.nn.Conv2d(8, 32, 1).to(DEV), torch.nn.Conv2d(32, 48, 1, bias=bias).to(DEV)
+    with torch.no_grad():
+        for p in list(body.parameters()) + list(head.parameters()):
+            p.copy_(torch.randn(p.shape, generator=g).to(DEV) * 0.5)
+    target = torch.randint(48, (2, 12, 20), generator=g)
+    target[torch.rand(2, 12, 20, generator=g) < 0.3] = -100
+    with torch.autocast("cuda", dtype=low):
+        features = body(image)
+        assert features.dtype == low
+        features.retain_grad()
+        loss = vs.compute_bin_cross_entropy(features, head.weight, target.to(DEV), head.bias)
+    loss.backward()
+    assert loss.dtype == torch.float32 and features.grad.dtype == low
+    params = [head.weight] + ([head.bias] if bias else [])
+    assert all(p.grad.dtype == torch.float32 and p.grad.shape == p.shape for p in params)
+    # the definition on what the call rounds: features and parameters in 16 bits
+    f6, w6 = (x.detach().cpu().double().requires_grad_(True) for x in (features, head.weight.to(low)))
+    b6 = head.bias.detach().to(low).cpu().double().requires_grad_(True) if bias else None
+    want = torch.nn.functional.cross_entropy(torch.nn.functional.conv2d(f6, w6, b6), target)
+    want.backward()
+    # 32 features of below 8 x 2.5: a logit's products and their sum are off by 34 u of their sizes' sum, below 200, and the
+    # log sum's own error comes on top, twice for the difference
+    assert abs(float(loss.detach()) - float(want.detach())) <= 2 * (34 * B.U * 200 + B.tile_sum(48) + 100 * B.U)
+    # derivatives are rounded to 16 bits and so are the gradients' sums: two half steps of every term at most, and in float16
+    # the fixed step of its subnormal numbers, under 2^12 of scale for the derivatives
+    half = B.HALF_STEP[low]
+    n = int((target >= 0).sum())
+    z = torch.nn.functional.conv2d(f6, w6, b6).detach().movedim(1, -1).reshape(-1, 48)
+    ds = torch.softmax(z, 1)
+    live = target.reshape(-1) >= 0
+    ds[live, target.reshape(-1)[live]] -= 1
+    ds = (ds * live[:, None]).abs() / n
+    err = ds * (half * 1.01) + 2e-5 / n + (2.0 ** -36 / n if low == torch.float16 else 0.0)
+    rows = f6.detach().movedim(1, -1).reshape(-1, 32)
+    pairs = [(features.grad, f6.grad, (err @ w6.detach().reshape(48, 32).abs()).reshape(2, 12, 20, 32).movedim(-1, 1)),
+             (head.weight.grad, w6.grad, (err.T @ rows.abs()).reshape(48, 32, 1, 1))]
+    if bias:
+        pairs.append((head.bias.grad, b6.grad, err.sum(0)))
+    for got, ref, tol in pairs:
+        B.close(got, ref, tol + (half + 8 * B.U) * ref.abs() + B.TINY[low], "gradient")
+
+
 # ------------------------------------------------------------------ calls that are refused
 def test_forward_mode_tangents_are_refused():
     import torch.autograd.forward_ad as fwad
