@@ -278,6 +278,9 @@ class ViewSynthesisLoss:
         other bins as one: ``logits``, ``teacher_logits`` [B,bins,H,W], ``weights`` [B,H,W] or None (a pixel of weight 0
         is left out).  The gradient reaches ``logits``."""
         from .vocab_losses import top_logits, topk_distillation_loss
+        if logits.shape != teacher_logits.shape:
+            raise ValueError("student and teacher must have the same bins over the same pixels, not %s and %s"
+                             % (tuple(logits.shape), tuple(teacher_logits.shape)))
         top = top_logits(teacher_logits.movedim(1, -1), min(int(k), teacher_logits.shape[1]), temperature)
         return topk_distillation_loss(logits.movedim(1, -1), top.values, top.indices, top.lse, temperature=temperature,
                                       weights=weights)

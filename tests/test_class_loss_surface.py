@@ -3,6 +3,8 @@ import os
 import subprocess
 import sys
 
+import pytest
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
@@ -28,3 +30,17 @@ print("fine")
 """
     done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert done.returncode == 0 and done.stdout.strip().endswith("fine"), done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("shape", [(1, 6, 3, 5), (1, 4, 3, 4), (2, 4, 3, 5), (4, 3, 5)])
+def test_bins_of_student_and_teacher_have_to_be_the_same(shape):
+    """A teacher of more bins would make its pixels NaN, one of fewer would be matched bin by bin with other depths."""
+    import types
+
+    import torch
+    from mde_amd.trainer_loss import ViewSynthesisLoss
+    vs = ViewSynthesisLoss(types.SimpleNamespace(height=3, width=5))
+    with pytest.raises(ValueError, match="same bins"):
+        vs.compute_bin_distillation(torch.zeros(1, 4, 3, 5), torch.zeros(shape), k=2)
+    with pytest.raises(ValueError, match="GPU"):
+        vs.compute_bin_distillation(torch.zeros(1, 4, 3, 5), torch.zeros(1, 4, 3, 5), k=2)
