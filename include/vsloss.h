@@ -475,7 +475,8 @@ int vsl_distill_bwd(const vsl_distill_desc* desc, const float* stats, const floa
  * matrix cores with float32 accumulation; in the backward call the derivative of a logit is rounded to the operands'
  * type before it meets weight and hidden (scaled, so that float16 keeps it: by the row's largest for grad_hidden, by the
  * largest of all for grad_weight and grad_bias).  grad_hidden of a row depends on nothing but that row.
- * A class whose bias is -infinity is masked out, whatever its weights hold.
+ * A class whose bias is -infinity is masked out, whatever its weights hold.  An infinity in hidden or weight makes the logits
+ * that its products make; in grad_hidden a derivative of 0 times an infinite weight is NaN.
  *
  * vsl_linear_ce_fwd: row_loss [rows] (scratch unless VSL_REDUCE_NONE); stats [2][rows], the maximum of a row's logits and the log2 of its sum of
  * exponentials above that (kept apart: a maximum of float32's lowest value would swallow the logarithm); loss and

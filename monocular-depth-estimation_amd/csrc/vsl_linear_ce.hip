@@ -302,6 +302,9 @@ __device__ __forceinline__ void tile_of(int64_t block, int64_t tiles_m, int64_t 
 // ------------------------------------------------------------------------------------------------------------------
 struct LogitArgs {
   Operands op;
+  // float32 by planes: the operands as they were given
+  const float *given_a, *given_b;
+  int64_t given_lda, given_ldb;
   const void* bias;
   const int64_t* target;
   int64_t class0;      // first class of the piece
@@ -370,6 +373,45 @@ __device__ __forceinline__ float take_plane(float& z) {
 // T: the tensors' type; SPLIT: float32 by planes of bfloat16.  8192 x 131072 x 4096 bfloat16: forward 6.7 ms, 1305 TFLOP/s,
 // derivatives 8 x 0.99 ms, 1110; bound by the matrix instructions at the power the card allows, then by the epilogue's
 // exponentials, which no other tile's products cover (a large tile fills its CU).  2011 x 32003 x 1000 float16: 165 and 206 us.
+// A tile by planes in which something is not finite is made again from the floats themselves: an infinity has no planes (what is
+// left of it is infinity minus infinity), and a logit of -infinity is a masked class however its product was formed.  A wave
+// makes its part alone, its fragments straight from memory; 1 % of the direct form's rate is enough for it.
+template <typename S>
+__device__ __forceinline__ void exact_if_not_finite(const LogitArgs& a, int m0, int n0, Tile<S>& t) {
+  float probe[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < S::IM; ++i)
+#pragma unroll
+    for (int j = 0; j < S::JN; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) probe[r & 1] = fmaf(t.acc[i][j][r], 0.0f, probe[r & 1]);
+  if (!__any(probe[0] + probe[1] != 0.0f)) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
+  const float *pa[S::IM], *pb[S::JN];
+#pragma unroll
+  for (int i = 0; i < S::IM; ++i) {
+    pa[i] = a.given_a + (int64_t)min(m0 + (wm * S::IM + i) * 32 + (lane & 31), a.op.M - 1) * a.given_lda;
+#pragma unroll
+    for (int j = 0; j < S::JN; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) t.acc[i][j][r] = 0.0f;
+  }
+#pragma unroll
+  for (int j = 0; j < S::JN; ++j) pb[j] = a.given_b + (int64_t)min(n0 + (wn * S::JN + j) * 32 + (lane & 31), a.op.N - 1) * a.given_ldb;
+  for (int k0 = 0; k0 < a.op.dim; k0 += 2) {
+    const int k = k0 + (lane >> 5);
+    float fa[S::IM], fb[S::JN];
+#pragma unroll
+    for (int i = 0; i < S::IM; ++i) fa[i] = k < a.op.dim ? pa[i][k] : 0.0f;
+#pragma unroll
+    for (int j = 0; j < S::JN; ++j) fb[j] = k < a.op.dim ? pb[j][k] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < S::IM; ++i)
+#pragma unroll
+      for (int j = 0; j < S::JN; ++j) t.acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[i], fb[j], t.acc[i][j], 0, 0, 0);
+  }
+}
+
 enum { kStatistics, kDerivatives, kRowDerivatives };  // of the logits; derivatives of one gradient, or of one per row
 template <typename T, typename S, int WHAT, bool SPLIT, int FORM>
 __global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
@@ -382,6 +424,7 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
   const int m0 = tm * S::BM, n0 = tn * S::BN;
   Tile<S> t;
   tile_product<O, S, SPLIT, FORM>(a.op, m0, n0, 0, (SPLIT ? kPairs : 1) * a.op.kblocks, lds, t);
+  if constexpr (SPLIT) exact_if_not_finite<S>(a, m0, n0, t);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
   const int half = lane >> 5;
   const bool biased = a.bias || m0 + S::BM > a.op.M;
@@ -1521,6 +1564,9 @@ void run_forward(const vsl_linear_ce_desc* d, const Forward& f, float* row_loss,
           l.copy_weight ? l.planes * l.dim_padded : d->weight_stride, l.copy_hidden ? l.planes * l.dim_padded : d->hidden_stride,
           (int)d->vocab, (int)d->rows, (int)(l.dim_padded / Kind<O>::BK), l.dim_padded, l.dim_padded, l.tail,
           (int)d->dim};
+  if constexpr (SPLIT) a.given_a = (const T*)d->weight, a.given_b = (const T*)d->hidden;
+  a.given_lda = d->weight_stride;
+  a.given_ldb = d->hidden_stride;
   a.bias = d->bias;
   a.target = d->target;
   a.rows_padded = l.rows_padded;
@@ -1613,6 +1659,9 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
     LogitArgs a{};
     a.op = {weight + v0 * ldw, hidden, ldw, ldh, (int)classes, (int)d->rows, (int)(l.dim_padded / Kind<O>::BK), l.dim_padded,
             l.dim_padded, l.tail, (int)d->dim};
+    if constexpr (SPLIT) a.given_a = (const T*)d->weight + v0 * d->weight_stride, a.given_b = (const T*)d->hidden;
+    a.given_lda = d->weight_stride;
+    a.given_ldb = d->hidden_stride;
     a.bias = d->bias;
     a.target = d->target;
     a.class0 = v0;

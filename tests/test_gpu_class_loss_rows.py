@@ -234,6 +234,47 @@ def test_rows_of_very_different_gradients_keep_their_digits(rows, vocab, dim, bi
     B.close(got[0], want, 2 * B.HALF_STEP[dtype] * want.abs().cpu() + fixed, "grad hidden")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab,dim", [(40, 300, 96), (12, 500, 3000), (1030, 4000, 330), (2100, 8200, 128), (1500, 5000, 512)])
+@pytest.mark.parametrize("strided", [False, True])
+def test_infinite_operands_mean_the_same_at_every_size(rows, vocab, dim, strided, dtype):
+    """float32 directly, in parts and by planes: a class at -infinity by its weight is masked, a row that has only such
+    classes adds nothing, and a row that meets +infinity is NaN; no other row is."""
+    import mde_amd.vocab_losses as L
+    h, w, b, z, t = exact_operands(rows, vocab, dim, 0.0, dtype, 9)
+    h, w = h.double(), w.double()
+    h[:, 5], w[:, 5] = 1.0, -1.0
+    w[7, 5] = -INF                                          # masked: every row has a positive feature there
+    h[3, 5] = INF                                           # nothing is left of this row
+    h[rows - 2, 4], w[:, 4] = INF, 1.0                      # +infinity, and against class 7 infinity minus infinity
+    t[t == 7] = 8
+    h, w = h.to(dtype), w.to(dtype)
+    z = h.double() @ w.double().T + b.double()
+    fine = [r for r in range(rows) if r not in (3, rows - 2)]
+    assert bool((z[3] == -INF).all()) and bool((z[fine, 7] == -INF).all()) and bool(torch.isnan(z[rows - 2, 7]))
+    place = lambda x: torch.nn.functional.pad(x, (3, 2)).to(DEV)[:, 3:-2] if strided else x.to(DEV)
+    leaves = [place(h).detach().requires_grad_(True), place(w).detach().requires_grad_(True), b.to(DEV).requires_grad_(True)]
+    out = L.linear_cross_entropy(leaves[0], leaves[1], t.to(DEV), leaves[2], reduction="none")
+    loss, ltol, ds, dtol = B.linear_ce(z[fine], t[fine])
+    B.close(out[fine], loss, ltol, "row losses")
+    assert float(out[3].detach()) == 0.0 and bool(torch.isnan(out[rows - 2]))
+    up = torch.ones(rows, device=DEV)
+    up[rows - 2] = 0.0                                      # not asked for: the row's NaN stays out of the sums
+    gh, gw, gb = (g.detach().cpu().double() for g in torch.autograd.grad(out, leaves, up))
+    cols = [c for c in range(dim) if c != 5]
+    # 0 times -infinity where the masked class meets grad_hidden's feature 5: as in any product with it
+    assert bool(torch.isnan(gh[:, 5]).all()) and not gh[3, cols].any() and not gh[rows - 2, cols].any()
+    half, n = B.HALF_STEP[dtype], max(rows, vocab) + 4
+    floor = 2.0 ** -36 if dtype == torch.float16 else 0.0
+    err = dtol + ds.abs() * half * 1.01 + floor
+    h6, w6 = h.double()[fine], w.double()[:, cols]
+    for name, got, want, tol in (
+            ("grad hidden", gh[fine][:, cols], ds @ w6, err @ w6.abs() + n * B.U * (ds.abs() @ w6.abs())),
+            ("grad weight", gw, ds.T @ h6, err.T @ h6.abs() + n * B.U * (ds.abs().T @ h6.abs())),
+            ("grad bias", gb, ds.sum(0), err.sum(0) + n * B.U * ds.abs().sum(0))):
+        B.close(got, want, tol + (half + 8 * B.U) * want.abs() + B.TINY[dtype], name)
+
+
 # ------------------------------------------------------------------ the trainer's surface
 @pytest.mark.parametrize("low", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("bias", [True, False])
