@@ -142,6 +142,94 @@ def test_linear_cross_entropy_does_not_feel_an_offset_of_the_logits(rows, vocab,
     check_linear_ce(h, w, b, t, z)
 
 
+# ------------------------------------------------------------------ masks of the type's lowest value
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tail", [False, True])
+def test_distillation_of_lowest_values(tail, dtype):
+    """Classes masked by the type's lowest value, and rows that hold nothing else: uniform ones."""
+    low = torch.finfo(dtype).min
+    for rows, vocab, k in SHAPES:
+        x = shifted(rows, vocab, 0.0, dtype, vocab + 3)
+        live = max(k, vocab // 2)
+        x[:, live:] = low
+        val, idx = teacher(rows, live, k, vocab + 4, torch.float32)
+        lse = (torch.logsumexp(val.double(), 1) + 0.1).float() if tail and live > k else None
+        check_distill(x, val, idx, lse, 1.0)
+        x[:] = low
+        lse = (torch.logsumexp(val.double(), 1) + 0.1).float() if tail and vocab > k else None
+        check_distill(x, val, idx, lse, 1.0)
+        if not tail:                                        # a teacher whose k are all masked alike
+            check_distill(shifted(rows, vocab, 0.0, dtype, vocab), torch.full((rows, k), low, dtype=dtype), idx, None, 1.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("temperature", [1.0, SMALL, 40.0])
+def test_top_logits_log_sums_row_by_row(temperature, dtype):
+    import mde_amd.vocab_losses as L
+    low = torch.finfo(dtype).min
+    for vocab in (9, 60, 128, 300, 900, 2048, 5000, 70001):
+        x = shifted(8, vocab, 0.0, dtype, vocab)
+        x[1] = low
+        x[2, vocab // 2:] = low
+        x[3, 4:] = -INF
+        x[4] += 500
+        x[5] -= 2000
+        z = x.double() / temperature
+        want = torch.logsumexp(z - z.max(1, keepdim=True).values, 1) + z.max(1).values
+        got = L.top_logits(x.to(DEV), 4, temperature).lse
+        # the largest / T is rounded twice, its sum with the logarithm once; beyond float32 the sum is infinite
+        beyond = want.abs() > torch.finfo(torch.float32).max
+        assert torch.equal(got.cpu()[beyond], torch.full_like(got.cpu()[beyond], -INF))
+        tol = B.log_sum_error(z, B.stream_sum(vocab)) + 4 * B.U * want.abs()
+        B.close(got.cpu()[~beyond], want[~beyond], tol[~beyond], "log sum")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab,dim", [(5, 40, 24), (12, 500, 3000), (40, 3000, 64), (200, 300, 96), (70, 9001, 1003), (1500, 5000, 512)])
+def test_linear_cross_entropy_of_lowest_biases(rows, vocab, dim, dtype):
+    """Beside other classes such a bias masks as -infinity does, to the bit; a row of nothing else is uniform."""
+    import mde_amd.vocab_losses as L
+    low = torch.finfo(dtype).min
+    h, w, b, _, t = exact_operands(rows, vocab, dim, 0.0, dtype, 11)
+    masked = torch.arange(vocab) % 3 == 1
+    t[masked[t]] -= 1
+    outs = []
+    for value in (low, -INF):
+        b2 = torch.where(masked, torch.full_like(b, value), b)
+        leaves = [x.to(DEV).requires_grad_(True) for x in (h, w, b2)]
+        rows_out = L.linear_cross_entropy(leaves[0], leaves[1], t.to(DEV), leaves[2], reduction="none")
+        mean = L.linear_cross_entropy(leaves[0], leaves[1], t.to(DEV), leaves[2])
+        outs.append([rows_out.detach(), mean.detach()] + list(torch.autograd.grad(mean, leaves)))
+    for a, c in zip(*outs):
+        assert bool(torch.isfinite(a).all()) and torch.equal(a, c)
+    if dtype == torch.float16:
+        return                                              # its lowest value is an ordinary logit
+    b[:] = low
+    z = b.double().expand(rows, vocab).clone()
+    assert torch.equal((z + h.double() @ w.double().T).float().double(), z)
+    check_linear_ce(h, w, b, t, z)
+
+
+@pytest.mark.parametrize("weighted", [False, True])
+def test_the_mean_is_the_sum_over_its_divisor(weighted):
+    import mde_amd.vocab_losses as L
+    for rows, vocab, k in ((7000, 60, 5), (300, 3000, 8)):
+        x = shifted(rows, vocab, 0.0, torch.float32, rows).to(DEV)
+        val, idx = (a.to(DEV) for a in teacher(rows, vocab, k, 5, torch.float32))
+        weights = torch.rand(rows, generator=gen(6)).to(DEV) if weighted else None
+        each, total, mean = (L.topk_distillation_loss(x, val, idx, weights=weights, reduction=r).double() for r in ("none", "sum", "mean"))
+        count = weights.double().sum() if weighted else rows
+        assert float((total - each.sum()).abs()) <= B.U * float(each.sum())
+        assert float((mean - each.sum() / count).abs()) <= B.U * float(each.sum() / count)
+        h, w, b, _, t = exact_operands(rows, vocab, 24, 0.0, torch.float32, 12)
+        t[::5] = -100
+        args = (h.to(DEV), w.to(DEV), t.to(DEV), b.to(DEV))
+        each, total, mean = (L.linear_cross_entropy(*args, reduction=r).double() for r in ("none", "sum", "mean"))
+        count = int((t != -100).sum())
+        assert float((total - each.sum()).abs()) <= B.U * float(each.sum())
+        assert float((mean - each.sum() / count).abs()) <= B.U * float(each.sum() / count)
+
+
 # ------------------------------------------------------------------ rows beside other rows
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("vocab", [12, 60, 128, 250, 500, 1000])
