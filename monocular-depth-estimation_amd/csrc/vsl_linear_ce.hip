@@ -16,6 +16,7 @@
 // product's own rounding is, and the sums stay float32.  Six bfloat16 products run 2.7 times faster than one float32
 // product; their operands are laid out as three planes per row, and the main loop walks the six pairs of planes one after
 // the other, smallest first.
+#include <algorithm>
 #include <type_traits>
 
 #include "vsl_vocab.hpp"
@@ -1348,8 +1349,27 @@ Layout layout_of(const vsl_linear_ce_desc* d) {
   return l;
 }
 
+// Pieces of the vocabulary: at most this many derivatives (256 MiB in 16 bits, twice), and at most a GiB of a weight that is laid
+// out (300 x 131072 x 4096 bfloat16: one piece 2.48 ms, two 2.55, four 2.58).  Smaller pieces would stay in the last-level cache, but every piece reads and writes grad_hidden's sums:
+// at 8192 x 131072 x 4096 in bfloat16 2^26, 2^27 and 2^28 derivatives take 29.6, 29.3 and 29.3 ms.  Pieces are equal but for a
+// tile: a short last one costs nearly as much as a whole one.
+constexpr int64_t kPieceElements = 1LL << 27, kPieceWeight = 1LL << 30;
+static_assert(kMostParts <= kPieceElements && kMostParts / kPad / kPartRows < 65536, "logits in parts are one piece, their rows one grid");
+struct Pieces {
+  int64_t piece, pieces;  // classes of a piece, the last may have fewer
+};
+// derivatives: of a class; laid_out: bytes a class takes in a layout, 0 without any; tile: what a single piece is padded to
+Pieces pieces_of(const vsl_linear_ce_desc* d, int64_t derivatives, int64_t laid_out, int64_t tile) {
+  int64_t most = d->vocab;
+  if (derivatives > 0) most = std::min(most, std::max(kPieceElements / derivatives / kPad, (int64_t)1) * kPad);
+  if (laid_out > 0) most = std::min(most, std::max(kPieceWeight / laid_out / kPad, (int64_t)1) * kPad);
+  const int64_t n = ceil_div(d->vocab, most), piece = round_up(ceil_div(d->vocab, n), n == 1 ? tile : kPad);
+  return {piece, ceil_div(d->vocab, piece)};
+}
+
 struct Forward {
   Layout l;
+  Pieces p;
   void *hidden, *weight;
   float2* partial;
   float* target_logit;
@@ -1363,8 +1383,9 @@ Forward forward_workspace(const vsl_linear_ce_desc* d, void* base) {
   const Layout& l = f.l;
   const int s = l.size * l.planes;
   Arena a{(char*)base};
+  f.p = pieces_of(d, 0, l.copy_weight && l.logits.splits == 1 ? l.dim_padded * s : 0, kPad);
   f.hidden = l.copy_hidden ? a.take((size_t)d->rows * l.dim_padded * s) : nullptr;
-  f.weight = l.copy_weight ? a.take((size_t)d->vocab * l.dim_padded * s) : nullptr;
+  f.weight = l.copy_weight ? a.take((size_t)(f.p.pieces == 1 ? d->vocab : f.p.piece) * l.dim_padded * s) : nullptr;
   if (l.logits.splits > 1) {
     f.parts = (float*)a.take((size_t)l.logits.splits * d->rows * d->vocab * 4);
     f.pairs = (double*)a.take((size_t)d->rows * 2 * sizeof(double));
@@ -1378,12 +1399,6 @@ Forward forward_workspace(const vsl_linear_ce_desc* d, void* base) {
   return f;
 }
 
-// Pieces of the vocabulary whose derivatives hold at most this many elements: 256 MiB in 16 bits, twice.  Smaller pieces
-// would stay in the last-level cache, but every piece reads and writes grad_hidden's sums: at 8192 x 131072 x 4096 in
-// bfloat16 2^26, 2^27 and 2^28 elements take 29.6, 29.3 and 29.3 ms.
-constexpr int64_t kPieceElements = 1LL << 27;
-static_assert(kMostParts <= kPieceElements && kMostParts / kPad / kPartRows < 65536, "logits in parts are one piece, their rows one grid");
-
 constexpr int64_t kBiasBlocks = 1024;
 
 // grad_hidden of few rows takes a large weight as it lies: transposing it first reads and writes it once more.
@@ -1395,7 +1410,7 @@ constexpr int64_t kColumnsRows = 128, kColumnsBytes = 16 << 20;
 struct Backward {
   Layout l;
   bool columns;
-  int64_t piece, pieces, vocab_padded;
+  int64_t piece, pieces;
   Plan plan_h, plan_w;
   void *hidden, *weight, *hidden_t, *weight_t, *delta, *delta_t;
   float *sum_h, *sum_w, *sum_b, *row_scale, *row_size, *out_scale, *largest, *parts;
@@ -1405,20 +1420,21 @@ Backward backward_workspace(const vsl_linear_ce_desc* d, uint32_t mask, void* ba
   Backward b{};
   b.l = layout_of(d);
   const int s = b.l.size * b.l.planes;
-  b.piece = kPieceElements / (b.l.rows_padded > 0 ? b.l.rows_padded : 1) / kPad * kPad;
-  if (b.piece < kPad) b.piece = kPad;
-  if (b.piece > round_up(d->vocab, kPad)) b.piece = round_up(d->vocab, kPad);
-  b.pieces = ceil_div(d->vocab, b.piece);
-  b.vocab_padded = round_up(d->vocab, kPad);
   const bool gh = mask & 1, gw = mask & 2, gb = mask & 4;
-  Arena a{(char*)base};
-  b.hidden = b.l.copy_hidden ? a.take((size_t)d->rows * b.l.dim_padded * s) : nullptr;
-  b.weight = b.l.copy_weight ? a.take((size_t)d->vocab * b.l.dim_padded * s) : nullptr;
-  b.hidden_t = gw ? a.take((size_t)d->dim * b.l.rows_padded * s) : nullptr;
   // dim: a piece that runs over the end of a row has to end in the next one (kStagedColumns)
   const bool columns = !b.l.split && d->rows <= kColumnsRows && d->dim >= 8 && d->vocab * d->dim * size_of(d->type) >= kColumnsBytes;
   b.columns = gh && columns;
-  b.weight_t = gh && !b.columns ? a.take((size_t)d->dim * b.vocab_padded * s) : nullptr;
+  // the same pieces whichever gradients are asked for, so that each has the same bits alone; whole where the logits come in parts
+  const bool parts = b.l.logits.splits > 1;
+  const int64_t tile = parts ? 64 : kShapes[b.l.logits.shape].bm;
+  const Pieces p = parts ? Pieces{round_up(d->vocab, tile), 1} : pieces_of(d, b.l.rows_padded, columns && !b.l.copy_weight ? 0 : b.l.dim_padded * s, tile);
+  b.piece = p.piece;
+  b.pieces = p.pieces;
+  Arena a{(char*)base};
+  b.hidden = b.l.copy_hidden ? a.take((size_t)d->rows * b.l.dim_padded * s) : nullptr;
+  b.weight = b.l.copy_weight ? a.take((size_t)(b.pieces == 1 ? d->vocab : b.piece) * b.l.dim_padded * s) : nullptr;
+  b.hidden_t = gw ? a.take((size_t)d->dim * b.l.rows_padded * s) : nullptr;
+  b.weight_t = gh && !b.columns ? a.take((size_t)d->dim * b.piece * s) : nullptr;
   b.delta = gh ? a.take((size_t)b.l.rows_padded * b.piece * s) : nullptr;
   b.delta_t = gw || gb ? a.take((size_t)b.l.rows_padded * b.piece * s) : nullptr;
   b.plan_h = plan_of(d->dim, d->rows, b.l.steps(b.piece), b.l.type, true, columns);
@@ -1459,8 +1475,10 @@ struct LayoutLaunch {
     const int64_t b = ceil_div(rows, 4);
     add({in, out, stride, rows, width, (int)cols, false, {}, b < 16384 ? b : 16384});
   }
-  void transpose(const void* in, int64_t stride, int64_t rows, int64_t cols, int64_t width, const Contributes& with, void* out) {
-    add({in, out, stride, rows, width, (int)cols, true, with, width / 64 * ceil_div(cols, 64)});
+  // covers the first `padded` columns of out's rows (a multiple of 64), zeros behind `rows`
+  void transpose(const void* in, int64_t stride, int64_t rows, int64_t cols, int64_t width, int64_t padded, const Contributes& with,
+                 void* out) {
+    add({in, out, stride, rows, width, (int)cols, true, with, padded / 64 * ceil_div(cols, 64)});
   }
   template <typename T, bool SPLIT>
   void run(hipStream_t s) {
@@ -1555,37 +1573,43 @@ void run_forward(const vsl_linear_ce_desc* d, const Forward& f, float* row_loss,
                  float* divisor, hipStream_t s) {
   typedef std::conditional_t<SPLIT, __bf16, T> O;
   const Layout& l = f.l;
-  LogitArgs a{};
-  LayoutLaunch lay;
-  if (l.copy_hidden) lay.copy(d->hidden, d->hidden_stride, d->rows, d->dim, l.dim_padded, f.hidden);
-  if (l.copy_weight) lay.copy(d->weight, d->weight_stride, d->vocab, d->dim, l.dim_padded, f.weight);
-  lay.run<T, SPLIT>(s);
-  a.op = {l.copy_weight ? f.weight : d->weight, l.copy_hidden ? f.hidden : d->hidden,
-          l.copy_weight ? l.planes * l.dim_padded : d->weight_stride, l.copy_hidden ? l.planes * l.dim_padded : d->hidden_stride,
-          (int)d->vocab, (int)d->rows, (int)(l.dim_padded / Kind<O>::BK), l.dim_padded, l.dim_padded, l.tail,
-          (int)d->dim};
-  if constexpr (SPLIT) a.given_a = (const T*)d->weight, a.given_b = (const T*)d->hidden;
-  a.given_lda = d->weight_stride;
-  a.given_ldb = d->hidden_stride;
-  a.bias = d->bias;
-  a.target = d->target;
-  a.rows_padded = l.rows_padded;
-  if constexpr (!SPLIT)
-    if (f.parts) {
-      launch_parts<T>(a.op, l, f.parts, s);
-      auto rows = [&](auto kernel, int threads) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)d->rows), dim3(threads), 0, s,
-                           Parts{f.parts, l.logits.splits, d->rows, d->vocab, d->bias}, d->target, d->ignore_index, d->z_loss,
-                           row_loss, stats, d->reduction, f.pairs, loss, divisor);
-      };
-      if (d->vocab > 2048) rows(k_ce_parts_rows<T, 1024>, 1024);  // 10544 classes of two rows: 8.9 us, with 256 threads 17.6
-      else rows(k_ce_parts_rows<T, kThreads>, kThreads);
-      if (d->reduction != VSL_REDUCE_NONE && d->rows > 1) launch_sum_pairs(f.pairs, d->rows, d->reduction, loss, divisor, s);
-      return;
-    }
-  a.partial = f.partial;
-  a.target_logit = f.target_logit;
-  const int tiles = launch_logits<T, kStatistics, SPLIT>(a, l.logits.shape, l.staged, s);
+  const O* hidden = (const O*)(l.copy_hidden ? f.hidden : d->hidden);
+  int tiles = 0;
+  for (int64_t p = 0; p < f.p.pieces; ++p) {
+    const int64_t v0 = p * f.p.piece, classes = d->vocab - v0 < f.p.piece ? d->vocab - v0 : f.p.piece;
+    const T* given = (const T*)d->weight + v0 * d->weight_stride;
+    LayoutLaunch lay;
+    if (l.copy_hidden && p == 0) lay.copy(d->hidden, d->hidden_stride, d->rows, d->dim, l.dim_padded, f.hidden);
+    if (l.copy_weight) lay.copy(given, d->weight_stride, classes, d->dim, l.dim_padded, f.weight);
+    lay.run<T, SPLIT>(s);
+    LogitArgs a{};
+    a.op = {l.copy_weight ? f.weight : (const void*)given, hidden, l.copy_weight ? l.planes * l.dim_padded : d->weight_stride,
+            l.copy_hidden ? l.planes * l.dim_padded : d->hidden_stride, (int)classes, (int)d->rows,
+            (int)(l.dim_padded / Kind<O>::BK), l.dim_padded, l.dim_padded, l.tail, (int)d->dim};
+    if constexpr (SPLIT) a.given_a = given, a.given_b = (const T*)d->hidden;
+    a.given_lda = d->weight_stride;
+    a.given_ldb = d->hidden_stride;
+    a.bias = d->bias;
+    a.target = d->target;
+    a.class0 = v0;
+    a.rows_padded = l.rows_padded;
+    if constexpr (!SPLIT)
+      if (f.parts) {
+        launch_parts<T>(a.op, l, f.parts, s);
+        auto rows = [&](auto kernel, int threads) {
+          hipLaunchKernelGGL(kernel, dim3((unsigned)d->rows), dim3(threads), 0, s,
+                             Parts{f.parts, l.logits.splits, d->rows, d->vocab, d->bias}, d->target, d->ignore_index, d->z_loss,
+                             row_loss, stats, d->reduction, f.pairs, loss, divisor);
+        };
+        if (d->vocab > 2048) rows(k_ce_parts_rows<T, 1024>, 1024);  // 10544 classes of two rows: 8.9 us, with 256 threads 17.6
+        else rows(k_ce_parts_rows<T, kThreads>, kThreads);
+        if (d->reduction != VSL_REDUCE_NONE && d->rows > 1) launch_sum_pairs(f.pairs, d->rows, d->reduction, loss, divisor, s);
+        return;
+      }
+    a.partial = f.partial + tiles * l.rows_padded;
+    a.target_logit = f.target_logit;
+    tiles += launch_logits<T, kStatistics, SPLIT>(a, l.logits.shape, l.staged, s);
+  }
   // few rows: more lanes each, so that no lane walks many tiles (16 rows of 512 tiles: 14 us with 16 lanes a row); many rows:
   // more of them a block, so that fewer sums are left
   auto rows = [&](auto kernel, int per_block, int threads) {
@@ -1635,31 +1659,33 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
     hipLaunchKernelGGL(k_ce_largest, dim3(sc.partials), dim3(kThreads), 0, s, sc);
     hipLaunchKernelGGL(k_ce_scale, dim3((unsigned)ceil_div(l.rows_padded, kThreads)), dim3(kThreads), 0, s, sc);
   }
-  LayoutLaunch lay;
-  if (l.copy_hidden) lay.copy(d->hidden, d->hidden_stride, d->rows, d->dim, l.dim_padded, b.hidden);
-  if (l.copy_weight) lay.copy(d->weight, d->weight_stride, d->vocab, d->dim, l.dim_padded, b.weight);
-  if (grad_weight)
-    lay.transpose(d->hidden, d->hidden_stride, d->rows, d->dim, l.rows_padded,
-                  Contributes{d->target, stats, row_scale, nullptr, d->ignore_index}, b.hidden_t);
-  if (grad_hidden && !b.columns)
-    lay.transpose(d->weight, d->weight_stride, d->vocab, d->dim, b.vocab_padded, Contributes{nullptr, nullptr, nullptr, d->bias, 0},
-                  b.weight_t);
-  lay.run<T, SPLIT>(s);
   const O* hidden = (const O*)(l.copy_hidden ? b.hidden : d->hidden);
-  const O* weight = (const O*)(l.copy_weight ? b.weight : d->weight);
   const int64_t ldh = l.copy_hidden ? l.planes * l.dim_padded : d->hidden_stride;
   const int64_t ldw = l.copy_weight ? l.planes * l.dim_padded : d->weight_stride;
   for (int64_t p = 0; p < b.pieces; ++p) {
     const int64_t v0 = p * b.piece, classes = d->vocab - v0 < b.piece ? d->vocab - v0 : b.piece;
+    const T* given = (const T*)d->weight + v0 * d->weight_stride;
+    const T* bias = d->bias ? (const T*)d->bias + v0 : nullptr;
     int shape = b.pieces == 1 ? l.logits.shape : plan_of(classes, d->rows, l.steps(d->dim), l.type, false, l.staged).shape;
     if (sizeof(O) == 2 && shape == kThin) shape = kNarrow;
     // what the derivative kernel covers: whole steps of K (32 float32, 64 in 16 bits) for the two products that follow
     const int64_t padded = round_up(classes, b.parts ? 64 : kShapes[shape].bm);
     const int64_t rows_covered = round_up(d->rows, b.parts ? 64 : kShapes[shape].bn);
+    LayoutLaunch lay;
+    if (p == 0) {
+      if (l.copy_hidden) lay.copy(d->hidden, d->hidden_stride, d->rows, d->dim, l.dim_padded, b.hidden);
+      if (grad_weight)
+        lay.transpose(d->hidden, d->hidden_stride, d->rows, d->dim, l.rows_padded, l.rows_padded,
+                      Contributes{d->target, stats, row_scale, nullptr, d->ignore_index}, b.hidden_t);
+    }
+    if (l.copy_weight) lay.copy(given, d->weight_stride, classes, d->dim, l.dim_padded, b.weight);
+    if (grad_hidden && !b.columns)
+      lay.transpose(given, d->weight_stride, classes, d->dim, b.piece, padded, Contributes{nullptr, nullptr, nullptr, bias, 0}, b.weight_t);
+    lay.run<T, SPLIT>(s);
     LogitArgs a{};
-    a.op = {weight + v0 * ldw, hidden, ldw, ldh, (int)classes, (int)d->rows, (int)(l.dim_padded / Kind<O>::BK), l.dim_padded,
+    a.op = {l.copy_weight ? b.weight : (const void*)given, hidden, ldw, ldh, (int)classes, (int)d->rows, (int)(l.dim_padded / Kind<O>::BK), l.dim_padded,
             l.dim_padded, l.tail, (int)d->dim};
-    if constexpr (SPLIT) a.given_a = (const T*)d->weight + v0 * d->weight_stride, a.given_b = (const T*)d->hidden;
+    if constexpr (SPLIT) a.given_a = given, a.given_b = (const T*)d->hidden;
     a.given_lda = d->weight_stride;
     a.given_ldb = d->hidden_stride;
     a.bias = d->bias;
@@ -1694,8 +1720,8 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
     int shapes[2], n = 0;
     FinishLaunch finish, finish_rows;
     if (grad_hidden) {
-      g[n].op = {(const O*)b.weight_t + v0, b.delta, l.planes * b.vocab_padded, l.planes * b.piece, (int)d->dim, (int)d->rows,
-                 (int)(padded / Kind<O>::BK), b.vocab_padded, b.piece, 8, 0};
+      g[n].op = {b.weight_t, b.delta, l.planes * b.piece, l.planes * b.piece, (int)d->dim, (int)d->rows,
+                 (int)(padded / Kind<O>::BK), b.piece, b.piece, 8, 0};
       g[n].add = p > 0;
       g[n].sum = b.sum_h;
       g[n].out = grad_hidden;
@@ -1704,11 +1730,11 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
       g[n].splits = b.plan_h.splits;
       shapes[n++] = b.plan_h.shape;
       if (b.columns) {
-        g[0].op.A = (const T*)d->weight + v0 * d->weight_stride;
+        g[0].op.A = given;
         g[0].op.lda = d->weight_stride;
         g[0].op.rows_of_k = (int)classes;
         g[0].whole = d->dim % 4 == 0;
-        g[0].op.bias = d->bias ? (const T*)d->bias + v0 : nullptr;
+        g[0].op.bias = bias;
       }
       if (b.sum_h && p == b.pieces - 1)
         (uniform ? finish : finish_rows).add(b.sum_h, b.plan_h.splits, d->rows * d->dim, grad_hidden, row_size, d->dim);
@@ -1735,14 +1761,14 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
     if (grad_bias) {
       // few classes: their rows in parts, so that more than a block per class works on them
       const int parts = b.sum_b ? (int)(kBiasBlocks / classes < 1 ? 1 : kBiasBlocks / classes) : 1;
-      auto bias = [&](auto kernel, int per_block) {
+      auto sum_rows = [&](auto kernel, int per_block) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(classes * parts, per_block)), dim3(kThreads), 0, s,
                            (const void*)b.delta_t, l.planes * l.rows_padded, l.rows_padded, rows_covered, (int)classes, parts,
                            parts > 1 ? b.sum_b : nullptr, scale, grad_bias + v0);
       };
       // few rows: a block per class would have little to add up (57 rows, 90227 classes: 58 us, with 8 lanes 5)
-      if (rows_covered <= 1024) bias(k_ce_bias<T, SPLIT, 8>, kThreads / 8);
-      else bias(k_ce_bias<T, SPLIT, kThreads>, 1);
+      if (rows_covered <= 1024) sum_rows(k_ce_bias<T, SPLIT, 8>, kThreads / 8);
+      else sum_rows(k_ce_bias<T, SPLIT, kThreads>, 1);
       if (parts > 1) finish.add(b.sum_b, parts, classes, grad_bias + v0);
     }
     finish.run<T>(scale, s);

@@ -363,6 +363,26 @@ def test_infinite_operands_mean_the_same_at_every_size(rows, vocab, dim, strided
         B.close(got, want, tol + (half + 8 * B.U) * want.abs() + B.TINY[dtype], name)
 
 
+# ------------------------------------------------------------------ pieces of the vocabulary
+@pytest.mark.parametrize("rows,vocab,dim,dtype,off", [
+    (2048, 70001, 330, torch.float32, 0),                   # by planes, pieces of 2^27 derivatives
+    (300, 70001, 4096, torch.float32, 0),                   # by planes, pieces of 2^30 bytes of weight, forward as well
+    (1200, 140000, 4099, torch.bfloat16, 1),                 # rows that 16-byte loads cannot take, copied piece by piece
+    (300, 140000, 4000, torch.float16, 0),                   # only the transposed weight goes in pieces
+    (100, 40000, 4096, torch.float32, 1),                   # few rows: the weight as it lies
+    (1030, 257, 64, torch.bfloat16, 0), (1030, 129, 96, torch.float32, 3), (9000, 100, 40, torch.float16, 0)])   # one, ragged
+def test_linear_cross_entropy_lays_out_piece_by_piece(rows, vocab, dim, dtype, off):
+    from test_gpu_vocab_losses import ce_inputs, check_ce
+    h, w, b, t = ce_inputs(rows, vocab, dim, dtype, rows + dim, bias=True)
+    t[torch.rand(rows, generator=gen(21)) < 0.2] = -100
+    masked = torch.cat([torch.arange(vocab - 3, vocab), torch.arange(5, vocab, 301)])
+    b[masked], w[masked] = -INF, float("nan")
+    t = torch.where(torch.isin(t, masked), torch.ones_like(t), t)
+    wide = torch.zeros(vocab, dim + 2 * off, dtype=dtype, device=DEV)
+    wide[:, off:off + dim] = w.to(DEV)
+    check_ce(h, w, b, t, on_device=(h.to(DEV), wide[:, off:off + dim]))
+
+
 # ------------------------------------------------------------------ the trainer's surface
 @pytest.mark.parametrize("low", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("bias", [True, False])
