@@ -914,9 +914,14 @@ __device__ __forceinline__ void store_tile(const GradArgs& a, int m0, int n0, co
   static_assert(kWide * S::BN * (int)sizeof(T) <= S::kLds && kPieces >= 16 && S::WM % kHalves == 0, "tile through LDS");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
   float scale[S::JN];
+  if (a.scale.rows) {
 #pragma unroll
-  for (int j = 0; j < S::JN; ++j)
-    scale[j] = a.scale.rows ? a.scale.rows[min(n0 + (wn * S::JN + j) * 32 + (lane & 31), a.op.N - 1)] : a.scale.get();
+    for (int j = 0; j < S::JN; ++j) scale[j] = a.scale.rows[min(n0 + (wn * S::JN + j) * 32 + (lane & 31), a.op.N - 1)];
+  } else {
+    scale[0] = a.scale.get();
+#pragma unroll
+    for (int j = 1; j < S::JN; ++j) scale[j] = scale[0];
+  }
 #pragma unroll
   for (int h = 0; h < kHalves; ++h) {
     if (h) __syncthreads();
