@@ -56,7 +56,8 @@ inline torch::Tensor per_row(const std::optional<torch::Tensor>& t, const char* 
 }
 
 inline double temperature_of(double value) {
-  TORCH_CHECK_VALUE(value >= 1e-4 && value <= 1e4, "temperature must lie in 1e-4..1e4, not ", value);
+  const float t = (float)value;   /* as the library holds it: float32's 1e-4 is a little below the double one */
+  TORCH_CHECK_VALUE(t >= 1e-4f && t <= 1e4f, "temperature must lie in 1e-4..1e4, not ", value);
   return value;
 }
 

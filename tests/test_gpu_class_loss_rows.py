@@ -86,6 +86,22 @@ def test_distillation_does_not_feel_an_offset_of_the_teachers_values(offset, t, 
             check_distill(x, val, idx, (torch.logsumexp(val.double() / t, 1) + 0.1).float(), t)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("t", [torch.tensor(1e-4).item(), 1e4])
+@pytest.mark.parametrize("tail", [False, True])
+def test_distillation_at_the_extreme_temperatures(t, tail, dtype):
+    for rows, vocab, k in SHAPES:
+        x = shifted(rows, vocab, 0.0, dtype, vocab + 5)
+        val, idx = teacher(rows, vocab, k, vocab + 6, torch.float32)
+        lse = None
+        if tail:                                            # the whole sum over some more classes like the k, as float32 holds it
+            z = val.double() / t
+            lse = (z.max(1).values + torch.logsumexp(z - z.max(1, keepdim=True).values, 1) + 0.1).float()
+            if float(lse.abs().max()) > 3e3:                # no digit left for what the k leave over: only rows that are whole
+                continue
+        check_distill(x, val, idx, lse, t)
+
+
 def exact_operands(rows, vocab, dim, offset, dtype, seed):
     """hidden, weight, bias whose logits float32 holds exactly whatever the order of the sums: small whole numbers times a power
     of two, few of a row's features not zero."""
