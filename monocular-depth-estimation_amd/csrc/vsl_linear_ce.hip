@@ -1012,7 +1012,7 @@ struct FinishJob {
   int splits;
   int64_t n;
   int64_t blocks;
-  const float* row_scale;  // ROWS: of rows of `width` elements, otherwise jobs' scale
+  const float* row_scale;  // ROWS: of rows of `width` elements, or NULL: jobs' scale
   int64_t width;
 };
 struct FinishJobs {
@@ -1026,7 +1026,7 @@ __global__ __launch_bounds__(kThreads) void k_ce_finish(FinishJobs jobs) {
   int which = 0;
   while (block >= jobs.job[which].blocks) block -= jobs.job[which++].blocks;  // the grid is the sum of the jobs' blocks
   const FinishJob& j = jobs.job[which];
-  const float scale = ROWS ? 0.0f : jobs.scale.get();
+  const float scale = jobs.scale.get();
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   auto sum = [&](int64_t i, int s0, int s1) {
     f32x4 v{0.0f, 0.0f, 0.0f, 0.0f};
@@ -1044,7 +1044,7 @@ __global__ __launch_bounds__(kThreads) void k_ce_finish(FinishJobs jobs) {
   auto store = [&](int64_t i, const f32x4& v) {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (i + e < j.n) ((T*)j.out)[i + e] = (T)((ROWS ? j.row_scale[(i + e) / j.width] : scale) * v[e]);
+      if (i + e < j.n) ((T*)j.out)[i + e] = (T)((ROWS && j.row_scale ? j.row_scale[(i + e) / j.width] : scale) * v[e]);
   };
   if (j.splits < kDealtSplits) {
     for (int64_t i = (block * kThreads + threadIdx.x) * 4; i < j.n; i += j.blocks * kThreads * 4) store(i, sum(i, 0, j.splits));
@@ -1499,10 +1499,10 @@ struct FinishLaunch {
     jobs.job[n++] = {sum, out, splits, elements, b < 65536 ? b : 65536, row_scale, width};
     blocks += jobs.job[n - 1].blocks;
   }
-  template <typename T, bool ROWS = false>
-  void run(const OutScale& scale, hipStream_t s) {
+  template <typename T>
+  void run(const OutScale& scale, bool rows, hipStream_t s) {
     jobs.scale = scale;
-    if (n) hipLaunchKernelGGL((k_ce_finish<T, ROWS>), dim3((unsigned)blocks), dim3(kThreads), 0, s, jobs);
+    if (n) hipLaunchKernelGGL((rows ? k_ce_finish<T, true> : k_ce_finish<T, false>), dim3((unsigned)blocks), dim3(kThreads), 0, s, jobs);
   }
 };
 
@@ -1723,7 +1723,7 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
     }
     GradArgs g[2] = {};
     int shapes[2], n = 0;
-    FinishLaunch finish, finish_rows;
+    FinishLaunch finish;
     if (grad_hidden) {
       g[n].op = {b.weight_t, b.delta, l.planes * b.piece, l.planes * b.piece, (int)d->dim, (int)d->rows,
                  (int)(padded / Kind<O>::BK), b.piece, b.piece, 8, 0};
@@ -1742,7 +1742,7 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
         g[0].op.bias = bias;
       }
       if (b.sum_h && p == b.pieces - 1)
-        (uniform ? finish : finish_rows).add(b.sum_h, b.plan_h.splits, d->rows * d->dim, grad_hidden, row_size, d->dim);
+        finish.add(b.sum_h, b.plan_h.splits, d->rows * d->dim, grad_hidden, row_size, d->dim);
     }
     if (grad_weight) {
       g[n].op = {b.hidden_t, b.delta_t, l.planes * l.rows_padded, l.planes * l.rows_padded, (int)d->dim, (int)classes,
@@ -1776,8 +1776,7 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
       else sum_rows(k_ce_bias<T, SPLIT, kThreads>, 1);
       if (parts > 1) finish.add(b.sum_b, parts, classes, grad_bias + v0);
     }
-    finish.run<T>(scale, s);
-    finish_rows.run<T, true>(scale, s);
+    finish.run<T>(scale, !uniform, s);
   }
 }
 
