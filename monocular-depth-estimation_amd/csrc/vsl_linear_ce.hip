@@ -6,6 +6,11 @@
 //              operands' type and written as [rows, piece] and as [piece, rows]; then
 //              grad_hidden += d weight_piece (float32 across the pieces) and grad_weight_piece = d^T hidden.
 //
+// d is rounded because a second plane for the rest of it would double both gradient products and the derivatives' traffic.
+// Gradients that are rounded to 16 bits at the end lose little by it: off against float64 by 1.8e-3 of their size instead of
+// 1.7e-3 (8192 x 131072 x 4096 bfloat16), 4.1e-4 instead of 3.8e-4 (2011 x 32003 x 1000 float16), 2.2e-3 instead of 1.7e-3
+// (92160 x 128 x 256 bfloat16).
+//
 // All three products are C[M,N] = A[M,K] B[N,K]^T with K contiguous in both operands, so that one main loop serves them:
 // the transposed weight and hidden that the two gradient products need are laid out once per call.  Recomputing z costs
 // a fourth product (a third more operations than keeping the logits) and spares rows * vocab float32 of memory traffic.
@@ -371,14 +376,16 @@ __device__ __forceinline__ float take_plane(float& z) {
   return h;
 }
 
-// T: the tensors' type; SPLIT: float32 by planes of bfloat16.  8192 x 131072 x 4096 bfloat16: forward 6.7 ms, 1305 TFLOP/s,
-// derivatives 8 x 0.99 ms, 1110; bound by the matrix instructions at the power the card allows, then by the epilogue's
-// exponentials, which no other tile's products cover (a large tile fills its CU).  2011 x 32003 x 1000 float16: 165 and 206 us.
-// A tile by planes in which something is not finite is made again from the floats themselves: an infinity has no planes (what is
-// left of it is infinity minus infinity), and a logit of -infinity is a masked class however its product was formed.  A wave
-// makes its part alone, its fragments straight from memory; 1 % of the direct form's rate is enough for it.
+// T: the tensors' type; SPLIT: float32 by planes of bfloat16.  8192 x 131072 x 4096 bfloat16: forward 6.98 ms, 1260 TFLOP/s,
+// derivatives 8 x 1.01 ms, 1089; bound by the matrix instructions at the power the card allows, then by the epilogue's
+// exponentials, which no other tile's products cover (a large tile fills its CU).  2011 x 32003 x 1000 float16: 149 and 187 us.
+// Logits by planes that are not finite are made again from the floats themselves: an infinity has no planes (what is left of it
+// is infinity minus infinity), and a logit of -infinity is a masked class however its product was formed.  A wave makes its
+// blocks alone, the fragments straight from memory; 1 % of the direct form's rate is enough for it.  Finite logits keep their
+// bits, so that no row feels another's: they wait in a piece of LDS of the wave's own (a tile's steps are done with it, the
+// epilogues use its beginning), since a block more in registers would spill.
 template <typename S>
-__device__ __forceinline__ void exact_if_not_finite(const LogitArgs& a, int m0, int n0, Tile<S>& t) {
+__device__ __forceinline__ void exact_if_not_finite(const LogitArgs& a, int m0, int n0, char* lds, Tile<S>& t) {
   float probe[2] = {0.0f, 0.0f};
 #pragma unroll
   for (int i = 0; i < S::IM; ++i)
@@ -387,30 +394,32 @@ __device__ __forceinline__ void exact_if_not_finite(const LogitArgs& a, int m0, 
 #pragma unroll
       for (int r = 0; r < 16; ++r) probe[r & 1] = fmaf(t.acc[i][j][r], 0.0f, probe[r & 1]);
   if (!__any(probe[0] + probe[1] != 0.0f)) return;
+  constexpr int kBlock = 32 * 32 * sizeof(float);
+  static_assert(S::WM * S::BN * sizeof(float2) + S::BM * sizeof(float) + S::WM * S::WN * kBlock <= S::kLds, "blocks that wait");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
-  const float *pa[S::IM], *pb[S::JN];
+  volatile float* planes = (volatile float*)(lds + S::kLds - (wave + 1) * kBlock) + lane;
 #pragma unroll
-  for (int i = 0; i < S::IM; ++i) {
-    pa[i] = a.given_a + (int64_t)min(m0 + (wm * S::IM + i) * 32 + (lane & 31), a.op.M - 1) * a.given_lda;
+  for (int i = 0; i < S::IM; ++i)
 #pragma unroll
-    for (int j = 0; j < S::JN; ++j)
+    for (int j = 0; j < S::JN; ++j) {
+      const float* pa = a.given_a + (int64_t)min(m0 + (wm * S::IM + i) * 32 + (lane & 31), a.op.M - 1) * a.given_lda;
+      const float* pb = a.given_b + (int64_t)min(n0 + (wn * S::JN + j) * 32 + (lane & 31), a.op.N - 1) * a.given_ldb;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) t.acc[i][j][r] = 0.0f;
-  }
+      for (int r = 0; r < 16; ++r) {
+        planes[64 * r] = t.acc[i][j][r];
+        t.acc[i][j][r] = 0.0f;
+      }
+#pragma unroll 1
+      for (int k0 = 0; k0 < a.op.dim; k0 += 2) {
+        const int k = k0 + (lane >> 5);
+        t.acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(k < a.op.dim ? pa[k] : 0.0f, k < a.op.dim ? pb[k] : 0.0f, t.acc[i][j], 0, 0, 0);
+      }
 #pragma unroll
-  for (int j = 0; j < S::JN; ++j) pb[j] = a.given_b + (int64_t)min(n0 + (wn * S::JN + j) * 32 + (lane & 31), a.op.N - 1) * a.given_ldb;
-  for (int k0 = 0; k0 < a.op.dim; k0 += 2) {
-    const int k = k0 + (lane >> 5);
-    float fa[S::IM], fb[S::JN];
-#pragma unroll
-    for (int i = 0; i < S::IM; ++i) fa[i] = k < a.op.dim ? pa[i][k] : 0.0f;
-#pragma unroll
-    for (int j = 0; j < S::JN; ++j) fb[j] = k < a.op.dim ? pb[j][k] : 0.0f;
-#pragma unroll
-    for (int i = 0; i < S::IM; ++i)
-#pragma unroll
-      for (int j = 0; j < S::JN; ++j) t.acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[i], fb[j], t.acc[i][j], 0, 0, 0);
-  }
+      for (int r = 0; r < 16; ++r) {
+        const float z = planes[64 * r];  // what the lane itself has put there
+        if (z * 0.0f == 0.0f) t.acc[i][j][r] = z;
+      }
+    }
 }
 
 enum { kStatistics, kDerivatives, kRowDerivatives };  // of the logits; derivatives of one gradient, or of one per row
@@ -425,7 +434,7 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
   const int m0 = tm * S::BM, n0 = tn * S::BN;
   Tile<S> t;
   tile_product<O, S, SPLIT, FORM>(a.op, m0, n0, 0, (SPLIT ? kPairs : 1) * a.op.kblocks, lds, t);
-  if constexpr (SPLIT) exact_if_not_finite<S>(a, m0, n0, t);
+  if constexpr (SPLIT) exact_if_not_finite<S>(a, m0, n0, lds, t);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
   const int half = lane >> 5;
   const bool biased = a.bias || m0 + S::BM > a.op.M;
@@ -872,7 +881,8 @@ __device__ __forceinline__ void transpose_job(const LayoutJob& j, int64_t block,
   }
 }
 
-// 8192 x 4096 and 131072 x 4096 bfloat16 transposed: 434 us, 5.3 TB/s read and written; float32 2.6 TB/s.
+// 16384 x 4096 bfloat16 transposed: 49 us, 5.5 TB/s read and written; planes of 1536 x 512 and 10007 x 512 float32, as they lie
+// and transposed: 20 us.
 template <typename T, bool SPLIT>
 __global__ __launch_bounds__(kThreads) void k_layout(LayoutJobs jobs) {
   __shared__ __attribute__((aligned(16))) char lds[64 * 65 * 4];
@@ -961,7 +971,7 @@ __device__ __forceinline__ void store_tile(const GradArgs& a, int m0, int n0, co
   }
 }
 
-// 8192 x 131072 x 4096 bfloat16, both products of a piece: 1.735 ms, 1267 TFLOP/s, bound as k_ce_logits is.
+// 8192 x 131072 x 4096 bfloat16, both products of a piece: 1.757 ms, 1252 TFLOP/s, bound as k_ce_logits is.
 template <typename T, typename S, bool SPLIT, int FORM>
 __global__ __launch_bounds__(S::kThreads) void k_ce_grad(GradJobs jobs) {
   const int which = blockIdx.x >= jobs.first ? 1 : 0;
@@ -1004,7 +1014,7 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_grad(GradJobs jobs) {
 }
 
 // out = scale * the sum of the splits, in their order: four elements a thread; many splits are dealt to the four waves; up to
-// three sums in one launch.  8192 x 4096 float32 to bfloat16: 53 us, 3.8 TB/s.
+// three sums in one launch.  8192 x 4096 float32 to bfloat16: 49 us, 4.1 TB/s.
 constexpr int kDealtSplits = 8;  // at least
 struct FinishJob {
   const float* sum;

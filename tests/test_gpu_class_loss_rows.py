@@ -379,6 +379,29 @@ def test_infinite_operands_mean_the_same_at_every_size(rows, vocab, dim, strided
         B.close(got, want, tol + (half + 8 * B.U) * want.abs() + B.TINY[dtype], name)
 
 
+@pytest.mark.parametrize("rows,vocab,dim", [(40, 300, 96), (1500, 5000, 512), (2100, 8200, 128)])
+def test_a_row_that_is_not_finite_changes_no_bit_of_another(rows, vocab, dim):
+    """Every third row of hidden infinite or NaN, and a class that is masked out with weights of NaN: the others as without."""
+    import mde_amd.vocab_losses as L
+    g = gen(13)
+    h, w, b = torch.randn(rows, dim, generator=g), torch.randn(vocab, dim, generator=g) / math.sqrt(dim), torch.zeros(vocab)
+    t = torch.randint(vocab - 4, (rows,), generator=g)
+    b[vocab - 4:] = -INF
+    fine = torch.arange(rows) % 3 != 1
+    outs = []
+    for spoiled in (False, True):
+        h2, w2 = h.clone(), w.clone()
+        if spoiled:
+            h2[1::6, 7], h2[4::6, 9] = INF, float("nan")
+            w2[vocab - 4:] = float("nan")
+        leaves = [h2.to(DEV).requires_grad_(True), w2.to(DEV), b.to(DEV)]
+        out = L.linear_cross_entropy(leaves[0], leaves[1], t.to(DEV), leaves[2], reduction="none")
+        (grad,) = torch.autograd.grad(out, leaves[:1], torch.ones(rows, device=DEV))
+        outs.append((out.detach().cpu()[fine], grad.cpu()[fine]))
+        assert bool(torch.isfinite(out[fine]).all()) and bool(torch.isnan(out[~fine]).all()) == spoiled
+    assert all(torch.equal(x, y) for x, y in zip(*outs))
+
+
 # ------------------------------------------------------------------ pieces of the vocabulary
 @pytest.mark.parametrize("rows,vocab,dim,dtype,off", [
     (2048, 70001, 330, torch.float32, 0),                   # by planes, pieces of 2^27 derivatives
