@@ -358,7 +358,7 @@ __global__ __launch_bounds__(kThreads) void k_top_rows(TopArgs a) {
 // elements reach.  Then, from the start (what was read is in L2 still), the elements that reach the bound are collected,
 // and whenever more than `trigger` are there the k largest of them are kept and the bound rises to the k-th.  A group of
 // which more passes than the buffer holds (rising rows) is collected again, vector by vector.
-// 4096 x 131072 bfloat16, k = 64: 267 us, 4.0 TB/s read, vector instructions 74 % busy; 1 x 50021, k = 32: 10 us, latency.
+// 4096 x 131072 bfloat16, k = 64: 268 us, 4.0 TB/s read, vector instructions 75 % busy; 1 x 50021, k = 32: 10 us, latency.
 constexpr int kProbe = 4;
 constexpr int kGroup = 2;
 constexpr int kTrigger = 512;  // at most; see trigger below
@@ -943,8 +943,8 @@ struct ShortRow {
 constexpr int kResident = 2048;  // blocks of 256 threads that 256 CUs hold: what walks short rows
 
 // Forward pass of short rows: maximum, the teacher's entries from an LDS line, then the sum over all classes or, with a rest
-// class, over those that are not the teacher's.  1474560 x 128 bfloat16, k = 8, rest class: 149 us, 3.3 TB/s; bound by
-// vector instructions (79 % busy), the exponentials and the two-float logarithms of q.
+// class, over those that are not the teacher's.  1474560 x 128 bfloat16, k = 8, rest class: 146 us, 3.4 TB/s; bound by
+// vector instructions (78 % busy), the exponentials and the two-float logarithms of q.
 
 template <typename T, int L, int NV>
 __global__ __launch_bounds__(kThreads) void k_distill_rows(DistillArgs a) {
@@ -1085,7 +1085,7 @@ __global__ __launch_bounds__(kThreads) void k_distill_rows(DistillArgs a) {
 }
 
 // The gradient of a short row: every class as if it were not the teacher's goes to an LDS line, the teacher's entries
-// overwrite theirs there, and the line goes out.  1474560 x 128 bfloat16, k = 8: 167 us, 5.2 TB/s read and written.
+// overwrite theirs there, and the line goes out.  1474560 x 128 bfloat16, k = 8: 165 us, 5.3 TB/s read and written.
 template <typename T, int L, int NV>
 __global__ __launch_bounds__(kThreads) void k_distill_rows_grad(DistillArgs a) {
   constexpr int E = Vec<T>::E, G = kThreads / L, W = L * NV * E;
@@ -1217,7 +1217,7 @@ __device__ __forceinline__ void close_row(const DistillArgs& a, int64_t row, flo
 constexpr int kMaxSegment = 1 << 17;  // elements of a segment: one bit of LDS each says whether the class is the teacher's
 
 // Forward pass of long rows, a block per row or segment: one read, running maximum and sum per thread; with a rest class
-// (REST) the teacher's classes are left out of them by a bit map.  4096 x 131072 bfloat16: 231 us, 4.6 TB/s.
+// (REST) the teacher's classes are left out of them by a bit map.  4096 x 131072 bfloat16: 225 us, 4.8 TB/s.
 constexpr int kWide = 4;  // vectors a thread has under way
 template <typename T, bool REST>
 __global__ __launch_bounds__(kThreads) void k_distill_stream(DistillArgs a) {
@@ -1301,7 +1301,7 @@ __global__ __launch_bounds__(kThreads) void k_distill_join(DistillArgs a) {
 }
 
 // The gradient of a long row: every class as if it were not the teacher's, then, behind a barrier, the teacher's own.
-// 4096 x 131072 bfloat16: 428 us, 5.0 TB/s read and written.
+// 4096 x 131072 bfloat16: 425 us, 5.0 TB/s read and written.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_distill_grad(DistillArgs a) {
   constexpr int E = Vec<T>::E, kTile = kThreads * E;
