@@ -376,16 +376,14 @@ __device__ __forceinline__ float take_plane(float& z) {
   return h;
 }
 
-// T: the tensors' type; SPLIT: float32 by planes of bfloat16.  8192 x 131072 x 4096 bfloat16: forward 6.98 ms, 1260 TFLOP/s,
-// derivatives 8 x 1.01 ms, 1089; bound by the matrix instructions at the power the card allows, then by the epilogue's
-// exponentials, which no other tile's products cover (a large tile fills its CU).  2011 x 32003 x 1000 float16: 149 and 187 us.
 // Logits by planes that are not finite are made again from the floats themselves: an infinity has no planes (what is left of it
-// is infinity minus infinity), and a logit of -infinity is a masked class however its product was formed.  A wave makes its
-// blocks alone, the fragments straight from memory; 1 % of the direct form's rate is enough for it.  Finite logits keep their
-// bits, so that no row feels another's: they wait in a piece of LDS of the wave's own (a tile's steps are done with it, the
-// epilogues use its beginning), since a block more in registers would spill.
+// is infinity minus infinity), and a logit of -infinity is a masked class however its product was formed.  A wave makes its own,
+// four classes of 32 rows in either half at a time as sixteen products of 4 x 4, whose four registers are those of four classes in
+// the tile; larger products would not fit beside the tile.  The fragments come straight from memory, at some hundredths of the
+// direct form's rate.  Finite logits keep their bits, so that no row feels another's; those of masked classes and of rows that
+// do not count are left as they are.
 template <typename S>
-__device__ __forceinline__ void exact_if_not_finite(const LogitArgs& a, int m0, int n0, char* lds, Tile<S>& t) {
+__device__ __forceinline__ void exact_if_not_finite(const LogitArgs& a, int m0, int n0, Tile<S>& t) {
   float probe[2] = {0.0f, 0.0f};
 #pragma unroll
   for (int i = 0; i < S::IM; ++i)
@@ -394,35 +392,46 @@ __device__ __forceinline__ void exact_if_not_finite(const LogitArgs& a, int m0, 
 #pragma unroll
       for (int r = 0; r < 16; ++r) probe[r & 1] = fmaf(t.acc[i][j][r], 0.0f, probe[r & 1]);
   if (!__any(probe[0] + probe[1] != 0.0f)) return;
-  constexpr int kBlock = 32 * 32 * sizeof(float);
-  static_assert(S::WM * S::BN * sizeof(float2) + S::BM * sizeof(float) + S::WM * S::WN * kBlock <= S::kLds, "blocks that wait");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
-  volatile float* planes = (volatile float*)(lds + S::kLds - (wave + 1) * kBlock) + lane;
 #pragma unroll
   for (int i = 0; i < S::IM; ++i)
 #pragma unroll
-    for (int j = 0; j < S::JN; ++j) {
-      const float* pa = a.given_a + (int64_t)min(m0 + (wm * S::IM + i) * 32 + (lane & 31), a.op.M - 1) * a.given_lda;
-      const float* pb = a.given_b + (int64_t)min(n0 + (wn * S::JN + j) * 32 + (lane & 31), a.op.N - 1) * a.given_ldb;
+    for (int j = 0; j < S::JN; ++j)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        planes[64 * r] = t.acc[i][j][r];
-        t.acc[i][j][r] = 0.0f;
-      }
-#pragma unroll 1
-      for (int k0 = 0; k0 < a.op.dim; k0 += 2) {
-        const int k = k0 + (lane >> 5);
-        t.acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(k < a.op.dim ? pa[k] : 0.0f, k < a.op.dim ? pb[k] : 0.0f, t.acc[i][j], 0, 0, 0);
-      }
+      for (int r4 = 0; r4 < 4; ++r4) {
+        bool wrong[4], any = false;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float z = planes[64 * r];  // what the lane itself has put there
-        if (z * 0.0f == 0.0f) t.acc[i][j][r] = z;
+        for (int e = 0; e < 4; ++e) any |= wrong[e] = t.acc[i][j][4 * r4 + e] * 0.0f != 0.0f;
+        if (!__any(any)) continue;
+        int m = m0 + (wm * S::IM + i) * 32 + 8 * r4 + 4 * (lane >> 5) + (lane & 3), n = n0 + (wn * S::JN + j) * 32 + (lane & 31);
+        const bool masked = m >= a.op.M || (a.bias && ((const float*)a.bias)[a.class0 + m] == ninf());
+        const bool counts = n < a.op.N && a.target[n] != a.ignore_index;
+        any = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) any |= wrong[e] = wrong[e] && counts && !__shfl((int)masked, (lane & 32) + e, 64);
+        if (!__any(any)) continue;
+        asm volatile("" : "+v"(m), "+v"(n));  // addresses of these classes alone: made for all in advance they would spill
+        const float* pa = a.given_a + (int64_t)min(m, a.op.M - 1) * a.given_lda;
+        const float* pb = a.given_b + (int64_t)min(n, a.op.N - 1) * a.given_ldb;
+        f32x4 z{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k = 0; k < a.op.dim && __any(any);) {  // until all are NaN, if they become that
+          const int end = min(k + 64, a.op.dim);
+#pragma unroll 4
+          for (; k < end; ++k) z = __builtin_amdgcn_mfma_f32_4x4x1f32(pa[k], pb[k], z, 0, 0, 0);
+          any = false;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) any |= wrong[e] && z[e] == z[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (wrong[e]) t.acc[i][j][4 * r4 + e] = z[e];
       }
-    }
 }
 
 enum { kStatistics, kDerivatives, kRowDerivatives };  // of the logits; derivatives of one gradient, or of one per row
+// T: the tensors' type; SPLIT: float32 by planes of bfloat16.  8192 x 131072 x 4096 bfloat16: forward 6.98 ms, 1260 TFLOP/s,
+// derivatives 8 x 1.01 ms, 1089; bound by the matrix instructions at the power the card allows, then by the epilogue's
+// exponentials, which no other tile's products cover (a large tile fills its CU).  2011 x 32003 x 1000 float16: 149 and 187 us.
 template <typename T, typename S, int WHAT, bool SPLIT, int FORM>
 __global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
   constexpr bool DELTA = WHAT != kStatistics, ROWS = WHAT == kRowDerivatives;
@@ -434,7 +443,7 @@ __global__ __launch_bounds__(S::kThreads) void k_ce_logits(LogitArgs a) {
   const int m0 = tm * S::BM, n0 = tn * S::BN;
   Tile<S> t;
   tile_product<O, S, SPLIT, FORM>(a.op, m0, n0, 0, (SPLIT ? kPairs : 1) * a.op.kblocks, lds, t);
-  if constexpr (SPLIT) exact_if_not_finite<S>(a, m0, n0, lds, t);
+  if constexpr (SPLIT) exact_if_not_finite<S>(a, m0, n0, t);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
   const int half = lane >> 5;
   const bool biased = a.bias || m0 + S::BM > a.op.M;
@@ -1365,9 +1374,9 @@ Layout layout_of(const vsl_linear_ce_desc* d) {
 }
 
 // Pieces of the vocabulary: at most this many derivatives (256 MiB in 16 bits, twice), and at most a GiB of a weight that is laid
-// out (300 x 131072 x 4096 bfloat16: one piece 2.48 ms, two 2.55, four 2.58).  Smaller pieces would stay in the last-level cache, but every piece reads and writes grad_hidden's sums:
-// at 8192 x 131072 x 4096 in bfloat16 2^26, 2^27 and 2^28 derivatives take 29.6, 29.3 and 29.3 ms.  Pieces are equal but for a
-// tile: a short last one costs nearly as much as a whole one.
+// out (300 x 131072 x 4096 bfloat16: one piece 2.48 ms, two 2.55, four 2.58).  Smaller pieces would stay in the last-level cache,
+// but every piece reads and writes grad_hidden's sums: at 8192 x 131072 x 4096 in bfloat16 2^26, 2^27 and 2^28 derivatives take
+// 29.6, 29.3 and 29.3 ms.  Pieces are equal but for a tile: a short last one costs nearly as much as a whole one.
 constexpr int64_t kPieceElements = 1LL << 27, kPieceWeight = 1LL << 30;
 static_assert(kMostParts <= kPieceElements && kMostParts / kPad / kPartRows < 65536, "logits in parts are one piece, their rows one grid");
 struct Pieces {
@@ -1442,7 +1451,8 @@ Backward backward_workspace(const vsl_linear_ce_desc* d, uint32_t mask, void* ba
   // the same pieces whichever gradients are asked for, so that each has the same bits alone; whole where the logits come in parts
   const bool parts = b.l.logits.splits > 1;
   const int64_t tile = parts ? 64 : kShapes[b.l.logits.shape].bm;
-  const Pieces p = parts ? Pieces{round_up(d->vocab, tile), 1} : pieces_of(d, b.l.rows_padded, columns && !b.l.copy_weight ? 0 : b.l.dim_padded * s, tile);
+  const int64_t laid_out = columns && !b.l.copy_weight ? 0 : b.l.dim_padded * s;
+  const Pieces p = parts ? Pieces{round_up(d->vocab, tile), 1} : pieces_of(d, b.l.rows_padded, laid_out, tile);
   b.piece = p.piece;
   b.pieces = p.pieces;
   Arena a{(char*)base};
@@ -1512,7 +1522,8 @@ struct FinishLaunch {
   template <typename T>
   void run(const OutScale& scale, bool rows, hipStream_t s) {
     jobs.scale = scale;
-    if (n) hipLaunchKernelGGL((rows ? k_ce_finish<T, true> : k_ce_finish<T, false>), dim3((unsigned)blocks), dim3(kThreads), 0, s, jobs);
+    const auto kernel = rows ? k_ce_finish<T, true> : k_ce_finish<T, false>;
+    if (n) hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kThreads), 0, s, jobs);
   }
 };
 
@@ -1606,6 +1617,7 @@ void run_forward(const vsl_linear_ce_desc* d, const Forward& f, float* row_loss,
     a.given_ldb = d->hidden_stride;
     a.bias = d->bias;
     a.target = d->target;
+    a.ignore_index = d->ignore_index;
     a.class0 = v0;
     a.rows_padded = l.rows_padded;
     if constexpr (!SPLIT)
@@ -1652,7 +1664,8 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
   const bool uniform = d->reduction != VSL_REDUCE_NONE && d->z_loss == 0.0f;
   const float* row_scale = uniform ? nullptr : b.row_scale;
   const float* row_size = uniform ? nullptr : b.row_size;
-  const OutScale scale = uniform ? OutScale{g_loss, mean_of, nullptr, nullptr, unit} : OutScale{nullptr, nullptr, b.out_scale, nullptr, unit};
+  const OutScale scale = uniform ? OutScale{g_loss, mean_of, nullptr, nullptr, unit}
+                                 : OutScale{nullptr, nullptr, b.out_scale, nullptr, unit};
   if (!uniform) {
     ScaleArgs sc{};
     sc.g_loss = g_loss;
@@ -1695,11 +1708,12 @@ void run_backward(const vsl_linear_ce_desc* d, const Backward& b, const float* s
     }
     if (l.copy_weight) lay.copy(given, d->weight_stride, classes, d->dim, l.dim_padded, b.weight);
     if (grad_hidden && !b.columns)
-      lay.transpose(given, d->weight_stride, classes, d->dim, b.piece, padded, Contributes{nullptr, nullptr, nullptr, bias, 0}, b.weight_t);
+      lay.transpose(given, d->weight_stride, classes, d->dim, b.piece, padded, Contributes{nullptr, nullptr, nullptr, bias, 0},
+                    b.weight_t);
     lay.run<T, SPLIT>(s);
     LogitArgs a{};
-    a.op = {l.copy_weight ? b.weight : (const void*)given, hidden, ldw, ldh, (int)classes, (int)d->rows, (int)(l.dim_padded / Kind<O>::BK), l.dim_padded,
-            l.dim_padded, l.tail, (int)d->dim};
+    a.op = {l.copy_weight ? b.weight : (const void*)given, hidden, ldw, ldh, (int)classes, (int)d->rows,
+            (int)(l.dim_padded / Kind<O>::BK), l.dim_padded, l.dim_padded, l.tail, (int)d->dim};
     if constexpr (SPLIT) a.given_a = given, a.given_b = (const T*)d->hidden;
     a.given_lda = d->weight_stride;
     a.given_ldb = d->hidden_stride;
