@@ -416,7 +416,6 @@ __device__ __forceinline__ void exact_if_not_finite(const LogitArgs& a, int m0, 
         f32x4 z{0.0f, 0.0f, 0.0f, 0.0f};
         for (int k = 0; k < a.op.dim && __any(any);) {  // until all are NaN, if they become that
           const int end = min(k + 64, a.op.dim);
-#pragma unroll 4
           for (; k < end; ++k) z = __builtin_amdgcn_mfma_f32_4x4x1f32(pa[k], pb[k], z, 0, 0, 0);
           any = false;
 #pragma unroll
